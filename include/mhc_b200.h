@@ -346,6 +346,73 @@ MHC_API int mhc_layer_bwd_static(const float* grad_out, const float* x, const fl
                          size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Embedding lookup into residual streams, and its gradient.  No counterpart in
+ * the reference, whose models start from embeddings made elsewhere.
+ *   out[t, i, :] = scales[i] * weight[ids[t], :]        t < tokens, i < n <= 32
+ * ids are int64 (ids_64 != 0) or int32; weight [vocab, hidden] and out
+ * [tokens, n, hidden] are fp32 or bf16 each (products in fp32, rounded once);
+ * scales is a HOST array of n floats, read before the call returns.  An id
+ * outside [0, vocab) gives a row of NaN and reads nothing.
+ * ------------------------------------------------------------------------- */
+MHC_API int mhc_stream_embedding_fwd(const void* ids, int32_t ids_64, const void* weight, int32_t weight_bf16,
+                             void* out, int32_t out_bf16, const float* scales, int64_t tokens,
+                             int32_t n, int64_t hidden, int64_t vocab, void* stream);
+/* grad_weight[v, :] = sum over t with ids[t] = v, v != padding_idx, of
+ * sum_i scales[i] grad_out[t, i, :], fp32 sums in token order (bitwise
+ * reproducible); the whole [vocab, hidden] gradient is written, rows without a
+ * token as zeros.  Ids outside [0, vocab) add nothing; padding_idx < 0: none.
+ * grad_weight must be 16-byte aligned. */
+MHC_API size_t mhc_stream_embedding_bwd_workspace_bytes(int64_t tokens, int64_t hidden);
+MHC_API int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, const void* ids, int32_t ids_64,
+                             void* grad_weight, int32_t gw_bf16, const float* scales, int64_t tokens,
+                             int32_t n, int64_t hidden, int64_t vocab, int64_t padding_idx,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits.  No counterpart in the reference, which
+ * saves whole bf16 copies (ops.py:394-470).
+ * A row of cols values is kept as int8 codes, padded with zeros to
+ * mhc_checkpoint8_pitch(cols) = 128 * ceil(cols / 128) bytes, and one exponent
+ * byte E per 32 codes (pitch / 32 a row): a code stands for code * 2^(E - 127).
+ * With a = max |x| of a block, E >= 1 is the smallest with
+ * a < 127.5 * 2^(E - 127), and code = x / 2^(E - 127) rounded to nearest, ties
+ * to even (at E = 249 held to +-63: 64 would stand for 2^128).  E = 255: the block held an infinity or a NaN and stands for NaNs.
+ * codes must be 16-byte and exponents 4-byte aligned.
+ * ------------------------------------------------------------------------- */
+MHC_API int64_t mhc_checkpoint8_pitch(int64_t cols);
+/* x [rows, cols] fp32 or bf16, rows row_stride elements apart */
+MHC_API int mhc_checkpoint8_pack(const void* x, int32_t x_bf16, int64_t row_stride, int8_t* codes,
+                         uint8_t* exponents, int64_t rows, int64_t cols, void* stream);
+/* out [rows, cols] contiguous, fp32 or bf16 (both exact) */
+MHC_API int mhc_checkpoint8_unpack(const int8_t* codes, const uint8_t* exponents, void* out,
+                           int32_t out_bf16, int64_t rows, int64_t cols, void* stream);
+/* RMSNorm (mhc_rmsnorm_fwd) of x [rows, cols] fp32 or bf16, out in x's type,
+ * that also packs x in the same pass. */
+MHC_API int mhc_rmsnorm_checkpoint8_fwd(const void* x, int32_t x_bf16, const float* weight, void* out,
+                                float* rms, int8_t* codes, uint8_t* exponents, int64_t rows,
+                                int64_t cols, float eps, void* stream);
+/* Its backward at the restored input xh (rms is the forward's):
+ *   grad_x = (g w - xh sum(g w xh) / (cols rms^2)) / rms, in g's type
+ *   grad_weight = sum over rows of g xh / rms (fixed order) */
+MHC_API size_t mhc_rmsnorm_checkpoint8_bwd_workspace_bytes(int64_t rows, int64_t cols);
+MHC_API int mhc_rmsnorm_checkpoint8_bwd(const void* grad_out, int32_t g_bf16, const int8_t* codes,
+                                const uint8_t* exponents, const float* weight, const float* rms,
+                                void* grad_x, float* grad_weight, int64_t rows, int64_t cols,
+                                void* workspace, size_t workspace_bytes, void* stream);
+/* Weight gradient of a linear layer from its kept input:
+ *   grad_weight[o, k] = sum_t grad_out[t, o] xh[t, k]        [out_features, in_features]
+ * grad_out [tokens, out_features] fp32 or bf16, rows row_stride elements apart;
+ * grad_weight fp32 or bf16, contiguous.  fp32 grad_out is used in full
+ * precision; sums are fp32 and in a fixed order. */
+MHC_API size_t mhc_checkpoint8_weight_grad_workspace_bytes(int64_t tokens, int64_t out_features,
+                                                   int64_t in_features, int32_t g_bf16, int32_t gw_bf16);
+MHC_API int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16, int64_t row_stride,
+                                const int8_t* codes, const uint8_t* exponents, void* grad_weight,
+                                int32_t gw_bf16, int64_t tokens, int64_t out_features,
+                                int64_t in_features, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* ---------------------------------------------------------------------------
  * Device error word.  No counterpart in the reference.  Kernels that wait on
  * asynchronous copies (TMA + mbarrier) bound every wait; a wait that runs out
  * sets this word to nonzero and the kernel abandons its work (its outputs are

@@ -73,6 +73,19 @@ SIGNATURES = {
                                   [_P] * 7 + [_I64, _I32, _I64, _I32, _F, _F, _P, _SZ, _P]),
     "mhc_layer_bwd_static": (ctypes.c_int,
                              [_P] * 12 + [_I64, _I32, _I64, _I32, _F, _F, _P, _SZ, _P]),
+    "mhc_stream_embedding_fwd": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _I32, _P, _I64, _I32, _I64, _I64, _P]),
+    "mhc_stream_embedding_bwd_workspace_bytes": (_SZ, [_I64, _I64]),
+    "mhc_stream_embedding_bwd": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _I32, _P, _I64, _I32, _I64, _I64, _I64,
+                                                _P, _SZ, _P]),
+    "mhc_checkpoint8_pitch": (_I64, [_I64]),
+    "mhc_checkpoint8_pack": (ctypes.c_int, [_P, _I32, _I64, _P, _P, _I64, _I64, _P]),
+    "mhc_checkpoint8_unpack": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I64, _P]),
+    "mhc_rmsnorm_checkpoint8_fwd": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _I64, _I64, _F, _P]),
+    "mhc_rmsnorm_checkpoint8_bwd_workspace_bytes": (_SZ, [_I64, _I64]),
+    "mhc_rmsnorm_checkpoint8_bwd": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
+    "mhc_checkpoint8_weight_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
+    "mhc_checkpoint8_weight_grad": (ctypes.c_int, [_P, _I32, _I64, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _SZ,
+                                                   _P]),
     "mhc_device_error_word": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int32), ctypes.c_int32]),
     "mhc_profile_enable": (ctypes.c_int, [ctypes.c_int]),
     "mhc_profile_report": (ctypes.c_int, [ctypes.c_char_p, _SZ]),

@@ -21,6 +21,26 @@ from .ops import (
     stream_distribute_mix_add,
 )
 
+# Operators beyond the reference's API: attributes of the package, left out of
+# __all__, which names exactly what the reference exports.
+from .checkpoint8 import (  # noqa: F401
+    Checkpoint8,
+    checkpoint8_pack,
+    checkpoint8_recompute,
+    checkpoint8_unpack,
+    checkpoint8_weight_grad,
+    linear_checkpoint8,
+    rmsnorm_checkpoint8,
+    rmsnorm_checkpoint8_bwd,
+    rmsnorm_checkpoint8_fwd,
+)
+from .embedding import (  # noqa: F401
+    StreamEmbedding,
+    stream_embedding,
+    stream_embedding_bwd,
+    stream_embedding_fwd,
+)
+
 __all__ = [
     "MHCLayer",
     "MHCResidualWrapper",

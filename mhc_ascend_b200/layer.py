@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .checkpoint8 import checkpoint8_recompute, rmsnorm_checkpoint8
 from .ops import (
     MHCLayerStaticFunction,
     compute_rms,
@@ -50,11 +51,16 @@ class MHCLayer(nn.Module):
             arithmetic): static-H inference, and dynamic-H training and
             inference at n <= 4 (n == 4 for training), hidden % 64 == 0.  Off
             by default: like the reference, the layer then returns fp32.
+        checkpoint_8bit: in training, keep the input streams in 8 bits (33/32
+            bytes a value) and nothing else; the backward restores them and
+            runs the forward kernels again.  The gradients are the layer's at
+            the restored input.
     """
 
     def __init__(self, hidden_dim: int, expansion_rate: int = 4, num_sinkhorn_iters: int = 20,
                  sinkhorn_eps: float = 1e-8, rmsnorm_eps: float = 1e-5,
-                 use_dynamic_h: bool = True, alpha_init: float = 0.01, bf16_io: bool = False):
+                 use_dynamic_h: bool = True, alpha_init: float = 0.01, bf16_io: bool = False,
+                 checkpoint_8bit: bool = False):
         super().__init__()
         self.hidden_dim = hidden_dim
         self.expansion_rate = expansion_rate
@@ -63,6 +69,7 @@ class MHCLayer(nn.Module):
         self.rmsnorm_eps = rmsnorm_eps
         self.use_dynamic_h = use_dynamic_h
         self.bf16_io = bf16_io
+        self.checkpoint_8bit = checkpoint_8bit
         n, C = expansion_rate, hidden_dim
         nC = n * C
         self.rmsnorm_weight = nn.Parameter(torch.ones(hidden_dim, dtype=torch.float32))
@@ -86,35 +93,44 @@ class MHCLayer(nn.Module):
         assert n == self.expansion_rate, f"Expected expansion_rate={self.expansion_rate}, got {n}"
         assert C == self.hidden_dim, f"Expected hidden_dim={self.hidden_dim}, got {C}"
         if self.use_dynamic_h:
-            args = (self.rmsnorm_weight, self.phi_pre, self.phi_post, self.phi_res,
-                    self.alpha_pre, self.alpha_post, self.alpha_res, self.b_pre, self.b_post,
-                    self.b_res, self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps)
+            params = (self.rmsnorm_weight, self.phi_pre, self.phi_post, self.phi_res,
+                      self.alpha_pre, self.alpha_post, self.alpha_res, self.b_pre, self.b_post,
+                      self.b_res)
+        else:
+            params = (self.rmsnorm_weight, self.H_pre, self.H_post, self.H_res)
+        if self.checkpoint_8bit and torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params)):
+            if x.dtype not in (torch.float32, torch.bfloat16):
+                x = x.float()
+            return checkpoint8_recompute(self._run, x, *params)
+        return self._run(x, *params)
+
+    def _run(self, x, *params):
+        """The layer on x with the given parameters."""
+        B, n, C = x.shape
+        if self.use_dynamic_h:
+            args = (*params, self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps)
             bf16 = self.bf16_io and x.dtype == torch.bfloat16
             xin = x if bf16 else x.float()
             if (not self.training) and (not torch.is_grad_enabled()):
                 return mhc_layer_fused_dynamic_inference(xin, *args, bf16_io=bf16)
             return mhc_layer_fused_dynamic_training(xin, *args, bf16_io=bf16)
         hp = (self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps)
+        w, H_pre, H_post, H_res = params
         if n > 8:
             # the fused static kernels cover n <= 8; wider rates run the
             # reference's own composition (layer.py:142-170) over this
             # library's CUDA operators, with one Sinkhorn for the shared H_res
             xf = x.float()
-            M = sinkhorn_knopp(torch.exp(self.H_res.float()).unsqueeze(0), hp[0], hp[1])
-            y = rmsnorm(stream_aggregate(xf, self.H_pre.unsqueeze(0).expand(B, -1)),
-                        self.rmsnorm_weight, hp[2])
-            return stream_distribute_mix_add(y, self.H_post.unsqueeze(0).expand(B, -1),
+            M = sinkhorn_knopp(torch.exp(H_res.float()).unsqueeze(0), hp[0], hp[1])
+            y = rmsnorm(stream_aggregate(xf, H_pre.unsqueeze(0).expand(B, -1)), w, hp[2])
+            return stream_distribute_mix_add(y, H_post.unsqueeze(0).expand(B, -1),
                                              M.expand(B, -1, -1), xf)
-        if not torch.is_grad_enabled() or not (x.requires_grad or any(
-                p.requires_grad for p in (self.rmsnorm_weight, self.H_pre, self.H_post,
-                                          self.H_res))):
+        if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, *params)):
             bf16 = self.bf16_io and x.dtype == torch.bfloat16
-            out, _ = mhc_layer_fwd_static(x if bf16 else x.float(), self.rmsnorm_weight,
-                                          self.H_pre, self.H_post, self.H_res, *hp,
+            out, _ = mhc_layer_fwd_static(x if bf16 else x.float(), w, H_pre, H_post, H_res, *hp,
                                           save_rms=False, bf16_io=bf16)
             return out
-        return MHCLayerStaticFunction.apply(x.float(), self.rmsnorm_weight, self.H_pre,
-                                            self.H_post, self.H_res, *hp)
+        return MHCLayerStaticFunction.apply(x.float(), w, H_pre, H_post, H_res, *hp)
 
     def extra_repr(self) -> str:
         return (f"hidden_dim={self.hidden_dim}, expansion_rate={self.expansion_rate}, "
@@ -137,7 +153,8 @@ class MHCResidualWrapper(nn.Module):
 
     Streams: [residual, branch_output, 0.1*residual, 0.01*residual, ...]
     ('decay') or zeros beyond the first two ('zero'); the mHC output is averaged
-    over streams.  ``use_post_norm`` is accepted and, as in the reference
+    over streams.  With ``checkpoint_8bit`` (an argument of the layer) the
+    residual and the branch output are kept in 8 bits for the backward.  ``use_post_norm`` is accepted and, as in the reference
     (layer.py:261), forced off.
     """
 
@@ -166,10 +183,12 @@ class MHCResidualWrapper(nn.Module):
             # n = 4, dynamic H: the streams are built inside the layer's kernels
             # and the mean is written by its output pass -- no [B*T, n, C]
             # tensor in either direction
-            output = wrapper_fused_dynamic(
-                residual, branch_output, self.residual_mode, m.rmsnorm_weight, m.phi_pre,
-                m.phi_post, m.phi_res, m.alpha_pre, m.alpha_post, m.alpha_res, m.b_pre, m.b_post,
-                m.b_res, m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
+            params = (m.rmsnorm_weight, m.phi_pre, m.phi_post, m.phi_res, m.alpha_pre, m.alpha_post,
+                      m.alpha_res, m.b_pre, m.b_post, m.b_res)
+            if m.checkpoint_8bit and torch.is_grad_enabled():
+                output = checkpoint8_recompute(self._fused, residual, branch_output, *params, kept=2)
+            else:
+                output = self._fused(residual, branch_output, *params)
             return output.reshape(B, T, C) if T > 1 else output
         # one CUDA pass packs the streams, one averages them (the reference
         # runs n - 1 scalings, a stack and a mean as framework ops)
@@ -178,6 +197,11 @@ class MHCResidualWrapper(nn.Module):
         if T > 1:
             output = output.reshape(B, T, C)
         return output
+
+    def _fused(self, residual, branch_output, *params):
+        m = self.mhc
+        return wrapper_fused_dynamic(residual, branch_output, self.residual_mode, *params,
+                                     m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
 
     def forward_prenorm(self, residual: torch.Tensor, branch_output: torch.Tensor,
                         norm_weight: torch.Tensor, norm_eps: float = 1e-5):
@@ -194,14 +218,15 @@ class MHCResidualWrapper(nn.Module):
         r2, b2 = residual.reshape(-1, C), branch_output.reshape(-1, C)
         m = self.mhc
         if wrapper_fused_supported(r2, b2, self.expansion_rate, C, m.use_dynamic_h) and \
-                self.residual_mode in ("decay", "zero"):
+                self.residual_mode in ("decay", "zero") and not m.checkpoint_8bit:
             hidden, normed = wrapper_fused_dynamic_prenorm(
                 r2, b2, self.residual_mode, norm_weight, norm_eps, m.rmsnorm_weight, m.phi_pre,
                 m.phi_post, m.phi_res, m.alpha_pre, m.alpha_post, m.alpha_res, m.b_pre, m.b_post,
                 m.b_res, m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
             return hidden.reshape(shape), normed.reshape(shape)
         hidden = self.forward(residual, branch_output)
-        return hidden, rmsnorm(hidden.reshape(-1, C), norm_weight, norm_eps).reshape(shape)
+        norm = rmsnorm_checkpoint8 if m.checkpoint_8bit else rmsnorm
+        return hidden, norm(hidden.reshape(-1, C), norm_weight, norm_eps).reshape(shape)
 
     def extra_repr(self) -> str:
         return (f"hidden_dim={self.hidden_dim}, expansion_rate={self.expansion_rate}, "
