@@ -1,79 +1,547 @@
-// Weight gradient of a linear layer from its input kept in 8 bits:
+// Weight gradient of a linear layer from its input kept in 8 bits, on tcgen05:
 //   gW[o, k] = sum_t g[t, o] xh[t, k]
+//
+// xh is exact in bf16 (checkpoint8.cuh), so a bf16 g makes every product exact
+// and the sum is formed in fp32 in tensor memory.  An fp32 g is cut into three
+// bf16 terms of 8 significant bits each (exact, by truncation), three MMAs a
+// step.
+//
+// A pair of CTAs (cta_group::2) computes 256 x 256 tiles of gW: M = 256 rows o
+// (A = g, 128 of them in each CTA), N = 256 columns k (B = xh, 128 expanded by
+// each CTA).  Both operands are MN-major: a token is a row of g and of the
+// codes, and the contraction runs over tokens, so neither is transposed.  Why a
+// pair: a CTA then expands and stores 128 columns for 128 x 256 products; alone
+// it would expand 256, and with the MMAs' own operand reads that is more than
+// shared memory's 128 bytes a cycle.
+//
+// Warps of a CTA: 0 issues the TMA loads of g, 1 the MMAs (of the pair, in the
+// even CTA), 2 owns the tensor memory, 4..7 empty accumulators, 8..15 read
+// codes straight from global memory (L2), two stages ahead of their use, and
+// store xh in the 128-byte-swizzled layout that the MMA reads.  A stage is 64
+// tokens.  Two accumulators of 256 columns fill tensor memory, so a tile is
+// written while the next one is summed.
+//
+// Accumulating MMAs truncate (a relative shrink of about 2e-8 each, measured on
+// the layer's projection), so a chain is kept to kChain stages: 4096 tokens
+// or 256 MMAs; what follows is added in fp32 in global memory by the thread that
+// wrote the sum before.  A bf16 gW needs no such cut (kMaxChain16).
 #include "checkpoint8.cuh"
+#include "tma.cuh"
 
 namespace mhc {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16;
+constexpr int kTok = 64;                       // tokens of a stage
+constexpr int kTileO = 256, kTileK = 256;      // tile of a pair
+constexpr uint32_t kOpBytes = kTok * 128 * 2;  // one operand of one CTA, one stage: 64 tokens x 128 bf16
+constexpr int kThreads = 512, kExpandWarps = 8;
+constexpr int kChain = 64;                     // stages summed in tensor memory before fp32 takes over
+constexpr int64_t kMaxChain16 = 1 << 18;       // tokens: 2^18 / 16 MMAs x 2e-8 is 3.3e-4, a twelfth of a bf16
+                                               // rounding; longer sums go through fp32 parts
 
-// A 64 x 64 tile of gW a block, 4 x 4 values a thread, 16 tokens at a time
-// through shared memory; the codes are expanded as they are staged.
-template <typename TG, typename TW>
-__global__ void __launch_bounds__(256)
-    wgrad_plain_kernel(const TG* __restrict__ g, int64_t stride, const int8_t* __restrict__ codes,
-                       const uint8_t* __restrict__ exps, TW* __restrict__ gw, int64_t T, int64_t O, int64_t K,
-                       int64_t pitch) {
-  __shared__ float sg[kDepth][kTile], sx[kDepth][kTile];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int64_t o0 = (int64_t)blockIdx.y * kTile, k0 = (int64_t)blockIdx.x * kTile;
-  float acc[4][4] = {};
-  for (int64_t t0 = 0; t0 < T; t0 += kDepth) {
-#pragma unroll
-    for (int e = tid; e < kDepth * kTile; e += 256) {
-      const int d = e / kTile, c = e % kTile;
-      const int64_t t = t0 + d;
-      sg[d][c] = t < T && o0 + c < O ? ck_f32(g[t * stride + o0 + c]) : 0.f;
-      float v[1] = {0.f};
-      if (t < T && k0 + c < K) ck_decode<1>(codes + t * pitch, exps + t * (pitch / kCkBlock), k0 + c, v);
-      sx[d][c] = v[0];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sg[d][ty * 4 + i], sx[d][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+template <int PLANES>
+struct WgCfg {
+  static constexpr uint32_t STAGE = (PLANES + 1) * kOpBytes;  // A planes, then B
+  static constexpr int STAGES = PLANES == 1 ? 6 : 3;
+  static constexpr uint32_t OFF_BAR = STAGES * STAGE;
+  static constexpr uint32_t SMEM = OFF_BAR + (3 * STAGES + 5) * 8 + 16 + 1024;  // + alignment of the ring
+};
+
+struct WgArgs {
+  const int8_t* codes;
+  const uint8_t* exps;
+  void* gw;
+  float* part;           // parts of split tiles: [unit][256][256]
+  int64_t T, O, K, pitch;
+  int tiles_o, tiles_k;
+  int full, splits;      // whole tiles, then each further tile in `splits` parts along the tokens
+  int units;
+};
+
+// Work of a pair: unit u is a whole tile or a part of one, as a range of stages.
+struct Unit {
+  int tile_o, tile_k, s0, s1, part;  // part < 0: into gw
+};
+__device__ __forceinline__ Unit unit_of(const WgArgs& a, int u) {
+  Unit r;
+  const int nst = (int)((a.T + kTok - 1) / kTok);
+  int tile = u;
+  r.s0 = 0; r.s1 = nst; r.part = -1;
+  if (u >= a.full) {
+    const int v = u - a.full, s = v % a.splits;
+    tile = a.full + v / a.splits;
+    r.part = v;
+    r.s0 = (int)((int64_t)nst * s / a.splits);
+    r.s1 = (int)((int64_t)nst * (s + 1) / a.splits);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t o = o0 + ty * 4 + i, k = k0 + tx * 4 + j;
-      if (o < O && k < K) ck_store(gw + o * K + k, acc[i][j]);
-    }
+  // bands of 8 tile columns, rows of tiles within a band: pairs that run
+  // together read the same few rows of tiles and the same 8 columns from L2
+  constexpr int BAND = 8;
+  const int band = tile / (BAND * a.tiles_o), w = min(BAND, a.tiles_k - band * BAND), in = tile - band * BAND * a.tiles_o;
+  r.tile_o = in / w;
+  r.tile_k = band * BAND + in % w;
+  return r;
 }
 
-template <typename TG, typename TW>
-int launch_plain(const void* g, int64_t stride, const int8_t* codes, const uint8_t* exps, void* gw, int64_t T,
-                 int64_t O, int64_t K, cudaStream_t st) {
-  ProfScope p("checkpoint8_weight_grad", st);
-  const dim3 grid((unsigned)((K + kTile - 1) / kTile), (unsigned)((O + kTile - 1) / kTile));
-  wgrad_plain_kernel<TG, TW><<<grid, 256, 0, st>>>((const TG*)g, stride, codes, exps, (TW*)gw, T, O, K, ck_pitch(K));
-  return check_launch("checkpoint8_weight_grad");
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrive on the barrier at this offset in the even CTA
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .b32 ra;\n mapa.shared::cluster.u32 ra, %0, 0;\n"
+      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool poll_cluster(uint32_t addr, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(addr), "r"(parity), "r"(kSuspendNs)
+      : "memory");
+  return done != 0;
+}
+// Bounded wait; gives up early once another warp of the CTA has.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  const uint32_t addr = smem_u32(bar);
+  if (poll_cluster(addr, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 0; it < kSpinLimit; ++it) {
+    if (poll_cluster(addr, parity)) return true;
+    if (*stop) return false;
+    if (global_ns() - t0 > kWaitLimitNs) break;
+  }
+  atomicExch(&g_mhc_device_error, 1);
+  *stop = 1;
+  return false;
+}
+
+// MN-major operand, 128-byte swizzle: atoms of 64 elements x 8 tokens, the next
+// 64 elements 8192 bytes on, the next 8 tokens 1024
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D fp32, A and B bf16, both MN-major, 256 x 256
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((kTileK >> 3) << 17) |
+                            ((kTileO >> 4) << 24);
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(kIdesc), "r"(accumulate)
+      : "memory");
+}
+// arrives at this offset in both CTAs once the pair's MMAs issued so far are done
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+// Two codes -> two bf16 values.  With the low 7 bits set into the mantissa of
+// 128 (0x43nn) a byte reads 128 + low7; less 128, or 256 where its sign is set,
+// that is the code, and the product with the power-of-two step is exact.
+// sel picks the two bytes.
+__device__ __forceinline__ uint32_t expand2(uint32_t low, uint32_t sign, uint32_t sel, __nv_bfloat162 step) {
+  uint32_t a = __byte_perm(low, 0x43434343u, sel), k = __byte_perm(sign, 0x43434343u, sel);
+  const __nv_bfloat162 d = __hmul2(__hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&k)), step);
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+// Columns [c, c + 32) of one output row: add what is there if `more`, store.
+__device__ __forceinline__ void put_row(float* p, float (&v)[32], int64_t left, bool vec, bool more) {
+  if (vec && left >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      if (more) {
+        const float4 b = *reinterpret_cast<const float4*>(p + j);
+        o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
+      }
+      *reinterpret_cast<float4*>(p + j) = o;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) p[j] = more ? p[j] + v[j] : v[j];
+  }
+}
+__device__ __forceinline__ void put_row(__nv_bfloat16* p, float (&v)[32], int64_t left, bool vec, bool) {
+  if (vec && left >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = v[j + i];
+      ck_save(p + j, w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) ck_store(p + j, v[j]);
+  }
+}
+
+template <int PLANES, typename TW>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    wgrad_kernel(const __grid_constant__ CUtensorMap gmap, const WgArgs a) {
+  using Cfg = WgCfg<PLANES>;
+  constexpr int S = Cfg::STAGES;
+  extern __shared__ unsigned char raw[];
+  unsigned char* ring = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);  // the same offset in both CTAs
+  uint64_t* afull = reinterpret_cast<uint64_t*>(ring + Cfg::OFF_BAR);  // [S] this CTA's part of g has landed
+  uint64_t* full = afull + S;                                          // [S] (even CTA) both operands of both CTAs
+  uint64_t* empty = full + S;                                          // [S] the stage's MMAs are done
+  uint64_t* dfull = empty + S;                                         // [2] an accumulator is whole
+  uint64_t* dempty = dfull + 2;                                        // [2] (even CTA) it has been read in both CTAs
+  uint64_t* idle = dempty + 2;                                         // every MMA issued is done
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(idle + 1);
+  volatile int* stop = reinterpret_cast<volatile int*>(tslot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cta_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&afull[s], 1);
+      mbar_init(&full[s], 2 * kExpandWarps);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&dfull[b], 1);
+      mbar_init(&dempty[b], 8);
+    }
+    mbar_init(idle, 1);
+    *stop = 0;
+    fence_mbar_init();
+    prefetch_tmap(&gmap);
+  }
+  fence_before();
+  __syncthreads();
+  cluster_barrier();
+  fence_after();
+  const uint32_t tmem = *tslot;
+
+  if (warp == 0) {
+    if (lane == 0) {  // ---- g: two boxes of 64 columns x 64 tokens a plane ----
+      int it = 0;
+      for (int u = pair; u < a.units && !*stop; u += pairs) {
+        const Unit q = unit_of(a, u);
+        const int o = q.tile_o * kTileO + (int)rank * 128;
+        for (int st = q.s0; st < q.s1; ++st, ++it) {
+          const int s = it % S;
+          if (it >= S && !wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop)) goto loads_done;
+          unsigned char* dst = ring + s * Cfg::STAGE;
+          mbar_expect_tx(&afull[s], PLANES * kOpBytes);
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p) {
+            tma_load_3d(dst + p * kOpBytes, &gmap, o, st * kTok, p, &afull[s]);
+            tma_load_3d(dst + p * kOpBytes + kOpBytes / 2, &gmap, o + 64, st * kTok, p, &afull[s]);
+          }
+        }
+      }
+    loads_done:
+      // nothing may land after the block is gone
+      for (int j = it > S ? it - S : 0; j < it; ++j) mbar_wait(&afull[j % S], (uint32_t)((j / S) & 1));
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {  // ---- MMAs of the pair ----
+      int it = 0, acc = 0;
+      for (int u = pair; u < a.units; u += pairs) {
+        const Unit q = unit_of(a, u);
+        const int cut = (sizeof(TW) == 4 || q.part >= 0) ? kChain : q.s1 - q.s0;
+        for (int st = q.s0; st < q.s1; ++acc) {
+          const int b = acc & 1, end = min(st + cut, q.s1);
+          if (acc >= 2 && !wait_bar(&dempty[b], (uint32_t)((acc / 2 - 1) & 1), stop)) goto mma_done;
+          fence_after();
+          const uint32_t d = tmem + 256u * b;
+          for (int first = st; st < end; ++st, ++it) {
+            const int s = it % S;
+            if (!wait_bar(&full[s], (uint32_t)((it / S) & 1), stop)) goto mma_done;
+            fence_after();
+            const uint32_t base = smem_u32(ring + s * Cfg::STAGE);
+#pragma unroll
+            for (int p = PLANES - 1; p >= 0; --p)  // smallest terms first
+#pragma unroll
+              for (int k = 0; k < kTok / 16; ++k)
+                mma_pair(d, mn_desc(base + p * kOpBytes + k * 2048), mn_desc(base + PLANES * kOpBytes + k * 2048),
+                         (st > first || p < PLANES - 1 || k > 0) ? 1u : 0u);
+            commit_pair(&empty[s]);
+          }
+          commit_pair(&dfull[b]);
+        }
+      }
+    mma_done:
+      commit_pair(idle);
+      mbar_wait(idle, 0u);
+    }
+  } else if (warp >= 8) {
+    // ---- expand: a thread takes one token's block of 32 codes a stage ----
+    const int e = tid - 256;                             // 0 .. 255
+    const int tok = (e & 7) | ((e >> 5) << 3);           // eight lanes: eight tokens, so that 16-byte stores meet no
+    const int blk = (e >> 3) & 3;                        // bank twice under the swizzle
+    const uint32_t row = (uint32_t)(PLANES * kOpBytes + (blk >> 1) * (kOpBytes / 2) + tok * 128);
+    uint4 c0[2], c1[2];
+    uint32_t ex[2];
+    // the fetch runs two stages ahead of the store
+    int fu = pair, fs = 0, fe = 0;
+    int64_t fk = 0;
+    auto ahead = [&](int slot) {  // fetch the next stage, if there is one
+      if (fs >= fe) {
+        if (fu >= a.units) return;
+        const Unit q = unit_of(a, fu);
+        fs = q.s0;
+        fe = q.s1;
+        fk = (int64_t)q.tile_k * kTileK + rank * 128 + blk * 32;
+      }
+      const int64_t t = (int64_t)fs * kTok + tok;
+      c0[slot] = c1[slot] = make_uint4(0u, 0u, 0u, 0u);
+      ex[slot] = 1u;
+      if (t < a.T && fk < a.pitch) {
+        const uint4* p = reinterpret_cast<const uint4*>(a.codes + t * a.pitch + fk);
+        c0[slot] = __ldg(p);
+        c1[slot] = __ldg(p + 1);
+        ex[slot] = __ldg(a.exps + (t * a.pitch + fk) / kCkBlock);
+      }
+      if (++fs >= fe) fu += pairs;
+    };
+    auto put = [&](int it, int slot) -> bool {
+      const int s = it % S;
+      bool ok = it < S || wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      const uint16_t sb = ex[slot] == 255u ? 0x7fc0 : (uint16_t)(ex[slot] << 7);
+      const __nv_bfloat162 step = __halves2bfloat162(__ushort_as_bfloat16(sb), __ushort_as_bfloat16(sb));
+      const uint32_t w[8] = {c0[slot].x, c0[slot].y, c0[slot].z, c0[slot].w,
+                             c1[slot].x, c1[slot].y, c1[slot].z, c1[slot].w};
+      unsigned char* dst = ring + s * Cfg::STAGE + row;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 o;
+        const uint32_t l0 = w[2 * j] & 0x7f7f7f7fu, s0 = w[2 * j] & 0x80808080u;
+        const uint32_t l1 = w[2 * j + 1] & 0x7f7f7f7fu, s1 = w[2 * j + 1] & 0x80808080u;
+        o.x = expand2(l0, s0, 0x4140, step);
+        o.y = expand2(l0, s0, 0x4342, step);
+        o.z = expand2(l1, s1, 0x4140, step);
+        o.w = expand2(l1, s1, 0x4342, step);
+        *reinterpret_cast<uint4*>(dst + ((((blk & 1) * 4 + j) ^ (tok & 7)) << 4)) = o;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        ok = wait_bar(&afull[s], (uint32_t)((it / S) & 1), stop);
+        if (ok) arrive_leader(&full[s]);
+      }
+      return __all_sync(0xffffffffu, ok);
+    };
+    int total = 0;
+    for (int u = pair; u < a.units; u += pairs) {
+      const Unit q = unit_of(a, u);
+      total += q.s1 - q.s0;
+    }
+    ahead(0);
+    ahead(1);
+    for (int it = 0; it < total; it += 2) {
+      if (!put(it, 0)) break;
+      ahead(0);
+      if (it + 1 < total) {
+        if (!put(it + 1, 1)) break;
+        ahead(1);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- accumulators -> gW or a part ----
+    const int q4 = warp & 3, rr = (int)rank * 128 + 32 * q4 + lane;
+    int acc = 0;
+    bool ok = true;
+    for (int u = pair; u < a.units && ok; u += pairs) {
+      const Unit q = unit_of(a, u);
+      const bool parts = q.part >= 0;
+      const int cut = (sizeof(TW) == 4 || parts) ? kChain : q.s1 - q.s0;
+      const int64_t o = (int64_t)q.tile_o * kTileO + rr, k0 = (int64_t)q.tile_k * kTileK;
+      for (int st = q.s0; st < q.s1; st += cut, ++acc) {
+        const int b = acc & 1;
+        ok = wait_bar(&dfull[b], (uint32_t)((acc / 2) & 1), stop);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        const bool more = st > q.s0;
+#pragma unroll 1
+        for (int c = 0; c < kTileK; c += 32) {
+          float v[32];
+          tmem_ld32(tmem + 256u * b + ((uint32_t)(32 * q4) << 16) + (uint32_t)c, v);
+          if (parts) {
+            put_row(a.part + ((int64_t)q.part * kTileO + rr) * kTileK + c, v, 32, true, more);
+          } else if (o < a.O && k0 + c < a.K) {
+            TW* p = reinterpret_cast<TW*>(a.gw) + o * a.K + k0 + c;
+            put_row(p, v, a.K - k0 - c, (reinterpret_cast<uintptr_t>(p) & 15) == 0, more);
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader(&dempty[b]);
+      }
+    }
+  }
+  // the other CTA may still arrive here, or read this one's operands
+  __syncthreads();
+  cluster_barrier();
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// Sum of a tile's parts, in order, into gW.
+template <typename TW>
+__global__ void __launch_bounds__(256)
+    wgrad_join_kernel(const WgArgs a) {
+  const Unit q = unit_of(a, a.full + (int)(blockIdx.x / (kTileO / 4)) * a.splits);
+  const int rr = (blockIdx.x % (kTileO / 4)) * 4 + (threadIdx.x >> 6), c = (threadIdx.x & 63) * 4;
+  const int64_t o = (int64_t)q.tile_o * kTileO + rr, k = (int64_t)q.tile_k * kTileK + c;
+  if (o >= a.O || k >= a.K) return;
+  const float* p = a.part + ((int64_t)q.part * kTileO + rr) * kTileK + c;
+  float4 s = *reinterpret_cast<const float4*>(p);
+  for (int i = 1; i < a.splits; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(p + (int64_t)i * kTileO * kTileK);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  TW* d = reinterpret_cast<TW*>(a.gw) + o * a.K + k;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (k + j < a.K) ck_store(d + j, v[j]);
+}
+
+// g as bf16 planes [PLANES][T][width] for the TMA: fp32 cut into three terms of
+// 8 bits by truncation (their sum is exact), or rows that the TMA cannot read
+// (start or stride not a multiple of 16 bytes) copied.
+template <typename TG>
+__global__ void __launch_bounds__(256)
+    wgrad_planes_kernel(const TG* __restrict__ g, int64_t stride, __nv_bfloat16* __restrict__ out, int64_t T, int64_t O,
+                        int64_t width) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < T * width; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / width, o = i - t * width;
+    if constexpr (sizeof(TG) == 2) {
+      out[i] = o < O ? g[t * stride + o] : __float2bfloat16_rn(0.f);
+    } else {
+      float r = o < O ? g[t * stride + o] : 0.f;
+      const bool fine = (__float_as_uint(r) & 0x7f800000u) != 0x7f800000u;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        const uint32_t top = __float_as_uint(r) & 0xffff0000u;
+        const bool nan = !fine && p == 0 && r != r;
+        out[(int64_t)p * T * width + i] = __ushort_as_bfloat16(nan ? (uint16_t)0x7fc0 : (uint16_t)(top >> 16));
+        r = fine ? r - __uint_as_float(top) : 0.f;
+      }
+    }
+  }
+}
+
+struct WgPlan {
+  bool parts_only;
+  int tiles_o, tiles_k, full, splits, pairs, units;
+  int64_t width;
+  size_t part_bytes;
+};
+WgPlan wg_plan(int64_t T, int64_t O, int64_t K, bool w16) {
+  WgPlan p;
+  p.tiles_o = (int)((O + kTileO - 1) / kTileO);
+  p.tiles_k = (int)((K + kTileK - 1) / kTileK);
+  p.width = (O + 7) / 8 * 8;
+  const int tiles = p.tiles_o * p.tiles_k, most = num_sms() / 2;
+  const int64_t stages = (T + kTok - 1) / kTok;
+  p.parts_only = w16 && T > kMaxChain16;
+  // Whole rounds of tiles, one a pair; the tiles of the last, partial round are
+  // split along the tokens over all pairs, at least 4 stages a part.
+  const int rest = p.parts_only ? tiles : tiles % most;
+  p.full = tiles - rest;
+  p.splits = 1;
+  if (rest > 0) {
+    int64_t s = most / rest;
+    if (s > stages / 4) s = stages / 4;
+    p.splits = s < 1 ? 1 : (int)s;
+  }
+  if (p.splits == 1 && !p.parts_only) p.full = tiles;
+  p.units = p.full + (tiles - p.full) * p.splits;
+  p.pairs = p.units < most ? p.units : most;
+  p.part_bytes = (size_t)(tiles - p.full) * p.splits * kTileO * kTileK * sizeof(float);
+  return p;
+}
+
+template <int PLANES, typename TW>
+int launch_wgrad(const CUtensorMap& map, const WgArgs& a, const WgPlan& pl, cudaStream_t st) {
+  auto kern = wgrad_kernel<PLANES, TW>;
+  constexpr uint32_t smem = WgCfg<PLANES>::SMEM;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return fail(MHC_ERR_CUDA, "checkpoint8_weight_grad: cannot reserve %u bytes of shared memory", smem);
+  {
+    ProfScope p("checkpoint8_weight_grad", st);
+    kern<<<2 * pl.pairs, kThreads, smem, st>>>(map, a);
+    const int rc = check_launch("checkpoint8_weight_grad");
+    if (rc) return rc;
+  }
+  const int rest = pl.tiles_o * pl.tiles_k - pl.full;
+  if (rest == 0) return MHC_OK;
+  ProfScope p("checkpoint8_weight_join", st);
+  wgrad_join_kernel<TW><<<(unsigned)rest * (kTileO / 4), 256, 0, st>>>(a);
+  return check_launch("checkpoint8_weight_join");
 }
 
 }  // namespace
 
-int wgrad_device_error(int* value, bool) {
-  *value = 0;  // nothing waits here
-  return MHC_OK;
+int wgrad_device_error(int* value, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(value, g_mhc_device_error, sizeof(int));
+  const int zero = 0;
+  if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(g_mhc_device_error, &zero, sizeof(int));
+  return e == cudaSuccess ? MHC_OK : fail(MHC_ERR_CUDA, "mhc_device_error_word: %s", cudaGetErrorString(e));
 }
 
 }  // namespace mhc
 
 using namespace mhc;
 
-extern "C" size_t mhc_checkpoint8_weight_grad_workspace_bytes(int64_t, int64_t, int64_t, int32_t, int32_t) {
-  return 0;
+// Sized for rows that need a copy of g, whatever their layout turns out to be.
+extern "C" size_t mhc_checkpoint8_weight_grad_workspace_bytes(int64_t tokens, int64_t out_features,
+                                                              int64_t in_features, int32_t g_bf16, int32_t gw_bf16) {
+  if (tokens < 1 || out_features < 1 || in_features < 1) return 0;
+  const WgPlan p = wg_plan(tokens, out_features, in_features, gw_bf16 != 0);
+  const size_t planes = (size_t)tokens * p.width * 2 * (g_bf16 ? 1 : 3);
+  return (planes + 255) / 256 * 256 + p.part_bytes;
 }
 
 extern "C" int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16, int64_t row_stride,
                                            const int8_t* codes, const uint8_t* exponents, void* grad_weight,
                                            int32_t gw_bf16, int64_t tokens, int64_t out_features,
-                                           int64_t in_features, void*, size_t, void* stream) {
+                                           int64_t in_features, void* workspace, size_t workspace_bytes,
+                                           void* stream) {
   const char* what = "checkpoint8_weight_grad";
   MHC_REQUIRE(tokens >= 0 && out_features >= 1 && in_features >= 1, MHC_ERR_INVALID_ARG,
               "%s: tokens must be >= 0, out_features and in_features >= 1 (got %lld, %lld, %lld)", what,
@@ -94,9 +562,42 @@ extern "C" int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16,
               what);
   MHC_REQUIRE(aligned16(codes) && (reinterpret_cast<uintptr_t>(exponents) & 3) == 0, MHC_ERR_ALIGNMENT,
               "%s: codes must be 16-byte and exponents 4-byte aligned", what);
-#define MHC_WGRAD(TG, TW) \
-  launch_plain<TG, TW>(grad_out, row_stride, codes, exponents, grad_weight, tokens, out_features, in_features, st)
-  return g_bf16 ? (gw_bf16 ? MHC_WGRAD(__nv_bfloat16, __nv_bfloat16) : MHC_WGRAD(__nv_bfloat16, float))
-                : (gw_bf16 ? MHC_WGRAD(float, __nv_bfloat16) : MHC_WGRAD(float, float));
-#undef MHC_WGRAD
+  const WgPlan pl = wg_plan(tokens, out_features, in_features, gw_bf16 != 0);
+  const bool copy = !g_bf16 || !aligned16(grad_out) || (row_stride % 8) != 0 || row_stride >= (1ll << 38);
+  const size_t planes = ((size_t)tokens * pl.width * 2 * (g_bf16 ? 1 : 3) + 255) / 256 * 256;
+  const size_t need = (copy ? planes : 0) + pl.part_bytes;
+  MHC_REQUIRE(need == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= need),
+              MHC_ERR_WORKSPACE, "%s: workspace too small", what);
+  const void* src = grad_out;
+  int64_t stride = tokens == 1 ? pl.width : row_stride;
+  char* ws = (char*)workspace;
+  if (copy) {
+    ProfScope p("checkpoint8_weight_planes", st);
+    const int64_t blocks = (tokens * pl.width + 1023) / 1024, most = 16ll * num_sms();
+    const unsigned nb = (unsigned)(blocks < most ? blocks : most);
+    if (g_bf16)
+      wgrad_planes_kernel<<<nb, 256, 0, st>>>((const __nv_bfloat16*)grad_out, row_stride, (__nv_bfloat16*)ws, tokens,
+                                              out_features, pl.width);
+    else
+      wgrad_planes_kernel<<<nb, 256, 0, st>>>((const float*)grad_out, row_stride, (__nv_bfloat16*)ws, tokens,
+                                              out_features, pl.width);
+    const int rc = check_launch("checkpoint8_weight_planes");
+    if (rc) return rc;
+    src = ws;
+    stride = pl.width;
+    ws += planes;
+  }
+  CUtensorMap map;
+  const int np = g_bf16 ? 1 : 3;
+  if (!make_tmap_3d(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, src, copy ? pl.width : out_features, tokens, np, stride * 2,
+                    copy ? (uint64_t)tokens * pl.width * 2 : (uint64_t)stride * 2, 64, kTok, 1,
+                    CU_TENSOR_MAP_SWIZZLE_128B))
+    return fail(MHC_ERR_CUDA, "%s: cannot encode the tensor map", what);
+  WgArgs a;
+  a.codes = codes; a.exps = exponents; a.gw = grad_weight; a.part = (float*)ws;
+  a.T = tokens; a.O = out_features; a.K = in_features; a.pitch = ck_pitch(in_features);
+  a.tiles_o = pl.tiles_o; a.tiles_k = pl.tiles_k; a.full = pl.full; a.splits = pl.splits; a.units = pl.units;
+  if (g_bf16)
+    return gw_bf16 ? launch_wgrad<1, __nv_bfloat16>(map, a, pl, st) : launch_wgrad<1, float>(map, a, pl, st);
+  return gw_bf16 ? launch_wgrad<3, __nv_bfloat16>(map, a, pl, st) : launch_wgrad<3, float>(map, a, pl, st);
 }
