@@ -15,16 +15,17 @@
 // shared memory's 128 bytes a cycle.
 //
 // Warps of a CTA: 0 issues the TMA loads of g, 1 the MMAs (of the pair, in the
-// even CTA), 2 owns the tensor memory, 4..7 empty accumulators, 8..15 read
-// codes straight from global memory (L2), two stages ahead of their use, and
-// store xh in the 128-byte-swizzled layout that the MMA reads.  A stage is 64
-// tokens.  Two accumulators of 256 columns fill tensor memory, so a tile is
-// written while the next one is summed.
+// even CTA), 2 owns the tensor memory, 3 reports g's arrival to the even CTA,
+// 4..11 take finished accumulators, 12..19 expand: two groups of four warps, each
+// every other stage (a stage is 64 tokens), read codes straight from global
+// memory (L2) a turn ahead and store xh in the 128-byte-swizzled layout that the
+// MMA reads.  Two accumulators of 256 columns fill tensor memory, so one is
+// read while the next is summed.
 //
 // Accumulating MMAs truncate (a relative shrink of about 2e-8 each, measured on
-// the layer's projection), so a chain is kept to kChain stages: 4096 tokens
-// or 256 MMAs; what follows is added in fp32 in global memory by the thread that
-// wrote the sum before.  A bf16 gW needs no such cut (kMaxChain16).
+// the layer's projection), so a chain is kept to 64 MMAs; warps 4..11 add the
+// chains in fp32 registers, 128 a thread, which is why registers are moved
+// between the roles (setmaxnreg).
 #include "checkpoint8.cuh"
 #include "tma.cuh"
 
@@ -34,17 +35,21 @@ namespace {
 constexpr int kTok = 64;                       // tokens of a stage
 constexpr int kTileO = 256, kTileK = 256;      // tile of a pair
 constexpr uint32_t kOpBytes = kTok * 128 * 2;  // one operand of one CTA, one stage: 64 tokens x 128 bf16
-constexpr int kThreads = 512, kExpandWarps = 8;
-constexpr int kChain = 64;                     // stages summed in tensor memory before fp32 takes over
-constexpr int64_t kMaxChain16 = 1 << 18;       // tokens: 2^18 / 16 MMAs x 2e-8 is 3.3e-4, a twelfth of a bf16
-                                               // rounding; longer sums go through fp32 parts
+constexpr int kOutWarp = 4, kOutWarps = 8, kExpandWarp = 12, kExpandWarps = 8;
+constexpr int kThreads = 32 * (kExpandWarp + kExpandWarps);
+// registers a thread by role; launched with 96 each, and 128 x 32 + 256 x 160 +
+// 256 x 64 = 640 x 96
+constexpr int kRegsFew = 32, kRegsOut = 160, kRegsExpand = 64;
 
 template <int PLANES>
 struct WgCfg {
   static constexpr uint32_t STAGE = (PLANES + 1) * kOpBytes;  // A planes, then B
   static constexpr int STAGES = PLANES == 1 ? 6 : 3;
-  static constexpr uint32_t OFF_BAR = STAGES * STAGE;
+  static constexpr int CHAIN = PLANES == 1 ? 16 : 5;          // stages summed in tensor memory: 64 / 60 MMAs
+  static constexpr uint32_t OFF_OUT = STAGES * STAGE;         // 4 KB a warp that writes: 32 x 32 values on their way out
+  static constexpr uint32_t OFF_BAR = OFF_OUT + kOutWarps * 4096;
   static constexpr uint32_t SMEM = OFF_BAR + (3 * STAGES + 5) * 8 + 16 + 1024;  // + alignment of the ring
+  static_assert(SMEM <= 232448, "227 KB a block");
 };
 
 struct WgArgs {
@@ -91,11 +96,15 @@ __device__ __forceinline__ uint32_t cta_rank() {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// arrive on the barrier at this offset in the even CTA
+// Arrive on the barrier at this offset in the even CTA.  What is handed over is
+// this CTA's own shared memory (already fenced to the async proxy by its
+// writers) and tensor memory, so the release need not reach past the CTA: at
+// cluster scope it waits for the warp's code loads in flight, and the 4096^2
+// product of 8192 tokens took 648 us instead of 379.
 __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
   asm volatile(
       "{\n .reg .b32 ra;\n mapa.shared::cluster.u32 ra, %0, 0;\n"
-      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n}\n" ::"r"(smem_u32(bar))
+      " mbarrier.arrive.shared::cluster.b64 _, [ra];\n}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
 __device__ __forceinline__ bool poll_cluster(uint32_t addr, uint32_t parity) {
@@ -150,20 +159,21 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
 }
+template <int R>
+__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
 // Two codes -> two bf16 values.  With the low 7 bits set into the mantissa of
 // 128 (0x43nn) a byte reads 128 + low7; less 128, or 256 where its sign is set,
@@ -175,37 +185,26 @@ __device__ __forceinline__ uint32_t expand2(uint32_t low, uint32_t sign, uint32_
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// Columns [c, c + 32) of one output row: add what is there if `more`, store.
-__device__ __forceinline__ void put_row(float* p, float (&v)[32], int64_t left, bool vec, bool more) {
-  if (vec && left >= 32) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      if (more) {
-        const float4 b = *reinterpret_cast<const float4*>(p + j);
-        o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
-      }
-      *reinterpret_cast<float4*>(p + j) = o;
-    }
+// Four values of an output row, `left` of them inside it.
+__device__ __forceinline__ void put4(float* p, const float4& v, int64_t left) {
+  if (left >= 4 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    *reinterpret_cast<float4*>(p) = v;
   } else {
+    const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < left) p[j] = more ? p[j] + v[j] : v[j];
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = w[j];
   }
 }
-__device__ __forceinline__ void put_row(__nv_bfloat16* p, float (&v)[32], int64_t left, bool vec, bool) {
-  if (vec && left >= 32) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = v[j + i];
-      ck_save(p + j, w);
-    }
+__device__ __forceinline__ void put4(__nv_bfloat16* p, const float4& v, int64_t left) {
+  if (left >= 4 && (reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+    __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
   } else {
+    const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < left) ck_store(p + j, v[j]);
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = __float2bfloat16_rn(w[j]);
   }
 }
 
@@ -235,12 +234,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&afull[s], 1);
-      mbar_init(&full[s], 2 * kExpandWarps);
+      mbar_init(&full[s], kExpandWarps + 2);  // a group of four warps and the report of g, in each CTA
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&dfull[b], 1);
-      mbar_init(&dempty[b], 8);
+      mbar_init(&dempty[b], 2 * kOutWarps);
     }
     mbar_init(idle, 1);
     *stop = 0;
@@ -253,163 +252,209 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = *tslot;
 
-  if (warp == 0) {
-    if (lane == 0) {  // ---- g: two boxes of 64 columns x 64 tokens a plane ----
-      int it = 0;
-      for (int u = pair; u < a.units && !*stop; u += pairs) {
-        const Unit q = unit_of(a, u);
-        const int o = q.tile_o * kTileO + (int)rank * 128;
-        for (int st = q.s0; st < q.s1; ++st, ++it) {
-          const int s = it % S;
-          if (it >= S && !wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop)) goto loads_done;
-          unsigned char* dst = ring + s * Cfg::STAGE;
-          mbar_expect_tx(&afull[s], PLANES * kOpBytes);
-#pragma unroll
-          for (int p = 0; p < PLANES; ++p) {
-            tma_load_3d(dst + p * kOpBytes, &gmap, o, st * kTok, p, &afull[s]);
-            tma_load_3d(dst + p * kOpBytes + kOpBytes / 2, &gmap, o + 64, st * kTok, p, &afull[s]);
-          }
-        }
-      }
-    loads_done:
-      // nothing may land after the block is gone
-      for (int j = it > S ? it - S : 0; j < it; ++j) mbar_wait(&afull[j % S], (uint32_t)((j / S) & 1));
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {  // ---- MMAs of the pair ----
-      int it = 0, acc = 0;
-      for (int u = pair; u < a.units; u += pairs) {
-        const Unit q = unit_of(a, u);
-        const int cut = (sizeof(TW) == 4 || q.part >= 0) ? kChain : q.s1 - q.s0;
-        for (int st = q.s0; st < q.s1; ++acc) {
-          const int b = acc & 1, end = min(st + cut, q.s1);
-          if (acc >= 2 && !wait_bar(&dempty[b], (uint32_t)((acc / 2 - 1) & 1), stop)) goto mma_done;
-          fence_after();
-          const uint32_t d = tmem + 256u * b;
-          for (int first = st; st < end; ++st, ++it) {
+  if (warp < kOutWarp) {
+    fewer_regs<kRegsFew>();
+    if (warp == 0) {
+      if (lane == 0) {  // ---- g: two boxes of 64 columns x 64 tokens a plane ----
+        int it = 0;
+        for (int u = pair; u < a.units && !*stop; u += pairs) {
+          const Unit q = unit_of(a, u);
+          const int o = q.tile_o * kTileO + (int)rank * 128;
+          for (int st = q.s0; st < q.s1; ++st, ++it) {
             const int s = it % S;
-            if (!wait_bar(&full[s], (uint32_t)((it / S) & 1), stop)) goto mma_done;
-            fence_after();
-            const uint32_t base = smem_u32(ring + s * Cfg::STAGE);
+            if (it >= S && !wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop)) goto loads_done;
+            unsigned char* dst = ring + s * Cfg::STAGE;
+            mbar_expect_tx(&afull[s], PLANES * kOpBytes);
 #pragma unroll
-            for (int p = PLANES - 1; p >= 0; --p)  // smallest terms first
-#pragma unroll
-              for (int k = 0; k < kTok / 16; ++k)
-                mma_pair(d, mn_desc(base + p * kOpBytes + k * 2048), mn_desc(base + PLANES * kOpBytes + k * 2048),
-                         (st > first || p < PLANES - 1 || k > 0) ? 1u : 0u);
-            commit_pair(&empty[s]);
+            for (int p = 0; p < PLANES; ++p) {
+              tma_load_3d(dst + p * kOpBytes, &gmap, o, st * kTok, p, &afull[s]);
+              tma_load_3d(dst + p * kOpBytes + kOpBytes / 2, &gmap, o + 64, st * kTok, p, &afull[s]);
+            }
           }
-          commit_pair(&dfull[b]);
+        }
+      loads_done:
+        // nothing may land after the block is gone
+        for (int j = it > S ? it - S : 0; j < it; ++j) mbar_wait(&afull[j % S], (uint32_t)((j / S) & 1));
+      }
+    } else if (warp == 1) {
+      if (lane == 0 && rank == 0) {  // ---- MMAs of the pair ----
+        int it = 0, acc = 0;
+        for (int u = pair; u < a.units; u += pairs) {
+          const Unit q = unit_of(a, u);
+          for (int st = q.s0; st < q.s1; ++acc) {
+            const int b = acc & 1, end = min(st + Cfg::CHAIN, q.s1);
+            if (acc >= 2 && !wait_bar(&dempty[b], (uint32_t)((acc / 2 - 1) & 1), stop)) goto mma_done;
+            fence_after();
+            const uint32_t d = tmem + 256u * b;
+            for (int first = st; st < end; ++st, ++it) {
+              const int s = it % S;
+              if (!wait_bar(&full[s], (uint32_t)((it / S) & 1), stop)) goto mma_done;
+              fence_after();
+              const uint32_t base = smem_u32(ring + s * Cfg::STAGE);
+#pragma unroll
+              for (int p = PLANES - 1; p >= 0; --p)  // smallest terms first
+#pragma unroll
+                for (int k = 0; k < kTok / 16; ++k)
+                  mma_pair(d, mn_desc(base + p * kOpBytes + k * 2048), mn_desc(base + PLANES * kOpBytes + k * 2048),
+                           (st > first || p < PLANES - 1 || k > 0) ? 1u : 0u);
+              commit_pair(&empty[s]);
+            }
+            commit_pair(&dfull[b]);
+          }
+        }
+      mma_done:
+        commit_pair(idle);
+        mbar_wait(idle, 0u);
+      }
+    } else if (warp == 3) {
+      if (lane == 0) {  // ---- g has landed: tell the even CTA ----
+        int it = 0;
+        for (int u = pair; u < a.units && !*stop; u += pairs) {
+          const Unit q = unit_of(a, u);
+          for (int st = q.s0; st < q.s1; ++st, ++it) {
+            if (!wait_bar(&afull[it % S], (uint32_t)((it / S) & 1), stop)) break;
+            arrive_leader(&full[it % S]);
+          }
         }
       }
-    mma_done:
-      commit_pair(idle);
-      mbar_wait(idle, 0u);
     }
-  } else if (warp >= 8) {
-    // ---- expand: a thread takes one token's block of 32 codes a stage ----
-    const int e = tid - 256;                             // 0 .. 255
-    const int tok = (e & 7) | ((e >> 5) << 3);           // eight lanes: eight tokens, so that 16-byte stores meet no
-    const int blk = (e >> 3) & 3;                        // bank twice under the swizzle
+  } else if (warp >= kExpandWarp) {
+    // ---- expand: a thread takes one block of 32 codes of two tokens a turn ----
+    fewer_regs<kRegsExpand>();
+    const int group = (warp - kExpandWarp) >> 2, e = tid & 127;
+    const int tok = (e & 7) | ((e >> 5) << 3);  // eight lanes: eight tokens, so that 16-byte stores meet no bank twice
+    const int blk = (e >> 3) & 3;               // under the swizzle; the second token is 32 on
     const uint32_t row = (uint32_t)(PLANES * kOpBytes + (blk >> 1) * (kOpBytes / 2) + tok * 128);
-    uint4 c0[2], c1[2];
+    const int64_t turn = 2 * kTok * a.pitch, second = 32 * a.pitch;
+    uint4 c[2][2];
     uint32_t ex[2];
-    // the fetch runs two stages ahead of the store
+    // the stage that is fetched next: every other one of the pair's stages
     int fu = pair, fs = 0, fe = 0;
-    int64_t fk = 0;
-    auto ahead = [&](int slot) {  // fetch the next stage, if there is one
-      if (fs >= fe) {
-        if (fu >= a.units) return;
+    int64_t off = 0, t = 0;
+    auto enter = [&](int over) {  // the first unit with more than `over` stages left to skip
+      while (fu < a.units) {
         const Unit q = unit_of(a, fu);
-        fs = q.s0;
+        fs = q.s0 + over;
         fe = q.s1;
-        fk = (int64_t)q.tile_k * kTileK + rank * 128 + blk * 32;
+        if (fs < fe) {
+          const int64_t k = (int64_t)q.tile_k * kTileK + rank * 128 + blk * 32;
+          t = k < a.pitch ? (int64_t)fs * kTok + tok : a.T;  // no columns here: zeros
+          off = t * a.pitch + k;
+          return;
+        }
+        over = fs - fe;
+        fu += pairs;
       }
-      const int64_t t = (int64_t)fs * kTok + tok;
-      c0[slot] = c1[slot] = make_uint4(0u, 0u, 0u, 0u);
-      ex[slot] = 1u;
-      if (t < a.T && fk < a.pitch) {
-        const uint4* p = reinterpret_cast<const uint4*>(a.codes + t * a.pitch + fk);
-        c0[slot] = __ldg(p);
-        c1[slot] = __ldg(p + 1);
-        ex[slot] = __ldg(a.exps + (t * a.pitch + fk) / kCkBlock);
-      }
-      if (++fs >= fe) fu += pairs;
     };
-    auto put = [&](int it, int slot) -> bool {
-      const int s = it % S;
-      bool ok = it < S || wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop);
-      if (!__all_sync(0xffffffffu, ok)) return false;
-      const uint16_t sb = ex[slot] == 255u ? 0x7fc0 : (uint16_t)(ex[slot] << 7);
-      const __nv_bfloat162 step = __halves2bfloat162(__ushort_as_bfloat16(sb), __ushort_as_bfloat16(sb));
-      const uint32_t w[8] = {c0[slot].x, c0[slot].y, c0[slot].z, c0[slot].w,
-                             c1[slot].x, c1[slot].y, c1[slot].z, c1[slot].w};
-      unsigned char* dst = ring + s * Cfg::STAGE + row;
+    auto fetch = [&]() {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint4 o;
-        const uint32_t l0 = w[2 * j] & 0x7f7f7f7fu, s0 = w[2 * j] & 0x80808080u;
-        const uint32_t l1 = w[2 * j + 1] & 0x7f7f7f7fu, s1 = w[2 * j + 1] & 0x80808080u;
-        o.x = expand2(l0, s0, 0x4140, step);
-        o.y = expand2(l0, s0, 0x4342, step);
-        o.z = expand2(l1, s1, 0x4140, step);
-        o.w = expand2(l1, s1, 0x4342, step);
-        *reinterpret_cast<uint4*>(dst + ((((blk & 1) * 4 + j) ^ (tok & 7)) << 4)) = o;
+      for (int h = 0; h < 2; ++h) {
+        c[h][0] = c[h][1] = make_uint4(0u, 0u, 0u, 0u);
+        ex[h] = 1u;
+        if (fu < a.units && t + 32 * h < a.T) {
+          const uint4* p = reinterpret_cast<const uint4*>(a.codes + off + h * second);
+          c[h][0] = __ldg(p);
+          c[h][1] = __ldg(p + 1);
+          ex[h] = __ldg(a.exps + ((off + h * second) >> 5));
+        }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        ok = wait_bar(&afull[s], (uint32_t)((it / S) & 1), stop);
-        if (ok) arrive_leader(&full[s]);
+      fs += 2;
+      off += turn;
+      t += 2 * kTok;
+      if (fs >= fe && fu < a.units) {
+        const int over = fs - fe;
+        fu += pairs;
+        enter(over);
       }
-      return __all_sync(0xffffffffu, ok);
     };
     int total = 0;
     for (int u = pair; u < a.units; u += pairs) {
       const Unit q = unit_of(a, u);
       total += q.s1 - q.s0;
     }
-    ahead(0);
-    ahead(1);
-    for (int it = 0; it < total; it += 2) {
-      if (!put(it, 0)) break;
-      ahead(0);
-      if (it + 1 < total) {
-        if (!put(it + 1, 1)) break;
-        ahead(1);
+    enter(group);
+    fetch();
+    for (int it = group; it < total; it += 2) {
+      const int s = it % S;
+      const bool ok = it < S || wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      unsigned char* dst = ring + s * Cfg::STAGE + row;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint16_t sb = ex[h] == 255u ? 0x7fc0 : (uint16_t)(ex[h] << 7);
+        const __nv_bfloat162 step = __halves2bfloat162(__ushort_as_bfloat16(sb), __ushort_as_bfloat16(sb));
+        const uint32_t w[8] = {c[h][0].x, c[h][0].y, c[h][0].z, c[h][0].w, c[h][1].x, c[h][1].y, c[h][1].z, c[h][1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4 o;
+          const uint32_t l0 = w[2 * j] & 0x7f7f7f7fu, s0 = w[2 * j] & 0x80808080u;
+          const uint32_t l1 = w[2 * j + 1] & 0x7f7f7f7fu, s1 = w[2 * j + 1] & 0x80808080u;
+          o.x = expand2(l0, s0, 0x4140, step);
+          o.y = expand2(l0, s0, 0x4342, step);
+          o.z = expand2(l1, s1, 0x4140, step);
+          o.w = expand2(l1, s1, 0x4342, step);
+          *reinterpret_cast<uint4*>(dst + h * 4096 + ((((blk & 1) * 4 + j) ^ (tok & 7)) << 4)) = o;
+        }
       }
+      fetch();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_leader(&full[s]);
     }
-  } else if (warp >= 4) {
-    // ---- accumulators -> gW or a part ----
-    const int q4 = warp & 3, rr = (int)rank * 128 + 32 * q4 + lane;
+  } else {
+    // ---- accumulators -> fp32 sums -> gW or a part ----
+    more_regs<kRegsOut>();
+    const int w8 = warp - kOutWarp, q4 = w8 & 3, half = w8 >> 2;  // 32 rows, 128 columns a warp
+    unsigned char* mine = ring + Cfg::OFF_OUT + w8 * 4096;
+    const uint32_t src = tmem + ((uint32_t)(32 * q4) << 16) + 128u * half;
     int acc = 0;
     bool ok = true;
     for (int u = pair; u < a.units && ok; u += pairs) {
       const Unit q = unit_of(a, u);
-      const bool parts = q.part >= 0;
-      const int cut = (sizeof(TW) == 4 || parts) ? kChain : q.s1 - q.s0;
-      const int64_t o = (int64_t)q.tile_o * kTileO + rr, k0 = (int64_t)q.tile_k * kTileK;
-      for (int st = q.s0; st < q.s1; st += cut, ++acc) {
+      float sum[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) sum[j] = 0.f;
+      for (int st = q.s0; st < q.s1; st += Cfg::CHAIN, ++acc) {
         const int b = acc & 1;
         ok = wait_bar(&dfull[b], (uint32_t)((acc / 2) & 1), stop);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
-        const bool more = st > q.s0;
-#pragma unroll 1
-        for (int c = 0; c < kTileK; c += 32) {
-          float v[32];
-          tmem_ld32(tmem + 256u * b + ((uint32_t)(32 * q4) << 16) + (uint32_t)c, v);
-          if (parts) {
-            put_row(a.part + ((int64_t)q.part * kTileO + rr) * kTileK + c, v, 32, true, more);
-          } else if (o < a.O && k0 + c < a.K) {
-            TW* p = reinterpret_cast<TW*>(a.gw) + o * a.K + k0 + c;
-            put_row(p, v, a.K - k0 - c, (reinterpret_cast<uintptr_t>(p) & 15) == 0, more);
-          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v[16];
+          tmem_ld16(src + 256u * b + 16u * i, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[16 * i + j] += v[j];
         }
         fence_before();
         __syncwarp();
         if (lane == 0) arrive_leader(&dempty[b]);
+      }
+      if (!ok) break;
+      // 32 x 32 values at a time through shared memory (16-byte columns exchanged
+      // by row, no bank twice), so that eight lanes write 128 bytes of a row
+      const int r0 = (int)rank * 128 + 32 * q4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+              make_float4(sum[32 * i + 4 * j], sum[32 * i + 4 * j + 1], sum[32 * i + 4 * j + 2], sum[32 * i + 4 * j + 3]);
+        __syncwarp();
+        const int col = 128 * half + 32 * i + 4 * (lane & 7);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = 4 * j + (lane >> 3);
+          const float4 v = *reinterpret_cast<const float4*>(mine + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          if (q.part >= 0) {
+            *reinterpret_cast<float4*>(a.part + ((int64_t)q.part * kTileO + r0 + r) * kTileK + col) = v;
+          } else {
+            const int64_t o = (int64_t)q.tile_o * kTileO + r0 + r, k = (int64_t)q.tile_k * kTileK + col;
+            if (o < a.O) put4(reinterpret_cast<TW*>(a.gw) + o * a.K + k, v, a.K - k);
+          }
+        }
       }
     }
   }
@@ -466,22 +511,20 @@ __global__ void __launch_bounds__(256)
 }
 
 struct WgPlan {
-  bool parts_only;
   int tiles_o, tiles_k, full, splits, pairs, units;
   int64_t width;
   size_t part_bytes;
 };
-WgPlan wg_plan(int64_t T, int64_t O, int64_t K, bool w16) {
+WgPlan wg_plan(int64_t T, int64_t O, int64_t K) {
   WgPlan p;
   p.tiles_o = (int)((O + kTileO - 1) / kTileO);
   p.tiles_k = (int)((K + kTileK - 1) / kTileK);
   p.width = (O + 7) / 8 * 8;
   const int tiles = p.tiles_o * p.tiles_k, most = num_sms() / 2;
   const int64_t stages = (T + kTok - 1) / kTok;
-  p.parts_only = w16 && T > kMaxChain16;
   // Whole rounds of tiles, one a pair; the tiles of the last, partial round are
   // split along the tokens over all pairs, at least 4 stages a part.
-  const int rest = p.parts_only ? tiles : tiles % most;
+  const int rest = tiles % most;
   p.full = tiles - rest;
   p.splits = 1;
   if (rest > 0) {
@@ -489,7 +532,7 @@ WgPlan wg_plan(int64_t T, int64_t O, int64_t K, bool w16) {
     if (s > stages / 4) s = stages / 4;
     p.splits = s < 1 ? 1 : (int)s;
   }
-  if (p.splits == 1 && !p.parts_only) p.full = tiles;
+  if (p.splits == 1) p.full = tiles;
   p.units = p.full + (tiles - p.full) * p.splits;
   p.pairs = p.units < most ? p.units : most;
   p.part_bytes = (size_t)(tiles - p.full) * p.splits * kTileO * kTileK * sizeof(float);
@@ -530,9 +573,9 @@ using namespace mhc;
 
 // Sized for rows that need a copy of g, whatever their layout turns out to be.
 extern "C" size_t mhc_checkpoint8_weight_grad_workspace_bytes(int64_t tokens, int64_t out_features,
-                                                              int64_t in_features, int32_t g_bf16, int32_t gw_bf16) {
+                                                              int64_t in_features, int32_t g_bf16, int32_t) {
   if (tokens < 1 || out_features < 1 || in_features < 1) return 0;
-  const WgPlan p = wg_plan(tokens, out_features, in_features, gw_bf16 != 0);
+  const WgPlan p = wg_plan(tokens, out_features, in_features);
   const size_t planes = (size_t)tokens * p.width * 2 * (g_bf16 ? 1 : 3);
   return (planes + 255) / 256 * 256 + p.part_bytes;
 }
@@ -562,7 +605,7 @@ extern "C" int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16,
               what);
   MHC_REQUIRE(aligned16(codes) && (reinterpret_cast<uintptr_t>(exponents) & 3) == 0, MHC_ERR_ALIGNMENT,
               "%s: codes must be 16-byte and exponents 4-byte aligned", what);
-  const WgPlan pl = wg_plan(tokens, out_features, in_features, gw_bf16 != 0);
+  const WgPlan pl = wg_plan(tokens, out_features, in_features);
   const bool copy = !g_bf16 || !aligned16(grad_out) || (row_stride % 8) != 0 || row_stride >= (1ll << 38);
   const size_t planes = ((size_t)tokens * pl.width * 2 * (g_bf16 ? 1 : 3) + 255) / 256 * 256;
   const size_t need = (copy ? planes : 0) + pl.part_bytes;
