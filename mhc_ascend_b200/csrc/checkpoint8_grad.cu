@@ -15,12 +15,12 @@
 // shared memory's 128 bytes a cycle.
 //
 // Warps of a CTA: 0 issues the TMA loads of g, 1 the MMAs (of the pair, in the
-// even CTA), 2 owns the tensor memory, 3 reports g's arrival to the even CTA,
-// 4..11 take finished accumulators, 12..19 expand: two groups of four warps, each
-// every other stage (a stage is 64 tokens), read codes straight from global
-// memory (L2) a turn ahead and store xh in the 128-byte-swizzled layout that the
-// MMA reads.  Two accumulators of 256 columns fill tensor memory, so one is
-// read while the next is summed.
+// even CTA), 2 owns the tensor memory and issues the TMA loads of the codes, 3
+// reports g's arrival to the even CTA, 4..11 take finished accumulators, 12..19
+// expand: two groups of four warps, each every other stage (a stage is 64
+// tokens), turn codes into xh in the 128-byte-swizzled layout that the MMA reads.
+// Two accumulators of 256 columns fill tensor memory, so one is read while the
+// next is summed.
 //
 // Accumulating MMAs truncate (a relative shrink of about 2e-8 each, measured on
 // the layer's projection), so a chain is kept to 64 MMAs; warps 4..11 add the
@@ -44,16 +44,17 @@ constexpr int kRegsFew = 32, kRegsOut = 160, kRegsExpand = 64;
 template <int PLANES>
 struct WgCfg {
   static constexpr uint32_t STAGE = (PLANES + 1) * kOpBytes;  // A planes, then B
-  static constexpr int STAGES = PLANES == 1 ? 6 : 3;
+  static constexpr int STAGES = PLANES == 1 ? 5 : 2;
+  static constexpr int CODES = PLANES == 1 ? 4 : 8;           // stages of codes: 64 tokens x 128 bytes each
   static constexpr int CHAIN = PLANES == 1 ? 16 : 5;          // stages summed in tensor memory: 64 / 60 MMAs
-  static constexpr uint32_t OFF_OUT = STAGES * STAGE;         // 4 KB a warp that writes: 32 x 32 values on their way out
+  static constexpr uint32_t OFF_CODES = STAGES * STAGE;
+  static constexpr uint32_t OFF_OUT = OFF_CODES + CODES * kOpBytes / 2;  // 4 KB a warp that writes: 32 x 32 values on their way out
   static constexpr uint32_t OFF_BAR = OFF_OUT + kOutWarps * 4096;
-  static constexpr uint32_t SMEM = OFF_BAR + (3 * STAGES + 5) * 8 + 16 + 1024;  // + alignment of the ring
+  static constexpr uint32_t SMEM = OFF_BAR + (3 * STAGES + 2 * CODES + 5) * 8 + 16 + 1024;  // + alignment of the ring
   static_assert(SMEM <= 232448, "227 KB a block");
 };
 
 struct WgArgs {
-  const int8_t* codes;
   const uint8_t* exps;
   void* gw;
   float* part;           // parts of split tiles: [unit][256][256]
@@ -210,15 +211,17 @@ __device__ __forceinline__ void put4(__nv_bfloat16* p, const float4& v, int64_t 
 
 template <int PLANES, typename TW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    wgrad_kernel(const __grid_constant__ CUtensorMap gmap, const WgArgs a) {
+    wgrad_kernel(const __grid_constant__ CUtensorMap gmap, const __grid_constant__ CUtensorMap cmap, const WgArgs a) {
   using Cfg = WgCfg<PLANES>;
-  constexpr int S = Cfg::STAGES;
+  constexpr int S = Cfg::STAGES, SC = Cfg::CODES;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);  // the same offset in both CTAs
   uint64_t* afull = reinterpret_cast<uint64_t*>(ring + Cfg::OFF_BAR);  // [S] this CTA's part of g has landed
   uint64_t* full = afull + S;                                          // [S] (even CTA) both operands of both CTAs
   uint64_t* empty = full + S;                                          // [S] the stage's MMAs are done
-  uint64_t* dfull = empty + S;                                         // [2] an accumulator is whole
+  uint64_t* cfull = empty + S;                                         // [SC] codes have landed
+  uint64_t* cempty = cfull + SC;                                       // [SC] they have been read
+  uint64_t* dfull = cempty + SC;                                       // [2] an accumulator is whole
   uint64_t* dempty = dfull + 2;                                        // [2] (even CTA) it has been read in both CTAs
   uint64_t* idle = dempty + 2;                                         // every MMA issued is done
   uint32_t* tslot = reinterpret_cast<uint32_t*>(idle + 1);
@@ -237,6 +240,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&full[s], kExpandWarps + 2);  // a group of four warps and the report of g, in each CTA
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < SC; ++s) {
+      mbar_init(&cfull[s], 1);
+      mbar_init(&cempty[s], 4);
+    }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&dfull[b], 1);
       mbar_init(&dempty[b], 2 * kOutWarps);
@@ -245,6 +252,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     *stop = 0;
     fence_mbar_init();
     prefetch_tmap(&gmap);
+    prefetch_tmap(&cmap);
   }
   fence_before();
   __syncthreads();
@@ -306,6 +314,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         commit_pair(idle);
         mbar_wait(idle, 0u);
       }
+    } else if (warp == 2) {
+      if (lane == 0) {  // ---- codes; columns past the rows' end and tokens past T read as zeros ----
+        int it = 0;
+        for (int u = pair; u < a.units && !*stop; u += pairs) {
+          const Unit q = unit_of(a, u);
+          for (int st = q.s0; st < q.s1; ++st, ++it) {
+            const int s = it % SC;
+            if (it >= SC && !wait_bar(&cempty[s], (uint32_t)((it / SC - 1) & 1), stop)) goto codes_done;
+            mbar_expect_tx(&cfull[s], kOpBytes / 2);
+            tma_load_2d(ring + Cfg::OFF_CODES + s * (kOpBytes / 2), &cmap, q.tile_k * kTileK + (int)rank * 128, st * kTok,
+                        &cfull[s]);
+          }
+        }
+      codes_done:
+        for (int j = it > SC ? it - SC : 0; j < it; ++j) mbar_wait(&cfull[j % SC], (uint32_t)((j / SC) & 1));
+      }
     } else if (warp == 3) {
       if (lane == 0) {  // ---- g has landed: tell the even CTA ----
         int it = 0;
@@ -325,10 +349,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int tok = (e & 7) | ((e >> 5) << 3);  // eight lanes: eight tokens, so that 16-byte stores meet no bank twice
     const int blk = (e >> 3) & 3;               // under the swizzle; the second token is 32 on
     const uint32_t row = (uint32_t)(PLANES * kOpBytes + (blk >> 1) * (kOpBytes / 2) + tok * 128);
-    const int64_t turn = 2 * kTok * a.pitch, second = 32 * a.pitch;
-    uint4 c[2][2];
-    uint32_t ex[2];
-    // the stage that is fetched next: every other one of the pair's stages
+    const uint32_t from = (uint32_t)(Cfg::OFF_CODES + tok * 128);
+    const int64_t wide = a.pitch / kCkBlock, turn = 2 * kTok * wide;
+    // The exponents come from global memory, fetched two turns before their use:
+    // the walk is over every other one of the pair's stages.
     int fu = pair, fs = 0, fe = 0;
     int64_t off = 0, t = 0;
     auto enter = [&](int over) {  // the first unit with more than `over` stages left to skip
@@ -338,25 +362,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         fe = q.s1;
         if (fs < fe) {
           const int64_t k = (int64_t)q.tile_k * kTileK + rank * 128 + blk * 32;
-          t = k < a.pitch ? (int64_t)fs * kTok + tok : a.T;  // no columns here: zeros
-          off = t * a.pitch + k;
+          t = k < a.pitch ? (int64_t)fs * kTok + tok : a.T;  // no columns here: the codes are zeros
+          off = t * wide + k / kCkBlock;
           return;
         }
         over = fs - fe;
         fu += pairs;
       }
     };
-    auto fetch = [&]() {
+    auto fetch = [&](uint32_t (&ex)[2]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        c[h][0] = c[h][1] = make_uint4(0u, 0u, 0u, 0u);
         ex[h] = 1u;
-        if (fu < a.units && t + 32 * h < a.T) {
-          const uint4* p = reinterpret_cast<const uint4*>(a.codes + off + h * second);
-          c[h][0] = __ldg(p);
-          c[h][1] = __ldg(p + 1);
-          ex[h] = __ldg(a.exps + ((off + h * second) >> 5));
-        }
+        if (fu < a.units && t + 32 * h < a.T) ex[h] = __ldg(a.exps + off + h * 32 * wide);
       }
       fs += 2;
       off += turn;
@@ -372,12 +390,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Unit q = unit_of(a, u);
       total += q.s1 - q.s0;
     }
+    uint32_t e0[2], e1[2];
     enter(group);
-    fetch();
-    for (int it = group; it < total; it += 2) {
-      const int s = it % S;
-      const bool ok = it < S || wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop);
-      if (!__all_sync(0xffffffffu, ok)) break;
+    fetch(e0);
+    fetch(e1);
+    auto expand = [&](int it, uint32_t (&ex)[2]) -> bool {
+      const int s = it % S, sc = it % SC;
+      bool ok = wait_bar(&cfull[sc], (uint32_t)((it / SC) & 1), stop);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      uint4 c[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          c[h][j] = *reinterpret_cast<const uint4*>(ring + from + sc * (kOpBytes / 2) + h * 4096 + (((2 * blk + j) ^ (tok & 7)) << 4));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&cempty[sc]);
+      ok = it < S || wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop);
+      if (!__all_sync(0xffffffffu, ok)) return false;
       unsigned char* dst = ring + s * Cfg::STAGE + row;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -396,10 +426,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(dst + h * 4096 + ((((blk & 1) * 4 + j) ^ (tok & 7)) << 4)) = o;
         }
       }
-      fetch();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) arrive_leader(&full[s]);
+      fetch(ex);
+      return true;
+    };
+    for (int it = group; it < total; it += 4) {
+      if (!expand(it, e0)) break;
+      if (it + 2 < total && !expand(it + 2, e1)) break;
     }
   } else {
     // ---- accumulators -> fp32 sums -> gW or a part ----
@@ -459,6 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   }
   // the other CTA may still arrive here, or read this one's operands
+  __syncwarp();
   __syncthreads();
   cluster_barrier();
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -540,14 +576,14 @@ WgPlan wg_plan(int64_t T, int64_t O, int64_t K) {
 }
 
 template <int PLANES, typename TW>
-int launch_wgrad(const CUtensorMap& map, const WgArgs& a, const WgPlan& pl, cudaStream_t st) {
+int launch_wgrad(const CUtensorMap& map, const CUtensorMap& codes, const WgArgs& a, const WgPlan& pl, cudaStream_t st) {
   auto kern = wgrad_kernel<PLANES, TW>;
   constexpr uint32_t smem = WgCfg<PLANES>::SMEM;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return fail(MHC_ERR_CUDA, "checkpoint8_weight_grad: cannot reserve %u bytes of shared memory", smem);
   {
     ProfScope p("checkpoint8_weight_grad", st);
-    kern<<<2 * pl.pairs, kThreads, smem, st>>>(map, a);
+    kern<<<2 * pl.pairs, kThreads, smem, st>>>(map, codes, a);
     const int rc = check_launch("checkpoint8_weight_grad");
     if (rc) return rc;
   }
@@ -636,11 +672,15 @@ extern "C" int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16,
                     copy ? (uint64_t)tokens * pl.width * 2 : (uint64_t)stride * 2, 64, kTok, 1,
                     CU_TENSOR_MAP_SWIZZLE_128B))
     return fail(MHC_ERR_CUDA, "%s: cannot encode the tensor map", what);
+  CUtensorMap cmap;
+  if (!make_tmap_2d(&cmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, tokens, ck_pitch(in_features), ck_pitch(in_features),
+                    kTok, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+    return fail(MHC_ERR_CUDA, "%s: cannot encode the tensor map", what);
   WgArgs a;
-  a.codes = codes; a.exps = exponents; a.gw = grad_weight; a.part = (float*)ws;
+  a.exps = exponents; a.gw = grad_weight; a.part = (float*)ws;
   a.T = tokens; a.O = out_features; a.K = in_features; a.pitch = ck_pitch(in_features);
   a.tiles_o = pl.tiles_o; a.tiles_k = pl.tiles_k; a.full = pl.full; a.splits = pl.splits; a.units = pl.units;
   if (g_bf16)
-    return gw_bf16 ? launch_wgrad<1, __nv_bfloat16>(map, a, pl, st) : launch_wgrad<1, float>(map, a, pl, st);
-  return gw_bf16 ? launch_wgrad<3, __nv_bfloat16>(map, a, pl, st) : launch_wgrad<3, float>(map, a, pl, st);
+    return gw_bf16 ? launch_wgrad<1, __nv_bfloat16>(map, cmap, a, pl, st) : launch_wgrad<1, float>(map, cmap, a, pl, st);
+  return gw_bf16 ? launch_wgrad<3, __nv_bfloat16>(map, cmap, a, pl, st) : launch_wgrad<3, float>(map, cmap, a, pl, st);
 }
