@@ -17,12 +17,12 @@ The reference has no counterpart (it saves bf16 copies, ops.py:394-470).
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence
 
 import torch
 
-from . import _C
-from .ops import _DevGuard, _f32, _lib, _require_cuda, _stream, _workspace
+from .ops import _f32, _launch, _lib, _require_cuda, _workspace
 
 BLOCK, PITCH = 32, 128
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -44,7 +44,7 @@ class Checkpoint8:
         dtype: type it had (what ``unpack`` returns by default)
     """
 
-    __slots__ = ("codes", "exponents", "shape", "dtype")
+    __slots__ = ("codes", "exponents", "shape", "dtype", "rows", "cols")
 
     def __init__(self, codes: torch.Tensor, exponents: torch.Tensor, shape: Sequence[int], dtype: torch.dtype):
         self.shape = torch.Size(shape)
@@ -53,25 +53,15 @@ class Checkpoint8:
         if dtype not in _FLOATS:
             raise RuntimeError(f"Checkpoint8: dtype must be float32 or bfloat16 (got {dtype})")
         _require_cuda("Checkpoint8", codes, exponents)
-        pitch = _pitch(self.shape[-1])
-        rows = self.rows
+        self.cols = self.shape[-1]
+        self.rows = rows = math.prod(self.shape[:-1])
+        pitch = _pitch(self.cols)
         if codes.dtype != torch.int8 or codes.shape != (rows, pitch) or not codes.is_contiguous():
             raise RuntimeError(f"Checkpoint8: codes must be a contiguous int8 [{rows}, {pitch}] tensor")
         if exponents.dtype != torch.uint8 or exponents.shape != (rows, pitch // BLOCK) \
                 or not exponents.is_contiguous():
             raise RuntimeError(f"Checkpoint8: exponents must be a contiguous uint8 [{rows}, {pitch // BLOCK}] tensor")
         self.codes, self.exponents, self.dtype = codes, exponents, dtype
-
-    @property
-    def cols(self) -> int:
-        return self.shape[-1]
-
-    @property
-    def rows(self) -> int:
-        r = 1
-        for d in self.shape[:-1]:
-            r *= d
-        return r
 
     def unpack(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return checkpoint8_unpack(self, dtype)
@@ -82,8 +72,9 @@ class Checkpoint8:
 
 def _empty(shape, dtype, device):
     c = object.__new__(Checkpoint8)
-    c.shape, c.dtype = torch.Size(shape), dtype
-    rows, pitch = c.rows, _pitch(shape[-1])
+    c.shape, c.dtype, c.cols = shape, dtype, shape[-1]
+    c.rows = rows = math.prod(shape[:-1])
+    pitch = _pitch(c.cols)
     c.codes = torch.empty(rows, pitch, dtype=torch.int8, device=device)
     c.exponents = torch.empty(rows, pitch // BLOCK, dtype=torch.uint8, device=device)
     return c
@@ -112,10 +103,8 @@ def checkpoint8_pack(x: torch.Tensor) -> Checkpoint8:
         raise RuntimeError(f"{what}: x must have a last dimension of at least 1")
     x2, stride = _rows2d(x.detach())
     kept = _empty(x.shape, x.dtype, x.device)
-    with _DevGuard(x):
-        rc = _lib.mhc_checkpoint8_pack(x2.data_ptr(), x.dtype == torch.bfloat16, stride, kept.codes.data_ptr(),
-                                       kept.exponents.data_ptr(), x2.size(0), x2.size(1), _stream(x.device))
-    _C.check(rc, what)
+    _launch("mhc_checkpoint8_pack", x.device, x2.data_ptr(), x.dtype == torch.bfloat16, stride,
+            kept.codes.data_ptr(), kept.exponents.data_ptr(), x2.size(0), x2.size(1))
     return kept
 
 
@@ -127,10 +116,8 @@ def checkpoint8_unpack(kept: Checkpoint8, dtype: Optional[torch.dtype] = None) -
         raise RuntimeError(f"{what}: dtype must be float32 or bfloat16 (got {dtype})")
     dev = kept.codes.device
     out = torch.empty(kept.shape, dtype=dtype, device=dev)
-    with _DevGuard(out):
-        rc = _lib.mhc_checkpoint8_unpack(kept.codes.data_ptr(), kept.exponents.data_ptr(), out.data_ptr(),
-                                         dtype == torch.bfloat16, kept.rows, kept.cols, _stream(dev))
-    _C.check(rc, what)
+    _launch("mhc_checkpoint8_unpack", dev, kept.codes.data_ptr(), kept.exponents.data_ptr(), out.data_ptr(),
+            dtype == torch.bfloat16, kept.rows, kept.cols)
     return out
 
 
@@ -152,11 +139,9 @@ def rmsnorm_checkpoint8_fwd(inp: torch.Tensor, weight: torch.Tensor, eps: float 
     out = torch.empty_like(x)
     rows = kept.rows
     rms = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with _DevGuard(x):
-        rc = _lib.mhc_rmsnorm_checkpoint8_fwd(x.data_ptr(), x.dtype == torch.bfloat16, w.data_ptr(), out.data_ptr(),
-                                              rms.data_ptr(), kept.codes.data_ptr(), kept.exponents.data_ptr(),
-                                              rows, kept.cols, float(eps), _stream(x.device))
-    _C.check(rc, what)
+    _launch("mhc_rmsnorm_checkpoint8_fwd", x.device, x.data_ptr(), x.dtype == torch.bfloat16, w.data_ptr(),
+            out.data_ptr(), rms.data_ptr(), kept.codes.data_ptr(), kept.exponents.data_ptr(), rows, kept.cols,
+            float(eps))
     return out, rms, kept
 
 
@@ -174,12 +159,9 @@ def rmsnorm_checkpoint8_bwd(grad_out: torch.Tensor, kept: Checkpoint8, weight: t
     gx = torch.empty_like(g)
     gw = torch.empty(cols, dtype=torch.float32, device=g.device)
     ws = _workspace(_lib.mhc_rmsnorm_checkpoint8_bwd_workspace_bytes(rows, cols), g.device)
-    with _DevGuard(g):
-        rc = _lib.mhc_rmsnorm_checkpoint8_bwd(g.data_ptr(), g.dtype == torch.bfloat16, kept.codes.data_ptr(),
-                                              kept.exponents.data_ptr(), w.data_ptr(), r.data_ptr(), gx.data_ptr(),
-                                              gw.data_ptr(), rows, cols, ws.data_ptr(), ws.numel(),
-                                              _stream(g.device))
-    _C.check(rc, what)
+    _launch("mhc_rmsnorm_checkpoint8_bwd", g.device, g.data_ptr(), g.dtype == torch.bfloat16, kept.codes.data_ptr(),
+            kept.exponents.data_ptr(), w.data_ptr(), r.data_ptr(), gx.data_ptr(), gw.data_ptr(), rows, cols,
+            ws.data_ptr(), ws.numel())
     return gx, gw
 
 
@@ -229,11 +211,8 @@ def checkpoint8_weight_grad(grad_out: torch.Tensor, kept: Checkpoint8,
     gw = torch.empty(O, K, dtype=dtype, device=g.device)
     g16, w16 = g.dtype == torch.bfloat16, dtype == torch.bfloat16
     ws = _workspace(_lib.mhc_checkpoint8_weight_grad_workspace_bytes(T, O, K, g16, w16), g.device)
-    with _DevGuard(g):
-        rc = _lib.mhc_checkpoint8_weight_grad(g.data_ptr(), g16, stride, kept.codes.data_ptr(),
-                                              kept.exponents.data_ptr(), gw.data_ptr(), w16, T, O, K, ws.data_ptr(),
-                                              ws.numel(), _stream(g.device))
-    _C.check(rc, what)
+    _launch("mhc_checkpoint8_weight_grad", g.device, g.data_ptr(), g16, stride, kept.codes.data_ptr(),
+            kept.exponents.data_ptr(), gw.data_ptr(), w16, T, O, K, ws.data_ptr(), ws.numel())
     return gw
 
 

@@ -307,7 +307,7 @@ RowPlan row_plan(int64_t cols, bool vec) {
 
 template <typename T>
 bool vec_ok(const void* p, int64_t cols, int64_t stride) {
-  return aligned16(p) && cols % 8 == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
+  return (reinterpret_cast<uintptr_t>(p) & (8 * sizeof(T) - 1)) == 0 && cols % 8 == 0 && stride % 8 == 0;
 }
 
 template <typename T>
@@ -341,7 +341,7 @@ int launch_unpack(const int8_t* codes, const uint8_t* exps, T* out, int64_t rows
 template <typename T>
 int launch_norm_fwd(const T* x, const float* w, T* out, float* rms, int8_t* codes, uint8_t* exps, int64_t rows,
                     int64_t cols, float eps, cudaStream_t st) {
-  const bool vec = vec_ok<T>(x, cols, cols) && aligned16(out) && aligned16(w);
+  const bool vec = vec_ok<T>(x, cols, cols) && vec_ok<T>(out, cols, cols) && vec_ok<float>(w, cols, cols);
   const RowPlan pl = row_plan(cols, vec);
   const int64_t pitch = ck_pitch(cols);
   ProfScope p("rmsnorm_checkpoint8_fwd", st);
@@ -369,7 +369,7 @@ int norm_bwd_blocks(int64_t rows, int64_t cols) {
 template <typename T>
 int launch_norm_bwd(const T* g, const int8_t* codes, const uint8_t* exps, const float* w, const float* rms, T* gx,
                     float* gw, int64_t rows, int64_t cols, float* part, cudaStream_t st) {
-  const bool vec = vec_ok<T>(g, cols, cols) && aligned16(gx) && aligned16(w);
+  const bool vec = vec_ok<T>(g, cols, cols) && vec_ok<T>(gx, cols, cols) && vec_ok<float>(w, cols, cols);
   const RowPlan pl = row_plan(cols, vec);
   const int64_t pitch = ck_pitch(cols);
   const int blocks = norm_bwd_blocks(rows, cols);

@@ -75,12 +75,12 @@ __device__ __forceinline__ float ck_f32(__nv_bfloat16 v) { return __bfloat162flo
 __device__ __forceinline__ void ck_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void ck_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// V consecutive values as floats: V = 8 with 16-byte accesses (the address is
-// 16-byte aligned), V = 1 plain
+// V consecutive values as floats: V = 8 in one access of 32 (fp32) or 16 (bf16)
+// bytes, aligned to its size, V = 1 plain
 __device__ __forceinline__ void ck_load(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p));
 }
 __device__ __forceinline__ void ck_load(const __nv_bfloat16* p, float (&v)[8]) {
   const uint4 a = *reinterpret_cast<const uint4*>(p);
@@ -95,8 +95,9 @@ template <typename T>
 __device__ __forceinline__ void ck_load(const T* p, float (&v)[1]) { v[0] = ck_f32(*p); }
 
 __device__ __forceinline__ void ck_save(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void ck_save(__nv_bfloat16* p, const float (&v)[8]) {
   uint4 r;

@@ -16,8 +16,7 @@ from typing import Optional, Sequence, Union
 import torch
 import torch.nn as nn
 
-from . import _C
-from .ops import _DevGuard, _lib, _require_cuda, _stream, _workspace
+from .ops import _launch, _lib, _require_cuda, _workspace
 
 _FLOATS = (torch.float32, torch.bfloat16)
 MAX_STREAMS = 32
@@ -62,12 +61,8 @@ def stream_embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, num_streams: i
     idc = _check_ids(what, ids)
     V, C = weight.shape
     out = torch.empty(*ids.shape, n, C, dtype=dtype, device=weight.device)
-    with _DevGuard(weight):
-        rc = _lib.mhc_stream_embedding_fwd(idc.data_ptr(), ids.dtype == torch.int64, weight.data_ptr(),
-                                           weight.dtype == torch.bfloat16, out.data_ptr(),
-                                           dtype == torch.bfloat16, sc, idc.numel(), n, C, V,
-                                           _stream(weight.device))
-    _C.check(rc, what)
+    _launch("mhc_stream_embedding_fwd", weight.device, idc.data_ptr(), ids.dtype == torch.int64, weight.data_ptr(),
+            weight.dtype == torch.bfloat16, out.data_ptr(), dtype == torch.bfloat16, sc, idc.numel(), n, C, V)
     return out
 
 
@@ -92,11 +87,9 @@ def stream_embedding_bwd(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddin
     gw = torch.empty(V, C, dtype=dtype, device=g.device)
     T = idc.numel()
     ws = _workspace(_lib.mhc_stream_embedding_bwd_workspace_bytes(T, C), g.device)
-    with _DevGuard(g):
-        rc = _lib.mhc_stream_embedding_bwd(g.data_ptr(), g.dtype == torch.bfloat16, idc.data_ptr(),
-                                           ids.dtype == torch.int64, gw.data_ptr(), dtype == torch.bfloat16,
-                                           sc, T, n, C, V, pad, ws.data_ptr(), ws.numel(), _stream(g.device))
-    _C.check(rc, what)
+    _launch("mhc_stream_embedding_bwd", g.device, g.data_ptr(), g.dtype == torch.bfloat16, idc.data_ptr(),
+            ids.dtype == torch.int64, gw.data_ptr(), dtype == torch.bfloat16, sc, T, n, C, V, pad, ws.data_ptr(),
+            ws.numel())
     return gw
 
 

@@ -81,6 +81,25 @@ class _DevGuard:
         self.g.__exit__(*a)
 
 
+_bound = {}  # entry points by name
+
+
+def _launch(name, device, *args):
+    """Call the entry point `name` with `args` and the current stream of
+    `device`, with that device current; raise on an error status."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound[name] = getattr(_C.load(), name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _C.check(rc, name)
+
+
 # =============================================================================
 # Sinkhorn-Knopp
 # =============================================================================
