@@ -5,11 +5,18 @@
 namespace mhc {
 namespace {
 
-// Row and unit (of V columns) of a flat unit index, stepped without divisions.
-struct UnitWalk {
-  int64_t row;
-  int64_t u;
-  __device__ __forceinline__ UnitWalk(int64_t i, int64_t U) : row(i / U), u(i % U) {}
+// ---------------------------------------------------------------------------
+// pack / unpack: one pass, bound by HBM.  A warp takes spans of 256 columns of a
+// row, a lane 8 of them (32 or 16 bytes in, 8 bytes of codes out), kUnroll spans
+// at once so that enough loads are in flight.  EVEN: rows that 16- or 32-byte
+// accesses fit; the spans then run over the rows without a gap.
+// ---------------------------------------------------------------------------
+constexpr int kPackThreads = 256, kUnroll = 4;
+
+// Row and column of a lane's unit in a list of units, U (EVEN) or 32 * spans a row
+struct Walk {
+  int64_t row, u;
+  __device__ __forceinline__ Walk(int64_t i, int64_t U) : row(i / U), u(i % U) {}
   __device__ __forceinline__ void step(int64_t drow, int64_t du, int64_t U) {
     row += drow;
     u += du;
@@ -17,118 +24,154 @@ struct UnitWalk {
   }
 };
 
-// ---------------------------------------------------------------------------
-// pack / unpack: one pass, bound by HBM.  A thread takes units of 8 columns
-// (32 or 16 bytes in, 8 bytes of codes out), kUnroll of them so that enough
-// loads are in flight.  Rows whose start or width breaks 16-byte accesses take
-// one column per lane instead (a block is then a warp).
-// ---------------------------------------------------------------------------
-constexpr int kPackThreads = 256, kUnroll = 4;
-
-template <typename T, int V>
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(kPackThreads)
     pack_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict__ codes,
-                uint8_t* __restrict__ exps, int64_t rows, int64_t cols, int64_t U) {
-  const int64_t pitch = U * V, total = rows * U;
+                uint8_t* __restrict__ exps, int64_t rows, int64_t cols, int64_t pitch, int64_t U) {
+  __shared__ __align__(16) float sm[EVEN ? 1 : kPackThreads * 8];
+  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
   const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
   const int64_t drow = kPackThreads / U, du = kPackThreads % U;
-  UnitWalk at(first, U);
-  float v[kUnroll][V];
+  Walk at(first, U);
+  float v[kUnroll][8];
   int64_t row[kUnroll], col[kUnroll];
 #pragma unroll
   for (int k = 0; k < kUnroll; ++k) {
     row[k] = at.row;
-    col[k] = at.u * V;
+    col[k] = at.u * 8;
+    if (EVEN) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[k][j] = 0.f;
-    if (at.row < rows && col[k] < cols) {  // V = 8: cols % 8 == 0, so a unit lies in the row or past it
-      ck_load(x + at.row * stride + col[k], v[k]);
+      for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+      if (at.row < rows && col[k] < cols) ck_load(x + at.row * stride + col[k], v[k]);  // cols % 8 == 0
+    } else {  // U % 32 == 0: the warp is in one row
+      ck_load_any(x + at.row * stride, col[k] - 8 * (threadIdx.x & 31), at.row < rows ? cols : 0, mine, v[k]);
     }
-    at.step(drow, du, U);
-  }
-#pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
-    const bool on = first + (int64_t)k * kPackThreads < total;
-    ck_encode<V>(v[k], codes + row[k] * pitch, exps + row[k] * (pitch / kCkBlock), col[k], on);
-  }
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kPackThreads)
-    unpack_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
-                  T* __restrict__ out, int64_t rows, int64_t cols, int64_t U, int64_t pitch) {
-  const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
-  const int64_t drow = kPackThreads / U, du = kPackThreads % U;
-  UnitWalk at(first, U);
-  float v[kUnroll][V];
-  int64_t row[kUnroll], col[kUnroll];
-#pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
-    row[k] = at.row;
-    col[k] = at.u * V;
-    if (at.row < rows && col[k] < cols)
-      ck_decode<V>(codes + at.row * pitch, exps + at.row * (pitch / kCkBlock), col[k], v[k]);
     at.step(drow, du, U);
   }
 #pragma unroll
   for (int k = 0; k < kUnroll; ++k)
-    if (row[k] < rows && col[k] < cols) ck_save(out + row[k] * cols + col[k], v[k]);
+    ck_encode(v[k], codes + row[k] * pitch, exps + row[k] * (pitch / kCkBlock), col[k], row[k] < rows && col[k] < pitch);
+}
+
+template <typename T, bool EVEN>
+__global__ void __launch_bounds__(kPackThreads)
+    unpack_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
+                  T* __restrict__ out, int64_t rows, int64_t cols, int64_t pitch, int64_t U) {
+  __shared__ __align__(16) float sm[EVEN ? 1 : kPackThreads * 8];
+  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
+  const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
+  const int64_t drow = kPackThreads / U, du = kPackThreads % U;
+  Walk at(first, U);
+  uint2 w[kUnroll];
+  uint32_t E[kUnroll];
+  int64_t row[kUnroll], col[kUnroll];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) {
+    row[k] = at.row;
+    col[k] = at.u * 8;
+    w[k] = make_uint2(0u, 0u);
+    E[k] = 1u;
+    if (at.row < rows && col[k] < cols) {
+      w[k] = *reinterpret_cast<const uint2*>(codes + at.row * pitch + col[k]);
+      E[k] = exps[(at.row * pitch + col[k]) / kCkBlock];
+    }
+    at.step(drow, du, U);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) {
+    float v[8];
+    ck_decode(w[k], E[k], v);
+    if (EVEN) {
+      if (row[k] < rows && col[k] < cols) ck_save(out + row[k] * cols + col[k], v);
+    } else {
+      ck_save_any(out + row[k] * cols, col[k] - 8 * (threadIdx.x & 31), row[k] < rows ? cols : 0, mine, v);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
 // RMSNorm.  r = sqrt(mean x^2 + eps), y = x / r * w, and the codes of x, in one
-// pass over x: a row stays in its block's registers between the sum and the
-// output (UPT units of V columns a thread).
+// pass over x: a row stays in registers between the sum and the output, UPT
+// units of 8 columns a thread.  WARP: rows of at most 1024 columns belong to a
+// warp, 8 to a block, and need no barrier; longer ones to a block.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float block_total(float v, float* red) {
+constexpr int kWarpCols = 1024, kWarpRows = 8;
+
+// Sum over the row's threads, the same in each.
+template <bool WARP>
+__device__ __forceinline__ float row_total(float v, float* red) {
   v = warp_sum(v);
+  if (WARP) return v;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   if (lane == 0) red[warp] = v;
   __syncthreads();
-  float s = 0.f;
-  for (int w = 0; w < nw; ++w) s += red[w];
-  return s;
+  return warp_sum(lane < nw ? red[lane] : 0.f);
+}
+// Column of a thread's unit k, of the first unit of its warp
+template <bool WARP>
+__device__ __forceinline__ int64_t unit_col(int k) {
+  return 8 * (WARP ? (int64_t)(k * 32 + (threadIdx.x & 31)) : (int64_t)k * blockDim.x + threadIdx.x);
 }
 
-// Most threads of a block by the share of a row that one thread holds: more
-// than 512 only where the largest share needs them.
-constexpr int row_threads(int V, int UPT) { return UPT == (V == 8 ? 4 : 16) ? 1024 : 512; }
+// Eight weights; columns past the end read as zero
+__device__ __forceinline__ void load_w(const float* w, int64_t c, int64_t cols, float (&v)[8]) {
+  if (c + 8 <= cols && (reinterpret_cast<uintptr_t>(w) & 31) == 0) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(w + c)), b = __ldg(reinterpret_cast<const float4*>(w + c + 4));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? __ldg(w + c + j) : 0.f;
+  }
+}
 
-template <typename T, int V, int UPT>
-__global__ void __launch_bounds__(row_threads(V, UPT))
+// Most threads of a block by the share of a row that one thread holds
+constexpr int row_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : UPT == 4 ? 1024 : 512; }
+
+template <typename T, int UPT, bool WARP, bool EVEN>
+__global__ void __launch_bounds__(row_threads(UPT, WARP))
     norm_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, T* __restrict__ out,
                     float* __restrict__ rms, int8_t* __restrict__ codes, uint8_t* __restrict__ exps,
-                    int64_t cols, int64_t pitch, float eps) {
+                    int64_t rows, int64_t cols, int64_t pitch, float eps) {
   __shared__ float red[32];
-  const int64_t row = blockIdx.x;
+  __shared__ __align__(16) float sm[EVEN ? 1 : row_threads(UPT, WARP) * 8];
+  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
+  const int lane = threadIdx.x & 31;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (WARP && row >= rows) return;
   const T* xr = x + row * cols;
-  float v[UPT][V];
+  float v[UPT][8];
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < UPT; ++k) {
-    const int64_t c = ((int64_t)k * blockDim.x + threadIdx.x) * V;
+    const int64_t c = unit_col<WARP>(k);
+    if (EVEN) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[k][j] = 0.f;
-    if (c < cols) ck_load(xr + c, v[k]);
+      for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+      if (c < cols) ck_load(xr + c, v[k]);
+    } else {
+      ck_load_any(xr, c - 8 * lane, cols, mine, v[k]);
+    }
   }
 #pragma unroll
   for (int k = 0; k < UPT; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) ss = fmaf(v[k][j], v[k][j], ss);
-  const float r = sqrtf(block_total(ss, red) / (float)cols + eps);
-  const float ir = 1.0f / r;
-  if (threadIdx.x == 0) rms[row] = r;
+    for (int j = 0; j < 8; ++j) ss = fmaf(v[k][j], v[k][j], ss);
+  const float r = sqrtf(row_total<WARP>(ss, red) / (float)cols + eps), ir = 1.0f / r;
+  if (WARP ? lane == 0 : threadIdx.x == 0) rms[row] = r;
 #pragma unroll
   for (int k = 0; k < UPT; ++k) {
-    const int64_t c = ((int64_t)k * blockDim.x + threadIdx.x) * V;
-    if (c < cols) {
-      float o[V], wv[V];
-      ck_load(w + c, wv);
+    const int64_t c = unit_col<WARP>(k);
+    float o[8], wv[8];
+    load_w(w, c, cols, wv);
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = v[k][j] * ir * wv[j];
-      ck_save(out + row * cols + c, o);
+    for (int j = 0; j < 8; ++j) o[j] = v[k][j] * ir * wv[j];
+    if (EVEN) {
+      if (c < cols) ck_save(out + row * cols + c, o);
+    } else {
+      ck_save_any(out + row * cols, c - 8 * lane, cols, mine, o);
     }
-    ck_encode<V>(v[k], codes + row * pitch, exps + row * (pitch / kCkBlock), c, c < pitch);
+    ck_encode(v[k], codes + row * pitch, exps + row * (pitch / kCkBlock), c, c < pitch);
   }
 }
 
@@ -139,6 +182,8 @@ __global__ void __launch_bounds__(1024)
                          float* __restrict__ rms, int8_t* __restrict__ codes, uint8_t* __restrict__ exps,
                          int64_t cols, int64_t pitch, float eps) {
   __shared__ float red[32];
+  __shared__ __align__(16) float sm[1024 * 8];
+  float* mine = sm + (threadIdx.x >> 5) * 256;
   const int64_t row = blockIdx.x;
   const T* xr = x + row * cols;
   float ss = 0.f;
@@ -146,98 +191,169 @@ __global__ void __launch_bounds__(1024)
     const float t = ck_f32(xr[c]);
     ss = fmaf(t, t, ss);
   }
-  const float r = sqrtf(block_total(ss, red) / (float)cols + eps);
-  const float ir = 1.0f / r;
+  const float r = sqrtf(row_total<false>(ss, red) / (float)cols + eps), ir = 1.0f / r;
   if (threadIdx.x == 0) rms[row] = r;
-  for (int64_t c = threadIdx.x; c - threadIdx.x < pitch; c += blockDim.x) {
-    float v[1] = {c < cols ? ck_f32(xr[c]) : 0.f};
-    if (c < cols) ck_store(out + row * cols + c, v[0] * ir * w[c]);
-    ck_encode<1>(v, codes + row * pitch, exps + row * (pitch / kCkBlock), c, c < pitch);
+  for (int64_t c0 = (threadIdx.x >> 5) * 256; c0 < pitch; c0 += 8 * blockDim.x) {
+    const int64_t c = c0 + 8 * (threadIdx.x & 31);
+    float v[8], o[8], wv[8];
+    ck_load_any(xr, c0, cols, mine, v);
+    load_w(w, c, cols, wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = v[j] * ir * wv[j];
+    ck_save_any(out + row * cols, c0, cols, mine, o);
+    ck_encode(v, codes + row * pitch, exps + row * (pitch / kCkBlock), c, c < pitch);
   }
 }
 
 // Backward at the restored input xh:
 //   gx = (g w - xh * D / (cols r^2)) / r,  D = sum_c g w xh
 //   gw = sum over rows of g xh / r
-// A block walks rows blockIdx.x, + gridDim.x, ...; its threads keep their
+// A block (or warp) walks every (its count)-th row; its threads keep their
 // columns' share of gw in registers over all of them, so g and the codes are
 // read once and gw leaves as one row of partial sums a block, added in block
-// order by norm_gw_kernel: no atomics, the same bits every time.
-template <typename T, int V, int UPT>
-__global__ void __launch_bounds__(row_threads(V, UPT))
+// order by norm_gw_kernel: no atomics, the same bits every time.  The next
+// row's g and codes are loaded before this row's sum is waited for.
+template <typename T, int UPT, bool WARP, bool EVEN>
+__global__ void __launch_bounds__(row_threads(UPT, WARP))
     norm_bwd_kernel(const T* __restrict__ g, const int8_t* __restrict__ codes,
                     const uint8_t* __restrict__ exps, const float* __restrict__ w,
                     const float* __restrict__ rms, T* __restrict__ gx, float* __restrict__ part,
                     int64_t rows, int64_t cols, int64_t pitch) {
   __shared__ float red[2][32];
-  float acc[UPT][V];
+  __shared__ __align__(16) float sm[EVEN && !WARP ? 1 : row_threads(UPT, WARP) * 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* mine = sm + (EVEN ? 0 : warp * 256);
+  float acc[UPT][8];
 #pragma unroll
   for (int k = 0; k < UPT; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[k][j] = 0.f;
-  int buf = 0;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, buf ^= 1) {
-    float gv[UPT][V], xv[UPT][V];
-    float d = 0.f;
+    for (int j = 0; j < 8; ++j) acc[k][j] = 0.f;
+  float ng[UPT][8];  // the row ahead
+  uint2 nc[UPT];
+  uint32_t ne[UPT];
+  float nr = 1.f;
+  auto fetch = [&](int64_t row) {
+    if (row < rows) {
+      nr = rms[row];
 #pragma unroll
-    for (int k = 0; k < UPT; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + threadIdx.x) * V;
+      for (int k = 0; k < UPT; ++k) {
+        const int64_t c = unit_col<WARP>(k);
+        nc[k] = make_uint2(0u, 0u);
+        ne[k] = 1u;
+        if (c < pitch) {
+          nc[k] = *reinterpret_cast<const uint2*>(codes + row * pitch + c);
+          ne[k] = exps[(row * pitch + c) / kCkBlock];
+        }
+        if (EVEN) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) gv[k][j] = xv[k][j] = 0.f;
-      if (c < cols) {
-        ck_load(g + row * cols + c, gv[k]);
-        ck_decode<V>(codes + row * pitch, exps + row * (pitch / kCkBlock), c, xv[k]);
-      }
-    }
-    const float r = rms[row], ir = 1.0f / r;
-#pragma unroll
-    for (int k = 0; k < UPT; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + threadIdx.x) * V;
-      float wv[V];
-      if (c < cols) {
-        ck_load(w + c, wv);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          acc[k][j] = fmaf(gv[k][j] * ir, xv[k][j], acc[k][j]);
-          gv[k][j] *= wv[j];
-          d = fmaf(gv[k][j], xv[k][j], d);
+          for (int j = 0; j < 8; ++j) ng[k][j] = 0.f;
+          if (c < cols) ck_load(g + row * cols + c, ng[k]);
+        } else {
+          ck_load_any(g + row * cols, c - 8 * lane, cols, mine, ng[k]);
         }
       }
     }
-    // two buffers: a block writes red[buf] again only after the barrier of the row between
-    const float coef = block_total(d, red[buf]) / ((float)cols * r * r);
+  };
+  const int64_t first = WARP ? (int64_t)blockIdx.x * kWarpRows + warp : (int64_t)blockIdx.x;
+  const int64_t hop = WARP ? (int64_t)gridDim.x * kWarpRows : (int64_t)gridDim.x;
+  fetch(first);
+  int buf = 0;
+  for (int64_t row = first; row < rows; row += hop, buf ^= 1) {
+    float gv[UPT][8], xv[UPT][8];
+    const float r = nr, ir = 1.0f / r;
+    float d = 0.f;
 #pragma unroll
     for (int k = 0; k < UPT; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + threadIdx.x) * V;
-      if (c < cols) {
-        float o[V];
+      float wv[8];
+      load_w(w, unit_col<WARP>(k), cols, wv);
+      ck_decode(nc[k], ne[k], xv[k]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = (gv[k][j] - xv[k][j] * coef) * ir;
-        ck_save(gx + row * cols + c, o);
+      for (int j = 0; j < 8; ++j) {
+        acc[k][j] = fmaf(ng[k][j] * ir, xv[k][j], acc[k][j]);
+        gv[k][j] = ng[k][j] * wv[j];
+        d = fmaf(gv[k][j], xv[k][j], d);
+      }
+    }
+    fetch(row + hop);
+    // two buffers: a block writes red[buf] again only after the barrier of the row between
+    const float coef = row_total<WARP>(d, red[buf]) / ((float)cols * r * r);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      const int64_t c = unit_col<WARP>(k);
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = (gv[k][j] - xv[k][j] * coef) * ir;
+      if (EVEN) {
+        if (c < cols) ck_save(gx + row * cols + c, o);
+      } else {
+        ck_save_any(gx + row * cols, c - 8 * lane, cols, mine, o);
       }
     }
   }
+  if (WARP) {  // the warps' shares, added in warp order
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) {
-    const int64_t c = ((int64_t)k * blockDim.x + threadIdx.x) * V;
-    if (c < cols) {
-      float* p = part + (int64_t)blockIdx.x * cols + c;
+    for (int k = 0; k < UPT; ++k) {
+      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < V; ++j) p[j] = acc[k][j];
+      for (int j = 0; j < 8; ++j) sm[warp * 256 + j * 32 + lane] = acc[k][j];
+      __syncthreads();
+      float s = 0.f;
+      for (int q = 0; q < kWarpRows; ++q) s += sm[q * 256 + threadIdx.x];
+      const int64_t c = (k * 32 + lane) * 8 + (threadIdx.x >> 5);  // word j * 32 + lane holds column 8 lane + j
+      if (c < cols) part[(int64_t)blockIdx.x * cols + c] = s;
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < UPT; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t c = unit_col<WARP>(k) + j;
+        if (c < cols) part[(int64_t)blockIdx.x * cols + c] = acc[k][j];
+      }
   }
 }
 
-// Long rows: two passes a row, gw added up in the block's own row of partials.
-template <typename T>
-__global__ void __launch_bounds__(1024)
+// Rows too long for that: g and the codes are read twice (the second time from
+// L2), and the block's share of gw is kept in shared memory (KEEP) or, past
+// kKeepCols columns, in its row of partial sums.
+constexpr int kLongThreads = 512;
+constexpr int64_t kKeepCols = 49152;  // 192 KB
+
+template <typename T, bool EVEN, bool KEEP>
+__global__ void __launch_bounds__(kLongThreads)
     norm_bwd_long_kernel(const T* __restrict__ g, const int8_t* __restrict__ codes,
                          const uint8_t* __restrict__ exps, const float* __restrict__ w,
                          const float* __restrict__ rms, T* __restrict__ gx, float* __restrict__ part,
                          int64_t rows, int64_t cols, int64_t pitch) {
+  extern __shared__ __align__(16) float keep[];  // [8][units]: value j of unit u at j * units + u
   __shared__ float red[2][32];
-  float* p = part + (int64_t)blockIdx.x * cols;
-  for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) p[c] = 0.f;
+  __shared__ __align__(16) float sm[EVEN ? 1 : kLongThreads * 8];
+  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
+  const int lane = threadIdx.x & 31;
+  const int64_t units = pitch / 8;
+  float* p = KEEP ? keep : part + (int64_t)blockIdx.x * cols;
+  auto slot = [&](int64_t c, int j) -> int64_t { return KEEP ? j * units + c / 8 : c + j; };
+  // each unit is always the same thread's
+  for (int64_t c = 8 * threadIdx.x; c < cols; c += 8 * kLongThreads)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) p[slot(c, j)] = 0.f;
+  auto unit = [&](const T* gr, const int8_t* cr, const uint8_t* er, int64_t c, float (&gv)[8], float (&xv)[8]) {
+    uint2 q = make_uint2(0u, 0u);
+    uint32_t E = 1u;
+    if (c < pitch) {
+      q = *reinterpret_cast<const uint2*>(cr + c);
+      E = er[c / kCkBlock];
+    }
+    ck_decode(q, E, xv);
+    if (EVEN) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gv[j] = 0.f;
+      if (c < cols) ck_load(gr + c, gv);
+    } else {
+      ck_load_any(gr, c - 8 * lane, cols, mine, gv);
+    }
+  };
   int buf = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, buf ^= 1) {
     const int8_t* cr = codes + row * pitch;
@@ -245,20 +361,37 @@ __global__ void __launch_bounds__(1024)
     const T* gr = g + row * cols;
     const float r = rms[row], ir = 1.0f / r;
     float d = 0.f;
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
-      float xv[1];
-      ck_decode<1>(cr, er, c, xv);
-      const float gv = ck_f32(gr[c]);
-      p[c] = fmaf(gv * ir, xv[0], p[c]);
-      d = fmaf(gv * w[c], xv[0], d);
+    for (int64_t c0 = 8 * (threadIdx.x & ~31); c0 < cols; c0 += 8 * kLongThreads) {
+      const int64_t c = c0 + 8 * lane;
+      float gv[8], xv[8], wv[8];
+      unit(gr, cr, er, c, gv, xv);
+      load_w(w, c, cols, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (c + j < cols) p[slot(c, j)] = fmaf(gv[j] * ir, xv[j], p[slot(c, j)]);
+        d = fmaf(gv[j] * wv[j], xv[j], d);
+      }
     }
-    const float coef = block_total(d, red[buf]) / ((float)cols * r * r);
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
-      float xv[1];
-      ck_decode<1>(cr, er, c, xv);
-      ck_store(gx + row * cols + c, (ck_f32(gr[c]) * w[c] - xv[0] * coef) * ir);
+    const float coef = row_total<false>(d, red[buf]) / ((float)cols * r * r);
+    for (int64_t c0 = 8 * (threadIdx.x & ~31); c0 < cols; c0 += 8 * kLongThreads) {
+      const int64_t c = c0 + 8 * lane;
+      float gv[8], xv[8], wv[8];
+      unit(gr, cr, er, c, gv, xv);
+      load_w(w, c, cols, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gv[j] = (gv[j] * wv[j] - xv[j] * coef) * ir;
+      if (EVEN) {
+        if (c < cols) ck_save(gx + row * cols + c, gv);
+      } else {
+        ck_save_any(gx + row * cols, c0, cols, mine, gv);
+      }
     }
   }
+  if (KEEP)
+    for (int64_t c = 8 * threadIdx.x; c < cols; c += 8 * kLongThreads)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < cols) part[(int64_t)blockIdx.x * cols + c + j] = p[slot(c, j)];
 }
 
 // gw[c] = sum of part[0..blocks)[c]: 32 columns a block, 8 threads a column,
@@ -282,110 +415,129 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// How a row of `cols` columns is laid over a block: V columns a unit, UPT units
-// a thread, `threads` threads; UPT = 0: the row does not fit the registers.
+// How a row is laid over threads: UPT units a thread, `threads` a block; warp:
+// one row a warp; UPT = 0: the row does not fit the registers.
 struct RowPlan {
-  int V, UPT, threads;
+  int UPT, threads;
+  bool warp;
 };
-RowPlan row_plan(int64_t cols, bool vec) {
-  const int64_t U = vec ? ck_pitch(cols) / 8 : ck_pitch(cols);
-  const int cand[3] = {1, 2, 4};
-  const int wide[4] = {1, 4, 8, 16};
-  if (vec) {
-    for (int upt : cand) {
-      const int64_t th = (((U + upt - 1) / upt) + 31) / 32 * 32;
-      if (th <= row_threads(8, upt)) return {8, upt, (int)th};
-    }
-  } else {
-    for (int upt : wide) {
-      const int64_t th = (((U + upt - 1) / upt) + 31) / 32 * 32;
-      if (th <= row_threads(1, upt)) return {1, upt, (int)th};
-    }
+RowPlan row_plan(int64_t cols) {
+  const int64_t pitch = ck_pitch(cols), U = pitch / 8;
+  if (pitch <= kWarpCols) return {pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows, true};
+  for (int upt : {1, 2, 4}) {
+    const int64_t th = (((U + upt - 1) / upt) + 31) / 32 * 32;
+    // two units a thread from 2048 columns on: fewer warps meet at the barrier
+    if (th <= row_threads(upt, false)) return {upt, (int)th, false};
   }
-  return {1, 0, 1024};
+  return {0, 1024, false};
 }
 
 template <typename T>
-bool vec_ok(const void* p, int64_t cols, int64_t stride) {
+bool even_rows(const void* p, int64_t cols, int64_t stride) {
   return (reinterpret_cast<uintptr_t>(p) & (8 * sizeof(T) - 1)) == 0 && cols % 8 == 0 && stride % 8 == 0;
+}
+
+// Units of a row in pack's and unpack's list, and the list's blocks
+int64_t list_units(int64_t cols, bool even, bool padded) {
+  const int64_t u = ((padded ? ck_pitch(cols) : cols) + 7) / 8;
+  return even ? u : (u + 31) / 32 * 32;
+}
+int64_t list_blocks(int64_t rows, int64_t U) {
+  return (rows * U + kPackThreads * kUnroll - 1) / (kPackThreads * kUnroll);
 }
 
 template <typename T>
 int launch_pack(const T* x, int64_t stride, int8_t* codes, uint8_t* exps, int64_t rows, int64_t cols,
                 cudaStream_t st) {
-  const bool vec = vec_ok<T>(x, cols, stride);
-  const int64_t U = ck_pitch(cols) / (vec ? 8 : 1);
-  const int64_t blocks = (rows * U + kPackThreads * kUnroll - 1) / (kPackThreads * kUnroll);
+  const bool even = even_rows<T>(x, cols, stride);
+  const int64_t U = list_units(cols, even, true), blocks = list_blocks(rows, U), pitch = ck_pitch(cols);
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "checkpoint8_pack: %lld x %lld values are too many",
               (long long)rows, (long long)cols);
   ProfScope p("checkpoint8_pack", st);
-  if (vec) pack_kernel<T, 8><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, U);
-  else pack_kernel<T, 1><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, U);
+  if (even) pack_kernel<T, true><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, pitch, U);
+  else pack_kernel<T, false><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, pitch, U);
   return check_launch("checkpoint8_pack");
 }
 
 template <typename T>
 int launch_unpack(const int8_t* codes, const uint8_t* exps, T* out, int64_t rows, int64_t cols, cudaStream_t st) {
-  const bool vec = vec_ok<T>(out, cols, cols);
-  const int64_t U = (cols + (vec ? 7 : 0)) / (vec ? 8 : 1);
-  const int64_t blocks = (rows * U + kPackThreads * kUnroll - 1) / (kPackThreads * kUnroll);
+  const bool even = even_rows<T>(out, cols, cols);
+  const int64_t U = list_units(cols, even, false), blocks = list_blocks(rows, U), pitch = ck_pitch(cols);
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "checkpoint8_unpack: %lld x %lld values are too many",
               (long long)rows, (long long)cols);
   ProfScope p("checkpoint8_unpack", st);
-  const int64_t pitch = ck_pitch(cols);
-  if (vec) unpack_kernel<T, 8><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, U, pitch);
-  else unpack_kernel<T, 1><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, U, pitch);
+  if (even) unpack_kernel<T, true><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, pitch, U);
+  else unpack_kernel<T, false><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, pitch, U);
   return check_launch("checkpoint8_unpack");
 }
+
+// LAUNCH(kernel) with the variant of KERNEL that the plan asks for
+#define MHC_ROW_VARIANTS(KERNEL, LAUNCH)                                                                 \
+  if (pl.warp) {                                                           \
+    if (pl.UPT == 1) { if (even) LAUNCH((KERNEL<T, 1, true, true>)); else LAUNCH((KERNEL<T, 1, true, false>)); } \
+    else if (pl.UPT == 2) { if (even) LAUNCH((KERNEL<T, 2, true, true>)); else LAUNCH((KERNEL<T, 2, true, false>)); } \
+    else { if (even) LAUNCH((KERNEL<T, 4, true, true>)); else LAUNCH((KERNEL<T, 4, true, false>)); }       \
+  } else if (pl.UPT == 1) { if (even) LAUNCH((KERNEL<T, 1, false, true>)); else LAUNCH((KERNEL<T, 1, false, false>)); } \
+  else { if (even) LAUNCH((KERNEL<T, 2, false, true>)); else LAUNCH((KERNEL<T, 2, false, false>)); }
 
 template <typename T>
 int launch_norm_fwd(const T* x, const float* w, T* out, float* rms, int8_t* codes, uint8_t* exps, int64_t rows,
                     int64_t cols, float eps, cudaStream_t st) {
-  const bool vec = vec_ok<T>(x, cols, cols) && vec_ok<T>(out, cols, cols) && vec_ok<float>(w, cols, cols);
-  const RowPlan pl = row_plan(cols, vec);
+  const bool even = even_rows<T>(x, cols, cols) && even_rows<T>(out, cols, cols);
+  const RowPlan pl = row_plan(cols);
   const int64_t pitch = ck_pitch(cols);
+  const unsigned blocks = (unsigned)(pl.warp ? (rows + kWarpRows - 1) / kWarpRows : rows);
   ProfScope p("rmsnorm_checkpoint8_fwd", st);
-#define MHC_NORM_FWD(VV, UU) \
-  norm_fwd_kernel<T, VV, UU><<<(unsigned)rows, pl.threads, 0, st>>>(x, w, out, rms, codes, exps, cols, pitch, eps)
-  if (pl.UPT == 0)
-    norm_fwd_long_kernel<T><<<(unsigned)rows, pl.threads, 0, st>>>(x, w, out, rms, codes, exps, cols, pitch, eps);
-  else if (pl.V == 8 && pl.UPT == 1) MHC_NORM_FWD(8, 1);
-  else if (pl.V == 8 && pl.UPT == 2) MHC_NORM_FWD(8, 2);
-  else if (pl.V == 8) MHC_NORM_FWD(8, 4);
-  else if (pl.UPT == 1) MHC_NORM_FWD(1, 1);
-  else if (pl.UPT == 4) MHC_NORM_FWD(1, 4);
-  else if (pl.UPT == 8) MHC_NORM_FWD(1, 8);
-  else MHC_NORM_FWD(1, 16);
+#define MHC_NORM_FWD(KERN) KERN<<<blocks, pl.threads, 0, st>>>(x, w, out, rms, codes, exps, rows, cols, pitch, eps)
+  if (pl.UPT == 0) {
+    norm_fwd_long_kernel<T><<<blocks, pl.threads, 0, st>>>(x, w, out, rms, codes, exps, cols, pitch, eps);
+  } else if (!pl.warp && pl.UPT == 4) {
+    if (even) MHC_NORM_FWD((norm_fwd_kernel<T, 4, false, true>));
+    else MHC_NORM_FWD((norm_fwd_kernel<T, 4, false, false>));
+  } else {
+    MHC_ROW_VARIANTS(norm_fwd_kernel, MHC_NORM_FWD)
+  }
 #undef MHC_NORM_FWD
   return check_launch("rmsnorm_checkpoint8_fwd");
 }
 
+// Rows whose backward does not fit the registers
+bool long_bwd(const RowPlan& pl) { return !pl.warp && (pl.UPT == 0 || pl.UPT == 4); }
+
+// Blocks of the backward: as many as run at once (the gradient of the weight
+// leaves as one row a block), no more than there are rows for.
 int norm_bwd_blocks(int64_t rows, int64_t cols) {
-  // two blocks an SM at most; fewer rows than that: one block a row
-  const int64_t most = 2 * (int64_t)num_sms();
-  return (int)(rows < most ? (rows > 0 ? rows : 1) : most);
+  const RowPlan pl = row_plan(cols);
+  const int64_t need = pl.warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
+  const int64_t most = (int64_t)num_sms() * (long_bwd(pl) || pl.threads <= 256 ? 2 : 1);
+  return (int)(need < most ? (need > 0 ? need : 1) : most);
 }
 
 template <typename T>
 int launch_norm_bwd(const T* g, const int8_t* codes, const uint8_t* exps, const float* w, const float* rms, T* gx,
                     float* gw, int64_t rows, int64_t cols, float* part, cudaStream_t st) {
-  const bool vec = vec_ok<T>(g, cols, cols) && vec_ok<T>(gx, cols, cols) && vec_ok<float>(w, cols, cols);
-  const RowPlan pl = row_plan(cols, vec);
+  const bool even = even_rows<T>(g, cols, cols) && even_rows<T>(gx, cols, cols);
+  const RowPlan pl = row_plan(cols);
   const int64_t pitch = ck_pitch(cols);
   const int blocks = norm_bwd_blocks(rows, cols);
   {
     ProfScope p("rmsnorm_checkpoint8_bwd", st);
-#define MHC_NORM_BWD(VV, UU) \
-  norm_bwd_kernel<T, VV, UU><<<blocks, pl.threads, 0, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch)
-    if (pl.UPT == 0)
-      norm_bwd_long_kernel<T><<<blocks, pl.threads, 0, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch);
-    else if (pl.V == 8 && pl.UPT == 1) MHC_NORM_BWD(8, 1);
-    else if (pl.V == 8 && pl.UPT == 2) MHC_NORM_BWD(8, 2);
-    else if (pl.V == 8) MHC_NORM_BWD(8, 4);
-    else if (pl.UPT == 1) MHC_NORM_BWD(1, 1);
-    else if (pl.UPT == 4) MHC_NORM_BWD(1, 4);
-    else if (pl.UPT == 8) MHC_NORM_BWD(1, 8);
-    else MHC_NORM_BWD(1, 16);
+#define MHC_NORM_BWD(KERN) KERN<<<blocks, pl.threads, 0, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch)
+    if (long_bwd(pl)) {
+      const bool keep = cols <= kKeepCols;
+      const size_t bytes = keep ? (size_t)pitch * sizeof(float) : 0;
+      auto go = [&](auto kern) -> int {
+        if (bytes && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+          return fail(MHC_ERR_CUDA, "rmsnorm_checkpoint8_bwd: cannot reserve %zu bytes of shared memory", bytes);
+        kern<<<blocks, kLongThreads, bytes, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch);
+        return MHC_OK;
+      };
+      const int rc = keep ? (even ? go(norm_bwd_long_kernel<T, true, true>) : go(norm_bwd_long_kernel<T, false, true>))
+                          : (even ? go(norm_bwd_long_kernel<T, true, false>) : go(norm_bwd_long_kernel<T, false, false>));
+      if (rc) return rc;
+    } else {
+      MHC_ROW_VARIANTS(norm_bwd_kernel, MHC_NORM_BWD)
+    }
 #undef MHC_NORM_BWD
     const int rc = check_launch("rmsnorm_checkpoint8_bwd");
     if (rc) return rc;

@@ -75,8 +75,8 @@ __device__ __forceinline__ float ck_f32(__nv_bfloat16 v) { return __bfloat162flo
 __device__ __forceinline__ void ck_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void ck_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// V consecutive values as floats: V = 8 in one access of 32 (fp32) or 16 (bf16)
-// bytes, aligned to its size, V = 1 plain
+// A thread works on units of 8 consecutive columns; four lanes hold a block.
+// Eight values in one access of 32 (fp32) or 16 (bf16) bytes, aligned to its size:
 __device__ __forceinline__ void ck_load(const float* p, float (&v)[8]) {
   asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
@@ -91,9 +91,6 @@ __device__ __forceinline__ void ck_load(const __nv_bfloat16* p, float (&v)[8]) {
     v[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
   }
 }
-template <typename T>
-__device__ __forceinline__ void ck_load(const T* p, float (&v)[1]) { v[0] = ck_f32(*p); }
-
 __device__ __forceinline__ void ck_save(float* p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
                "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
@@ -108,54 +105,68 @@ __device__ __forceinline__ void ck_save(__nv_bfloat16* p, const float (&v)[8]) {
   r.z = *reinterpret_cast<uint32_t*>(&h[2]); r.w = *reinterpret_cast<uint32_t*>(&h[3]);
   *reinterpret_cast<uint4*>(p) = r;
 }
-template <typename T>
-__device__ __forceinline__ void ck_save(T* p, const float (&v)[1]) { ck_store(p, v[0]); }
 
-// Codes and exponent of one unit of V values that starts at column c of its
-// row.  V = 8: the four lanes 4j .. 4j+3 hold one block; V = 1: the warp's 32
-// lanes do.  All lanes of the warp take part; lanes past the row's end pass
-// zeros, and `on` says whether the unit lies inside the padded row.
-template <int V>
-__device__ __forceinline__ void ck_encode(float (&v)[V], int8_t* codes, uint8_t* exps, int64_t c, bool on) {
+// Rows whose start or width breaks such accesses go through shared memory: the
+// warp's 256 consecutive columns [c0, c0 + 256) move as 8 coalesced accesses of
+// one value a lane, and change hands in `sm` (256 words of the warp's own).
+// (Columns one a lane throughout took 3 times as long.)  Values past the row's
+// end read as zero and are not written.
+__device__ __forceinline__ int ck_word(int w) { return w ^ (((w >> 5) & 1) << 2); }  // no bank twice either way
+template <typename T>
+__device__ __forceinline__ void ck_load_any(const T* row, int64_t c0, int64_t cols, float* sm, float (&v)[8]) {
+  const int lane = threadIdx.x & 31;
+  float t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = c0 + 32 * j + lane < cols ? ck_f32(row[c0 + 32 * j + lane]) : 0.f;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sm[ck_word(32 * j + lane)] = t[j];
+  __syncwarp();
+  const float4 a = *reinterpret_cast<const float4*>(sm + ck_word(8 * lane));
+  const float4 b = *reinterpret_cast<const float4*>(sm + ck_word(8 * lane + 4));
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void ck_save_any(T* row, int64_t c0, int64_t cols, float* sm, const float (&v)[8]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  *reinterpret_cast<float4*>(sm + ck_word(8 * lane)) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(sm + ck_word(8 * lane + 4)) = make_float4(v[4], v[5], v[6], v[7]);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c0 + 32 * j + lane < cols) ck_store(row + c0 + 32 * j + lane, sm[ck_word(32 * j + lane)]);
+}
+
+// Codes and exponent of the unit that starts at column c of its row.  All
+// lanes of the warp take part; values past the row's end are zeros, and `on`
+// says whether the unit lies inside the padded row.
+__device__ __forceinline__ void ck_encode(float (&v)[8], int8_t* codes, uint8_t* exps, int64_t c, bool on) {
   uint32_t m = abs_bits(v[0]);
 #pragma unroll
-  for (int j = 1; j < V; ++j) m = max(m, abs_bits(v[j]));
-  if constexpr (V == 8) {
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  } else {
-    m = __reduce_max_sync(0xffffffffu, m);
-  }
+  for (int j = 1; j < 8; ++j) m = max(m, abs_bits(v[j]));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const uint32_t E = ck_exponent(m);
   const float inv = ck_inverse(E);
   if (!on) return;
   if (E == kCkTop) {  // the largest finite values
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = fminf(fmaxf(v[j], -63.f * 0x1p122f), 63.f * 0x1p122f);
+    for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -63.f * 0x1p122f), 63.f * 0x1p122f);
   }
-  if constexpr (V == 8) {
-    uint2 w;
-    w.x = ck_pack4(ck_code(v[0], inv), ck_code(v[1], inv), ck_code(v[2], inv), ck_code(v[3], inv));
-    w.y = ck_pack4(ck_code(v[4], inv), ck_code(v[5], inv), ck_code(v[6], inv), ck_code(v[7], inv));
-    *reinterpret_cast<uint2*>(codes + c) = w;
-    if ((threadIdx.x & 3) == 0) exps[c / kCkBlock] = (uint8_t)E;
-  } else {
-    codes[c] = (int8_t)(ck_code(v[0], inv) & 0xff);
-    if ((threadIdx.x & 31) == 0) exps[c / kCkBlock] = (uint8_t)E;
-  }
+  uint2 w;
+  w.x = ck_pack4(ck_code(v[0], inv), ck_code(v[1], inv), ck_code(v[2], inv), ck_code(v[3], inv));
+  w.y = ck_pack4(ck_code(v[4], inv), ck_code(v[5], inv), ck_code(v[6], inv), ck_code(v[7], inv));
+  *reinterpret_cast<uint2*>(codes + c) = w;
+  if ((threadIdx.x & 3) == 0) exps[c / kCkBlock] = (uint8_t)E;
 }
 
-// The values of one unit of V codes at column c of its row.
-template <int V>
-__device__ __forceinline__ void ck_decode(const int8_t* codes, const uint8_t* exps, int64_t c, float (&v)[V]) {
-  const float step = ck_step(exps[c / kCkBlock]);
-  if constexpr (V == 8) {
-    const uint2 w = *reinterpret_cast<const uint2*>(codes + c);
-    ck_expand4(w.x, step, v);
-    ck_expand4(w.y, step, v + 4);
-  } else {
-    v[0] = (float)codes[c] * step;
-  }
+// The values of 8 codes.
+__device__ __forceinline__ void ck_decode(uint2 w, uint32_t E, float (&v)[8]) {
+  const float step = ck_step(E);
+  ck_expand4(w.x, step, v);
+  ck_expand4(w.y, step, v + 4);
 }
 
 }  // namespace mhc
