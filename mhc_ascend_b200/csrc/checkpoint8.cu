@@ -1,6 +1,7 @@
 // 8-bit activation checkpoints: pack, restore, and RMSNorm that keeps its
 // input in 8 bits (forward and backward).  Format: checkpoint8.cuh.
 #include "checkpoint8.cuh"
+#include "tma.cuh"
 
 namespace mhc {
 namespace {
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(row_threads(UPT, WARP))
                     float* __restrict__ rms, int8_t* __restrict__ codes, uint8_t* __restrict__ exps,
                     int64_t rows, int64_t cols, int64_t pitch, float eps) {
   __shared__ float red[32];
-  __shared__ __align__(16) float sm[EVEN ? 1 : row_threads(UPT, WARP) * 8];
+  extern __shared__ __align__(16) float sm[];  // uneven rows: 8 a thread
   float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
   const int lane = threadIdx.x & 31;
   const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -313,6 +314,163 @@ __global__ void __launch_bounds__(row_threads(UPT, WARP))
   }
 }
 
+// ---------------------------------------------------------------------------
+// Backward of rows of 1025 to 8192 columns that 16-byte copies fit: a block walks
+// its rows over a ring of them in shared memory filled by bulk copies, so that
+// what is in flight depends neither on registers nor on where the block's threads
+// are.  g and xh are read from there twice, for the sum and for the output, so
+// little is live across the barrier and 1024 threads fit an SM.  The barrier of
+// row i also says that everyone is done with row i - 1: thread 0 then refills its
+// place.  What bounds it is instructions (two expansions a value), hence two-wide
+// fp32 arithmetic and the weights in shared memory.
+// Measured at [16384, 7168] bf16: %BWD7168%; [8192, 4096] bf16: %BWD4096%.
+// ---------------------------------------------------------------------------
+constexpr int kRingMost = 8, kRingUPT = 2;
+
+struct Ring {
+  int stages, blocks;  // blocks an SM; stages = 0: no ring
+  uint32_t stage;      // bytes
+  int threads;
+};
+
+// values of a unit in shared memory
+__device__ __forceinline__ void smem_load(const float* p, float2 (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = make_float2(a.x, a.y); v[1] = make_float2(a.z, a.w);
+  v[2] = make_float2(b.x, b.y); v[3] = make_float2(b.z, b.w);
+}
+__device__ __forceinline__ void smem_load(const __nv_bfloat16* p, float2 (&v)[4]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t r[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = make_float2(__uint_as_float(r[j] << 16), __uint_as_float(r[j] & 0xffff0000u));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512, 2)
+    norm_bwd_ring_kernel(const T* __restrict__ g, const int8_t* __restrict__ codes,
+                         const uint8_t* __restrict__ exps, const float* __restrict__ w,
+                         const float* __restrict__ rms, T* __restrict__ gx, float* __restrict__ part,
+                         int64_t rows, int cols, int pitch, Ring plan) {
+  extern __shared__ __align__(128) unsigned char ring_sm[];
+  __shared__ uint64_t full[kRingMost];
+  __shared__ float red[2][16];
+  __shared__ int stop_s;
+  volatile int* stop = &stop_s;
+  constexpr int UPT = kRingUPT;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  const uint32_t gb = (uint32_t)cols * sizeof(T);  // bytes of a row of g; its codes follow
+  float* ws = reinterpret_cast<float*>(ring_sm + (uint32_t)plan.stages * plan.stage);
+  auto load = [&](int i, int s) {  // the block's row i into stage s; one thread
+    const int64_t row = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
+    if (row >= rows) return;
+    unsigned char* dst = ring_sm + (uint32_t)s * plan.stage;
+    mbar_expect_tx(&full[s], gb + (uint32_t)pitch);
+    bulk_load(dst, g + row * cols, gb, &full[s]);
+    bulk_load(dst + gb, codes + row * pitch, (uint32_t)pitch, &full[s]);
+  };
+  if (tid == 0) {
+    for (int s = 0; s < plan.stages; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+    *stop = 0;
+  }
+  for (int c = tid; c < cols; c += blockDim.x) ws[c] = w[c];
+  __syncthreads();
+  if (tid == 0)
+    for (int s = 0; s < plan.stages; ++s) load(s, s);
+  int c[UPT];
+  bool on[UPT];
+  float2 acc[UPT][4];
+  const uint8_t* ep = exps + (int64_t)blockIdx.x * (pitch / kCkBlock);
+  uint32_t ne[UPT];  // the exponents and r of the row ahead
+#pragma unroll
+  for (int k = 0; k < UPT; ++k) {
+    c[k] = 8 * (k * (int)blockDim.x + tid);
+    on[k] = c[k] < cols;
+    ne[k] = on[k] ? ep[c[k] / kCkBlock] : 1u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[k][j] = make_float2(0.f, 0.f);
+  }
+  float nr = rms[blockIdx.x];
+  const float share = 1.0f / (float)cols;
+  int i = 0, s = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, ++i) {
+    const unsigned char* at = ring_sm + (uint32_t)s * plan.stage;
+    if (!mbar_wait(&full[s], phase)) *stop = 1;
+    uint32_t E[UPT];
+    const float ir = 1.0f / nr;
+    float2 d2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      E[k] = ne[k];
+      if (on[k]) {
+        float2 gv[4], wv[4];
+        float xv[8];
+        smem_load(reinterpret_cast<const T*>(at) + c[k], gv);
+        smem_load(ws + c[k], wv);
+        ck_decode(*reinterpret_cast<const uint2*>(at + gb + c[k]), E[k], xv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 gx2 = __fmul2_rn(gv[j], make_float2(xv[2 * j], xv[2 * j + 1]));
+          acc[k][j] = __ffma2_rn(gx2, make_float2(ir, ir), acc[k][j]);
+          d2 = __ffma2_rn(gx2, wv[j], d2);
+        }
+      }
+    }
+    if (row + gridDim.x < rows) {
+      ep += (int64_t)gridDim.x * (pitch / kCkBlock);
+      nr = rms[row + gridDim.x];
+#pragma unroll
+      for (int k = 0; k < UPT; ++k)
+        if (on[k]) ne[k] = ep[c[k] / kCkBlock];
+    }
+    const float d = warp_sum(d2.x + d2.y);
+    if (lane == 0) red[i & 1][warp] = d;
+    __syncthreads();
+    if (*stop) break;
+    if (tid == 0 && i > 0) load(i - 1 + plan.stages, s == 0 ? plan.stages - 1 : s - 1);
+    float t = lane < nw ? red[i & 1][lane & 15] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);  // 16 warps at most
+    const float coef = -__shfl_sync(0xffffffffu, t, 0) * share * (ir * ir);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      if (on[k]) {
+        float2 gv[4], wv[4];
+        float xv[8], o[8];
+        smem_load(reinterpret_cast<const T*>(at) + c[k], gv);
+        smem_load(ws + c[k], wv);
+        ck_decode(*reinterpret_cast<const uint2*>(at + gb + c[k]), E[k], xv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 a = __ffma2_rn(make_float2(xv[2 * j], xv[2 * j + 1]), make_float2(coef, coef),
+                                      __fmul2_rn(gv[j], wv[j]));
+          const float2 b = __fmul2_rn(a, make_float2(ir, ir));
+          o[2 * j] = b.x;
+          o[2 * j + 1] = b.y;
+        }
+        ck_save(gx + row * cols + c[k], o);
+      }
+    }
+    if (++s == plan.stages) { s = 0; phase ^= 1; }
+  }
+  if (*stop && tid == 0)  // nothing may land after the block is gone
+    for (int k = i; k < i + plan.stages; ++k)
+      if ((int64_t)blockIdx.x + (int64_t)k * gridDim.x < rows)
+        mbar_wait(&full[k % plan.stages], (uint32_t)((k / plan.stages) & 1));
+#pragma unroll
+  for (int k = 0; k < UPT; ++k)
+    if (on[k]) {
+      float* p = part + (int64_t)blockIdx.x * cols + c[k];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[2 * j] = acc[k][j].x;
+        p[2 * j + 1] = acc[k][j].y;
+      }
+    }
+}
+
 // Rows too long for that: g and the codes are read twice (the second time from
 // L2), and the block's share of gw is kept in shared memory (KEEP) or, past
 // kKeepCols columns, in its row of partial sums.
@@ -421,12 +579,14 @@ struct RowPlan {
   int UPT, threads;
   bool warp;
 };
-RowPlan row_plan(int64_t cols) {
+RowPlan row_plan(int64_t cols, bool backward) {
   const int64_t pitch = ck_pitch(cols), U = pitch / 8;
   if (pitch <= kWarpCols) return {pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows, true};
+  // forward: four units a thread wherever that leaves four warps, since small
+  // blocks put more rows on an SM ([16384, 7168] bf16: %FWD7168%)
+  if (!backward && U >= 512 && U <= 4096) return {4, (int)(((U + 3) / 4 + 31) / 32 * 32), false};
   for (int upt : {1, 2, 4}) {
     const int64_t th = (((U + upt - 1) / upt) + 31) / 32 * 32;
-    // two units a thread from 2048 columns on: fewer warps meet at the barrier
     if (th <= row_threads(upt, false)) return {upt, (int)th, false};
   }
   return {0, 1024, false};
@@ -484,11 +644,12 @@ template <typename T>
 int launch_norm_fwd(const T* x, const float* w, T* out, float* rms, int8_t* codes, uint8_t* exps, int64_t rows,
                     int64_t cols, float eps, cudaStream_t st) {
   const bool even = even_rows<T>(x, cols, cols) && even_rows<T>(out, cols, cols);
-  const RowPlan pl = row_plan(cols);
+  const RowPlan pl = row_plan(cols, false);
   const int64_t pitch = ck_pitch(cols);
   const unsigned blocks = (unsigned)(pl.warp ? (rows + kWarpRows - 1) / kWarpRows : rows);
   ProfScope p("rmsnorm_checkpoint8_fwd", st);
-#define MHC_NORM_FWD(KERN) KERN<<<blocks, pl.threads, 0, st>>>(x, w, out, rms, codes, exps, rows, cols, pitch, eps)
+  const size_t staging = even ? 0 : (size_t)pl.threads * 32;
+#define MHC_NORM_FWD(KERN) KERN<<<blocks, pl.threads, staging, st>>>(x, w, out, rms, codes, exps, rows, cols, pitch, eps)
   if (pl.UPT == 0) {
     norm_fwd_long_kernel<T><<<blocks, pl.threads, 0, st>>>(x, w, out, rms, codes, exps, cols, pitch, eps);
   } else if (!pl.warp && pl.UPT == 4) {
@@ -504,12 +665,30 @@ int launch_norm_fwd(const T* x, const float* w, T* out, float* rms, int8_t* code
 // Rows whose backward does not fit the registers
 bool long_bwd(const RowPlan& pl) { return !pl.warp && (pl.UPT == 0 || pl.UPT == 4); }
 
+// Two to six blocks an SM, 1024 threads or less; the ring takes what the weights
+// leave of 224 KB.
+Ring ring_plan(int64_t rows, int64_t cols, size_t e) {
+  const int64_t U = (cols + 7) / 8;
+  Ring p = {0, 0, 0, 0};
+  // a block has to meet several rows for its ring to pay
+  if (ck_pitch(cols) <= kWarpCols || U > 1024 || rows < 8 * (int64_t)num_sms()) return p;
+  p.threads = (int)((((U + kRingUPT - 1) / kRingUPT) + 31) / 32 * 32);
+  p.blocks = 1024 / p.threads;
+  p.blocks = p.blocks < 2 ? 2 : p.blocks > 6 ? 6 : p.blocks;
+  p.stage = (uint32_t)((size_t)cols * e + ck_pitch(cols));
+  const size_t s = ((size_t)(224 * 1024 / p.blocks) - (size_t)cols * sizeof(float)) / p.stage;
+  p.stages = (int)(s > kRingMost ? kRingMost : s);
+  if (p.stages < 3) p.stages = 0;
+  return p;
+}
+
 // Blocks of the backward: as many as run at once (the gradient of the weight
 // leaves as one row a block), no more than there are rows for.
 int norm_bwd_blocks(int64_t rows, int64_t cols) {
-  const RowPlan pl = row_plan(cols);
+  const RowPlan pl = row_plan(cols, true);
+  const Ring ring = ring_plan(rows, cols, 2);  // the blocks are the same for both types
   const int64_t need = pl.warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
-  const int64_t most = (int64_t)num_sms() * (long_bwd(pl) || pl.threads <= 256 ? 2 : 1);
+  const int64_t most = (ring.stages > 0 ? ring.blocks : 2) * (int64_t)num_sms();
   return (int)(need < most ? (need > 0 ? need : 1) : most);
 }
 
@@ -517,11 +696,19 @@ template <typename T>
 int launch_norm_bwd(const T* g, const int8_t* codes, const uint8_t* exps, const float* w, const float* rms, T* gx,
                     float* gw, int64_t rows, int64_t cols, float* part, cudaStream_t st) {
   const bool even = even_rows<T>(g, cols, cols) && even_rows<T>(gx, cols, cols);
-  const RowPlan pl = row_plan(cols);
+  const RowPlan pl = row_plan(cols, true);
   const int64_t pitch = ck_pitch(cols);
   const int blocks = norm_bwd_blocks(rows, cols);
   {
     ProfScope p("rmsnorm_checkpoint8_bwd", st);
+    const Ring ring = ring_plan(rows, cols, sizeof(T));
+    if (even && ring.stages > 0) {
+      auto kern = norm_bwd_ring_kernel<T>;
+      const size_t bytes = (size_t)ring.stages * ring.stage + (size_t)cols * sizeof(float);
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+        return fail(MHC_ERR_CUDA, "rmsnorm_checkpoint8_bwd: cannot reserve %zu bytes of shared memory", bytes);
+      kern<<<blocks, ring.threads, bytes, st>>>(g, codes, exps, w, rms, gx, part, rows, (int)cols, (int)pitch, ring);
+    } else
 #define MHC_NORM_BWD(KERN) KERN<<<blocks, pl.threads, 0, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch)
     if (long_bwd(pl)) {
       const bool keep = cols <= kKeepCols;
@@ -564,6 +751,14 @@ int check_kept(const char* what, const int8_t* codes, const uint8_t* exps) {
 }
 
 }  // namespace
+
+int norm_device_error(int* value, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(value, g_mhc_device_error, sizeof(int));
+  const int zero = 0;
+  if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(g_mhc_device_error, &zero, sizeof(int));
+  return e == cudaSuccess ? MHC_OK : fail(MHC_ERR_CUDA, "mhc_device_error_word: %s", cudaGetErrorString(e));
+}
+
 }  // namespace mhc
 
 using namespace mhc;

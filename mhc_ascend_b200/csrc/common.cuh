@@ -68,8 +68,10 @@ int fwd_dynamic_check_args(const char* what, int64_t B, int n, int64_t C, int it
                            float s_eps, float r_eps);
 size_t fwd_dynamic_scratch_bytes(int64_t B, int n, int64_t C, bool need_rec);
 
-// The device error word of checkpoint8_grad.cu's bounded waits (each
-// translation unit that waits has its own); mhc_device_error_word joins them.
+// The device error words of checkpoint8.cu's and checkpoint8_grad.cu's bounded
+// waits (each translation unit that waits has its own);
+// mhc_device_error_word joins them.
+int norm_device_error(int* value, bool reset);
 int wgrad_device_error(int* value, bool reset);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -1384,10 +1384,11 @@ extern "C" int mhc_device_error_word(int32_t* value, int32_t reset) {
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_mhc_device_error, sizeof(int));
   if (e != cudaSuccess)
     return fail(MHC_ERR_CUDA, "mhc_device_error_word: %s", cudaGetErrorString(e));
-  int w = 0;  // the weight gradient's own word
-  const int rc = wgrad_device_error(&w, reset != 0);
+  int w[2] = {0, 0};  // the other units' own words
+  int rc = norm_device_error(&w[0], reset != 0);
+  if (!rc) rc = wgrad_device_error(&w[1], reset != 0);
   if (rc) return rc;
-  *value = v ? v : w;
+  *value = v ? v : w[0] ? w[0] : w[1];
   if (reset) {
     const int zero = 0;
     e = cudaMemcpyToSymbol(g_mhc_device_error, &zero, sizeof(int));
