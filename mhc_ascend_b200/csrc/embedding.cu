@@ -20,7 +20,7 @@ struct Scales {
   float s[kMaxStreams];
 };
 
-// units of 4 values (16 or 8 bytes) where the layout allows them, of one elsewhere
+// units of 4 or 8 values where the layout allows them, of one elsewhere
 __device__ __forceinline__ void load_unit(const float* p, float (&v)[4]) {
   const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -29,6 +29,15 @@ __device__ __forceinline__ void load_unit(const __nv_bfloat16* p, float (&v)[4])
   const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p));
   v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
   v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void load_unit(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+  const uint32_t r[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(r[j] << 16);
+    v[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
+  }
 }
 template <typename T>
 __device__ __forceinline__ void load_unit(const T* p, float (&v)[1]) { v[0] = ck_f32(*p); }
@@ -43,6 +52,11 @@ __device__ __forceinline__ void save_unit(__nv_bfloat16* p, const float (&v)[4])
   r.y = *reinterpret_cast<uint32_t*>(&b);
   *reinterpret_cast<uint2*>(p) = r;
 }
+__device__ __forceinline__ void save_unit(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void save_unit(__nv_bfloat16* p, const float (&v)[8]) { ck_save(p, v); }
 template <typename T>
 __device__ __forceinline__ void save_unit(T* p, const float (&v)[1]) { ck_store(p, v[0]); }
 
@@ -84,13 +98,13 @@ __global__ void __launch_bounds__(256)
 // to 9 bits, least significant first; block c owns the c-th eighth of the
 // positions.  Per digit: a histogram of the block's range in shared memory;
 // the exclusive sums over digits and blocks from the others' histograms
-// through distributed shared memory; then tiles of 2048 positions are ranked
+// through distributed shared memory; then tiles of 4096 positions are ranked
 // (per warp by ballots, across warps by a column sum) and scattered.  The
 // lists stay in L2.  Padding and invalid ids get the key V and sort last.
 // All other blocks write zeros over gW meanwhile: the sort costs a few
 // microseconds a digit on 8 SMs, and hides behind V C stores.
 // ---------------------------------------------------------------------------
-constexpr int kSortBlocks = 8, kSortThreads = 512, kSortItems = 4, kSortTile = kSortThreads * kSortItems;
+constexpr int kSortBlocks = 8, kSortThreads = 512, kSortItems = 8, kSortTile = kSortThreads * kSortItems;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortWarps = kSortThreads / 32;
 
 template <typename I>
@@ -101,6 +115,7 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
   if (blockIdx.x >= kSortBlocks) {
     const uint64_t nb = gridDim.x - kSortBlocks, b = blockIdx.x - kSortBlocks;
     const uint64_t units = zero_bytes / 16;
+#pragma unroll 4
     for (uint64_t u = b * kSortThreads + tid; u < units; u += nb * kSortThreads)
       reinterpret_cast<uint4*>(zero)[u] = make_uint4(0u, 0u, 0u, 0u);
     if (b == 0 && tid < (int)(zero_bytes & 15)) zero[units * 16 + tid] = 0;
@@ -130,7 +145,14 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
     };
     for (int d = tid; d < kDigits; d += kSortThreads) hist[d] = 0;
     __syncthreads();
-    for (uint32_t i = lo + tid; i < hi; i += kSortThreads) atomicAdd(&hist[(key_at(i) >> shift) & mask], 1u);
+    for (uint32_t i0 = lo + tid; i0 < hi; i0 += 8 * kSortThreads) {
+      uint32_t k[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j] = i0 + j * kSortThreads < hi ? key_at(i0 + j * kSortThreads) : 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j * kSortThreads < hi) atomicAdd(&hist[(k[j] >> shift) & mask], 1u);
+    }
     cluster.sync();
     {  // one digit a thread: everyone's count, and the counts of the blocks before this one
       uint32_t all = 0, before = 0;
@@ -153,18 +175,21 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
       base[tid] = wbase + inc - all + before;
     }
     cluster.sync();  // the histograms have been read: the next digit may clear them
+    uint32_t key[kSortItems], val[kSortItems];
+    auto fetch = [&](uint32_t t0) {
+#pragma unroll
+      for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t i = t0 + warp * (32 * kSortItems) + lane + 32 * k;
+        key[k] = i < hi ? key_at(i) : 0xffffffffu;
+        val[k] = i < hi ? (p > 0 ? __ldcg(vin + i) : i) : 0u;
+      }
+    };
+    if (lo < hi) fetch(lo);
     for (uint32_t t0 = lo; t0 < hi; t0 += kSortTile) {
       for (int e = tid; e < kSortWarps * kDigits; e += kSortThreads) (&wcnt[0][0])[e] = 0;
       __syncthreads();
-      uint32_t key[kSortItems], val[kSortItems], place[kSortItems];
+      uint32_t place[kSortItems];
       const uint32_t wfirst = t0 + warp * (32 * kSortItems) + lane;
-#pragma unroll
-      for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t i = wfirst + 32 * k;
-        const bool on = i < hi;
-        key[k] = on ? key_at(i) : 0xffffffffu;
-        val[k] = on ? (p > 0 ? __ldcg(vin + i) : i) : 0u;
-      }
 #pragma unroll
       for (int k = 0; k < kSortItems; ++k) {
         const bool on = wfirst + 32 * k < hi;
@@ -184,10 +209,13 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
       __syncthreads();
       {
         uint32_t run = base[tid];
+        uint32_t c[kSortWarps];
+#pragma unroll
+        for (int k = 0; k < kSortWarps; ++k) c[k] = wcnt[k][tid];
+#pragma unroll
         for (int k = 0; k < kSortWarps; ++k) {
-          const uint32_t c = wcnt[k][tid];
           wcnt[k][tid] = run;
-          run += c;
+          run += c[k];
         }
         base[tid] = run;
       }
@@ -199,6 +227,7 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
           __stcg(kout + at, key[k]);
           __stcg(vout + at, val[k]);
         }
+      if (t0 + kSortTile < hi) fetch(t0 + kSortTile);
       __syncthreads();
     }
     cluster.sync();  // release / acquire: the lists are whole before the next digit reads them
@@ -206,58 +235,78 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
 }
 
 // ---------------------------------------------------------------------------
-// gradient, launch 2: sums of the sorted positions, kChunk a block, a slice of
-// the columns a block.  Rows whose tokens all lie in the chunk are written;
-// the sums at its two ends, if their rows go on in a neighbour, are kept:
-// ends[chunk][0] for a row that began before the chunk, [1] for one that
-// begins in it and goes on.
+// gradient, launch 2: sums of the sorted positions, `chunk` of them and a slice of
+// the columns a block.  Rows whose tokens all lie in the chunk are written; the
+// sums at its two ends, if their rows go on in a neighbour, are kept:
+// ends[chunk][0] for a row that began before the chunk, [1] for one that begins in
+// it and goes on.  Bound by reading g: 8 or 16 loads of a thread are in flight,
+// and blocks that run together read neighbouring slices of the same rows.
+// A thread has NC x V columns: V = 4 or 8 in one access, or four single ones, a
+// block's width apart, where rows are not aligned.
 // launch 3: for each row that begins in a chunk and goes on, its sums are added
 // in chunk order and the row is written.
 // ---------------------------------------------------------------------------
-constexpr int kChunk = 32, kSumThreads = 128, kLoads = 8;
+constexpr int kMaxChunk = 64, kSumThreads = 128, kJoinThreads = 256;
 
-template <typename TG, typename TW, int V>
+template <typename TG, typename TW, int V, int NC>
 __global__ void __launch_bounds__(kSumThreads)
     embed_sum_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals,
                      const TG* __restrict__ g, TW* __restrict__ gw, float* __restrict__ ends, uint32_t T,
-                     uint32_t vocab, int n, int64_t C, const __grid_constant__ Scales sc) {
-  __shared__ uint32_t sk[kChunk + 2], sv[kChunk];
+                     uint32_t vocab, int n, int64_t C, const __grid_constant__ Scales sc, int chunk, uint32_t slices) {
+  constexpr int L = NC == 1 ? 8 : 4;  // rows of g in flight
+  __shared__ uint32_t sk[kMaxChunk + 2], sv[kMaxChunk];
   __shared__ float ss[kMaxStreams];
-  const uint32_t p0 = blockIdx.x * kChunk;
+  const uint32_t piece = blockIdx.x / slices;
+  const uint32_t p0 = piece * chunk;
   const int tid = threadIdx.x;
-  if (tid < kChunk + 2) {  // sk[1 + j] = key at p0 + j; neighbours on both sides
+  if (tid < chunk + 2) {  // sk[1 + j] = key at p0 + j; neighbours on both sides
     const int64_t q = (int64_t)p0 + tid - 1;
     sk[tid] = q >= 0 && q < (int64_t)T ? keys[q] : 0xffffffffu;
   }
-  if (tid < kChunk) sv[tid] = p0 + tid < T ? vals[p0 + tid] : 0u;
+  if (tid < chunk) sv[tid] = p0 + tid < T ? vals[p0 + tid] : 0u;
   if (tid < n) ss[tid] = sc.s[tid];
   __syncthreads();
-  int len = (int)min((uint32_t)kChunk, T - p0);
+  int len = (int)min((uint32_t)chunk, T - p0);
   while (len > 0 && sk[len] >= vocab) --len;  // padding sorts last
   if (len == 0) return;
-  const int64_t c = ((int64_t)blockIdx.y * kSumThreads + tid) * V;
+  const int64_t c = ((int64_t)(blockIdx.x - piece * slices) * (kSumThreads * NC) + tid) * V;
   if (c >= C) return;
-  float acc[V];
+  bool on[NC];
 #pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  int p = 0, i = 0;  // the load that is added next: stream i of position p
+  for (int m = 0; m < NC; ++m) on[m] = c + (int64_t)m * kSumThreads * V < C;
+  float acc[NC][V];
+#pragma unroll
+  for (int m = 0; m < NC; ++m)
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[m][j] = 0.f;
+  int p = 0, i = 0;  // what is added next: stream i of position p
   int first = 0;     // first position of the running row
   const int total = len * n;
   int lp = 0, li = 0;
-  for (int q = 0; q < total; q += kLoads) {
-    float v[kLoads][V];
+  const TG* at = g + (int64_t)sv[0] * n * C + c;  // what is loaded next
+  for (int q = 0; q < total; q += L) {
+    float v[L][NC][V];
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k)
+    for (int k = 0; k < L; ++k)
       if (q + k < total) {
-        load_unit(g + ((int64_t)sv[lp] * n + li) * C + c, v[k]);
-        if (++li == n) { li = 0; ++lp; }
+#pragma unroll
+        for (int m = 0; m < NC; ++m)
+          if (on[m]) load_unit(at + (int64_t)m * kSumThreads * V, v[k][m]);
+        at += C;
+        if (++li == n) {
+          li = 0;
+          if (++lp < len) at = g + (int64_t)sv[lp] * n * C + c;
+        }
       }
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k)
+    for (int k = 0; k < L; ++k)
       if (q + k < total) {
         const float s = ss[i];
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = fmaf(s, v[k][j], acc[j]);
+        for (int m = 0; m < NC; ++m)
+          if (on[m])
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[m][j] = fmaf(s, v[k][m][j], acc[m][j]);
         if (++i == n) {
           i = 0;
           const uint32_t key = sk[p + 1];
@@ -265,15 +314,17 @@ __global__ void __launch_bounds__(kSumThreads)
           if (!more) {
             const bool before = first == 0 && sk[0] == key;
             const bool after = p + 1 == len && sk[p + 2] == key;
-            if (!before && !after) {
-              save_unit(gw + (int64_t)key * C + c, acc);
-            } else {
-              float* e = ends + ((int64_t)blockIdx.x * 2 + (before ? 0 : 1)) * C + c;
+            float* e = ends + ((int64_t)piece * 2 + (before ? 0 : 1)) * C + c;
 #pragma unroll
-              for (int j = 0; j < V; ++j) e[j] = acc[j];
+            for (int m = 0; m < NC; ++m) {
+              const int64_t o = (int64_t)m * kSumThreads * V;
+              if (on[m]) {
+                if (!before && !after) save_unit(gw + (int64_t)key * C + c + o, acc[m]);
+                else save_unit(e + o, acc[m]);
+              }
+#pragma unroll
+              for (int j = 0; j < V; ++j) acc[m][j] = 0.f;
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] = 0.f;
             first = p + 1;
           }
           ++p;
@@ -282,33 +333,69 @@ __global__ void __launch_bounds__(kSumThreads)
   }
 }
 
+// A block joins one row's sums over kJoinThreads * V columns; where there are many,
+// a warp takes every eighth of them and the eight shares are added in order.
 template <typename TW, int V>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kJoinThreads)
     embed_join_kernel(const uint32_t* __restrict__ keys, TW* __restrict__ gw, const float* __restrict__ ends,
-                      uint32_t T, uint32_t vocab, int64_t C) {
-  const uint32_t p1 = (blockIdx.x + 1) * kChunk;  // first position of the next chunk (exists: the grid is one short)
-  const uint32_t key = keys[p1];
-  if (key >= vocab || keys[p1 - 1] != key) return;                     // no row goes on here
-  const uint32_t p0 = p1 - kChunk;
-  if (keys[p0] == key && p0 > 0 && keys[p0 - 1] == key) return;        // it began in an earlier chunk
-  uint32_t lo = p1, hi = T;                                            // first position past the row
+                      uint32_t T, uint32_t vocab, int64_t C, int chunk, uint32_t slices) {
+  __shared__ __align__(16) float part[8][32 * V];
+  const uint32_t piece = blockIdx.x / slices;
+  const uint32_t p1 = (piece + 1) * chunk;  // first position of the next chunk (exists: the grid is one short)
+  const uint32_t p0 = p1 - chunk;
+  const uint32_t key = keys[p1], last_key = keys[p1 - 1], first_key = keys[p0], before_key = p0 > 0 ? keys[p0 - 1] : ~0u;
+  if (key >= vocab || last_key != key) return;          // no row goes on here
+  if (first_key == key && before_key == key) return;    // it began in an earlier chunk
+  uint32_t lo = p1, hi = T;                             // first position past the row
   while (lo < hi) {
     const uint32_t m = lo + (hi - lo) / 2;
     if (keys[m] > key) hi = m; else lo = m + 1;
   }
-  const uint32_t last = (lo - 1) / kChunk;
-  const int64_t c = ((int64_t)blockIdx.y * kSumThreads + threadIdx.x) * V;
-  if (c >= C) return;
-  float acc[V];
-  load_unit(ends + ((int64_t)blockIdx.x * 2 + 1) * C + c, acc);
-#pragma unroll 8
-  for (uint32_t m = blockIdx.x + 1; m <= last; ++m) {
-    float v[V];
-    load_unit(ends + (int64_t)m * 2 * C + c, v);
+  const uint32_t last = (lo - 1) / chunk, count = last - piece;
+  const int64_t c0 = (int64_t)(blockIdx.x - piece * slices) * (kJoinThreads * V);
+  if (count <= 16) {
+    const int64_t c = c0 + threadIdx.x * V;
+    if (c >= C) return;
+    float acc[V];
+    load_unit(ends + ((int64_t)piece * 2 + 1) * C + c, acc);
+#pragma unroll 4
+    for (uint32_t m = piece + 1; m <= last; ++m) {
+      float v[V];
+      load_unit(ends + (int64_t)m * 2 * C + c, v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] += v[j];
+      for (int j = 0; j < V; ++j) acc[j] += v[j];
+    }
+    save_unit(gw + (int64_t)key * C + c, acc);
+    return;
   }
-  save_unit(gw + (int64_t)key * C + c, acc);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int sub = 0; sub < 8; ++sub) {
+    const int64_t c = c0 + (sub * 32 + lane) * V;
+    float acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+    if (c < C) {
+      if (warp == 0) load_unit(ends + ((int64_t)piece * 2 + 1) * C + c, acc);
+#pragma unroll 8
+      for (uint32_t m = piece + 1 + warp; m <= last; m += 8) {
+        float v[V];
+        load_unit(ends + (int64_t)m * 2 * C + c, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += v[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[warp][lane * V + j] = acc[j];
+    __syncthreads();
+    if (warp == 0 && c < C) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w)
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += part[w][lane * V + j];
+      save_unit(gw + (int64_t)key * C + c, acc);
+    }
+    __syncthreads();
+  }
 }
 
 int check_embed(const char* what, int64_t T, int32_t n, int64_t C, int64_t vocab, const float* scales) {
@@ -350,31 +437,44 @@ int launch_embed_fwd(const void* ids, const void* w, void* out, int64_t T, int n
 
 struct GradPlan {
   size_t list, ends;  // bytes of one list, of the end sums
+  int chunk;          // positions of a chunk
   int64_t chunks;
 };
+// The largest chunk (a power of two to 64) that leaves 2048 blocks: shorter chunks
+// join more sums, fewer blocks leave the GPU idle ([128, 32, 1280] in chunks of 32
+// took 200 us on its 12 blocks).
 GradPlan grad_plan(int64_t T, int64_t C) {
   GradPlan p;
   p.list = ((size_t)T * 4 + 255) / 256 * 256;
-  p.chunks = (T + kChunk - 1) / kChunk;
+  const int64_t slices = (C + 511) / 512;
+  p.chunk = kMaxChunk;
+  while (p.chunk > 1 && (T + p.chunk - 1) / p.chunk * slices < 2048) p.chunk /= 2;
+  p.chunks = (T + p.chunk - 1) / p.chunk;
   p.ends = (size_t)p.chunks * 2 * (size_t)C * sizeof(float);
   return p;
 }
 
-template <typename TG, typename TW, int V>
+template <typename TG, typename TW, int V, int NC>
 int launch_embed_sums(const uint32_t* keys, const uint32_t* vals, const void* g, void* gw, float* ends, int64_t T,
                       int n, int64_t C, int64_t vocab, const Scales& sc, const GradPlan& pl, cudaStream_t st) {
-  const unsigned slices = (unsigned)((C + kSumThreads * V - 1) / (kSumThreads * V));
   {
+    const int64_t slices = (C + kSumThreads * V * NC - 1) / (kSumThreads * V * NC), blocks = pl.chunks * slices;
+    MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: %lld tokens of %lld are too many",
+                (long long)T, (long long)C);
     ProfScope p("stream_embedding_sum", st);
-    embed_sum_kernel<TG, TW, V><<<dim3((unsigned)pl.chunks, slices), kSumThreads, 0, st>>>(
-        keys, vals, (const TG*)g, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, n, C, sc);
+    embed_sum_kernel<TG, TW, V, NC><<<(unsigned)blocks, kSumThreads, 0, st>>>(
+        keys, vals, (const TG*)g, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, n, C, sc, pl.chunk, (uint32_t)slices);
     const int rc = check_launch("stream_embedding_sum");
     if (rc) return rc;
   }
   if (pl.chunks < 2) return MHC_OK;
+  constexpr int W = V == 1 ? 1 : 4;
+  const int64_t slices = (C + kJoinThreads * W - 1) / (kJoinThreads * W), blocks = (pl.chunks - 1) * slices;
+  MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: %lld tokens of %lld are too many",
+              (long long)T, (long long)C);
   ProfScope p("stream_embedding_join", st);
-  embed_join_kernel<TW, V><<<dim3((unsigned)(pl.chunks - 1), slices), kSumThreads, 0, st>>>(
-      keys, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, C);
+  embed_join_kernel<TW, W><<<(unsigned)blocks, kJoinThreads, 0, st>>>(keys, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab,
+                                                                      C, pl.chunk, (uint32_t)slices);
   return check_launch("stream_embedding_join");
 }
 
@@ -458,13 +558,12 @@ extern "C" int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, co
   }
   const uint32_t* keys = (passes & 1) ? kb : ka;
   const uint32_t* vals = (passes & 1) ? vb : va;
-  const size_t eg = g_bf16 ? 2 : 4, ew = gw_bf16 ? 2 : 4;
-  const bool vec = hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(grad_out) & (4 * eg - 1)) == 0 &&
-                   (reinterpret_cast<uintptr_t>(grad_weight) & (4 * ew - 1)) == 0;
-#define MHC_SUMS(TG, TW)                                                                                          \
-  (vec ? launch_embed_sums<TG, TW, 4>(keys, vals, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st) \
-       : launch_embed_sums<TG, TW, 1>(keys, vals, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st))
-  return g_bf16 ? (gw_bf16 ? MHC_SUMS(__nv_bfloat16, __nv_bfloat16) : MHC_SUMS(__nv_bfloat16, float))
-                : (gw_bf16 ? MHC_SUMS(float, __nv_bfloat16) : MHC_SUMS(float, float));
+  // 16-byte loads of g, and stores of gW of 4 or 8 values
+  const bool vec = hidden % (g_bf16 ? 8 : 4) == 0 && aligned16(grad_out);
+#define MHC_SUMS(TG, TW, VV)                                                                                        \
+  (vec ? launch_embed_sums<TG, TW, VV, 1>(keys, vals, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st) \
+       : launch_embed_sums<TG, TW, 1, 4>(keys, vals, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st))
+  return g_bf16 ? (gw_bf16 ? MHC_SUMS(__nv_bfloat16, __nv_bfloat16, 8) : MHC_SUMS(__nv_bfloat16, float, 8))
+                : (gw_bf16 ? MHC_SUMS(float, __nv_bfloat16, 4) : MHC_SUMS(float, float, 4));
 #undef MHC_SUMS
 }
