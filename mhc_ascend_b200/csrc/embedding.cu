@@ -30,15 +30,6 @@ __device__ __forceinline__ void load_unit(const __nv_bfloat16* p, float (&v)[4])
   v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
   v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
 }
-__device__ __forceinline__ void load_unit(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-  const uint32_t r[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = __uint_as_float(r[j] << 16);
-    v[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
-  }
-}
 template <typename T>
 __device__ __forceinline__ void load_unit(const T* p, float (&v)[1]) { v[0] = ck_f32(*p); }
 
@@ -109,7 +100,7 @@ constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortWarps = kSortThrea
 
 template <typename I>
 __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThreads)
-    embed_sort_kernel(const I* __restrict__ ids, uint32_t* ka, uint32_t* va, uint32_t* kb, uint32_t* vb, uint32_t T,
+    embed_sort_kernel(const I* __restrict__ ids, uint2* la, uint2* lb, uint32_t T,
                       uint32_t vocab, int64_t pad, int passes, int bits, char* zero, uint64_t zero_bytes) {
   const int tid = threadIdx.x;
   if (blockIdx.x >= kSortBlocks) {
@@ -134,12 +125,10 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
 
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    uint32_t* kin = (p & 1) ? kb : ka;
-    uint32_t* vin = (p & 1) ? vb : va;
-    uint32_t* kout = (p & 1) ? ka : kb;
-    uint32_t* vout = (p & 1) ? va : vb;
+    const uint2* in = (p & 1) ? lb : la;  // (key, token)
+    uint2* out = (p & 1) ? la : lb;
     auto key_at = [&](uint32_t i) -> uint32_t {
-      if (p > 0) return __ldcg(kin + i);
+      if (p > 0) return __ldcg(&in[i].x);
       const int64_t id = (int64_t)ids[i];
       return (id >= 0 && id < (int64_t)vocab && id != pad) ? (uint32_t)id : vocab;
     };
@@ -175,13 +164,13 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
       base[tid] = wbase + inc - all + before;
     }
     cluster.sync();  // the histograms have been read: the next digit may clear them
-    uint32_t key[kSortItems], val[kSortItems];
+    uint2 item[kSortItems];
     auto fetch = [&](uint32_t t0) {
 #pragma unroll
       for (int k = 0; k < kSortItems; ++k) {
         const uint32_t i = t0 + warp * (32 * kSortItems) + lane + 32 * k;
-        key[k] = i < hi ? key_at(i) : 0xffffffffu;
-        val[k] = i < hi ? (p > 0 ? __ldcg(vin + i) : i) : 0u;
+        item[k] = make_uint2(0xffffffffu, 0u);
+        if (i < hi) item[k] = p > 0 ? __ldcg(in + i) : make_uint2(key_at(i), i);
       }
     };
     if (lo < hi) fetch(lo);
@@ -193,7 +182,7 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
 #pragma unroll
       for (int k = 0; k < kSortItems; ++k) {
         const bool on = wfirst + 32 * k < hi;
-        const uint32_t d = (key[k] >> shift) & mask;
+        const uint32_t d = (item[k].x >> shift) & mask;
         uint32_t peers = __ballot_sync(0xffffffffu, on);
         for (int b = 0; b < bits; ++b) {
           const uint32_t m = __ballot_sync(0xffffffffu, (d >> b) & 1u);
@@ -222,11 +211,8 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < kSortItems; ++k)
-        if (wfirst + 32 * k < hi) {
-          const uint32_t at = wcnt[warp][(key[k] >> shift) & mask] + place[k];
-          __stcg(kout + at, key[k]);
-          __stcg(vout + at, val[k]);
-        }
+        if (wfirst + 32 * k < hi)
+          __stcg(out + wcnt[warp][(item[k].x >> shift) & mask] + place[k], item[k]);
       if (t0 + kSortTile < hi) fetch(t0 + kSortTile);
       __syncthreads();
     }
@@ -241,57 +227,107 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
 // ends[chunk][0] for a row that began before the chunk, [1] for one that begins in
 // it and goes on.  Bound by reading g: 8 or 16 loads of a thread are in flight,
 // and blocks that run together read neighbouring slices of the same rows.
-// A thread has NC x V columns: V = 4 or 8 in one access, or four single ones, a
-// block's width apart, where rows are not aligned.
+// A thread has 16 bytes of columns.
 // launch 3: for each row that begins in a chunk and goes on, its sums are added
 // in chunk order and the row is written.
 // ---------------------------------------------------------------------------
 constexpr int kMaxChunk = 64, kSumThreads = 128, kJoinThreads = 256;
 
-template <typename TG, typename TW, int V, int NC>
+// 16 bytes from an address of any alignment, as 4 words: of two aligned accesses
+// (the second is mostly an L1 hit: it is the neighbour's first), a shift by words,
+// then by bits.  The accesses of several rows are issued before the first shift
+// waits for one.
+__device__ __forceinline__ void shift16(uint32_t sh, const uint4& a, const uint4& b, uint32_t (&o)[4]) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t t[6], u[5];
+#pragma unroll
+  for (int j = 0; j < 6; ++j) t[j] = (sh & 8) ? w[j + 2] : w[j];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) u[j] = (sh & 4) ? t[j + 1] : t[j];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(u[j], u[j + 1], (sh & 3) * 8);
+}
+__device__ __forceinline__ void unit_of_words(const float*, const uint32_t (&o)[4], float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(o[j]);
+}
+__device__ __forceinline__ void unit_of_words(const __nv_bfloat16*, const uint32_t (&o)[4], float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(o[j] << 16);
+    v[2 * j + 1] = __uint_as_float(o[j] & 0xffff0000u);
+  }
+}
+
+// EVEN: rows of g start on 16 bytes and gW's on four values.  Elsewhere bf16 rows
+// are read by shifts and their sums go through shared memory, so that the stores
+// are coalesced; fp32 rows are read and written one value a lane ([8192, 4, 4095]:
+// 118 us against 162 by shifts, whose registers halve what is in flight; bf16
+// [100003, 2, 1281] 241 us by shifts, 275 one value a lane).
+template <typename TG, typename TW, bool EVEN>
 __global__ void __launch_bounds__(kSumThreads)
-    embed_sum_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals,
-                     const TG* __restrict__ g, TW* __restrict__ gw, float* __restrict__ ends, uint32_t T,
-                     uint32_t vocab, int n, int64_t C, const __grid_constant__ Scales sc, int chunk, uint32_t slices) {
-  constexpr int L = NC == 1 ? 8 : 4;  // rows of g in flight
+    embed_sum_kernel(const uint2* __restrict__ list, const TG* __restrict__ g, TW* __restrict__ gw,
+                     float* __restrict__ ends, uint32_t T, uint32_t vocab, int n, int64_t C,
+                     const __grid_constant__ Scales sc, int chunk, uint32_t slices) {
+  constexpr int V = 16 / (int)sizeof(TG);
+  constexpr int L = EVEN ? 8 : 4;  // rows of g in flight
+  constexpr bool SINGLE = !EVEN && sizeof(TG) == 4;
+  const int width = blockDim.x;
   __shared__ uint32_t sk[kMaxChunk + 2], sv[kMaxChunk];
   __shared__ float ss[kMaxStreams];
+  __shared__ float sums[EVEN || SINGLE ? 1 : kSumThreads * V];
   const uint32_t piece = blockIdx.x / slices;
   const uint32_t p0 = piece * chunk;
   const int tid = threadIdx.x;
-  if (tid < chunk + 2) {  // sk[1 + j] = key at p0 + j; neighbours on both sides
-    const int64_t q = (int64_t)p0 + tid - 1;
-    sk[tid] = q >= 0 && q < (int64_t)T ? keys[q] : 0xffffffffu;
+  for (int j = tid; j < chunk + 2; j += width) {  // sk[1 + j] = key at p0 + j; neighbours on both sides
+    const int64_t q = (int64_t)p0 + j - 1;
+    const uint2 e = q >= 0 && q < (int64_t)T ? list[q] : make_uint2(0xffffffffu, 0u);
+    sk[j] = e.x;
+    if (j >= 1 && j <= chunk) sv[j - 1] = e.y;
   }
-  if (tid < chunk) sv[tid] = p0 + tid < T ? vals[p0 + tid] : 0u;
-  if (tid < n) ss[tid] = sc.s[tid];
+  if (tid < n) ss[tid] = sc.s[tid];  // n <= 32 <= width
   __syncthreads();
   int len = (int)min((uint32_t)chunk, T - p0);
   while (len > 0 && sk[len] >= vocab) --len;  // padding sorts last
   if (len == 0) return;
-  const int64_t c = ((int64_t)(blockIdx.x - piece * slices) * (kSumThreads * NC) + tid) * V;
-  if (c >= C) return;
-  bool on[NC];
+  const int64_t c0 = (int64_t)(blockIdx.x - piece * slices) * (width * V), c = c0 + tid * (SINGLE ? 1 : V);
+  const int have = SINGLE ? (int)max((int64_t)0, min((int64_t)V, (C - c + width - 1) / width))
+                          : (int)max((int64_t)0, min((int64_t)V, C - c));
+  if ((EVEN || SINGLE) && have == 0) return;
+  // The aligned accesses around a unit stay inside the tensor unless its token is
+  // the first or the last one, or rows are shorter than such an access.
+  auto edge = [&](uint32_t token) { return token == 0 || token == T - 1 || C < 16; };
+  float acc[V];
 #pragma unroll
-  for (int m = 0; m < NC; ++m) on[m] = c + (int64_t)m * kSumThreads * V < C;
-  float acc[NC][V];
-#pragma unroll
-  for (int m = 0; m < NC; ++m)
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[m][j] = 0.f;
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
   int p = 0, i = 0;  // what is added next: stream i of position p
   int first = 0;     // first position of the running row
   const int total = len * n;
   int lp = 0, li = 0;
   const TG* at = g + (int64_t)sv[0] * n * C + c;  // what is loaded next
   for (int q = 0; q < total; q += L) {
-    float v[L][NC][V];
+    uint4 v[L], w[EVEN || SINGLE ? 1 : L];
+    uint32_t sh[EVEN || SINGLE ? 1 : L];
 #pragma unroll
     for (int k = 0; k < L; ++k)
       if (q + k < total) {
-#pragma unroll
-        for (int m = 0; m < NC; ++m)
-          if (on[m]) load_unit(at + (int64_t)m * kSumThreads * V, v[k][m]);
+        if constexpr (EVEN) {
+          v[k] = __ldcs(reinterpret_cast<const uint4*>(at));
+        } else if constexpr (SINGLE) {
+          const uint32_t* word = reinterpret_cast<const uint32_t*>(at);
+          v[k].x = word[0];
+          if (have > 1) v[k].y = word[width];
+          if (have > 2) v[k].z = word[2 * width];
+          if (have > 3) v[k].w = word[3 * width];
+        } else {
+          sh[k] = 16;
+          if (have > 0 && !edge(sv[lp])) {
+            const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(at) & ~(uintptr_t)15);
+            sh[k] = (uint32_t)reinterpret_cast<uintptr_t>(at) & 15u;
+            v[k] = base[0];
+            w[k] = base[1];
+          }
+        }
         at += C;
         if (++li == n) {
           li = 0;
@@ -302,11 +338,21 @@ __global__ void __launch_bounds__(kSumThreads)
     for (int k = 0; k < L; ++k)
       if (q + k < total) {
         const float s = ss[i];
+        float u[V];
+        if constexpr (EVEN || SINGLE) {
+          const uint32_t o[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          unit_of_words(g, o, u);
+        } else if (sh[k] < 16) {
+          uint32_t o[4];
+          shift16(sh[k], v[k], w[k], o);
+          unit_of_words(g, o, u);
+        } else {
+          const TG* from = g + ((int64_t)sv[p] * n + i) * C + c;
 #pragma unroll
-        for (int m = 0; m < NC; ++m)
-          if (on[m])
+          for (int j = 0; j < V; ++j) u[j] = j < have ? ck_f32(from[j]) : 0.f;
+        }
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[m][j] = fmaf(s, v[k][m][j], acc[m][j]);
+        for (int j = 0; j < V; ++j) acc[j] = fmaf(s, u[j], acc[j]);
         if (++i == n) {
           i = 0;
           const uint32_t key = sk[p + 1];
@@ -314,17 +360,38 @@ __global__ void __launch_bounds__(kSumThreads)
           if (!more) {
             const bool before = first == 0 && sk[0] == key;
             const bool after = p + 1 == len && sk[p + 2] == key;
-            float* e = ends + ((int64_t)piece * 2 + (before ? 0 : 1)) * C + c;
+            float* e = ends + ((int64_t)piece * 2 + (before ? 0 : 1)) * C;
+            if (EVEN) {
+              if (!before && !after) save_unit(gw + (int64_t)key * C + c, acc);
+              else save_unit(e + c, acc);
+            } else if (SINGLE) {
 #pragma unroll
-            for (int m = 0; m < NC; ++m) {
-              const int64_t o = (int64_t)m * kSumThreads * V;
-              if (on[m]) {
-                if (!before && !after) save_unit(gw + (int64_t)key * C + c + o, acc[m]);
-                else save_unit(e + o, acc[m]);
+              for (int j = 0; j < V; ++j)
+                if (j < have) {
+                  if (!before && !after) ck_store(gw + (int64_t)key * C + c + j * width, acc[j]);
+                  else e[c + j * width] = acc[j];
+                }
+            } else {
+              float* mine = sums + (tid & ~31) * V;  // the warp's columns
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < V; ++j) mine[(tid & 31) * V + j] = acc[j];
+              __syncwarp();
+              const int64_t o = c0 + (tid & ~31) * V + (tid & 31);
+              const int left = (int)min((int64_t)(32 * V), C - o);  // of the row, from this lane's first on
+              if (!before && !after) {
+                TW* to = gw + (int64_t)key * C + o;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                  if (32 * j < left) ck_store(to + 32 * j, mine[32 * j + (tid & 31)]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                  if (32 * j < left) e[o + 32 * j] = mine[32 * j + (tid & 31)];
               }
-#pragma unroll
-              for (int j = 0; j < V; ++j) acc[m][j] = 0.f;
             }
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = 0.f;
             first = p + 1;
           }
           ++p;
@@ -337,19 +404,20 @@ __global__ void __launch_bounds__(kSumThreads)
 // a warp takes every eighth of them and the eight shares are added in order.
 template <typename TW, int V>
 __global__ void __launch_bounds__(kJoinThreads)
-    embed_join_kernel(const uint32_t* __restrict__ keys, TW* __restrict__ gw, const float* __restrict__ ends,
+    embed_join_kernel(const uint2* __restrict__ list, TW* __restrict__ gw, const float* __restrict__ ends,
                       uint32_t T, uint32_t vocab, int64_t C, int chunk, uint32_t slices) {
   __shared__ __align__(16) float part[8][32 * V];
   const uint32_t piece = blockIdx.x / slices;
   const uint32_t p1 = (piece + 1) * chunk;  // first position of the next chunk (exists: the grid is one short)
   const uint32_t p0 = p1 - chunk;
-  const uint32_t key = keys[p1], last_key = keys[p1 - 1], first_key = keys[p0], before_key = p0 > 0 ? keys[p0 - 1] : ~0u;
+  const uint32_t key = list[p1].x, last_key = list[p1 - 1].x, first_key = list[p0].x;
+  const uint32_t before_key = p0 > 0 ? list[p0 - 1].x : ~0u;
   if (key >= vocab || last_key != key) return;          // no row goes on here
   if (first_key == key && before_key == key) return;    // it began in an earlier chunk
   uint32_t lo = p1, hi = T;                             // first position past the row
   while (lo < hi) {
     const uint32_t m = lo + (hi - lo) / 2;
-    if (keys[m] > key) hi = m; else lo = m + 1;
+    if (list[m].x > key) hi = m; else lo = m + 1;
   }
   const uint32_t last = (lo - 1) / chunk, count = last - piece;
   const int64_t c0 = (int64_t)(blockIdx.x - piece * slices) * (kJoinThreads * V);
@@ -445,7 +513,7 @@ struct GradPlan {
 // took 200 us on its 12 blocks).
 GradPlan grad_plan(int64_t T, int64_t C) {
   GradPlan p;
-  p.list = ((size_t)T * 4 + 255) / 256 * 256;
+  p.list = ((size_t)T * 8 + 255) / 256 * 256;
   const int64_t slices = (C + 511) / 512;
   p.chunk = kMaxChunk;
   while (p.chunk > 1 && (T + p.chunk - 1) / p.chunk * slices < 2048) p.chunk /= 2;
@@ -454,26 +522,29 @@ GradPlan grad_plan(int64_t T, int64_t C) {
   return p;
 }
 
-template <typename TG, typename TW, int V, int NC>
-int launch_embed_sums(const uint32_t* keys, const uint32_t* vals, const void* g, void* gw, float* ends, int64_t T,
+template <typename TG, typename TW, bool EVEN>
+int launch_embed_sums(const uint2* list, const void* g, void* gw, float* ends, int64_t T,
                       int n, int64_t C, int64_t vocab, const Scales& sc, const GradPlan& pl, cudaStream_t st) {
   {
-    const int64_t slices = (C + kSumThreads * V * NC - 1) / (kSumThreads * V * NC), blocks = pl.chunks * slices;
+    // even slices of at most kSumThreads units of 16 bytes
+    const int64_t units = (C * (int64_t)sizeof(TG) + 15) / 16, slices = (units + kSumThreads - 1) / kSumThreads;
+    const int64_t threads = ((units + slices - 1) / slices + 31) / 32 * 32, blocks = pl.chunks * slices;
+
     MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: %lld tokens of %lld are too many",
                 (long long)T, (long long)C);
     ProfScope p("stream_embedding_sum", st);
-    embed_sum_kernel<TG, TW, V, NC><<<(unsigned)blocks, kSumThreads, 0, st>>>(
-        keys, vals, (const TG*)g, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, n, C, sc, pl.chunk, (uint32_t)slices);
+    embed_sum_kernel<TG, TW, EVEN><<<(unsigned)blocks, (unsigned)threads, 0, st>>>(
+        list, (const TG*)g, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, n, C, sc, pl.chunk, (uint32_t)slices);
     const int rc = check_launch("stream_embedding_sum");
     if (rc) return rc;
   }
   if (pl.chunks < 2) return MHC_OK;
-  constexpr int W = V == 1 ? 1 : 4;
+  constexpr int W = EVEN ? 4 : 1;
   const int64_t slices = (C + kJoinThreads * W - 1) / (kJoinThreads * W), blocks = (pl.chunks - 1) * slices;
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: %lld tokens of %lld are too many",
               (long long)T, (long long)C);
   ProfScope p("stream_embedding_join", st);
-  embed_join_kernel<TW, W><<<(unsigned)blocks, kJoinThreads, 0, st>>>(keys, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab,
+  embed_join_kernel<TW, W><<<(unsigned)blocks, kJoinThreads, 0, st>>>(list, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab,
                                                                       C, pl.chunk, (uint32_t)slices);
   return check_launch("stream_embedding_join");
 }
@@ -506,7 +577,7 @@ extern "C" int mhc_stream_embedding_fwd(const void* ids, int32_t ids_64, const v
 extern "C" size_t mhc_stream_embedding_bwd_workspace_bytes(int64_t tokens, int64_t hidden) {
   if (tokens < 0 || hidden < 1) return 0;
   const GradPlan p = grad_plan(tokens, hidden);
-  return 4 * p.list + p.ends;
+  return 2 * p.list + p.ends;
 }
 
 extern "C" int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, const void* ids, int32_t ids_64,
@@ -531,9 +602,8 @@ extern "C" int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, co
   const Scales sc = host_scales(scales, n);
   const GradPlan pl = grad_plan(tokens, hidden);
   char* ws = (char*)workspace;
-  uint32_t *ka = (uint32_t*)ws, *va = (uint32_t*)(ws + pl.list), *kb = (uint32_t*)(ws + 2 * pl.list),
-           *vb = (uint32_t*)(ws + 3 * pl.list);
-  float* ends = (float*)(ws + 4 * pl.list);
+  uint2 *la = (uint2*)ws, *lb = (uint2*)(ws + pl.list);
+  float* ends = (float*)(ws + 2 * pl.list);
   // keys are 0 .. vocab: equal digits of at most 9 bits
   int kbits = 1;
   while ((vocab >> kbits) != 0) ++kbits;
@@ -546,24 +616,22 @@ extern "C" int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, co
     const unsigned zb = (unsigned)((want < most ? want : most) + kSortBlocks - 1) / kSortBlocks * kSortBlocks;
     const dim3 grid(kSortBlocks + zb);
     if (ids_64)
-      embed_sort_kernel<int64_t><<<grid, kSortThreads, 0, st>>>((const int64_t*)ids, ka, va, kb, vb, (uint32_t)tokens,
+      embed_sort_kernel<int64_t><<<grid, kSortThreads, 0, st>>>((const int64_t*)ids, la, lb, (uint32_t)tokens,
                                                                 (uint32_t)vocab, padding_idx, passes, bits,
                                                                 (char*)grad_weight, gw_bytes);
     else
-      embed_sort_kernel<int32_t><<<grid, kSortThreads, 0, st>>>((const int32_t*)ids, ka, va, kb, vb, (uint32_t)tokens,
+      embed_sort_kernel<int32_t><<<grid, kSortThreads, 0, st>>>((const int32_t*)ids, la, lb, (uint32_t)tokens,
                                                                 (uint32_t)vocab, padding_idx, passes, bits,
                                                                 (char*)grad_weight, gw_bytes);
     rc = check_launch("stream_embedding_sort");
     if (rc) return rc;
   }
-  const uint32_t* keys = (passes & 1) ? kb : ka;
-  const uint32_t* vals = (passes & 1) ? vb : va;
-  // 16-byte loads of g, and stores of gW of 4 or 8 values
-  const bool vec = hidden % (g_bf16 ? 8 : 4) == 0 && aligned16(grad_out);
-#define MHC_SUMS(TG, TW, VV)                                                                                        \
-  (vec ? launch_embed_sums<TG, TW, VV, 1>(keys, vals, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st) \
-       : launch_embed_sums<TG, TW, 1, 4>(keys, vals, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st))
-  return g_bf16 ? (gw_bf16 ? MHC_SUMS(__nv_bfloat16, __nv_bfloat16, 8) : MHC_SUMS(__nv_bfloat16, float, 8))
-                : (gw_bf16 ? MHC_SUMS(float, __nv_bfloat16, 4) : MHC_SUMS(float, float, 4));
+  const uint2* list = (passes & 1) ? lb : la;
+  const bool even = hidden % (g_bf16 ? 8 : 4) == 0 && aligned16(grad_out);
+#define MHC_SUMS(TG, TW)                                                                                            \
+  (even ? launch_embed_sums<TG, TW, true>(list, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st)   \
+        : launch_embed_sums<TG, TW, false>(list, grad_out, grad_weight, ends, tokens, n, hidden, vocab, sc, pl, st))
+  return g_bf16 ? (gw_bf16 ? MHC_SUMS(__nv_bfloat16, __nv_bfloat16) : MHC_SUMS(__nv_bfloat16, float))
+                : (gw_bf16 ? MHC_SUMS(float, __nv_bfloat16) : MHC_SUMS(float, float));
 #undef MHC_SUMS
 }
