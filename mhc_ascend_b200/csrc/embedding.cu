@@ -83,35 +83,46 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// gradient, launch 1: the sort, and the zeros of the dense gradient.
-//
-// The first 8 blocks are one cluster that sorts (key, t) by radix digits of up
-// to 9 bits, least significant first; block c owns the c-th eighth of the
-// positions.  Per digit: a histogram of the block's range in shared memory;
-// the exclusive sums over digits and blocks from the others' histograms
-// through distributed shared memory; then tiles of 4096 positions are ranked
-// (per warp by ballots, across warps by a column sum) and scattered.  The
-// lists stay in L2.  Padding and invalid ids get the key V and sort last.
-// All other blocks write zeros over gW meanwhile: the sort costs a few
-// microseconds a digit on 8 SMs, and hides behind V C stores.
+// gradient, launch 1: the sort.  16 blocks, one cluster, sort (key, t) by radix
+// digits of up to 9 bits, least significant first; block c owns the c-th sixteenth
+// of the positions.  Per digit: a histogram of the block's range in shared memory;
+// the exclusive sums over digits and blocks from the others' histograms through
+// distributed shared memory; then tiles of 4096 positions are ranked (per warp by
+// ballots, across warps by a column sum) and scattered.  The lists stay in L2.
+// Padding and invalid ids get the key V and sort last.  (Clusters of 8: 103 us at
+// 100003 tokens against 63; ranking by match instructions in place of ballots:
+// 15% slower.)
+// launch 2, at the same time: zeros over gW, which is most of what is written.  It
+// may start as soon as the sort has (programmatic launch) and ends after it, so
+// that what follows finds both done.  In one kernel with the sort, whose
+// registers and clusters leave a block an SM, 1.07 GB took 197 us, here 143 us
+// (a block for each 16 KB: 8 blocks an SM that walk on took 170).
 // ---------------------------------------------------------------------------
-constexpr int kSortBlocks = 8, kSortThreads = 512, kSortItems = 8, kSortTile = kSortThreads * kSortItems;
+constexpr int kZeroThreads = 256, kZeroUnroll = 4;
+
+__global__ void __launch_bounds__(kZeroThreads)
+    embed_zero_kernel(uint4* __restrict__ zero, uint64_t bytes) {
+  const uint64_t units = bytes / 16, u = (uint64_t)blockIdx.x * (kZeroThreads * kZeroUnroll) + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < kZeroUnroll; ++j)
+    if (u + j * kZeroThreads < units) zero[u + j * kZeroThreads] = make_uint4(0u, 0u, 0u, 0u);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x < (bytes & 15)) reinterpret_cast<char*>(zero)[units * 16 + threadIdx.x] = 0;
+    // One block that waits for the sort keeps the whole launch from ending before
+    // it; were all to wait, the first of them would keep the others out.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  }
+}
+
+constexpr int kSortBlocks = 16, kSortThreads = 512, kSortItems = 8, kSortTile = kSortThreads * kSortItems;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortWarps = kSortThreads / 32;
 
 template <typename I>
 __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThreads)
     embed_sort_kernel(const I* __restrict__ ids, uint2* la, uint2* lb, uint32_t T,
-                      uint32_t vocab, int64_t pad, int passes, int bits, char* zero, uint64_t zero_bytes) {
+                      uint32_t vocab, int64_t pad, int passes, int bits) {
   const int tid = threadIdx.x;
-  if (blockIdx.x >= kSortBlocks) {
-    const uint64_t nb = gridDim.x - kSortBlocks, b = blockIdx.x - kSortBlocks;
-    const uint64_t units = zero_bytes / 16;
-#pragma unroll 4
-    for (uint64_t u = b * kSortThreads + tid; u < units; u += nb * kSortThreads)
-      reinterpret_cast<uint4*>(zero)[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (b == 0 && tid < (int)(zero_bytes & 15)) zero[units * 16 + tid] = 0;
-    return;
-  }
+  asm volatile("griddepcontrol.launch_dependents;");  // the zeros need nothing of this
   __shared__ uint32_t hist[kDigits];                 // this block's counts, read by the whole cluster
   __shared__ uint32_t base[kDigits];                 // next free place of each digit for this block
   __shared__ uint32_t wcnt[kSortWarps][kDigits];     // counts, then places, by warp
@@ -221,14 +232,14 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
 }
 
 // ---------------------------------------------------------------------------
-// gradient, launch 2: sums of the sorted positions, `chunk` of them and a slice of
+// gradient, launch 3: sums of the sorted positions, `chunk` of them and a slice of
 // the columns a block.  Rows whose tokens all lie in the chunk are written; the
 // sums at its two ends, if their rows go on in a neighbour, are kept:
 // ends[chunk][0] for a row that began before the chunk, [1] for one that begins in
 // it and goes on.  Bound by reading g: 8 or 16 loads of a thread are in flight,
 // and blocks that run together read neighbouring slices of the same rows.
 // A thread has 16 bytes of columns.
-// launch 3: for each row that begins in a chunk and goes on, its sums are added
+// launch 4: for each row that begins in a chunk and goes on, its sums are added
 // in chunk order and the row is written.
 // ---------------------------------------------------------------------------
 constexpr int kMaxChunk = 64, kSumThreads = 128, kJoinThreads = 256;
@@ -421,12 +432,12 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
   const uint32_t last = (lo - 1) / chunk, count = last - piece;
   const int64_t c0 = (int64_t)(blockIdx.x - piece * slices) * (kJoinThreads * V);
-  if (count <= 16) {
+  if (count <= 256) {
     const int64_t c = c0 + threadIdx.x * V;
     if (c >= C) return;
     float acc[V];
     load_unit(ends + ((int64_t)piece * 2 + 1) * C + c, acc);
-#pragma unroll 4
+#pragma unroll 16
     for (uint32_t m = piece + 1; m <= last; ++m) {
       float v[V];
       load_unit(ends + (int64_t)m * 2 * C + c, v);
@@ -610,20 +621,34 @@ extern "C" int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, co
   const int passes = (kbits + kDigitBits - 1) / kDigitBits, bits = (kbits + passes - 1) / passes;
   {
     ProfScope p("stream_embedding_sort", st);
-    // clusters of 8 blocks: the first sorts, the others clear, up to two blocks an SM
-    const uint64_t want = (gw_bytes + 16 * kSortThreads * 8 - 1) / (16 * kSortThreads * 8);
-    const uint64_t most = 2 * (uint64_t)num_sms() - kSortBlocks;
-    const unsigned zb = (unsigned)((want < most ? want : most) + kSortBlocks - 1) / kSortBlocks * kSortBlocks;
-    const dim3 grid(kSortBlocks + zb);
-    if (ids_64)
-      embed_sort_kernel<int64_t><<<grid, kSortThreads, 0, st>>>((const int64_t*)ids, la, lb, (uint32_t)tokens,
-                                                                (uint32_t)vocab, padding_idx, passes, bits,
-                                                                (char*)grad_weight, gw_bytes);
-    else
-      embed_sort_kernel<int32_t><<<grid, kSortThreads, 0, st>>>((const int32_t*)ids, la, lb, (uint32_t)tokens,
-                                                                (uint32_t)vocab, padding_idx, passes, bits,
-                                                                (char*)grad_weight, gw_bytes);
+    auto go = [&](auto kern, auto* id) -> int {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return fail(MHC_ERR_CUDA, "stream_embedding_bwd: no clusters of %d blocks", kSortBlocks);
+      kern<<<kSortBlocks, kSortThreads, 0, st>>>(id, la, lb, (uint32_t)tokens, (uint32_t)vocab, padding_idx, passes, bits);
+      return MHC_OK;
+    };
+    rc = ids_64 ? go(embed_sort_kernel<int64_t>, (const int64_t*)ids) : go(embed_sort_kernel<int32_t>, (const int32_t*)ids);
+    if (rc) return rc;
     rc = check_launch("stream_embedding_sort");
+    if (rc) return rc;
+  }
+  {
+    ProfScope p("stream_embedding_zero", st);
+    const uint64_t per = 16ull * kZeroThreads * kZeroUnroll, want = (gw_bytes + per - 1) / per;
+    MHC_REQUIRE(want < (1ull << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: a table of %lld x %lld is too large",
+                (long long)vocab, (long long)hidden);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)want);
+    cfg.blockDim = dim3(kZeroThreads);
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, embed_zero_kernel, (uint4*)grad_weight, (uint64_t)gw_bytes);
+    MHC_REQUIRE(e == cudaSuccess, MHC_ERR_CUDA, "stream_embedding_zero: launch failed: %s", cudaGetErrorString(e));
+    rc = check_launch("stream_embedding_zero");
     if (rc) return rc;
   }
   const uint2* list = (passes & 1) ? lb : la;
