@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(row_threads(UPT, WARP))
                     const uint8_t* __restrict__ exps, const float* __restrict__ w,
                     const float* __restrict__ rms, T* __restrict__ gx, float* __restrict__ part,
                     int64_t rows, int64_t cols, int64_t pitch) {
+  let_next_start();
   __shared__ float red[2][32];
   __shared__ __align__(16) float sm[EVEN && !WARP ? 1 : row_threads(UPT, WARP) * 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(512, 2)
                          const uint8_t* __restrict__ exps, const float* __restrict__ w,
                          const float* __restrict__ rms, T* __restrict__ gx, float* __restrict__ part,
                          int64_t rows, int cols, int pitch, Ring plan) {
+  let_next_start();
   extern __shared__ __align__(128) unsigned char ring_sm[];
   __shared__ uint64_t full[kRingMost];
   __shared__ float red[2][16];
@@ -483,6 +485,7 @@ __global__ void __launch_bounds__(kLongThreads)
                          const uint8_t* __restrict__ exps, const float* __restrict__ w,
                          const float* __restrict__ rms, T* __restrict__ gx, float* __restrict__ part,
                          int64_t rows, int64_t cols, int64_t pitch) {
+  let_next_start();
   extern __shared__ __align__(16) float keep[];  // [8][units]: value j of unit u at j * units + u
   __shared__ float red[2][32];
   __shared__ __align__(16) float sm[EVEN ? 1 : kLongThreads * 8];
@@ -557,6 +560,7 @@ __global__ void __launch_bounds__(kLongThreads)
 __global__ void __launch_bounds__(256)
     norm_gw_kernel(const float* __restrict__ part, float* __restrict__ gw, int blocks, int64_t cols) {
   __shared__ float s[8][32];
+  wait_for_previous();
   const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float t = 0.f;
@@ -730,7 +734,7 @@ int launch_norm_bwd(const T* g, const int8_t* codes, const uint8_t* exps, const 
     if (rc) return rc;
   }
   ProfScope p("rmsnorm_checkpoint8_gw", st);
-  norm_gw_kernel<<<(unsigned)((cols + 31) / 32), 256, 0, st>>>(part, gw, blocks, cols);
+  launch_early(norm_gw_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st, part, gw, blocks, cols);
   return check_launch("rmsnorm_checkpoint8_gw");
 }
 

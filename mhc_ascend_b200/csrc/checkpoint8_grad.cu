@@ -259,6 +259,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_barrier();
   fence_after();
   const uint32_t tmem = *tslot;
+  let_next_start();
+  wait_for_previous();
 
   if (warp < kOutWarp) {
     fewer_regs<kRegsFew>();
@@ -504,6 +506,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 template <typename TW>
 __global__ void __launch_bounds__(256)
     wgrad_join_kernel(const WgArgs a) {
+  wait_for_previous();
   const Unit q = unit_of(a, a.full + (int)(blockIdx.x / (kTileO / 4)) * a.splits);
   const int rr = (blockIdx.x % (kTileO / 4)) * 4 + (threadIdx.x >> 6), c = (threadIdx.x & 63) * 4;
   const int64_t o = (int64_t)q.tile_o * kTileO + rr, k = (int64_t)q.tile_k * kTileK + c;
@@ -528,6 +531,7 @@ template <typename TG>
 __global__ void __launch_bounds__(256)
     wgrad_planes_kernel(const TG* __restrict__ g, int64_t stride, __nv_bfloat16* __restrict__ out, int64_t T, int64_t O,
                         int64_t width) {
+  let_next_start();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < T * width; i += (int64_t)gridDim.x * 256) {
     const int64_t t = i / width, o = i - t * width;
     if constexpr (sizeof(TG) == 2) {
@@ -576,21 +580,24 @@ WgPlan wg_plan(int64_t T, int64_t O, int64_t K) {
 }
 
 template <int PLANES, typename TW>
-int launch_wgrad(const CUtensorMap& map, const CUtensorMap& codes, const WgArgs& a, const WgPlan& pl, cudaStream_t st) {
+int launch_wgrad(const CUtensorMap& map, const CUtensorMap& codes, const WgArgs& a, const WgPlan& pl, bool after_planes,
+                 cudaStream_t st) {
   auto kern = wgrad_kernel<PLANES, TW>;
   constexpr uint32_t smem = WgCfg<PLANES>::SMEM;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return fail(MHC_ERR_CUDA, "checkpoint8_weight_grad: cannot reserve %u bytes of shared memory", smem);
   {
     ProfScope p("checkpoint8_weight_grad", st);
-    kern<<<2 * pl.pairs, kThreads, smem, st>>>(map, codes, a);
+    const dim3 grid(2 * pl.pairs);
+    if (after_planes) launch_early(kern, grid, dim3(kThreads), smem, st, map, codes, a);
+    else kern<<<grid, kThreads, smem, st>>>(map, codes, a);
     const int rc = check_launch("checkpoint8_weight_grad");
     if (rc) return rc;
   }
   const int rest = pl.tiles_o * pl.tiles_k - pl.full;
   if (rest == 0) return MHC_OK;
   ProfScope p("checkpoint8_weight_join", st);
-  wgrad_join_kernel<TW><<<(unsigned)rest * (kTileO / 4), 256, 0, st>>>(a);
+  launch_early(wgrad_join_kernel<TW>, dim3((unsigned)rest * (kTileO / 4)), dim3(256), 0, st, a);
   return check_launch("checkpoint8_weight_join");
 }
 
@@ -681,6 +688,6 @@ extern "C" int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16,
   a.T = tokens; a.O = out_features; a.K = in_features; a.pitch = ck_pitch(in_features);
   a.tiles_o = pl.tiles_o; a.tiles_k = pl.tiles_k; a.full = pl.full; a.splits = pl.splits; a.units = pl.units;
   if (g_bf16)
-    return gw_bf16 ? launch_wgrad<1, __nv_bfloat16>(map, cmap, a, pl, st) : launch_wgrad<1, float>(map, cmap, a, pl, st);
-  return gw_bf16 ? launch_wgrad<3, __nv_bfloat16>(map, cmap, a, pl, st) : launch_wgrad<3, float>(map, cmap, a, pl, st);
+    return gw_bf16 ? launch_wgrad<1, __nv_bfloat16>(map, cmap, a, pl, copy, st) : launch_wgrad<1, float>(map, cmap, a, pl, copy, st);
+  return gw_bf16 ? launch_wgrad<3, __nv_bfloat16>(map, cmap, a, pl, copy, st) : launch_wgrad<3, float>(map, cmap, a, pl, copy, st);
 }

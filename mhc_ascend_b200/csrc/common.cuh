@@ -76,6 +76,25 @@ int wgrad_device_error(int* value, bool reset);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Launch that may start once every block of the launch before it in the stream
+// has called let_next_start() or ended (programmatic stream serialization); the
+// kernel calls wait_for_previous() before it touches anything that launch wrote
+// or still reads.
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
 #define MHC_REQUIRE(cond, code, ...)          \
   do {                                        \
     if (!(cond)) return ::mhc::fail((code), __VA_ARGS__); \
@@ -100,6 +119,9 @@ inline int num_sms() {
 // ---------------------------------------------------------------------------
 // Device helpers
 // ---------------------------------------------------------------------------
+
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -102,6 +102,7 @@ constexpr int kZeroThreads = 256, kZeroUnroll = 4;
 
 __global__ void __launch_bounds__(kZeroThreads)
     embed_zero_kernel(uint4* __restrict__ zero, uint64_t bytes) {
+  let_next_start();
   const uint64_t units = bytes / 16, u = (uint64_t)blockIdx.x * (kZeroThreads * kZeroUnroll) + threadIdx.x;
 #pragma unroll
   for (int j = 0; j < kZeroUnroll; ++j)
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(kZeroThreads)
     if (threadIdx.x < (bytes & 15)) reinterpret_cast<char*>(zero)[units * 16 + threadIdx.x] = 0;
     // One block that waits for the sort keeps the whole launch from ending before
     // it; were all to wait, the first of them would keep the others out.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_previous();
   }
 }
 
@@ -122,7 +123,7 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
     embed_sort_kernel(const I* __restrict__ ids, uint2* la, uint2* lb, uint32_t T,
                       uint32_t vocab, int64_t pad, int passes, int bits) {
   const int tid = threadIdx.x;
-  asm volatile("griddepcontrol.launch_dependents;");  // the zeros need nothing of this
+  let_next_start();  // the zeros need nothing of this
   __shared__ uint32_t hist[kDigits];                 // this block's counts, read by the whole cluster
   __shared__ uint32_t base[kDigits];                 // next free place of each digit for this block
   __shared__ uint32_t wcnt[kSortWarps][kDigits];     // counts, then places, by warp
@@ -284,6 +285,8 @@ __global__ void __launch_bounds__(kSumThreads)
   constexpr int L = EVEN ? 8 : 4;  // rows of g in flight
   constexpr bool SINGLE = !EVEN && sizeof(TG) == 4;
   const int width = blockDim.x;
+  let_next_start();
+  wait_for_previous();
   __shared__ uint32_t sk[kMaxChunk + 2], sv[kMaxChunk];
   __shared__ float ss[kMaxStreams];
   __shared__ float sums[EVEN || SINGLE ? 1 : kSumThreads * V];
@@ -418,6 +421,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     embed_join_kernel(const uint2* __restrict__ list, TW* __restrict__ gw, const float* __restrict__ ends,
                       uint32_t T, uint32_t vocab, int64_t C, int chunk, uint32_t slices) {
   __shared__ __align__(16) float part[8][32 * V];
+  wait_for_previous();
   const uint32_t piece = blockIdx.x / slices;
   const uint32_t p1 = (piece + 1) * chunk;  // first position of the next chunk (exists: the grid is one short)
   const uint32_t p0 = p1 - chunk;
@@ -544,8 +548,8 @@ int launch_embed_sums(const uint2* list, const void* g, void* gw, float* ends, i
     MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: %lld tokens of %lld are too many",
                 (long long)T, (long long)C);
     ProfScope p("stream_embedding_sum", st);
-    embed_sum_kernel<TG, TW, EVEN><<<(unsigned)blocks, (unsigned)threads, 0, st>>>(
-        list, (const TG*)g, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, n, C, sc, pl.chunk, (uint32_t)slices);
+    launch_early(embed_sum_kernel<TG, TW, EVEN>, dim3((unsigned)blocks), dim3((unsigned)threads), 0, st, list, (const TG*)g,
+                 (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab, n, C, sc, pl.chunk, (uint32_t)slices);
     const int rc = check_launch("stream_embedding_sum");
     if (rc) return rc;
   }
@@ -555,8 +559,8 @@ int launch_embed_sums(const uint2* list, const void* g, void* gw, float* ends, i
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: %lld tokens of %lld are too many",
               (long long)T, (long long)C);
   ProfScope p("stream_embedding_join", st);
-  embed_join_kernel<TW, W><<<(unsigned)blocks, kJoinThreads, 0, st>>>(list, (TW*)gw, ends, (uint32_t)T, (uint32_t)vocab,
-                                                                      C, pl.chunk, (uint32_t)slices);
+  launch_early(embed_join_kernel<TW, W>, dim3((unsigned)blocks), dim3(kJoinThreads), 0, st, list, (TW*)gw, ends, (uint32_t)T,
+               (uint32_t)vocab, C, pl.chunk, (uint32_t)slices);
   return check_launch("stream_embedding_join");
 }
 
@@ -637,16 +641,8 @@ extern "C" int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, co
     const uint64_t per = 16ull * kZeroThreads * kZeroUnroll, want = (gw_bytes + per - 1) / per;
     MHC_REQUIRE(want < (1ull << 31), MHC_ERR_UNSUPPORTED, "stream_embedding_bwd: a table of %lld x %lld is too large",
                 (long long)vocab, (long long)hidden);
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)want);
-    cfg.blockDim = dim3(kZeroThreads);
-    cfg.stream = st;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, embed_zero_kernel, (uint4*)grad_weight, (uint64_t)gw_bytes);
+    const cudaError_t e = launch_early(embed_zero_kernel, dim3((unsigned)want), dim3(kZeroThreads), 0, st,
+                                       (uint4*)grad_weight, (uint64_t)gw_bytes);
     MHC_REQUIRE(e == cudaSuccess, MHC_ERR_CUDA, "stream_embedding_zero: launch failed: %s", cudaGetErrorString(e));
     rc = check_launch("stream_embedding_zero");
     if (rc) return rc;
