@@ -15,15 +15,77 @@ namespace {
 constexpr int kPackThreads = 256, kUnroll = 4;
 
 // Row and column of a lane's unit in a list of units, U (EVEN) or 32 * spans a row
+// (64-bit divisions are a third of such a kernel's instructions: they are done in
+// 32 bits, or not at all, wherever the numbers allow)
 struct Walk {
-  int64_t row, u;
-  __device__ __forceinline__ Walk(int64_t i, int64_t U) : row(i / U), u(i % U) {}
-  __device__ __forceinline__ void step(int64_t drow, int64_t du, int64_t U) {
+  int64_t row, u, drow, du;
+  __device__ __forceinline__ Walk(int64_t i, int64_t U) : row(0), u(i), drow(0), du(kPackThreads) {
+    if (i >= U) {
+      if ((uint64_t)i >> 32) {
+        row = i / U;
+        u = i - row * U;
+      } else {
+        row = (uint32_t)i / (uint32_t)U;
+        u = (uint32_t)i % (uint32_t)U;
+      }
+    }
+    if (U <= kPackThreads) {
+      drow = kPackThreads / (int)U;
+      du = kPackThreads % (int)U;
+    }
+  }
+  __device__ __forceinline__ void step(int64_t U) {
     row += drow;
     u += du;
     if (u >= U) { u -= U; ++row; }
   }
 };
+
+// Rows without gaps and without padding: one list of units, and no index arithmetic
+// (which is what bounds the general kernels in bf16: [8192, 8192] 52 us against 33).
+template <typename T>
+__global__ void __launch_bounds__(kPackThreads)
+    pack_flat_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, uint8_t* __restrict__ exps, int64_t units) {
+  const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
+  x += 8 * first;
+  codes += 8 * first;
+  exps += first >> 2;
+  const int left = (int)min((units - first + kPackThreads - 1) / kPackThreads, (int64_t)kUnroll);
+  float v[kUnroll][8];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+    if (k < left) ck_load(x + 8 * kPackThreads * k, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) ck_encode(v[k], codes, exps, 8 * kPackThreads * k, k < left);
+}
+template <typename T>
+__global__ void __launch_bounds__(kPackThreads)
+    unpack_flat_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps, T* __restrict__ out,
+                       int64_t units) {
+  const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
+  codes += 8 * first;
+  exps += first >> 2;
+  out += 8 * first;
+  const int left = (int)min((units - first + kPackThreads - 1) / kPackThreads, (int64_t)kUnroll);
+  uint2 w[kUnroll];
+  uint32_t E[kUnroll];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k)
+    if (k < left) {
+      w[k] = *reinterpret_cast<const uint2*>(codes + 8 * kPackThreads * k);
+      E[k] = exps[kPackThreads / 4 * k];
+    }
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k)
+    if (k < left) {
+      float v[8];
+      ck_decode(w[k], E[k], v);
+      ck_save(out + 8 * kPackThreads * k, v);
+    }
+}
 
 template <typename T, bool EVEN>
 __global__ void __launch_bounds__(kPackThreads)
@@ -32,7 +94,6 @@ __global__ void __launch_bounds__(kPackThreads)
   __shared__ __align__(16) float sm[EVEN ? 1 : kPackThreads * 8];
   float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
   const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
-  const int64_t drow = kPackThreads / U, du = kPackThreads % U;
   Walk at(first, U);
   float v[kUnroll][8];
   int64_t row[kUnroll], col[kUnroll];
@@ -47,7 +108,7 @@ __global__ void __launch_bounds__(kPackThreads)
     } else {  // U % 32 == 0: the warp is in one row
       ck_load_any(x + at.row * stride, col[k] - 8 * (threadIdx.x & 31), at.row < rows ? cols : 0, mine, v[k]);
     }
-    at.step(drow, du, U);
+    at.step(U);
   }
 #pragma unroll
   for (int k = 0; k < kUnroll; ++k)
@@ -61,7 +122,6 @@ __global__ void __launch_bounds__(kPackThreads)
   __shared__ __align__(16) float sm[EVEN ? 1 : kPackThreads * 8];
   float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
   const int64_t first = (int64_t)blockIdx.x * (kPackThreads * kUnroll) + threadIdx.x;
-  const int64_t drow = kPackThreads / U, du = kPackThreads % U;
   Walk at(first, U);
   uint2 w[kUnroll];
   uint32_t E[kUnroll];
@@ -76,7 +136,7 @@ __global__ void __launch_bounds__(kPackThreads)
       w[k] = *reinterpret_cast<const uint2*>(codes + at.row * pitch + col[k]);
       E[k] = exps[(at.row * pitch + col[k]) / kCkBlock];
     }
-    at.step(drow, du, U);
+    at.step(U);
   }
 #pragma unroll
   for (int k = 0; k < kUnroll; ++k) {
@@ -326,8 +386,8 @@ __global__ void __launch_bounds__(row_threads(UPT, WARP), EVEN || WARP || UPT !=
 // row i also says that everyone is done with row i - 1: thread 0 then refills its
 // place.  What bounds it is instructions (two expansions a value), hence two-wide
 // fp32 arithmetic and the weights in shared memory.
-// Measured at [16384, 7168] bf16: 142 us, 4.2 TB/s (one row ahead in registers, a
-// block an SM: 203 us); [8192, 4096] bf16: 48 us.
+// Measured at [16384, 7168] bf16: 133 us, 4.5 TB/s (one row ahead in registers, a
+// block an SM: 203 us); [8192, 4096] bf16: 46 us.
 // ---------------------------------------------------------------------------
 constexpr int kRingMost = 8, kRingUPT = 2;
 
@@ -621,7 +681,9 @@ int launch_pack(const T* x, int64_t stride, int8_t* codes, uint8_t* exps, int64_
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "checkpoint8_pack: %lld x %lld values are too many",
               (long long)rows, (long long)cols);
   ProfScope p("checkpoint8_pack", st);
-  if (even) pack_kernel<T, true><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, pitch, U);
+  if (even && stride == cols && cols == pitch)
+    pack_flat_kernel<T><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, codes, exps, rows * U);
+  else if (even) pack_kernel<T, true><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, pitch, U);
   else pack_kernel<T, false><<<(unsigned)blocks, kPackThreads, 0, st>>>(x, stride, codes, exps, rows, cols, pitch, U);
   return check_launch("checkpoint8_pack");
 }
@@ -633,7 +695,9 @@ int launch_unpack(const int8_t* codes, const uint8_t* exps, T* out, int64_t rows
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "checkpoint8_unpack: %lld x %lld values are too many",
               (long long)rows, (long long)cols);
   ProfScope p("checkpoint8_unpack", st);
-  if (even) unpack_kernel<T, true><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, pitch, U);
+  if (even && cols == pitch)
+    unpack_flat_kernel<T><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows * U);
+  else if (even) unpack_kernel<T, true><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, pitch, U);
   else unpack_kernel<T, false><<<(unsigned)blocks, kPackThreads, 0, st>>>(codes, exps, out, rows, cols, pitch, U);
   return check_launch("checkpoint8_unpack");
 }

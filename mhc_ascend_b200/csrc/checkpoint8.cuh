@@ -57,26 +57,18 @@ __device__ __forceinline__ uint32_t ck_pack4(uint32_t a, uint32_t b, uint32_t c,
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 // Four codes -> four values.  The byte with its sign flipped, set into the low
-// byte of 2^23, is f = 2^23 + 128 + code, and f * step - (2^23 + 128) * step in one
-// fma is code * step, exactly (8 significant bits).  From E = 227 on the second
-// product leaves fp32, and the two steps are taken one by one.
-__device__ __forceinline__ void ck_expand4(uint32_t codes, float step, float minus, bool big, float* v) {
+// byte of 2^23, is 2^23 + 128 + code; the subtraction and the product with the
+// step are exact (8 significant bits).
+__device__ __forceinline__ void ck_expand4(uint32_t codes, float2 step, float* v) {
   const uint32_t u = codes ^ 0x80808080u;
-  float2 f[2];
-  f[0].x = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440));
-  f[0].y = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441));
-  f[1].x = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442));
-  f[1].y = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443));
+  const float2 minus = make_float2(-8388736.0f, -8388736.0f);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    if (big) {
-      f[j].x = (f[j].x - 8388736.0f) * step;
-      f[j].y = (f[j].y - 8388736.0f) * step;
-    } else {
-      f[j] = __ffma2_rn(f[j], make_float2(step, step), make_float2(minus, minus));
-    }
-    v[2 * j] = f[j].x;
-    v[2 * j + 1] = f[j].y;
+    float2 f = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + 2 * j)),
+                           __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + 2 * j)));
+    f = __fmul2_rn(__fadd2_rn(f, minus), step);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
   }
 }
 
@@ -176,9 +168,9 @@ __device__ __forceinline__ void ck_encode(float (&v)[8], int8_t* codes, uint8_t*
 
 // The values of 8 codes.
 __device__ __forceinline__ void ck_decode(uint2 w, uint32_t E, float (&v)[8]) {
-  const float step = ck_step(E), minus = -8388736.0f * step;
-  ck_expand4(w.x, step, minus, E >= 227u, v);
-  ck_expand4(w.y, step, minus, E >= 227u, v + 4);
+  const float2 step = make_float2(ck_step(E), ck_step(E));
+  ck_expand4(w.x, step, v);
+  ck_expand4(w.y, step, v + 4);
 }
 
 }  // namespace mhc
