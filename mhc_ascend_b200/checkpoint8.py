@@ -243,8 +243,13 @@ class LinearCheckpoint8Function(torch.autograd.Function):
 
 def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``torch.nn.functional.linear`` (x, weight and bias of one type, float32 or
-    bfloat16) that keeps x in 8 bits for the weight's gradient."""
+    bfloat16) that keeps x in 8 bits for the weight's gradient.  Under autocast
+    the three are cast to its type first, as for the plain layer."""
     _require_cuda("linear_checkpoint8", x, weight)
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        with torch.autocast("cuda", enabled=False):
+            return linear_checkpoint8(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype))
     _check_float("linear_checkpoint8", "x", x)
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise RuntimeError("linear_checkpoint8: x, weight and bias must have one type")
@@ -264,6 +269,7 @@ class Checkpoint8Function(torch.autograd.Function):
         packed = [checkpoint8_pack(t) for t in tensors[:kept]]
         ctx.save_for_backward(*[p for c in packed for p in (c.codes, c.exponents)], *tensors[kept:])
         ctx.function, ctx.kept = function, [(c.shape, c.dtype) for c in packed]
+        ctx.autocast = dict(enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"))
         return function(*tensors)
 
     @staticmethod
@@ -274,7 +280,7 @@ class Checkpoint8Function(torch.autograd.Function):
         tensors += [t.detach() for t in saved[2 * k:]]
         for t, n in zip(tensors, need):
             t.requires_grad_(n)
-        with torch.enable_grad():
+        with torch.enable_grad(), torch.autocast("cuda", **ctx.autocast):
             out = ctx.function(*tensors)
         outs = out if isinstance(out, tuple) else (out,)
         pairs = [(o, g) for o, g in zip(outs, grad_out) if g is not None and o.requires_grad]
@@ -291,6 +297,6 @@ def checkpoint8_recompute(function, *tensors: torch.Tensor, kept: int = 1):
     random numbers, and what it differentiates by has to be among ``tensors``."""
     if not 1 <= kept <= len(tensors):
         raise RuntimeError(f"checkpoint8_recompute: kept must be in [1, {len(tensors)}] (got {kept})")
-    if not torch.is_grad_enabled():
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
         return function(*tensors)
     return Checkpoint8Function.apply(function, kept, *tensors)

@@ -406,8 +406,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           c[h][j] = *reinterpret_cast<const uint4*>(ring + from + sc * (kOpBytes / 2) + h * 4096 + (((2 * blk + j) ^ (tok & 7)) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&cempty[sc]);
       ok = it < S || wait_bar(&empty[s], (uint32_t)((it / S - 1) & 1), stop);
       if (!__all_sync(0xffffffffu, ok)) return false;
       unsigned char* dst = ring + s * Cfg::STAGE + row;
@@ -430,7 +428,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) arrive_leader(&full[s]);
+      if (lane == 0) {
+        arrive_leader(&full[s]);
+        // Only now have all lanes used their codes.  Released straight after the
+        // loads were issued, the stage was refilled under some of them.
+        mbar_arrive(&cempty[sc]);
+      }
       fetch(ex);
       return true;
     };

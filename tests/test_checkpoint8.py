@@ -328,6 +328,21 @@ def test_weight_grad_of_many_tokens(cuda, tg):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tg,tw,T,O,K", [(BF16, F32, 8192, 4096, 4096), (BF16, BF16, 16384, 4096, 2048),
+                                         (F32, F32, 4096, 2048, 4096)])
+def test_weight_grad_on_a_full_gpu(cuda, tg, tw, T, O, K):
+    """Every SM at work, call after call: each stage's hand-overs between the
+    copies, the expanding warps and the MMAs have to hold under contention."""
+    x = torch.randn(T, K, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1))
+    g = torch.randn(T, O, device=cuda, generator=torch.Generator(device=cuda).manual_seed(2)).to(tg)
+    kept = mhc.checkpoint8_pack(x)
+    first = mhc.checkpoint8_weight_grad(g, kept, dtype=tw)
+    _wgrad_check(first, g, kept.unpack().double(), tw == BF16)
+    for _ in range(40):
+        assert torch.equal(mhc.checkpoint8_weight_grad(g, kept, dtype=tw), first)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tg", [BF16, F32])
 def test_weight_grad_layouts(cuda, tg):
     x, wide = acts(150, 72, seed=1), acts(150, 400, seed=2, dtype=tg).to(cuda)
@@ -468,3 +483,28 @@ def test_recompute_of_any_function(cuda):
     assert torch.equal(x.grad, xh.grad) and torch.equal(w.grad, wh.grad)
     with torch.no_grad():
         assert torch.equal(mhc.checkpoint8_recompute(f, x, w, s)[0], ra)
+
+
+@pytest.mark.gpu
+def test_autocast(cuda):
+    """The linear layer casts as torch's does, and what runs again runs under the
+    forward's autocast."""
+    x, w = acts(30, 64, seed=1).to(cuda).requires_grad_(True), acts(24, 64, seed=2).to(cuda).requires_grad_(True)
+    with torch.autocast("cuda", dtype=BF16):
+        out = mhc.linear_checkpoint8(x, w)
+        assert out.dtype == BF16 and torch.equal(out, torch.nn.functional.linear(x, w))
+        again = mhc.checkpoint8_recompute(torch.nn.functional.linear, x, w)
+    g = acts(30, 24, seed=3, dtype=BF16).to(cuda)
+    out.backward(g)
+    assert x.grad.dtype == F32 and w.grad.dtype == F32
+    _wgrad_check(w.grad, g.cpu(), restored64(x.detach().to(BF16)), True)
+    w.grad = None
+    again.backward(g)  # outside of autocast
+    xh = mhc.checkpoint8_pack(x).unpack()
+    _wgrad_check(w.grad, g.cpu(), xh.double().cpu(), True)
+
+
+@pytest.mark.gpu
+def test_recompute_without_gradients_keeps_nothing(cuda):
+    x = acts(9, 40, seed=1).to(cuda)
+    assert mhc.checkpoint8_recompute(torch.tanh, x).grad_fn is None
