@@ -46,6 +46,11 @@ struct WgCfg {
   static constexpr uint32_t STAGE = (PLANES + 1) * kOpBytes;  // A planes, then B
   static constexpr int STAGES = PLANES == 1 ? 5 : 2;
   static constexpr int CODES = PLANES == 1 ? 4 : 8;           // stages of codes: 64 tokens x 128 bytes each
+  // Parities tell a phase from the next only.  A group that has stored stage i knows
+  // that the MMAs of stage i - STAGES are done, so before it waits for those of
+  // i + 2 - STAGES no earlier phase of that barrier is open; and it meets a stage
+  // of codes again itself.
+  static_assert(STAGES >= 2 && CODES % 2 == 0, "two groups");
   static constexpr int CHAIN = PLANES == 1 ? 16 : 5;          // stages summed in tensor memory: 64 / 60 MMAs
   static constexpr uint32_t OFF_CODES = STAGES * STAGE;
   static constexpr uint32_t OFF_OUT = OFF_CODES + CODES * kOpBytes / 2;  // 4 KB a warp that writes: 32 x 32 values on their way out
