@@ -86,7 +86,15 @@ def _rows2d(t):
     cols = t.size(-1)
     if t.dim() == 2 and (t.stride(1) == 1 or cols == 1) and t.stride(0) >= cols:
         return t, t.stride(0)
-    return t.reshape(-1, cols).contiguous(), cols
+    return t.detach().reshape(-1, cols).contiguous(), cols
+
+
+def _dense(t):
+    return t if t.is_contiguous() else t.detach().contiguous()
+
+
+def _weight(t):
+    return t if t.dtype == torch.float32 and t.is_contiguous() else _f32(t)
 
 
 def _check_float(what, name, t):
@@ -101,7 +109,7 @@ def checkpoint8_pack(x: torch.Tensor) -> Checkpoint8:
     _check_float(what, "x", x)
     if x.dim() == 0 or x.size(-1) == 0:
         raise RuntimeError(f"{what}: x must have a last dimension of at least 1")
-    x2, stride = _rows2d(x.detach())
+    x2, stride = _rows2d(x)
     kept = _empty(x.shape, x.dtype, x.device)
     _launch("mhc_checkpoint8_pack", x.device, x2.data_ptr(), x.dtype == torch.bfloat16, stride,
             kept.codes.data_ptr(), kept.exponents.data_ptr(), x2.size(0), x2.size(1))
@@ -134,9 +142,9 @@ def rmsnorm_checkpoint8_fwd(inp: torch.Tensor, weight: torch.Tensor, eps: float 
         raise RuntimeError(f"{what}: inp must have a last dimension of at least 1")
     if weight.dim() != 1 or weight.size(0) != inp.size(-1):
         raise RuntimeError("Weight must be 1D with size equal to hidden_dim")
-    x, w = inp.detach().contiguous(), _f32(weight)
+    x, w = _dense(inp), _weight(weight)
     kept = _empty(x.shape, x.dtype, x.device)
-    out = torch.empty_like(x)
+    out = torch.empty_like(x, requires_grad=False)
     rows = kept.rows
     rms = torch.empty(rows, dtype=torch.float32, device=x.device)
     _launch("mhc_rmsnorm_checkpoint8_fwd", x.device, x.data_ptr(), x.dtype == torch.bfloat16, w.data_ptr(),
@@ -155,7 +163,7 @@ def rmsnorm_checkpoint8_bwd(grad_out: torch.Tensor, kept: Checkpoint8, weight: t
     rows, cols = kept.rows, kept.cols
     if weight.shape != (cols,) or rms.numel() != rows:
         raise RuntimeError(f"{what}: weight must be [{cols}] and rms [{rows}]")
-    g, w, r = grad_out.detach().contiguous(), _f32(weight), _f32(rms)
+    g, w, r = _dense(grad_out), _weight(weight), _weight(rms)
     gx = torch.empty_like(g)
     gw = torch.empty(cols, dtype=torch.float32, device=g.device)
     ws = _workspace(_lib.mhc_rmsnorm_checkpoint8_bwd_workspace_bytes(rows, cols), g.device)
@@ -206,7 +214,7 @@ def checkpoint8_weight_grad(grad_out: torch.Tensor, kept: Checkpoint8,
     if grad_out.dim() < 1 or grad_out.shape[:-1] != kept.shape[:-1] or grad_out.size(-1) == 0:
         raise RuntimeError(f"{what}: grad_out must be {tuple(kept.shape[:-1])} + [out_features] "
                            f"(got {tuple(grad_out.shape)})")
-    g, stride = _rows2d(grad_out.detach())
+    g, stride = _rows2d(grad_out)
     T, O, K = kept.rows, g.size(1), kept.cols
     gw = torch.empty(O, K, dtype=dtype, device=g.device)
     g16, w16 = g.dtype == torch.bfloat16, dtype == torch.bfloat16

@@ -83,7 +83,8 @@ def stream_embedding_bwd(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddin
     V = int(num_embeddings)
     pad = _padding(padding_idx, V)
     sc = _scales(scale, n)
-    idc, g = _check_ids(what, ids), grad_out.detach().contiguous()
+    idc = _check_ids(what, ids)
+    g = grad_out if grad_out.is_contiguous() else grad_out.detach().contiguous()
     gw = torch.empty(V, C, dtype=dtype, device=g.device)
     T = idc.numel()
     ws = _workspace(_lib.mhc_stream_embedding_bwd_workspace_bytes(T, C), g.device)
