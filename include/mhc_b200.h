@@ -403,9 +403,11 @@ MHC_API int mhc_rmsnorm_checkpoint8_bwd(const void* grad_out, int32_t g_bf16, co
  *   grad_weight[o, k] = sum_t grad_out[t, o] xh[t, k]        [out_features, in_features]
  * grad_out [tokens, out_features] fp32 or bf16, rows row_stride elements apart;
  * grad_weight fp32 or bf16, contiguous.  fp32 grad_out is used in full
- * precision; sums are fp32 and in a fixed order. */
+ * precision; sums are fp32 and in a fixed order.  The workspace is smaller for a
+ * bf16 grad_out whose start is 16-byte aligned and whose row_stride is a multiple
+ * of 8 (g_aligned): any other is copied there first. */
 MHC_API size_t mhc_checkpoint8_weight_grad_workspace_bytes(int64_t tokens, int64_t out_features,
-                                                   int64_t in_features, int32_t g_bf16, int32_t gw_bf16);
+                                                   int64_t in_features, int32_t g_bf16, int32_t g_aligned);
 MHC_API int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16, int64_t row_stride,
                                 const int8_t* codes, const uint8_t* exponents, void* grad_weight,
                                 int32_t gw_bf16, int64_t tokens, int64_t out_features,

@@ -218,7 +218,8 @@ def checkpoint8_weight_grad(grad_out: torch.Tensor, kept: Checkpoint8,
     T, O, K = kept.rows, g.size(1), kept.cols
     gw = torch.empty(O, K, dtype=dtype, device=g.device)
     g16, w16 = g.dtype == torch.bfloat16, dtype == torch.bfloat16
-    ws = _workspace(_lib.mhc_checkpoint8_weight_grad_workspace_bytes(T, O, K, g16, w16), g.device)
+    aligned = g16 and stride % 8 == 0 and g.data_ptr() % 16 == 0
+    ws = _workspace(_lib.mhc_checkpoint8_weight_grad_workspace_bytes(T, O, K, g16, aligned), g.device)
     _launch("mhc_checkpoint8_weight_grad", g.device, g.data_ptr(), g16, stride, kept.codes.data_ptr(),
             kept.exponents.data_ptr(), gw.data_ptr(), w16, T, O, K, ws.data_ptr(), ws.numel())
     return gw

@@ -622,12 +622,11 @@ int wgrad_device_error(int* value, bool reset) {
 
 using namespace mhc;
 
-// Sized for rows that need a copy of g, whatever their layout turns out to be.
 extern "C" size_t mhc_checkpoint8_weight_grad_workspace_bytes(int64_t tokens, int64_t out_features,
-                                                              int64_t in_features, int32_t g_bf16, int32_t) {
+                                                              int64_t in_features, int32_t g_bf16, int32_t g_aligned) {
   if (tokens < 1 || out_features < 1 || in_features < 1) return 0;
   const WgPlan p = wg_plan(tokens, out_features, in_features);
-  const size_t planes = (size_t)tokens * p.width * 2 * (g_bf16 ? 1 : 3);
+  const size_t planes = g_bf16 && g_aligned ? 0 : (size_t)tokens * p.width * 2 * (g_bf16 ? 1 : 3);
   return (planes + 255) / 256 * 256 + p.part_bytes;
 }
 
@@ -657,7 +656,7 @@ extern "C" int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16,
   MHC_REQUIRE(aligned16(codes) && (reinterpret_cast<uintptr_t>(exponents) & 3) == 0, MHC_ERR_ALIGNMENT,
               "%s: codes must be 16-byte and exponents 4-byte aligned", what);
   const WgPlan pl = wg_plan(tokens, out_features, in_features);
-  const bool copy = !g_bf16 || !aligned16(grad_out) || (row_stride % 8) != 0 || row_stride >= (1ll << 38);
+  const bool copy = !g_bf16 || !aligned16(grad_out) || (row_stride % 8) != 0;
   const size_t planes = ((size_t)tokens * pl.width * 2 * (g_bf16 ? 1 : 3) + 255) / 256 * 256;
   const size_t need = (copy ? planes : 0) + pl.part_bytes;
   MHC_REQUIRE(need == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= need),

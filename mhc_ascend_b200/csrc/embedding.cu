@@ -245,10 +245,10 @@ __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThrea
 // ---------------------------------------------------------------------------
 constexpr int kMaxChunk = 64, kSumThreads = 128, kJoinThreads = 256;
 
-// 16 bytes from an address of any alignment, as 4 words: of two aligned accesses
-// (the second is mostly an L1 hit: it is the neighbour's first), a shift by words,
-// then by bits.  The accesses of several rows are issued before the first shift
-// waits for one.
+// 16 bytes from an address of any alignment, as 4 words: of two aligned accesses, a
+// shift by words, then by bits.  The second access is the next lane's first and
+// comes from it by shuffles (read again: 166 us against 158 below).  The
+// accesses of several rows are issued before the first shift waits for one.
 __device__ __forceinline__ void shift16(uint32_t sh, const uint4& a, const uint4& b, uint32_t (&o)[4]) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   uint32_t t[6], u[5];
@@ -275,7 +275,9 @@ __device__ __forceinline__ void unit_of_words(const __nv_bfloat16*, const uint32
 // are read by shifts and their sums go through shared memory, so that the stores
 // are coalesced; fp32 rows are read and written one value a lane ([8192, 4, 4095]:
 // 118 us against 162 by shifts, whose registers halve what is in flight; bf16
-// [100003, 2, 1281] 241 us by shifts, 275 one value a lane).
+// [100003, 2, 1281] 152 us by shifts, 268 one value a lane).  What bounds bf16
+// there is latency: a warp's four rows in flight, then their sums, then the next
+// four; six rows, or registers for more blocks, were slower.
 template <typename TG, typename TW, bool EVEN>
 __global__ void __launch_bounds__(kSumThreads)
     embed_sum_kernel(const uint2* __restrict__ list, const TG* __restrict__ g, TW* __restrict__ gw,
@@ -311,6 +313,7 @@ __global__ void __launch_bounds__(kSumThreads)
   // The aligned accesses around a unit stay inside the tensor unless its token is
   // the first or the last one, or rows are shorter than such an access.
   auto edge = [&](uint32_t token) { return token == 0 || token == T - 1 || C < 16; };
+  const bool last = (tid & 31) == 31 || c + V >= C;  // no next lane that loads
   float acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
@@ -334,12 +337,11 @@ __global__ void __launch_bounds__(kSumThreads)
           if (have > 2) v[k].z = word[2 * width];
           if (have > 3) v[k].w = word[3 * width];
         } else {
-          sh[k] = 16;
-          if (have > 0 && !edge(sv[lp])) {
+          sh[k] = edge(sv[lp]) ? 16u : (uint32_t)reinterpret_cast<uintptr_t>(at) & 15u;  // the same in every lane
+          if (have > 0 && sh[k] < 16) {
             const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(at) & ~(uintptr_t)15);
-            sh[k] = (uint32_t)reinterpret_cast<uintptr_t>(at) & 15u;
             v[k] = base[0];
-            w[k] = base[1];
+            if (last) w[k] = base[1];
           }
         }
         at += C;
@@ -357,8 +359,13 @@ __global__ void __launch_bounds__(kSumThreads)
           const uint32_t o[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
           unit_of_words(g, o, u);
         } else if (sh[k] < 16) {
+          uint4 next;
+          next.x = __shfl_down_sync(0xffffffffu, v[k].x, 1);
+          next.y = __shfl_down_sync(0xffffffffu, v[k].y, 1);
+          next.z = __shfl_down_sync(0xffffffffu, v[k].z, 1);
+          next.w = __shfl_down_sync(0xffffffffu, v[k].w, 1);
           uint32_t o[4];
-          shift16(sh[k], v[k], w[k], o);
+          shift16(sh[k], v[k], last ? w[k] : next, o);
           unit_of_words(g, o, u);
         } else {
           const TG* from = g + ((int64_t)sv[p] * n + i) * C + c;

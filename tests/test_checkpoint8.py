@@ -75,6 +75,9 @@ def test_entry_points_validate_without_gpu():
         g, 1, st, c, p, gw, 0, T, O, K, None, 0, None)
     assert wg(T=-1) == -1 and wg(O=0) == -1 and wg(K=0) == -1 and wg(g=None) == -1 and wg(gw=None) == -1
     assert wg(st=7) == -1 and wg(c=odd) == -3 and wg(T=1 << 31) == -2
+    size = lambda *a: lib.mhc_checkpoint8_weight_grad_workspace_bytes(*a)  # noqa: E731
+    assert size(-1, 8, 8, 1, 1) == 0 and size(100, 8, 8, 1, 0) - size(100, 8, 8, 1, 1) >= 1600
+    assert wg(g=ctypes.c_void_p(18)) == -4 and "workspace" in _C.last_error()  # needs a copy
 
 
 # ---------------------------------------------------------------------------
