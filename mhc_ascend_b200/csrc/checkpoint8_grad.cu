@@ -26,6 +26,10 @@
 // the layer's projection), so a chain is kept to 64 MMAs; warps 4..11 add the
 // chains in fp32 registers, 128 a thread, which is why registers are moved
 // between the roles (setmaxnreg).
+//
+// 8192 tokens, 4096 x 4096: 220 us alone, 1.25 PFLOP/s, 76% of what cuBLAS reaches in
+// bf16; the tensor pipe is 67% busy, a stage takes about 980 cycles for 512 of MMAs
+// (the operands' traffic alone is 640 of shared memory; the rest is hand-overs).
 #include "checkpoint8.cuh"
 #include "tma.cuh"
 
