@@ -269,6 +269,14 @@ def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
 # Recomputation from 8 bits
 # =============================================================================
 
+def _forget(tensor):
+    """Keep nothing of a tensor that a graph wants to save."""
+
+
+def _forgotten(_):
+    raise RuntimeError("checkpoint8_recompute: function must not differentiate inside its forward pass")
+
+
 class Checkpoint8Function(torch.autograd.Function):
     """function(*tensors) that saves its first `kept` tensors in 8 bits and
     nothing of its inside; the backward restores them and runs it again."""
@@ -279,7 +287,16 @@ class Checkpoint8Function(torch.autograd.Function):
         ctx.save_for_backward(*[p for c in packed for p in (c.codes, c.exponents)], *tensors[kept:])
         ctx.function, ctx.kept = function, [(c.shape, c.dtype) for c in packed]
         ctx.autocast = dict(enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"))
-        return function(*tensors)
+        # With gradients on, as the caller has them and as the recomputation runs: a
+        # function that asks for the mode (as MHCLayer does) takes one path in both,
+        # and the backward differentiates what the forward returned.  The graph is
+        # made for that alone: it saves nothing and goes with this call.
+        inside = [t.detach().requires_grad_(n) for t, n in zip(tensors, ctx.needs_input_grad[2:])]
+        with torch.enable_grad(), torch.autograd.graph.saved_tensors_hooks(_forget, _forgotten):
+            out = function(*inside)
+        if isinstance(out, tuple):
+            return tuple(o.detach() if torch.is_tensor(o) else o for o in out)
+        return out.detach() if torch.is_tensor(out) else out
 
     @staticmethod
     def backward(ctx, *grad_out):

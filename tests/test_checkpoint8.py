@@ -511,3 +511,50 @@ def test_autocast(cuda):
 def test_recompute_without_gradients_keeps_nothing(cuda):
     x = acts(9, 40, seed=1).to(cuda)
     assert mhc.checkpoint8_recompute(torch.tanh, x).grad_fn is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dynamic,bf16,training", [(4, False, True, True), (8, False, True, True),
+                                                     (4, False, True, False), (4, False, False, False),
+                                                     (4, True, True, False), (4, True, False, False)])
+def test_layer_in_8_bits_runs_the_plain_layers_pass(cuda, n, dynamic, bf16, training):
+    """With gradients on, in training and in eval mode, the result has the plain
+    layer's type and bits, and so have the gradients at the restored input."""
+    torch.manual_seed(n)
+    layer = mhc.MHCLayer(128, n, use_dynamic_h=dynamic, alpha_init=0.3, bf16_io=bf16).to(cuda).train(training)
+    kept = mhc.MHCLayer(128, n, use_dynamic_h=dynamic, alpha_init=0.3, bf16_io=bf16,
+                        checkpoint_8bit=True).to(cuda).train(training)
+    kept.load_state_dict(layer.state_dict())
+    x = acts(40, n, 128, seed=n, dtype=BF16 if bf16 else F32).to(cuda)
+    xs = x.clone().requires_grad_(True)
+    out, want = kept(xs), layer(x.clone().requires_grad_(True))
+    assert out.dtype == want.dtype and torch.equal(out, want)
+    g = acts(40, n, 128, seed=5, dtype=want.dtype).to(cuda)
+    out.backward(g)
+    xh = mhc.checkpoint8_pack(x).unpack().requires_grad_(True)
+    layer(xh).backward(g)
+    assert torch.equal(xs.grad, xh.grad)
+    for (name, p), q in zip(kept.named_parameters(), layer.named_parameters()):
+        assert torch.equal(p.grad, q[1].grad), name
+
+
+@pytest.mark.gpu
+def test_recompute_runs_both_passes_in_one_mode(cuda):
+    """The function sees gradients on in both passes, and its first pass holds nothing."""
+    modes = []
+
+    def f(t):
+        modes.append(torch.is_grad_enabled())
+        return torch.tanh(t) if torch.is_grad_enabled() else t.sign()
+
+    x = acts(2048, 256, seed=1).to(cuda).requires_grad_(True)
+    mhc.checkpoint8_recompute(f, x).sum().backward()
+    assert modes == [True, True]
+    xh = mhc.checkpoint8_pack(x).unpack().requires_grad_(True)
+    torch.tanh(xh).sum().backward()
+    assert torch.equal(x.grad, xh.grad)
+    before = torch.cuda.memory_allocated()
+    out = mhc.checkpoint8_recompute(lambda t: torch.tanh(torch.tanh(t)), x)
+    assert torch.cuda.memory_allocated() - before <= out.numel() * 4 + x.numel() * 33 // 32 + 4096
+    with pytest.raises(RuntimeError, match="differentiate"):
+        mhc.checkpoint8_recompute(lambda t: torch.autograd.grad(torch.tanh(t).sum(), t)[0], x)
