@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(row_threads(UPT, WARP), EVEN || WARP || UPT !=
 // block an SM: 203 us); [8192, 4096] bf16: 45 us.
 // ---------------------------------------------------------------------------
 constexpr int kRingMost = 8, kRingUPT = 2;
+constexpr int kRingBytes = 224 * 1024;  // of an SM's blocks together, two at least
 
 struct Ring {
   int stages, blocks;  // blocks an SM; stages = 0: no ring
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(512, 2)
 // L2), and the block's share of gw is kept in shared memory (KEEP) or, past
 // kKeepCols columns, in its row of partial sums.
 constexpr int kLongThreads = 512;
-constexpr int64_t kKeepCols = 49152;  // 192 KB
+constexpr int64_t kKeepCols = 49152;  // 192 KB; a multiple of the rows' padding
 
 template <typename T, bool EVEN, bool KEEP>
 __global__ void __launch_bounds__(kLongThreads)
@@ -757,7 +758,7 @@ Ring ring_plan(int64_t rows, int64_t cols, size_t e) {
   p.blocks = 1024 / p.threads;
   p.blocks = p.blocks < 2 ? 2 : p.blocks > 6 ? 6 : p.blocks;
   p.stage = (uint32_t)((size_t)cols * e + ck_pitch(cols));
-  const size_t s = ((size_t)(224 * 1024 / p.blocks) - (size_t)cols * sizeof(float)) / p.stage;
+  const size_t s = ((size_t)(kRingBytes / p.blocks) - (size_t)cols * sizeof(float)) / p.stage;
   p.stages = (int)(s > kRingMost ? kRingMost : s);
   if (p.stages < 3) p.stages = 0;
   return p;
@@ -783,11 +784,15 @@ int launch_norm_bwd(const T* g, const int8_t* codes, const uint8_t* exps, const 
   {
     ProfScope p("rmsnorm_checkpoint8_bwd", st);
     const Ring ring = ring_plan(rows, cols, sizeof(T));
+    // The limit on dynamic shared memory belongs to the kernel, not to the launch:
+    // it is always set to the most that any width asks for, so that host threads
+    // with other widths cannot lower it in between.
     if (even && ring.stages > 0) {
       auto kern = norm_bwd_ring_kernel<T>;
       const size_t bytes = (size_t)ring.stages * ring.stage + (size_t)cols * sizeof(float);
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
-        return fail(MHC_ERR_CUDA, "rmsnorm_checkpoint8_bwd: cannot reserve %zu bytes of shared memory", bytes);
+      constexpr int most = kRingBytes / 2;
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+        return fail(MHC_ERR_CUDA, "rmsnorm_checkpoint8_bwd: cannot reserve %d bytes of shared memory", most);
       kern<<<blocks, ring.threads, bytes, st>>>(g, codes, exps, w, rms, gx, part, rows, (int)cols, (int)pitch, ring);
     } else
 #define MHC_NORM_BWD(KERN) KERN<<<blocks, pl.threads, 0, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch)
@@ -795,8 +800,9 @@ int launch_norm_bwd(const T* g, const int8_t* codes, const uint8_t* exps, const 
       const bool keep = cols <= kKeepCols;
       const size_t bytes = keep ? (size_t)pitch * sizeof(float) : 0;
       auto go = [&](auto kern) -> int {
-        if (bytes && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
-          return fail(MHC_ERR_CUDA, "rmsnorm_checkpoint8_bwd: cannot reserve %zu bytes of shared memory", bytes);
+        constexpr int most = (int)(kKeepCols * sizeof(float));
+        if (bytes && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+          return fail(MHC_ERR_CUDA, "rmsnorm_checkpoint8_bwd: cannot reserve %d bytes of shared memory", most);
         kern<<<blocks, kLongThreads, bytes, st>>>(g, codes, exps, w, rms, gx, part, rows, cols, pitch);
         return MHC_OK;
       };

@@ -558,3 +558,47 @@ def test_recompute_runs_both_passes_in_one_mode(cuda):
     assert torch.cuda.memory_allocated() - before <= out.numel() * 4 + x.numel() * 33 // 32 + 4096
     with pytest.raises(RuntimeError, match="differentiate"):
         mhc.checkpoint8_recompute(lambda t: torch.autograd.grad(torch.tanh(t).sum(), t)[0], x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [((2, 40000), (2, 33001), (1, 49152)), ((1184, 4096), (1184, 1032), (1184, 7168))])
+def test_rmsnorm_backward_from_several_host_threads(cuda, shapes):
+    """Calls of other widths in other threads, each on its own stream, take
+    nothing from each other (the kernels' limits on shared memory belong to the
+    process).  The entry point itself in a tight loop, so that calls overlap."""
+    import threading
+    lib = _C.load()
+
+    def case(rows, cols):
+        gen = torch.Generator(device=cuda).manual_seed(cols)
+        x, g = (torch.randn(rows, cols, device=cuda, generator=gen, dtype=BF16) for _ in range(2))
+        w = torch.rand(cols, device=cuda, generator=gen) + 0.5
+        _, rms, kept = mhc.rmsnorm_checkpoint8_fwd(x, w)
+        want = mhc.rmsnorm_checkpoint8_bwd(g, kept, w, rms)
+        got = torch.empty_like(want[0]), torch.empty_like(want[1])
+        size = lib.mhc_rmsnorm_checkpoint8_bwd_workspace_bytes(rows, cols)
+        ws, stream = torch.empty(size, dtype=torch.uint8, device=cuda), torch.cuda.Stream()
+        held = (g, kept, w, rms, ws, stream)
+        args = (g.data_ptr(), 1, kept.codes.data_ptr(), kept.exponents.data_ptr(), w.data_ptr(), rms.data_ptr(),
+                got[0].data_ptr(), got[1].data_ptr(), rows, cols, ws.data_ptr(), size, stream.cuda_stream)
+        return args, got, want, held
+
+    cases = [case(*s) for s in shapes]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(args):
+        for _ in range(2000):
+            if lib.mhc_rmsnorm_checkpoint8_bwd(*args):
+                errors.append(_C.last_error())
+                return
+
+    threads = [threading.Thread(target=work, args=(c[0],)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for _, got, want, _ in cases:
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
