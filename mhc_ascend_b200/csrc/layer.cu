@@ -309,8 +309,10 @@ bool launch_token_stream(const T* x, const float* w, float* rec, float* rms, T* 
   if (nbuf > 4) nbuf = 4;
   if (nbuf < 2) return false;
   const size_t smem = (size_t)nbuf * tok + (size_t)nbuf * 8;
+  // the limit belongs to the kernel: always the most, so that no other host
+  // thread's width lowers it before this launch
   cudaFuncSetAttribute(token_stream_fwd_kernel<N, T, DYN, GRAM>,
-                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)avail);
   const int64_t g = B < num_sms() ? B : num_sms();
   token_stream_fwd_kernel<N, T, DYN, GRAM><<<(unsigned)g, kTsThreads, smem, s>>>(
       x, w, rec, rms, out, B, C, r_eps, nbuf);
@@ -819,6 +821,8 @@ inline size_t wide_fwd_smem(int NM, int64_t C) { return (size_t)(NM * NM + 2 * N
 inline size_t wide_bwd_smem(int NM, int64_t C) {
   return (size_t)(NM * NM + 2 * NM + 2 * NM * 33 + 2 * C) * sizeof(float);
 }
+// the most of them, and the limit that is set at every launch: a limit of the
+// call's own size could be lowered by another host thread before the launch
 constexpr size_t kWideSmemMax = 200 * 1024;
 
 // Column sums of a [R][W] matrix in fixed order (chunks of rows, then the
@@ -870,13 +874,13 @@ int run_fwd_wide(const float* x, const float* w, const float* pp, const float* p
   {
     ProfScope _ps("wide_stream_fwd", s);
     if (NM == 8) {
-      cudaFuncSetAttribute(wide_stream_fwd_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(wide_stream_fwd_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmemMax);
       wide_stream_fwd_kernel<8><<<(unsigned)B, 256, smem, s>>>(x, w, Mb, rec, RS, out, n, C, r_eps);
     } else if (NM == 16) {
-      cudaFuncSetAttribute(wide_stream_fwd_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(wide_stream_fwd_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmemMax);
       wide_stream_fwd_kernel<16><<<(unsigned)B, 256, smem, s>>>(x, w, Mb, rec, RS, out, n, C, r_eps);
     } else {
-      cudaFuncSetAttribute(wide_stream_fwd_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(wide_stream_fwd_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmemMax);
       wide_stream_fwd_kernel<32><<<(unsigned)B, 256, smem, s>>>(x, w, Mb, rec, RS, out, n, C, r_eps);
     }
   }
@@ -915,13 +919,13 @@ int run_bwd_wide(const float* g, const float* x, const float* w, const float* pp
   {
     ProfScope _ps("wide_bwd_stream", s);
     if (NM == 8) {
-      cudaFuncSetAttribute(wide_bwd_stream_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(wide_bwd_stream_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmemMax);
       wide_bwd_stream_kernel<8><<<(unsigned)B, 256, smem, s>>>(g, x, w, rec, RS, ar, br, n, C, gx, gwt, ghh, gM, E);
     } else if (NM == 16) {
-      cudaFuncSetAttribute(wide_bwd_stream_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(wide_bwd_stream_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmemMax);
       wide_bwd_stream_kernel<16><<<(unsigned)B, 256, smem, s>>>(g, x, w, rec, RS, ar, br, n, C, gx, gwt, ghh, gM, E);
     } else {
-      cudaFuncSetAttribute(wide_bwd_stream_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(wide_bwd_stream_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmemMax);
       wide_bwd_stream_kernel<32><<<(unsigned)B, 256, smem, s>>>(g, x, w, rec, RS, ar, br, n, C, gx, gwt, ghh, gM, E);
     }
   }
