@@ -11,7 +11,8 @@ dimension.  The backward operators take the codes as they are:
 * ``checkpoint8_recompute`` -- any function of tensors: keeps its input packed
   and runs it again; ``MHCLayer(checkpoint_8bit=True)`` keeps its streams so.
 
-Each gradient is the exact gradient formula evaluated at the restored input.
+Each gradient is the exact gradient formula evaluated at the restored input;
+it is not differentiable again (autograd raises).
 The reference has no counterpart (it saves bf16 copies, ops.py:394-470).
 """
 
@@ -21,6 +22,7 @@ import math
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .ops import _f32, _launch, _lib, _require_cuda, _workspace
 
@@ -184,6 +186,7 @@ class RMSNormCheckpoint8Function(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         codes, exponents, weight, rms = ctx.saved_tensors
         kept = Checkpoint8(codes, exponents, *ctx.kept)
@@ -238,6 +241,7 @@ class LinearCheckpoint8Function(torch.autograd.Function):
         return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         codes, exponents, weight = ctx.saved_tensors
         gx = gw = gb = None
@@ -299,6 +303,7 @@ class Checkpoint8Function(torch.autograd.Function):
         return out.detach() if torch.is_tensor(out) else out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grad_out):
         saved, k = ctx.saved_tensors, len(ctx.kept)
         need = ctx.needs_input_grad[2:]

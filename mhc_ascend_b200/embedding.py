@@ -15,6 +15,7 @@ from typing import Optional, Sequence, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .ops import _launch, _lib, _require_cuda, _workspace
 
@@ -113,6 +114,7 @@ class StreamEmbeddingFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         (ids,) = ctx.saved_tensors
         rows, scale, padding_idx, dtype = ctx.args

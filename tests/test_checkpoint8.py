@@ -602,3 +602,17 @@ def test_rmsnorm_backward_from_several_host_threads(cuda, shapes):
     assert not errors, errors
     for _, got, want, _ in cases:
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_second_derivatives_raise(cuda):
+    """The kernels' gradients have no graph: differentiating one again raises
+    instead of leaving terms out."""
+    x, w = acts(9, 32, seed=1).to(cuda).requires_grad_(True), acts(7, 32, seed=2).to(cuda).requires_grad_(True)
+    v, ids = torch.ones(32, device=cuda, requires_grad=True), torch.arange(7, device=cuda)
+    for out, by in ((mhc.linear_checkpoint8(x, w), x), (mhc.linear_checkpoint8(x, w), w),
+                    (mhc.rmsnorm_checkpoint8(x, v), x), (mhc.checkpoint8_recompute(torch.tanh, x), x),
+                    (mhc.stream_embedding(ids, w, 2), w)):
+        grad, = torch.autograd.grad(out.square().sum(), by, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grad.sum().backward()
