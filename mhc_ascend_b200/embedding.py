@@ -24,13 +24,14 @@ MAX_STREAMS = 32
 
 
 def _scales(scale, n):
+    """The n scales as they are now, for the call and for its backward pass."""
     if isinstance(scale, (int, float)):
         vals = [float(scale)] * n
     else:
         vals = [float(v) for v in scale]
         if len(vals) != n:
             raise RuntimeError(f"stream_embedding: {n} streams need {n} scales (got {len(vals)})")
-    return (ctypes.c_float * n)(*vals)
+    return tuple(vals)
 
 
 def _check_ids(what, ids):
@@ -58,7 +59,7 @@ def stream_embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, num_streams: i
     dtype = weight.dtype if dtype is None else dtype
     if dtype not in _FLOATS:
         raise RuntimeError(f"{what}: dtype must be float32 or bfloat16 (got {dtype})")
-    sc = _scales(scale, n)
+    sc = (ctypes.c_float * n)(*_scales(scale, n))
     idc = _check_ids(what, ids)
     V, C = weight.shape
     out = torch.empty(*ids.shape, n, C, dtype=dtype, device=weight.device)
@@ -83,7 +84,7 @@ def stream_embedding_bwd(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddin
     n = _check_n(what, n)
     V = int(num_embeddings)
     pad = _padding(padding_idx, V)
-    sc = _scales(scale, n)
+    sc = (ctypes.c_float * n)(*_scales(scale, n))
     idc = _check_ids(what, ids)
     g = grad_out if grad_out.is_contiguous() else grad_out.detach().contiguous()
     gw = torch.empty(V, C, dtype=dtype, device=g.device)
@@ -108,6 +109,7 @@ class StreamEmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, ids, weight, num_streams, scale, padding_idx, dtype):
+        scale = _scales(scale, _check_n("stream_embedding", num_streams))  # the caller's list may change
         out = stream_embedding_fwd(ids, weight.detach(), num_streams, scale, dtype)
         ctx.save_for_backward(ids)
         ctx.args = (weight.size(0), scale, padding_idx, weight.dtype)

@@ -253,3 +253,15 @@ def test_offsets_past_32_bits(cuda):
     gw = mhc.stream_embedding_bwd(g, ids, V, dtype=BF16)
     assert float(gw[V - 1].float().sum()) == 2 * C and float(gw[V - 2].float().sum()) == C
     assert float(gw.sum(dtype=torch.float32)) == 5 * C
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [list, torch.tensor])
+def test_gradient_uses_the_forwards_scales(cuda, kind):
+    """Scales that change after the lookup change nothing in its gradient."""
+    scales = kind([1.0, 0.5])
+    w = torch.randn(6, 8, device=cuda, requires_grad=True)
+    out = mhc.stream_embedding(torch.tensor([1, 4], device=cuda), w, 2, scales)
+    scales[0] = 100.0
+    out.sum().backward()
+    assert torch.equal(w.grad.sum(1).cpu(), torch.tensor([0.0, 12.0, 0.0, 0.0, 12.0, 0.0]))
