@@ -281,6 +281,15 @@ def _forgotten(_):
     raise RuntimeError("checkpoint8_recompute: function must not differentiate inside its forward pass")
 
 
+def _holds_tensors(o):
+    """Whether o is a container with tensors inside."""
+    if isinstance(o, dict):
+        o = o.values()
+    elif not isinstance(o, (list, tuple)):
+        return False
+    return any(torch.is_tensor(v) or _holds_tensors(v) for v in o)
+
+
 class Checkpoint8Function(torch.autograd.Function):
     """function(*tensors) that saves its first `kept` tensors in 8 bits and
     nothing of its inside; the backward restores them and runs it again."""
@@ -298,9 +307,11 @@ class Checkpoint8Function(torch.autograd.Function):
         inside = [t.detach().requires_grad_(n) for t, n in zip(tensors, ctx.needs_input_grad[2:])]
         with torch.enable_grad(), torch.autograd.graph.saved_tensors_hooks(_forget, _forgotten):
             out = function(*inside)
-        if isinstance(out, tuple):
-            return tuple(o.detach() if torch.is_tensor(o) else o for o in out)
-        return out.detach() if torch.is_tensor(out) else out
+        outs = out if isinstance(out, tuple) else (out,)
+        if any(map(_holds_tensors, outs)):  # autograd would hand them out without a graph
+            raise RuntimeError("checkpoint8_recompute: function must return a tensor or a tuple of tensors")
+        outs = tuple(o.detach() if torch.is_tensor(o) else o for o in outs)
+        return outs if isinstance(out, tuple) else outs[0]
 
     @staticmethod
     @once_differentiable
@@ -321,10 +332,11 @@ class Checkpoint8Function(torch.autograd.Function):
 
 
 def checkpoint8_recompute(function, *tensors: torch.Tensor, kept: int = 1):
-    """Run ``function(*tensors)`` for training and keep only its first ``kept``
-    tensors, in 8 bits (float32 or bfloat16); the backward restores them and
-    recomputes.  The gradients are those of ``function`` at the restored
-    tensors.  ``function`` is called again with the same arguments: it draws no
+    """Run ``function(*tensors)`` (it returns a tensor or a tuple of them) for
+    training and keep only its first ``kept`` tensors, in 8 bits (float32 or
+    bfloat16); the backward restores them and recomputes.  The gradients are
+    those of ``function`` at the restored tensors.  ``function`` is called again
+    with the same arguments and gradients on, as in the first pass: it draws no
     random numbers, and what it differentiates by has to be among ``tensors``."""
     if not 1 <= kept <= len(tensors):
         raise RuntimeError(f"checkpoint8_recompute: kept must be in [1, {len(tensors)}] (got {kept})")

@@ -616,3 +616,16 @@ def test_second_derivatives_raise(cuda):
         grad, = torch.autograd.grad(out.square().sum(), by, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             grad.sum().backward()
+
+
+@pytest.mark.gpu
+def test_recompute_refuses_results_that_have_no_gradient(cuda):
+    """A list or a dict would pass through autograd without a graph."""
+    x = acts(9, 40, seed=1).to(cuda).requires_grad_(True)
+    for pack in (lambda t: [t * 2], lambda t: {"out": t * 2}, lambda t: (t * 2, [t])):
+        with pytest.raises(RuntimeError, match="tuple of tensors"):
+            mhc.checkpoint8_recompute(pack, x)
+    out, none, five, names = mhc.checkpoint8_recompute(lambda t: (t * 2, None, 5, ["a"]), x)
+    assert none is None and five == 5 and names == ["a"]
+    out.sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 2.0))
