@@ -256,7 +256,8 @@ class LinearCheckpoint8Function(torch.autograd.Function):
 
 def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``torch.nn.functional.linear`` (x, weight and bias of one type, float32 or
-    bfloat16) that keeps x in 8 bits for the weight's gradient.  Under autocast
+    bfloat16) that keeps x in 8 bits for the weight's gradient, and nothing of x
+    where the weight needs none.  Under autocast
     the three are cast to its type first, as for the plain layer."""
     _require_cuda("linear_checkpoint8", x, weight)
     if torch.is_autocast_enabled("cuda"):
@@ -266,6 +267,8 @@ def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     _check_float("linear_checkpoint8", "x", x)
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise RuntimeError("linear_checkpoint8: x, weight and bias must have one type")
+    if not (torch.is_grad_enabled() and weight.requires_grad):  # nobody will read the codes
+        return torch.nn.functional.linear(x, weight, bias)
     return LinearCheckpoint8Function.apply(x, weight, bias)
 
 

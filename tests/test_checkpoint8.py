@@ -629,3 +629,33 @@ def test_recompute_refuses_results_that_have_no_gradient(cuda):
     assert none is None and five == 5 and names == ["a"]
     out.sum().backward()
     assert torch.equal(x.grad, torch.full_like(x, 2.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["frozen", "no_grad", "autocast"])
+def test_linear_keeps_nothing_for_a_frozen_weight(cuda, mode):
+    """Without a weight gradient to come, x is neither packed nor kept."""
+    x, w = acts(4096, 512, seed=1).to(cuda).requires_grad_(True), (acts(64, 512, seed=2) * 0.1).to(cuda)
+    b = acts(64, seed=3).to(cuda).requires_grad_(True)
+    if mode == "no_grad":
+        w.requires_grad_(True)
+    with torch.set_grad_enabled(mode != "no_grad"), torch.autocast("cuda", dtype=BF16, enabled=mode == "autocast"):
+        mhc.linear_checkpoint8(x, w, b)  # the library's own buffers
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = mhc.linear_checkpoint8(x, w, b)
+        held, peak = torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before
+        assert torch.equal(out, torch.nn.functional.linear(x, w, b))
+    assert held <= out.numel() * 4 + w.numel() * 4 + 8192  # autocast keeps w's copy
+    if mode != "autocast":
+        assert peak <= 2 * out.numel() * 4 + 8192
+    if mode == "no_grad":
+        assert out.grad_fn is None
+        return
+    g = acts(4096, 64, seed=4, dtype=out.dtype).to(cuda)
+    out.backward(g)
+    xs, bs = (t.detach().clone().requires_grad_(True) for t in (x, b))
+    with torch.autocast("cuda", dtype=BF16, enabled=mode == "autocast"):
+        torch.nn.functional.linear(xs, w, bs).backward(g)
+    assert torch.equal(x.grad, xs.grad) and torch.equal(b.grad, bs.grad)
