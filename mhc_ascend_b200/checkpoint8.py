@@ -265,6 +265,8 @@ def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
         with torch.autocast("cuda", enabled=False):
             return linear_checkpoint8(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype))
     _check_float("linear_checkpoint8", "x", x)
+    if weight.dim() != 2:
+        raise RuntimeError(f"linear_checkpoint8: weight must be [out_features, in_features] (got {tuple(weight.shape)})")
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise RuntimeError("linear_checkpoint8: x, weight and bias must have one type")
     if not (torch.is_grad_enabled() and weight.requires_grad):  # nobody will read the codes

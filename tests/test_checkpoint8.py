@@ -659,3 +659,11 @@ def test_linear_keeps_nothing_for_a_frozen_weight(cuda, mode):
     with torch.autocast("cuda", dtype=BF16, enabled=mode == "autocast"):
         torch.nn.functional.linear(xs, w, bs).backward(g)
     assert torch.equal(x.grad, xs.grad) and torch.equal(b.grad, bs.grad)
+
+
+@pytest.mark.gpu
+def test_linear_refuses_a_weight_vector(cuda):
+    """Before the forward pass, not in the backward."""
+    x, w = torch.randn(8, 8, device=cuda), torch.randn(8, device=cuda, requires_grad=True)
+    with pytest.raises(RuntimeError, match="weight must be"):
+        mhc.linear_checkpoint8(x, w)
