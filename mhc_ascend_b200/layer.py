@@ -217,15 +217,16 @@ class MHCResidualWrapper(nn.Module):
         C = shape[-1]
         r2, b2 = residual.reshape(-1, C), branch_output.reshape(-1, C)
         m = self.mhc
+        keep = m.checkpoint_8bit and torch.is_grad_enabled()
         if wrapper_fused_supported(r2, b2, self.expansion_rate, C, m.use_dynamic_h) and \
-                self.residual_mode in ("decay", "zero") and not m.checkpoint_8bit:
+                self.residual_mode in ("decay", "zero") and not keep:
             hidden, normed = wrapper_fused_dynamic_prenorm(
                 r2, b2, self.residual_mode, norm_weight, norm_eps, m.rmsnorm_weight, m.phi_pre,
                 m.phi_post, m.phi_res, m.alpha_pre, m.alpha_post, m.alpha_res, m.b_pre, m.b_post,
                 m.b_res, m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
             return hidden.reshape(shape), normed.reshape(shape)
         hidden = self.forward(residual, branch_output)
-        norm = rmsnorm_checkpoint8 if m.checkpoint_8bit else rmsnorm
+        norm = rmsnorm_checkpoint8 if keep else rmsnorm
         return hidden, norm(hidden.reshape(-1, C), norm_weight, norm_eps).reshape(shape)
 
     def extra_repr(self) -> str:

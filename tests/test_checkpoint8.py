@@ -667,3 +667,29 @@ def test_linear_refuses_a_weight_vector(cuda):
     x, w = torch.randn(8, 8, device=cuda), torch.randn(8, device=cuda, requires_grad=True)
     with pytest.raises(RuntimeError, match="weight must be"):
         mhc.linear_checkpoint8(x, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4, 3])
+def test_wrapper_in_8_bits_without_gradients_is_the_plain_one(cuda, n):
+    """Output and norm in one pass where the plain wrapper has it, and no packing."""
+    torch.manual_seed(3)
+    plain = mhc.MHCResidualWrapper(64, n, alpha_init=0.2).to(cuda).eval()
+    kept = mhc.MHCResidualWrapper(64, n, alpha_init=0.2, checkpoint_8bit=True).to(cuda).eval()
+    kept.load_state_dict(plain.state_dict())
+    r, b, w = acts(3, 20, 64, seed=1).to(cuda), acts(3, 20, 64, seed=2).to(cuda), torch.rand(64, device=cuda) + 0.5
+
+    def launches(wrapper):
+        with torch.no_grad():
+            _C.profile_enable(True)
+            try:
+                out = wrapper.forward_prenorm(r, b, w)
+                torch.cuda.synchronize()
+                return out, sorted(_C.profile_report())
+            finally:
+                _C.profile_enable(False)
+
+    (hidden, normed), names = launches(kept)
+    (want, want_normed), want_names = launches(plain)
+    assert torch.equal(hidden, want) and torch.equal(normed, want_normed)
+    assert names == want_names and not any("checkpoint8" in k for k in names)
