@@ -57,6 +57,8 @@ class MHCLayer(nn.Module):
             the restored input.
     """
 
+    checkpoint_8bit = False  # of modules pickled before the argument was there
+
     def __init__(self, hidden_dim: int, expansion_rate: int = 4, num_sinkhorn_iters: int = 20,
                  sinkhorn_eps: float = 1e-8, rmsnorm_eps: float = 1e-5,
                  use_dynamic_h: bool = True, alpha_init: float = 0.01, bf16_io: bool = False,

@@ -693,3 +693,14 @@ def test_wrapper_in_8_bits_without_gradients_is_the_plain_one(cuda, n):
     (want, want_normed), want_names = launches(plain)
     assert torch.equal(hidden, want) and torch.equal(normed, want_normed)
     assert names == want_names and not any("checkpoint8" in k for k in names)
+
+
+def test_modules_pickled_before_the_flag_still_run():
+    layer = mhc.MHCLayer(64, 4)
+    state = dict(layer.__dict__)
+    del state["checkpoint_8bit"]
+    old = mhc.MHCLayer.__new__(mhc.MHCLayer)
+    old.__setstate__(state)  # as unpickling does
+    assert old.checkpoint_8bit is False
+    with pytest.raises(RuntimeError, match="CUDA"):
+        old(torch.randn(2, 4, 64))
