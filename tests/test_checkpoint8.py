@@ -704,3 +704,47 @@ def test_modules_pickled_before_the_flag_still_run():
     assert old.checkpoint_8bit is False
     with pytest.raises(RuntimeError, match="CUDA"):
         old(torch.randn(2, 4, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("per_sm,more,cols", [(8, 0, 1032), (8, -1, 1032), (8, -1, 4096), (8, 0, 4096), (16, 132, 1280),
+                                              (33, 116, 2048), (20, 41, 4096), (16, 32, 7168), (8, 117, 8192),
+                                              (8, 1, 8200), (9, 0, 1928)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rmsnorm_backward_of_training_batches(cuda, per_sm, more, cols, dtype):
+    """Rows enough that a block meets several of them: from 8 rows an SM and 1025
+    to 8192 columns on over a ring of rows in shared memory, whose places are
+    filled again and again; one row less and a wider row take other kernels."""
+    rows = per_sm * torch.cuda.get_device_properties(cuda).multi_processor_count + more
+    gen = torch.Generator(device=cuda).manual_seed(rows + cols)
+    loud = torch.exp(torch.randn(cols, device=cuda, generator=gen))
+    x, g = ((torch.randn(rows, cols, device=cuda, generator=gen) * loud).to(dtype) for _ in range(2))
+    w = torch.rand(cols, device=cuda, generator=gen) + 0.5
+    _, rms, kept = mhc.rmsnorm_checkpoint8_fwd(x, w)
+    gx, gw = mhc.rmsnorm_checkpoint8_bwd(g, kept, w, rms)
+    _, want, want_w, tol, tolw = _norm64(x, kept.unpack().double(), g, w, 1e-5)
+    half = UB if dtype == BF16 else 0.0
+    assert bool(((gx.double() - want).abs() <= tol + half * (want.abs() + tol)).all())
+    assert bool(((gw.double() - want_w).abs() <= tolw).all())
+    for _ in range(3):
+        again = mhc.rmsnorm_checkpoint8_bwd(g, kept, w, rms)
+        assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(700, 33001), (700, 40000), (601, 49152), (601, 49160), (333, 50001)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rmsnorm_backward_of_many_long_rows(cuda, rows, cols, dtype):
+    """Rows past the registers, several a block; past 49152 columns the weight's
+    share is kept outside of shared memory."""
+    gen = torch.Generator(device=cuda).manual_seed(cols)
+    x, g = (torch.randn(rows, cols, device=cuda, generator=gen).to(dtype) for _ in range(2))
+    w = torch.rand(cols, device=cuda, generator=gen) + 0.5
+    _, rms, kept = mhc.rmsnorm_checkpoint8_fwd(x, w)
+    gx, gw = mhc.rmsnorm_checkpoint8_bwd(g, kept, w, rms)
+    _, want, want_w, tol, tolw = _norm64(x, kept.unpack().double(), g, w, 1e-5)
+    half = UB if dtype == BF16 else 0.0
+    assert bool(((gx.double() - want).abs() <= tol + half * (want.abs() + tol)).all())
+    assert bool(((gw.double() - want_w).abs() <= tolw).all())
+    again = mhc.rmsnorm_checkpoint8_bwd(g, kept, w, rms)
+    assert torch.equal(again[0], gx) and torch.equal(again[1], gw)

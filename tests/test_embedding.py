@@ -265,3 +265,39 @@ def test_gradient_uses_the_forwards_scales(cuda, kind):
     scales[0] = 100.0
     out.sum().backward()
     assert torch.equal(w.grad.sum(1).cpu(), torch.tensor([0.0, 12.0, 0.0, 0.0, 12.0, 0.0]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [30000, 70000])  # 32 and 64 positions a block
+@pytest.mark.parametrize("kind,pad", [("text", None), ("text", 0), ("same", None)])
+@pytest.mark.parametrize("tg,tw,C,shift", [(BF16, BF16, 1281, 0), (BF16, F32, 1281, 1), (BF16, BF16, 1280, 0),
+                                           (BF16, F32, 1280, 1), (F32, F32, 1281, 0), (F32, BF16, 1284, 0),
+                                           (F32, F32, 1284, 1)])
+def test_gradient_of_training_batches(cuda, T, kind, pad, tg, tw, C, shift):
+    """Blocks of many positions and rows of several slices, in the layouts that
+    16-byte accesses fit and in those that they do not (an odd width; a start
+    that is `shift` values off)."""
+    n, V, scales = 2, 5000, [1.0, -0.625]
+    cpu = torch.Generator().manual_seed(T + C)
+    gen = torch.Generator(device=cuda).manual_seed(T + C)
+    ids = _ids(T, V, kind, cpu)
+    if pad is not None:
+        ids[torch.rand(T, generator=cpu) < 0.2] = pad
+    ids = ids.to(cuda)
+    store = torch.randn(T * n * C + shift, device=cuda, generator=gen).to(tg)
+    g = store[shift:].view(T, n, C)
+    got = mhc.stream_embedding_bwd(g, ids, V, scales, padding_idx=pad, dtype=tw)
+    want, mag = (torch.zeros(V, C, dtype=torch.float64, device=cuda) for _ in range(2))
+    keep = torch.arange(T, device=cuda) if pad is None else torch.nonzero(ids != pad).squeeze(1)
+    for i, s in enumerate(scales):
+        term = g[:, i].double()[keep] * s
+        want.index_add_(0, ids[keep], term)
+        mag.index_add_(0, ids[keep], term.abs())
+    count = torch.bincount(ids[keep], minlength=V).double() * n
+    bf16 = tw == BF16
+    _check_grad(got, want.cpu(), mag.cpu(), count.cpu(), bf16)
+    # over the whole table: a row's roundings are of random sign
+    err = (got.double() - want).norm()
+    bound = ((count.sqrt() + 8)[:, None] * U * mag).norm() + (UB * (1 + UB) * want.norm() if bf16 else 0)
+    assert float(err) <= float(bound)
+    assert torch.equal(got, mhc.stream_embedding_bwd(g, ids, V, scales, padding_idx=pad, dtype=tw))
