@@ -358,9 +358,9 @@ MHC_API int mhc_stream_embedding_fwd(const void* ids, int32_t ids_64, const void
                              void* out, int32_t out_bf16, const float* scales, int64_t tokens,
                              int32_t n, int64_t hidden, int64_t vocab, void* stream);
 /* grad_weight[v, :] = sum over t with ids[t] = v, v != padding_idx, of
- * sum_i scales[i] grad_out[t, i, :], fp32 sums in token order (bitwise
- * reproducible); the whole [vocab, hidden] gradient is written, rows without a
- * token as zeros.  Ids outside [0, vocab) add nothing; padding_idx < 0: none.
+ * sum_i scales[i] grad_out[t, i, :], fp32 sums in a fixed order (bitwise
+ * reproducible; token order within chunks, then the chunks' sums); the whole
+ * [vocab, hidden] gradient is written, rows without a token as zeros.  Ids outside [0, vocab) add nothing; padding_idx < 0: none.
  * grad_weight must be 16-byte aligned. */
 MHC_API size_t mhc_stream_embedding_bwd_workspace_bytes(int64_t tokens, int64_t hidden);
 MHC_API int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, const void* ids, int32_t ids_64,
@@ -376,7 +376,8 @@ MHC_API int mhc_stream_embedding_bwd(const void* grad_out, int32_t g_bf16, const
  * byte E per 32 codes (pitch / 32 a row): a code stands for code * 2^(E - 127).
  * With a = max |x| of a block, E >= 1 is the smallest with
  * a < 127.5 * 2^(E - 127), and code = x / 2^(E - 127) rounded to nearest, ties
- * to even (at E = 249 held to +-63: 64 would stand for 2^128).  E = 255: the block held an infinity or a NaN and stands for NaNs.
+ * to even (at E = 249 held to +-63: 64 would stand for 2^128).  E = 255: the
+ * block held an infinity or a NaN and stands for NaNs.
  * codes must be 16-byte and exponents 4-byte aligned.
  * ------------------------------------------------------------------------- */
 MHC_API int64_t mhc_checkpoint8_pitch(int64_t cols);

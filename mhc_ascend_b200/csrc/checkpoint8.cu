@@ -7,11 +7,13 @@ namespace mhc {
 namespace {
 
 // ---------------------------------------------------------------------------
-// pack / unpack: one pass, bound by HBM ([32768, 4096] fp32: 101 and 98 us, 6.7
-// and 6.9 TB/s; [8192, 8192] bf16: 33 and 28 us).  A warp takes spans of 256 columns of a
-// row, a lane 8 of them (32 or 16 bytes in, 8 bytes of codes out), kUnroll spans
-// at once so that enough loads are in flight.  EVEN: rows that 16- or 32-byte
-// accesses fit; the spans then run over the rows without a gap.
+// pack / unpack: one pass, bound by HBM (a call among others, [32768, 4096] fp32:
+// 97 and 104 us, 7.0 and 6.5 TB/s; [8192, 8192] bf16: 35 us each, 5.8 TB/s;
+// uneven rows, [8192, 8191] fp32: 59 and 70 us, bf16: 84 and 66 us).  A warp takes
+// spans of 256 columns of a row, a lane 8 of them (32 or 16 bytes in, 8 bytes of
+// codes out), kUnroll spans at once so that enough loads are in flight.  EVEN:
+// rows that 16- or 32-byte accesses fit; the spans then run over the rows without
+// a gap.
 // ---------------------------------------------------------------------------
 constexpr int kPackThreads = 256, kUnroll = 4;
 
@@ -43,7 +45,7 @@ struct Walk {
 };
 
 // Rows without gaps and without padding: one list of units, and no index arithmetic
-// (which is what bounds the general kernels in bf16: [8192, 8192] 52 us against 33).
+// (which is what bounds the general kernels in bf16: [8192, 8192] 54 us against 35).
 template <typename T>
 __global__ void __launch_bounds__(kPackThreads)
     pack_flat_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, uint8_t* __restrict__ exps, int64_t units) {
@@ -276,7 +278,8 @@ __global__ void __launch_bounds__(1024)
 // order by norm_gw_kernel: no atomics, the same bits every time.  The next
 // row's g and codes are loaded before this row's sum is waited for.
 // Uneven rows of a block are held to 64 registers, two blocks an SM: their loads
-// wait on shared memory ([8192, 4097] bf16: 104 us against 186).
+// wait on shared memory ([8192, 4097] bf16 by itself: 104 us against 186; among
+// other calls, with the weight's sums, 112).
 template <typename T, int UPT, bool WARP, bool EVEN>
 __global__ void __launch_bounds__(row_threads(UPT, WARP), EVEN || WARP || UPT != 2 ? 1 : 2)
     norm_bwd_kernel(const T* __restrict__ g, const int8_t* __restrict__ codes,
@@ -387,8 +390,9 @@ __global__ void __launch_bounds__(row_threads(UPT, WARP), EVEN || WARP || UPT !=
 // row i also says that everyone is done with row i - 1: thread 0 then refills its
 // place.  What bounds it is instructions (two expansions a value), hence two-wide
 // fp32 arithmetic and the weights in shared memory.
-// Measured at [16384, 7168] bf16: 126 us, 4.7 TB/s (one row ahead in registers, a
-// block an SM: 203 us); [8192, 4096] bf16: 45 us.
+// Measured at [16384, 7168] bf16: by itself 126 us, 4.7 TB/s (one row ahead in
+// registers, a block an SM: 203 us); among other calls, with the weight's sums, 137
+// us, [8192, 4096] bf16 58 us, fp32 72 us.
 // ---------------------------------------------------------------------------
 constexpr int kRingMost = 8, kRingUPT = 2;
 constexpr int kRingBytes = 224 * 1024;  // of an SM's blocks together, two at least
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(512, 2)
   }
   // The weights' first and second halves of units apart, so that eight lanes read
   // 128 bytes in a row: whole units met every bank twice (LSU 72% busy, 133 us
-  // against 126 at [16384, 7168] bf16).
+  // against 126 at [16384, 7168] bf16, by itself).
   const int units = cols / 8;
   for (int c = tid; c < cols; c += blockDim.x) ws[(((c >> 2) & 1) * units + (c >> 3)) * 4 + (c & 3)] = w[c];
   auto weights = [&](int c, float2 (&v)[4]) {
@@ -661,7 +665,8 @@ RowPlan row_plan(int64_t cols, bool backward) {
   const int64_t pitch = ck_pitch(cols), U = pitch / 8;
   if (pitch <= kWarpCols) return {pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows, true};
   // forward: four units a thread wherever that leaves four warps, since small
-  // blocks put more rows on an SM ([16384, 7168] bf16: 105 us, 5.6 TB/s, against 118)
+  // blocks put more rows on an SM ([16384, 7168] bf16 by itself: 105 us against 118;
+  // among other calls 110, 5.4 TB/s)
   if (!backward && U >= 512 && U <= 4096) return {4, (int)(((U + 3) / 4 + 31) / 32 * 32), false};
   for (int upt : {1, 2, 4}) {
     const int64_t th = (((U + upt - 1) / upt) + 31) / 32 * 32;

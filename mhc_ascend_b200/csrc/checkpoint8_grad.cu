@@ -27,9 +27,11 @@
 // chains in fp32 registers, 128 a thread, which is why registers are moved
 // between the roles (setmaxnreg).
 //
-// 8192 tokens, 4096 x 4096: 220 us alone, 1.25 PFLOP/s, 76% of what cuBLAS reaches in
-// bf16; the tensor pipe is 67% busy, a stage takes about 980 cycles for 512 of MMAs
-// (the operands' traffic alone is 640 of shared memory; the rest is hand-overs).
+// 8192 tokens, 4096 x 4096: 280 us a call in a continuous run, 985 TFLOP/s, 60% of
+// what cuBLAS reaches in bf16 in a burst and 70% of what it sustains (243 us in
+// short runs, 220 under the profiler on a cool GPU).  There the tensor pipe is 67%
+// busy, a stage takes about 980 cycles for 512 of MMAs (the operands' traffic alone
+// is 640 of shared memory; the rest is hand-overs).
 #include "checkpoint8.cuh"
 #include "tma.cuh"
 

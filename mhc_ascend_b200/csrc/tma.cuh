@@ -113,7 +113,7 @@ inline bool make_tmap_3d_f32(CUtensorMap* map, const void* base, uint64_t d0, ui
 constexpr uint32_t kSpinLimit = 1u << 26;  // ~seconds of polling, then give up
 
 // Error word set by bounded waits that timed out (one per translation unit
-// that includes this header; layer.cu exposes its copy through the C-ABI).
+// that includes this header; mhc_device_error_word joins those that wait).
 static __device__ int g_mhc_device_error = 0;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -72,7 +72,8 @@ def stream_embedding_bwd(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddin
                          scale: Union[float, Sequence[float]] = 1.0, padding_idx: Optional[int] = None,
                          dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Dense table gradient [num_embeddings, hidden] in ``dtype`` from the
-    streams' gradient (ids' shape + [n, hidden]); fp32 sums in token order."""
+    streams' gradient (ids' shape + [n, hidden]); fp32 sums in a fixed order
+    (token order within chunks of sorted tokens, then the chunks' sums)."""
     what = "stream_embedding_bwd"
     _require_cuda(what, grad_out, ids)
     if grad_out.dim() < 2 or grad_out.shape[:-2] != ids.shape:

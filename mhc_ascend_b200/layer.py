@@ -51,10 +51,10 @@ class MHCLayer(nn.Module):
             arithmetic): static-H inference, and dynamic-H training and
             inference at n <= 4 (n == 4 for training), hidden % 64 == 0.  Off
             by default: like the reference, the layer then returns fp32.
-        checkpoint_8bit: in training, keep the input streams in 8 bits (33/32
-            bytes a value) and nothing else; the backward restores them and
-            runs the forward kernels again.  The gradients are the layer's at
-            the restored input.
+        checkpoint_8bit: with gradients on, keep the input streams in 8 bits
+            (33/32 bytes a value) and nothing else; the backward restores them
+            and runs the forward kernels again.  The result is the plain
+            layer's, the gradients are the layer's at the restored input.
     """
 
     checkpoint_8bit = False  # of modules pickled before the argument was there
@@ -155,8 +155,10 @@ class MHCResidualWrapper(nn.Module):
 
     Streams: [residual, branch_output, 0.1*residual, 0.01*residual, ...]
     ('decay') or zeros beyond the first two ('zero'); the mHC output is averaged
-    over streams.  With ``checkpoint_8bit`` (an argument of the layer) the
-    residual and the branch output are kept in 8 bits for the backward.  ``use_post_norm`` is accepted and, as in the reference
+    over streams.  With ``checkpoint_8bit`` (an argument of the layer) the fused
+    pass (n = 4, dynamic H, fp32) keeps the residual and the branch output in 8
+    bits for the backward; elsewhere the layer keeps the n packed streams in 8
+    bits.  ``use_post_norm`` is accepted and, as in the reference
     (layer.py:261), forced off.
     """
 
