@@ -416,6 +416,94 @@ MHC_API int mhc_checkpoint8_weight_grad(const void* grad_out, int32_t g_bf16, in
                                 void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Dropout from a counter-based generator.  No counterpart in the reference, whose
+ * layers draw no random numbers.
+ *   out[i] = number(i) < drop ? 0 : x[i] / (1 - drop / 65536)       i < count
+ * x and out fp32 or bf16 (products in fp32, rounded once); 0 <= drop <= 65536, the
+ * probability in 65536ths.  number(i) is 16-bit number i % 8 of group
+ * position + i / 8 (mod 2^64) of the seed's stream: Philox4x32-10 at counter
+ * (group low, group high, 0, 0), key (seed low, seed high), word by word, low half
+ * first.  state, if not NULL, points to two device words (seed, position), read by
+ * the kernel in place of the arguments.  The backward pass is the same call on the
+ * gradient; nothing is stored.
+ * ------------------------------------------------------------------------- */
+MHC_API int mhc_dropout(const void* x, int32_t x_bf16, void* out, int64_t count, int32_t drop,
+                        const uint64_t* state, uint64_t seed, uint64_t position, void* stream);
+/* out[0..1] = state[0..1], then state[1] += groups (one atomic step, so that a
+ * captured graph takes new numbers each time, and overlapping calls different ones) */
+MHC_API int mhc_dropout_take(uint64_t* state, uint64_t* out, int64_t groups, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Residual addition and RMSNorm.  The reference normalises by itself
+ * (ops.py:87-136).  Rows of cols values, contiguous:
+ *   hidden = residual + dropout(branch)          (mhc_dropout's numbers, i = row cols + col)
+ *   r = sqrt(mean hidden^2 + eps),  out = hidden / r * weight
+ * residual and hidden have one type, branch and out another (fp32 or bf16 each);
+ * the norm is of hidden as it is returned.  rms [rows] may be NULL.  codes and
+ * exponents, if not NULL, receive out in 8 bits as mhc_checkpoint8_pack(out) does.
+ * hidden and out may not overlap the inputs.
+ * ------------------------------------------------------------------------- */
+MHC_API int mhc_add_rmsnorm_fwd(const void* residual, int32_t residual_bf16, const void* branch,
+                                int32_t branch_bf16, const float* weight, void* hidden, void* out,
+                                float* rms, int8_t* codes, uint8_t* exponents, int64_t rows,
+                                int64_t cols, float eps, int32_t drop, const uint64_t* state,
+                                uint64_t seed, uint64_t position, void* stream);
+/* The same without dropout, the output as 8-bit codes [rows, cols] (e4m3, or int8 if
+ * codes_int8) with fp32 scales: one a row, or, if grouped, one for each 128 columns
+ * [rows, ceil(cols / 128)].  With a = max |out| of a group, scale =
+ * max(a / 448, 2^-100) (int8: a / 127) and code = out / scale rounded to nearest,
+ * ties to even; a group with an infinity or a NaN has a NaN scale. */
+MHC_API int mhc_add_rmsnorm_coded(const void* residual, int32_t residual_bf16, const void* branch,
+                                  int32_t branch_bf16, const float* weight, void* hidden,
+                                  void* codes, int32_t codes_int8, float* scales, int32_t grouped,
+                                  int64_t rows, int64_t cols, float eps, void* stream);
+/* out = code * scale [rows, cols] */
+MHC_API int mhc_coded8_unpack(const void* codes, int32_t codes_int8, const float* scales,
+                              int32_t grouped, void* out, int32_t out_bf16, int64_t rows,
+                              int64_t cols, void* stream);
+/* Backward of mhc_add_rmsnorm_fwd from its hidden and rms:
+ *   gi = grad_hidden + (g w - hidden sum(g w hidden) / (cols r^2)) / r,  g = grad_out
+ *   grad_residual = gi,  grad_branch = dropout(gi),  grad_weight = sum over rows of g hidden / r
+ * grad_hidden may be NULL (zero), grad_branch too (not wanted: without dropout and
+ * with one type it equals grad_residual).  grad_weight's sums have a fixed order. */
+MHC_API size_t mhc_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
+MHC_API int mhc_add_rmsnorm_bwd(const void* grad_hidden, const void* grad_out, const void* hidden,
+                                int32_t residual_bf16, int32_t branch_bf16, const float* weight,
+                                const float* rms, void* grad_residual, void* grad_branch,
+                                float* grad_weight, int64_t rows, int64_t cols, int32_t drop,
+                                const uint64_t* state, uint64_t seed, uint64_t position,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities of given tokens, entropy and alternatives.  No counterpart in
+ * the reference.  logits [rows, vocab] fp32 or bf16, rows row_stride elements apart,
+ * vocab <= 2^21; targets int64 (targets_64 != 0) or int32.  With m = max x and
+ * s = sum exp(x - m) of a row:
+ *   logprob = x[target] - m - ln s,   entropy = -sum p ln p  (0 ln 0 = 0)
+ *   top_id, top_logprob [rows, top]: the `top` <= 32 largest logits, largest first,
+ *   ties (and +0, -0) to the lowest index; NaNs come last
+ *   stats [rows, 2] = (m, s), what the backward needs beside the entropy
+ * A target equal to ignore_index has logprob 0, any other outside [0, vocab) NaN.  A
+ * logit of -inf has probability 0; a row of nothing else has logprobs -inf and
+ * entropy 0.  A row with +inf or NaN has logprob, entropy and top_logprob NaN.
+ * ------------------------------------------------------------------------- */
+MHC_API int mhc_token_logprobs_fwd(const void* logits, int32_t logits_bf16, int64_t row_stride,
+                                   const void* targets, int32_t targets_64, int64_t ignore_index,
+                                   float* logprob, float* entropy, float* top_logprob,
+                                   int64_t* top_id, float* stats, int64_t rows, int64_t vocab,
+                                   int32_t top, void* stream);
+/* Gradient of the logits [rows, vocab], contiguous, in their type, from the
+ * gradients of the three results (each may be NULL; grad_top and top_id [rows, top]
+ * with top > 0).  A row of nothing but -inf gets zeros; a target outside
+ * [0, vocab) other than ignore_index gives its row NaNs. */
+MHC_API int mhc_token_logprobs_bwd(const void* logits, int32_t logits_bf16, int64_t row_stride,
+                                   const void* targets, int32_t targets_64, int64_t ignore_index,
+                                   const float* stats, const float* entropy, const int64_t* top_id,
+                                   const float* grad_logprob, const float* grad_entropy,
+                                   const float* grad_top, void* grad_logits, int64_t rows,
+                                   int64_t vocab, int32_t top, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Device error word.  No counterpart in the reference.  Kernels that wait on
  * asynchronous copies (TMA + mbarrier) bound every wait; a wait that runs out
  * sets this word to nonzero and the kernel abandons its work (its outputs are

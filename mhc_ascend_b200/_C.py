@@ -17,6 +17,7 @@ c_float_p = ctypes.c_void_p  # device pointers are passed as raw addresses
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
+_U64 = ctypes.c_uint64
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
 
@@ -86,6 +87,16 @@ SIGNATURES = {
     "mhc_checkpoint8_weight_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
     "mhc_checkpoint8_weight_grad": (ctypes.c_int, [_P, _I32, _I64, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _SZ,
                                                    _P]),
+    "mhc_dropout": (ctypes.c_int, [_P, _I32, _P, _I64, _I32, _P, _U64, _U64, _P]),
+    "mhc_dropout_take": (ctypes.c_int, [_P, _P, _I64, _P]),
+    "mhc_add_rmsnorm_fwd": (ctypes.c_int, [_P, _I32, _P, _I32] + [_P] * 6 + [_I64, _I64, _F, _I32, _P, _U64, _U64, _P]),
+    "mhc_add_rmsnorm_coded": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, _P, _I32, _P, _I32, _I64, _I64, _F, _P]),
+    "mhc_coded8_unpack": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _I32, _I64, _I64, _P]),
+    "mhc_add_rmsnorm_bwd_workspace_bytes": (_SZ, [_I64, _I64]),
+    "mhc_add_rmsnorm_bwd": (ctypes.c_int, [_P, _P, _P, _I32, _I32] + [_P] * 5 + [_I64, _I64, _I32, _P, _U64, _U64, _P,
+                                                                                  _SZ, _P]),
+    "mhc_token_logprobs_fwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64] + [_P] * 5 + [_I64, _I64, _I32, _P]),
+    "mhc_token_logprobs_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64] + [_P] * 7 + [_I64, _I64, _I32, _P]),
     "mhc_device_error_word": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int32), ctypes.c_int32]),
     "mhc_profile_enable": (ctypes.c_int, [ctypes.c_int]),
     "mhc_profile_report": (ctypes.c_int, [ctypes.c_char_p, _SZ]),

@@ -23,6 +23,13 @@ from .ops import (
 
 # Operators beyond the reference's API: attributes of the package, left out of
 # __all__, which names exactly what the reference exports.
+from .add_norm import (  # noqa: F401
+    Coded8,
+    add_rmsnorm,
+    add_rmsnorm_bwd,
+    add_rmsnorm_fwd,
+    add_rmsnorm_quantized,
+)
 from .checkpoint8 import (  # noqa: F401
     Checkpoint8,
     checkpoint8_pack,
@@ -34,11 +41,24 @@ from .checkpoint8 import (  # noqa: F401
     rmsnorm_checkpoint8_bwd,
     rmsnorm_checkpoint8_fwd,
 )
+from .counter_dropout import (  # noqa: F401
+    DropoutCounter,
+    StreamDropout,
+    dropout,
+    dropout_fwd,
+    dropout_groups,
+)
 from .embedding import (  # noqa: F401
     StreamEmbedding,
     stream_embedding,
     stream_embedding_bwd,
     stream_embedding_fwd,
+)
+from .logprobs import (  # noqa: F401
+    TokenLogprobs,
+    token_logprobs,
+    token_logprobs_bwd,
+    token_logprobs_fwd,
 )
 
 __all__ = [

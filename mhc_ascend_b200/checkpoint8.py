@@ -233,8 +233,9 @@ class LinearCheckpoint8Function(torch.autograd.Function):
     the gradient of x, which needs no x) are torch's."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        kept = checkpoint8_pack(x)
+    def forward(ctx, x, weight, bias, kept=None):
+        if kept is None:
+            kept = checkpoint8_pack(x)
         ctx.save_for_backward(kept.codes, kept.exponents, weight)
         ctx.kept = (kept.shape, kept.dtype)
         ctx.bias_dtype = None if bias is None else bias.dtype
@@ -251,19 +252,23 @@ class LinearCheckpoint8Function(torch.autograd.Function):
             gw = checkpoint8_weight_grad(grad_out, Checkpoint8(codes, exponents, *ctx.kept), weight.dtype)
         if ctx.needs_input_grad[2]:
             gb = grad_out.reshape(-1, grad_out.size(-1)).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
-        return gx, gw, gb
+        return gx, gw, gb, None
 
 
-def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                       kept: Optional[Checkpoint8] = None) -> torch.Tensor:
     """``torch.nn.functional.linear`` (x, weight and bias of one type, float32 or
     bfloat16) that keeps x in 8 bits for the weight's gradient, and nothing of x
-    where the weight needs none.  Under autocast
+    where the weight needs none.  ``kept`` is x in 8 bits where the caller has it
+    (``add_rmsnorm(..., keep=True)``): x is then not packed again.  Under autocast
     the three are cast to its type first, as for the plain layer."""
     _require_cuda("linear_checkpoint8", x, weight)
+    if kept is not None and (kept.shape != x.shape or kept.codes.device != x.device):
+        raise RuntimeError(f"linear_checkpoint8: kept must be x in 8 bits: {tuple(x.shape)} on {x.device}")
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
         with torch.autocast("cuda", enabled=False):
-            return linear_checkpoint8(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype))
+            return linear_checkpoint8(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype), kept)
     _check_float("linear_checkpoint8", "x", x)
     if weight.dim() != 2:
         raise RuntimeError(f"linear_checkpoint8: weight must be [out_features, in_features] (got {tuple(weight.shape)})")
@@ -271,7 +276,7 @@ def linear_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
         raise RuntimeError("linear_checkpoint8: x, weight and bias must have one type")
     if not (torch.is_grad_enabled() and weight.requires_grad):  # nobody will read the codes
         return torch.nn.functional.linear(x, weight, bias)
-    return LinearCheckpoint8Function.apply(x, weight, bias)
+    return LinearCheckpoint8Function.apply(x, weight, bias, kept)
 
 
 # =============================================================================

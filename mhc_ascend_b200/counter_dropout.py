@@ -1,0 +1,139 @@
+"""Dropout from a counter-based generator, with a mask that is never stored.
+
+Whether a value is dropped is a function of a seed and the value's place in a
+stream of random numbers, so the backward pass draws the same mask again and
+nothing is kept for it.  The same holds for ``checkpoint8_recompute``: a function
+that drops by a given (seed, position) gives the same result when it runs again.
+The reference has no counterpart (its layers draw no random numbers).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Tuple, Union
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .ops import _launch, _require_cuda
+
+GROUP = 8  # positions are counted in groups of eight values
+_FLOATS = (torch.float32, torch.bfloat16)
+_WORD = (1 << 64) - 1
+
+Rng = Union[Tuple[int, int], torch.Tensor]
+
+
+def dropout_groups(shape) -> int:
+    """Positions that a tensor of this shape takes up."""
+    return -(-math.prod(shape) // GROUP)
+
+
+def _drop(what, p):
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"{what}: p must be in [0, 1] (got {p})")
+    return round(p * 65536)
+
+
+def _source(what, rng, device):
+    """(state pointer or None, seed, position) for the C entry points."""
+    if torch.is_tensor(rng):
+        if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
+            raise RuntimeError(f"{what}: rng must be (seed, position) or a contiguous int64 tensor of the two")
+        if rng.device != device:
+            raise RuntimeError(f"{what}: rng must be on {device} (got {rng.device})")
+        return rng.data_ptr(), 0, 0
+    try:
+        seed, position = rng
+        return None, int(seed) & _WORD, int(position) & _WORD
+    except (TypeError, ValueError):
+        raise RuntimeError(f"{what}: rng must be (seed, position) or a contiguous int64 tensor of the two") from None
+
+
+def dropout_fwd(x: torch.Tensor, p: float, rng: Rng) -> torch.Tensor:
+    """x with values dropped (zero) with probability p and the others divided by
+    1 - p: float32 or bfloat16, a contiguous result.  p counts as the nearest
+    multiple of 2**-16.  Applied to a gradient it is the backward pass.
+
+    ``rng`` is (seed, position), or the two in an int64 CUDA tensor, read by the
+    kernel when it runs.  Value i in row-major order is decided by number i % 8 of
+    group position + i // 8 of the seed's stream; x takes up
+    ``dropout_groups(x.shape)`` positions."""
+    what = "dropout"
+    _require_cuda(what, x)
+    if x.dtype not in _FLOATS:
+        raise RuntimeError(f"{what}: x must be float32 or bfloat16 (got {x.dtype})")
+    drop = _drop(what, p)
+    source = _source(what, rng, x.device)
+    xc = x if x.is_contiguous() else x.detach().contiguous()
+    out = torch.empty_like(xc, requires_grad=False)
+    _launch("mhc_dropout", x.device, xc.data_ptr(), x.dtype == torch.bfloat16, out.data_ptr(), xc.numel(), drop, *source)
+    return out
+
+
+class DropoutFunction(torch.autograd.Function):
+    """Dropout that saves where its random numbers start, and no mask."""
+
+    @staticmethod
+    def forward(ctx, x, p, rng):
+        out = dropout_fwd(x, p, rng)
+        ctx.p, ctx.rng = p, None
+        if torch.is_tensor(rng):
+            ctx.save_for_backward(rng)
+        else:
+            ctx.rng = tuple(rng)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        rng = ctx.rng if ctx.rng is not None else ctx.saved_tensors[0]
+        return dropout_fwd(grad_out, ctx.p, rng), None, None
+
+
+def dropout(x: torch.Tensor, p: float, rng: Rng) -> torch.Tensor:
+    """``dropout_fwd`` with autograd.  An ``rng`` tensor must keep its value until
+    the backward pass (``DropoutCounter.take`` returns one that does)."""
+    return DropoutFunction.apply(x, p, rng)
+
+
+class DropoutCounter(nn.Module):
+    """Seed and position of a stream of random numbers, on the device: taking
+    numbers is one small kernel and no host step, so a captured graph takes new
+    ones each time it is replayed.  The state is a buffer of the module: it moves
+    with it and is saved with it."""
+
+    def __init__(self, seed: int = 0, position: int = 0):
+        super().__init__()
+        words = [v & _WORD for v in (int(seed), int(position))]
+        self.register_buffer("state", torch.tensor([v - (1 << 64) if v >> 63 else v for v in words], dtype=torch.int64))
+
+    def take(self, groups: int) -> torch.Tensor:
+        """(seed, position) for the next ``groups`` groups as an int64 tensor of its
+        own, and the position moved past them."""
+        _require_cuda("DropoutCounter.take", self.state)
+        if self.state.dtype != torch.int64 or not self.state.is_contiguous():
+            raise RuntimeError("DropoutCounter.take: state must be a contiguous int64 tensor")
+        out = torch.empty_like(self.state)
+        _launch("mhc_dropout_take", self.state.device, self.state.data_ptr(), out.data_ptr(), int(groups))
+        return out
+
+
+class StreamDropout(nn.Module):
+    """Dropout layer over its own ``DropoutCounter``; the identity in evaluation."""
+
+    def __init__(self, p: float, seed: int = 0):
+        super().__init__()
+        _drop("StreamDropout", p)
+        self.p = float(p)
+        self.counter = DropoutCounter(seed)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return x
+        return dropout(x, self.p, self.counter.take(dropout_groups(x.shape)))
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}"

@@ -1,6 +1,7 @@
 // 8-bit activation checkpoints: pack, restore, and RMSNorm that keeps its
 // input in 8 bits (forward and backward).  Format: checkpoint8.cuh.
 #include "checkpoint8.cuh"
+#include "rows.cuh"
 #include "tma.cuh"
 
 namespace mhc {
@@ -159,36 +160,6 @@ __global__ void __launch_bounds__(kPackThreads)
 // units of 8 columns a thread.  WARP: rows of at most 1024 columns belong to a
 // warp, 8 to a block, and need no barrier; longer ones to a block.
 // ---------------------------------------------------------------------------
-constexpr int kWarpCols = 1024, kWarpRows = 8;
-
-// Sum over the row's threads, the same in each.
-template <bool WARP>
-__device__ __forceinline__ float row_total(float v, float* red) {
-  v = warp_sum(v);
-  if (WARP) return v;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  return warp_sum(lane < nw ? red[lane] : 0.f);
-}
-// Column of a thread's unit k, of the first unit of its warp
-template <bool WARP>
-__device__ __forceinline__ int64_t unit_col(int k) {
-  return 8 * (WARP ? (int64_t)(k * 32 + (threadIdx.x & 31)) : (int64_t)k * blockDim.x + threadIdx.x);
-}
-
-// Eight weights; columns past the end read as zero
-__device__ __forceinline__ void load_w(const float* w, int64_t c, int64_t cols, float (&v)[8]) {
-  if (c + 8 <= cols && (reinterpret_cast<uintptr_t>(w) & 31) == 0) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(w + c)), b = __ldg(reinterpret_cast<const float4*>(w + c + 4));
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? __ldg(w + c + j) : 0.f;
-  }
-}
-
 // Most threads of a block by the share of a row that one thread holds
 constexpr int row_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : UPT == 4 ? 1024 : 512; }
 
@@ -633,28 +604,6 @@ __global__ void __launch_bounds__(kLongThreads)
         if (c + j < cols) part[(int64_t)blockIdx.x * cols + c + j] = p[slot(c, j)];
 }
 
-// gw[c] = sum of part[0..blocks)[c]: 32 columns a block, 8 threads a column,
-// each a fixed share of the partial rows.
-__global__ void __launch_bounds__(256)
-    norm_gw_kernel(const float* __restrict__ part, float* __restrict__ gw, int blocks, int64_t cols) {
-  __shared__ float s[8][32];
-  wait_for_previous();
-  const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  float t = 0.f;
-  if (c < cols)
-#pragma unroll 4
-    for (int b = q; b < blocks; b += 8) t += part[(int64_t)b * cols + c];
-  s[q][lane] = t;
-  __syncthreads();
-  if (q == 0 && c < cols) {
-    float a = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a += s[k][lane];
-    gw[c] = a;
-  }
-}
-
 // How a row is laid over threads: UPT units a thread, `threads` a block; warp:
 // one row a warp; UPT = 0: the row does not fit the registers.
 struct RowPlan {
@@ -673,11 +622,6 @@ RowPlan row_plan(int64_t cols, bool backward) {
     if (th <= row_threads(upt, false)) return {upt, (int)th, false};
   }
   return {0, 1024, false};
-}
-
-template <typename T>
-bool even_rows(const void* p, int64_t cols, int64_t stride) {
-  return (reinterpret_cast<uintptr_t>(p) & (8 * sizeof(T) - 1)) == 0 && cols % 8 == 0 && stride % 8 == 0;
 }
 
 // Units of a row in pack's and unpack's list, and the list's blocks

@@ -1,0 +1,654 @@
+// Log probabilities of given tokens, with entropy and the most likely
+// alternatives, and the gradient of the logits.
+//
+// With m = max x, s = sum exp(x - m) over a row of logits:
+//   log p_j = x_j - m - ln s,   H = ln s + sum exp(x - m) (m - x) / s
+// (both terms of H are >= 0: nothing cancels).  One pass over the row: a thread
+// keeps a running maximum, sum and sum of e t, t = (x - m) log2 e, and rescales
+// them when its maximum moves.  Minus infinity has probability 0 and adds nothing;
+// a row without anything else has s = 0.
+//
+// The k most likely, ties to the lowest index, in the same pass: every thread also
+// notes the maximum of each of its 32-value segments.  The k-th largest of the
+// threads' maxima bounds the k-th largest value from below, so only segments whose
+// maximum reaches it are read again (k of them unless values tie), and what reaches
+// it there is ranked by counting.  Where many values tie, or fewer than k threads
+// have any finite value, the k are taken one after the other instead.
+#include <cooperative_groups.h>
+
+#include "checkpoint8.cuh"
+
+namespace mhc {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr int kPer = 32;          // values of a thread's segment
+constexpr int kMostTop = 32;
+constexpr int kSegments = 128;    // segments and candidates that the fast selection takes
+constexpr int kCandidates = 512;
+constexpr int kMostTiles = 16;    // segments of a thread
+constexpr int kMostCluster = 8;
+
+__device__ __forceinline__ float minus_inf() { return __uint_as_float(0xff800000u); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// the larger; NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+constexpr float kTiny = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * inf out of e t
+
+// ---------------------------------------------------------------------------
+// A row as vectors of 16 bytes from the aligned address at or below its start;
+// the vectors at its ends are read value by value, with -inf outside the row.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Row {
+  static constexpr int VE = 16 / (int)sizeof(T);  // values of a vector
+  const T* base;  // aligned; value e of the row is base[shift + e]
+  int shift;
+  int64_t full0, full1, count, V;  // whole vectors, all vectors
+  __device__ __forceinline__ Row(const T* row, int64_t vocab) {
+    shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    base = row - shift;
+    V = vocab;
+    count = (shift + vocab + VE - 1) / VE;
+    full0 = shift ? 1 : 0;
+    full1 = (shift + vocab) / VE;
+  }
+  __device__ __forceinline__ int64_t index(int64_t v) const { return v * VE - shift; }  // of the vector's first value
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 load_vec(const Row<T>& r, int64_t v, int64_t end) {
+  if (v >= r.full0 && v < r.full1 && v < end) return *reinterpret_cast<const uint4*>(r.base + v * Row<T>::VE);
+  uint32_t w[4];
+  if (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t e = r.index(v) + j;
+      w[j] = v < end && e >= 0 && e < r.V ? reinterpret_cast<const uint32_t*>(r.base)[v * 4 + j] : 0xff800000u;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = 0u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t e = r.index(v) + 2 * j + i;
+        const uint32_t h =
+            v < end && e >= 0 && e < r.V ? reinterpret_cast<const uint16_t*>(r.base)[v * 8 + 2 * j + i] : 0xff80u;
+        w[j] |= h << (16 * i);
+      }
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Values 2 i and 2 i + 1 of a vector
+template <typename T>
+__device__ __forceinline__ float2 two(const uint4& u, int i) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4 (&u)[kPer / Row<T>::VE]) {
+  if (sizeof(T) == 4) {
+    float m = minus_inf();
+#pragma unroll
+    for (int q = 0; q < kPer / Row<T>::VE; ++q)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[q].x), __uint_as_float(u[q].y)),
+                         fmaxf(__uint_as_float(u[q].z), __uint_as_float(u[q].w))));
+    return m;
+  }
+  uint32_t m = 0xff80ff80u;
+  auto up = [&](uint32_t w) { asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w)); };
+#pragma unroll
+  for (int q = 0; q < kPer / Row<T>::VE; ++q) {
+    up(u[q].x);
+    up(u[q].y);
+    up(u[q].z);
+    up(u[q].w);
+  }
+  return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+}
+
+// ---------------------------------------------------------------------------
+// Order of the alternatives: a 64-bit key, larger first; no two are equal.
+// NaNs come last.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t key_of(float x, int64_t index) {
+  const uint32_t b = __float_as_uint(x + 0.f);  // one zero
+  const uint32_t o = x != x ? 0u : b ^ ((int32_t)b < 0 ? 0xffffffffu : 0x80000000u);
+  return (uint64_t)o << 32 | (uint32_t)~(uint32_t)index;
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return o == 0u ? __uint_as_float(0x7fc00000u) : __uint_as_float(o ^ ((int32_t)o < 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~(uint32_t)key; }
+
+__device__ __forceinline__ float bitonic_step(float v, int j, bool larger_low) {
+  const float o = __shfl_xor_sync(0xffffffffu, v, j);
+  const bool low = ((threadIdx.x & 31) & j) == 0;
+  return low == larger_low ? fmaxf(v, o) : fminf(v, o);
+}
+// Largest in lane 0
+__device__ __forceinline__ float warp_sort(float v) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) v = bitonic_step(v, j, ((threadIdx.x & 31) & k) == 0);
+  return v;
+}
+__device__ __forceinline__ float warp_merge(float v) {  // of a bitonic sequence
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) v = bitonic_step(v, j, true);
+  return v;
+}
+__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+struct Part {
+  float m, s, h;
+};
+// Bring a part to the maximum M >= its own
+__device__ __forceinline__ void rebase(Part& p, float M) {
+  const float t = fmaxf((p.m - M) * kLog2e, -1e30f), c = ex2(t);
+  p.h = c * fmaf(p.s, t, p.h);
+  p.s *= c;
+  p.m = M;
+}
+
+struct TopShared {
+  uint64_t best[kMostTop], joined[kMostTop];  // of the block, of the row's blocks together
+  uint64_t cand[kCandidates];
+  float lists[16][32];
+  uint64_t warps[16];
+  int seg[kSegments];
+  float bound;
+  int segments, candidates;
+};
+
+// The k largest keys of the vectors [v0, v1) of a row into sh.best, in order (0:
+// none left).  segmax: maxima of the threads' segments; tm: of all of a thread's.
+template <typename T, int THREADS>
+__device__ void select_top(const Row<T>& r, int64_t v0, int64_t v1, int k, int tiles, const float* segmax, float tm,
+                           TopShared& sh) {
+  constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float v = warp_sort(tm);
+  if (tid == 0) sh.segments = sh.candidates = 0;
+#pragma unroll
+  for (int half = W / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) sh.lists[warp][lane] = v;
+    __syncthreads();
+    if (warp < half) v = warp_merge(fmaxf(v, sh.lists[warp + half][31 - lane]));
+  }
+  if (tid == k - 1) sh.bound = v;  // k <= 32: a lane of warp 0
+  __syncthreads();
+  const float bound = sh.bound;
+  bool fast = bound > minus_inf();
+  if (fast) {
+    for (int it = 0; it < tiles; ++it)
+      if (segmax[it * THREADS + tid] >= bound) {
+        const int i = atomicAdd(&sh.segments, 1);
+        if (i < kSegments) sh.seg[i] = it * THREADS + tid;
+      }
+    __syncthreads();
+    const int n = sh.segments;
+    fast = n <= kSegments;
+    if (fast) {
+      for (int i = tid; i < n * VPT; i += THREADS) {
+        const int g = sh.seg[i / VPT];
+        const int64_t vec = v0 + (int64_t)(g / THREADS) * (THREADS * VPT) + (i % VPT) * THREADS + g % THREADS;
+        const uint4 u = load_vec(r, vec, v1);
+#pragma unroll
+        for (int j = 0; j < VE / 2; ++j) {
+          const float2 x = two<T>(u, j);
+          if (x.x >= bound) {
+            const int c = atomicAdd(&sh.candidates, 1);
+            if (c < kCandidates) sh.cand[c] = key_of(x.x, r.index(vec) + 2 * j);
+          }
+          if (x.y >= bound) {
+            const int c = atomicAdd(&sh.candidates, 1);
+            if (c < kCandidates) sh.cand[c] = key_of(x.y, r.index(vec) + 2 * j + 1);
+          }
+        }
+      }
+      __syncthreads();
+      const int c = sh.candidates;
+      fast = c <= kCandidates;
+      if (fast) {
+        for (int i = tid; i < c; i += THREADS) {
+          const uint64_t mine = sh.cand[i];
+          int rank = 0;
+          for (int j = 0; j < c; ++j) rank += sh.cand[j] > mine;
+          if (rank < k) sh.best[rank] = mine;
+        }
+      }
+    }
+  }
+  if (!fast) {  // one after the other; a thread looks again only when its best is taken
+    auto below = [&](uint64_t prev) {
+      uint64_t best = 0;
+      for (int64_t vec = v0 + tid; vec < v1; vec += THREADS) {
+        const uint4 u = load_vec(r, vec, v1);
+#pragma unroll
+        for (int j = 0; j < VE / 2; ++j) {
+          const float2 x = two<T>(u, j);
+          const int64_t e = r.index(vec) + 2 * j;
+          const uint64_t a = key_of(x.x, e), b = key_of(x.y, e + 1);
+          if (e >= 0 && e < r.V && a < prev && a > best) best = a;
+          if (e + 1 >= 0 && e + 1 < r.V && b < prev && b > best) best = b;
+        }
+      }
+      return best;
+    };
+    uint64_t mine = below(~0ull);
+    for (int i = 0; i < k; ++i) {
+      const uint64_t w = warp_max(mine);
+      __syncthreads();  // everyone has read the last round's
+      if (lane == 0) sh.warps[warp] = w;
+      __syncthreads();
+      const uint64_t top = warp_max(lane < W ? sh.warps[lane] : 0ull);
+      if (tid == 0) sh.best[i] = top;
+      if (top != 0 && mine == top) mine = below(top);
+    }
+  }
+  __syncthreads();
+}
+
+struct FwdArgs {
+  const void* logits;
+  int64_t stride, rows, V;
+  const void* targets;
+  int64_t ignore;
+  float *logprob, *entropy, *top_logprob, *stats;
+  int64_t* top_id;
+  int top, tiles;
+  bool ids64;
+};
+__device__ __forceinline__ int64_t target_of(const void* t, bool ids64, int64_t row) {
+  return ids64 ? static_cast<const int64_t*>(t)[row] : (int64_t)static_cast<const int32_t*>(t)[row];
+}
+__device__ __forceinline__ float value_of(const float* p) { return *p; }
+__device__ __forceinline__ float value_of(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// One row a cluster of CL blocks, each over its share of the row's vectors; block
+// 0 joins the shares through distributed shared memory.
+template <typename T, int THREADS, bool TOP, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS) logprobs_fwd_kernel(const FwdArgs p) {
+  constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  float* segmax = reinterpret_cast<float*>(dyn);
+  TopShared& sh = *reinterpret_cast<TopShared*>(dyn + (size_t)p.tiles * THREADS * sizeof(float));
+  __shared__ float red[3][W];
+  __shared__ Part part;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int CL = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
+  const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
+  const int64_t row = CLUSTER ? blockIdx.x / CL : blockIdx.x;
+  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
+  const int64_t each = (r.count + CL - 1) / CL;
+  const int64_t v0 = rank * each < r.count ? rank * each : r.count;
+  const int64_t v1 = v0 + each < r.count ? v0 + each : r.count;
+
+  float m = kLowest, tm = minus_inf();
+  float2 s2 = make_float2(0.f, 0.f), h2 = make_float2(0.f, 0.f);
+  int it = 0;
+  for (int64_t a = v0; a < v1; a += THREADS * VPT, ++it) {
+    uint4 u[VPT];
+#pragma unroll
+    for (int q = 0; q < VPT; ++q) u[q] = load_vec(r, a + q * THREADS + tid, v1);
+    const float mx = vec_max<T>(u);
+    if (TOP) {
+      segmax[it * THREADS + tid] = mx;
+      tm = fmaxf(tm, mx);
+    }
+    if (mx > m) {
+      const float t = fmaxf((m - mx) * kLog2e, -1e30f), c = ex2(t);
+      h2.x = c * fmaf(s2.x, t, h2.x);
+      h2.y = c * fmaf(s2.y, t, h2.y);
+      s2.x *= c;
+      s2.y *= c;
+      m = mx;
+    }
+    const float2 minus = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
+#pragma unroll
+    for (int q = 0; q < VPT; ++q)
+#pragma unroll
+      for (int j = 0; j < VE / 2; ++j) {
+        float2 t = __fmul2_rn(__fadd2_rn(two<T>(u[q], j), minus), scale);
+        t.x = max_nan(t.x, kTiny);
+        t.y = max_nan(t.y, kTiny);
+        const float2 e = make_float2(ex2(t.x), ex2(t.y));
+        s2 = __fadd2_rn(s2, e);
+        h2 = __ffma2_rn(e, t, h2);
+      }
+  }
+  // the threads' parts
+  Part mine = {m, s2.x + s2.y, h2.x + h2.y};
+  float M = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  rebase(mine, M);
+  mine.s = warp_sum(mine.s);
+  mine.h = warp_sum(mine.h);
+  if (lane == 0) {
+    red[0][warp] = M;
+    red[1][warp] = mine.s;
+    red[2][warp] = mine.h;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    Part w = {kLowest, 0.f, 0.f};
+    if (lane < W) w = {red[0][lane], red[1][lane], red[2][lane]};
+    M = w.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    rebase(w, M);
+    w.s = warp_sum(w.s);
+    w.h = warp_sum(w.h);
+    if (lane == 0) part = w;
+  }
+  if (TOP) select_top<T, THREADS>(r, v0, v1, p.top, it, segmax, tm, sh);
+  if (CLUSTER) {
+    cg::this_cluster().sync();
+    if (rank == 0) {
+      if (tid == 0) {
+        Part all = part;
+        for (int b = 1; b < CL; ++b) {
+          Part o = *cg::this_cluster().map_shared_rank(&part, b);
+          const float top = fmaxf(all.m, o.m);
+          rebase(all, top);
+          rebase(o, top);
+          all.s += o.s;
+          all.h += o.h;
+        }
+        part = all;
+      }
+      if (TOP) {
+        uint64_t* all = sh.cand;
+        for (int i = tid; i < CL * p.top; i += THREADS)
+          all[i] = cg::this_cluster().map_shared_rank(sh.best, i / p.top)[i % p.top];
+        __syncthreads();
+        for (int i = tid; i < CL * p.top; i += THREADS) {
+          const uint64_t key = all[i];
+          int place = 0;
+          for (int j = 0; j < CL * p.top; ++j) place += all[j] > key;
+          if (key != 0 && place < p.top) sh.joined[place] = key;
+        }
+      }
+    }
+    cg::this_cluster().sync();  // the others' shared memory has been read
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  const Part all = part;
+  const bool none = all.s == 0.f;
+  const float ln_s = logf(all.s);
+  if (TOP) {
+    const uint64_t* best = CLUSTER ? sh.joined : sh.best;
+    if (tid < p.top) {
+      const uint64_t key = best[tid];
+      p.top_logprob[row * p.top + tid] = none ? minus_inf() : (key_value(key) - all.m) - ln_s;
+      p.top_id[row * p.top + tid] = (int64_t)key_index(key);
+    }
+  }
+  if (tid == 0) {
+    const int64_t t = target_of(p.targets, p.ids64, row);
+    float lp = __uint_as_float(0x7fc00000u);
+    if (t == p.ignore) lp = 0.f;
+    else if (t >= 0 && t < p.V) lp = none ? minus_inf() : (value_of(r.base + r.shift + t) - all.m) - ln_s;
+    p.logprob[row] = lp;
+    p.entropy[row] = none ? 0.f : ln_s - all.h * kLn2 / all.s;
+    p.stats[2 * row] = all.m;
+    p.stats[2 * row + 1] = all.s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Gradient, from the row's m, s and H:
+//   gx_j = -p_j (G + gH (ln p_j + H)) + the given tokens' own gradients,
+//   G = g_logprob + sum g_top
+// and with t = (x - m) log2 e, e = 2^t: gx = e (A + B t).  The few places that have
+// a gradient of their own are written again after the block's others.
+// ---------------------------------------------------------------------------
+struct BwdArgs {
+  const void* logits;
+  int64_t stride, rows, V;
+  const void* targets;
+  int64_t ignore;
+  const float *stats, *entropy, *g_logprob, *g_entropy, *g_top;
+  const int64_t* top_id;
+  void* gx;
+  int top;
+  int64_t chunks;
+  bool ids64;
+};
+constexpr int kBwdThreads = 256;
+
+__device__ __forceinline__ float grad_of(float x, float m, float A, float B) {
+  const float t = max_nan((x - m) * kLog2e, kTiny);
+  return ex2(t) * fmaf(B, t, A);
+}
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs p) {
+  constexpr int VE = Row<T>::VE, VPT = kPer / VE;
+  __shared__ int64_t at[kMostTop + 1];
+  __shared__ float own[kMostTop + 1];
+  const int tid = threadIdx.x, B_ = blockDim.x;
+  const int64_t row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
+  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
+  T* out = static_cast<T*>(p.gx) + row * p.V;
+  const int64_t a = chunk * ((int64_t)B_ * VPT);
+  uint4 u[VPT];
+#pragma unroll
+  for (int q = 0; q < VPT; ++q) u[q] = load_vec(r, a + q * B_ + tid, r.count);
+  const float m = p.stats[2 * row], s = p.stats[2 * row + 1];
+  const bool none = s == 0.f;
+  for (int i = tid; i <= p.top; i += B_) {
+    if (i == 0) {
+      const int64_t t = target_of(p.targets, p.ids64, row);
+      const float g = p.g_logprob ? p.g_logprob[row] : 0.f;
+      const bool in = t >= 0 && t < p.V;
+      at[0] = in && t != p.ignore ? t : -1;
+      own[0] = t == p.ignore ? 0.f : in ? g : g * __uint_as_float(0x7fc00000u);
+    } else {
+      at[i] = p.top_id[row * p.top + i - 1];
+      own[i] = p.g_top[row * p.top + i - 1];
+    }
+  }
+  __syncthreads();
+  float G = own[0];
+  for (int i = 1; i <= p.top; ++i) G += own[i];
+  float A = 0.f, B = 0.f;
+  if (!none) {
+    const float gh = p.g_entropy ? p.g_entropy[row] : 0.f, inv = 1.0f / s;
+    A = -inv * fmaf(gh, p.entropy[row] - logf(s), G);
+    B = -inv * gh * kLn2;
+  }
+  const bool same = ((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) == (uintptr_t)r.shift;
+  const float2 A2 = make_float2(A, A), B2 = make_float2(B, B), minus = make_float2(-m, -m),
+               scale = make_float2(kLog2e, kLog2e);
+#pragma unroll
+  for (int q = 0; q < VPT; ++q) {
+    const int64_t v = a + q * B_ + tid;
+    if (v >= r.count) continue;
+    float o[VE];
+#pragma unroll
+    for (int j = 0; j < VE / 2; ++j) {
+      float2 t = __fmul2_rn(__fadd2_rn(two<T>(u[q], j), minus), scale);
+      t.x = max_nan(t.x, kTiny);
+      t.y = max_nan(t.y, kTiny);
+      const float2 g = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), __ffma2_rn(B2, t, A2));
+      o[2 * j] = g.x;
+      o[2 * j + 1] = g.y;
+    }
+    const int64_t e = r.index(v);
+    if (same && v >= r.full0 && v < r.full1) {
+      uint4 w;
+      if (sizeof(T) == 4) {
+        w = make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
+      } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(o[(2 * j) % VE], o[(2 * j + 1) % VE]);
+          h[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        w = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      *reinterpret_cast<uint4*>(out + e) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < VE; ++j)
+        if (e + j >= 0 && e + j < p.V) put(out + e + j, o[j]);
+    }
+  }
+  if (none) return;
+  __syncthreads();  // before these places are written again
+  const int64_t lo = r.index(a), hi = r.index(a + (int64_t)B_ * VPT);
+  for (int i = tid; i <= p.top; i += B_) {
+    const int64_t e = at[i];
+    if (e < 0 || e >= p.V || e < lo || e >= hi) continue;
+    float g = 0.f;
+    bool first = true;
+    for (int j = 0; j <= p.top; ++j)
+      if (at[j] == e) {
+        first = first && j >= i;
+        g += own[j];
+      }
+    if (first) put(out + e, g + grad_of(value_of(r.base + r.shift + e), m, A, B));
+  }
+}
+
+template <typename T, int THREADS, bool TOP>
+int launch_fwd(FwdArgs p, int CL, cudaStream_t st) {
+  constexpr int VE = Row<T>::VE;
+  const int64_t count = (p.V + VE - 1) / VE + 1, each = (count + CL - 1) / CL;
+  p.tiles = (int)((each + THREADS * (kPer / VE) - 1) / (THREADS * (kPer / VE)));
+  const size_t smem = TOP ? (size_t)p.tiles * THREADS * sizeof(float) + sizeof(TopShared) : 0;
+  ProfScope prof("token_logprobs_fwd", st);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)CL;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.rows * CL));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = CL > 1 ? 1 : 0;
+  if (CL > 1) cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, THREADS, TOP, true>, p);
+  else cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, THREADS, TOP, false>, p);
+  return check_launch("token_logprobs_fwd");
+}
+
+template <typename T>
+int pick_fwd(const FwdArgs& p, cudaStream_t st) {
+  // few rows: several blocks a row, so that the GPU is filled
+  int CL = 1;
+  while (CL < kMostCluster && p.rows * CL * 2 <= 2 * num_sms() && p.V >= (int64_t)CL * 2 * 2048) CL *= 2;
+  // a thread has at most kMostTiles segments
+  while (p.top > 0 && CL < kMostCluster && p.V + 16 > (int64_t)CL * 512 * kPer * kMostTiles) CL *= 2;
+  MHC_REQUIRE(p.rows * CL < (1ll << 31), MHC_ERR_UNSUPPORTED, "token_logprobs: %lld rows are too many", (long long)p.rows);
+  const bool small = (p.V + CL - 1) / CL <= 8192;
+  if (p.top > 0) return small ? launch_fwd<T, 128, true>(p, CL, st) : launch_fwd<T, 512, true>(p, CL, st);
+  return small ? launch_fwd<T, 128, false>(p, CL, st) : launch_fwd<T, 512, false>(p, CL, st);
+}
+
+int check_args(const char* what, int64_t rows, int64_t vocab, int64_t stride, int32_t top, int32_t bf16, const void* logits) {
+  MHC_REQUIRE(rows >= 0 && vocab >= 1, MHC_ERR_INVALID_ARG, "%s: rows must be >= 0 and vocab >= 1 (got %lld x %lld)", what,
+              (long long)rows, (long long)vocab);
+  MHC_REQUIRE(rows < (1ll << 31) && vocab <= (1ll << 21), MHC_ERR_UNSUPPORTED,
+              "%s: at most 2^31 - 1 rows of 2^21 logits (got %lld x %lld)", what, (long long)rows, (long long)vocab);
+  MHC_REQUIRE(stride >= vocab || rows <= 1, MHC_ERR_INVALID_ARG, "%s: row_stride %lld < vocab %lld", what, (long long)stride,
+              (long long)vocab);
+  MHC_REQUIRE(top >= 0 && top <= kMostTop && top <= vocab, MHC_ERR_UNSUPPORTED, "%s: top must be in [0, min(32, vocab)] (got %d)",
+              what, (int)top);
+  MHC_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (bf16 ? 1 : 3)) == 0, MHC_ERR_ALIGNMENT,
+              "%s: logits must be aligned to their type", what);
+  return MHC_OK;
+}
+
+}  // namespace
+}  // namespace mhc
+
+using namespace mhc;
+
+extern "C" int mhc_token_logprobs_fwd(const void* logits, int32_t logits_bf16, int64_t row_stride, const void* targets,
+                                      int32_t targets_64, int64_t ignore_index, float* logprob, float* entropy,
+                                      float* top_logprob, int64_t* top_id, float* stats, int64_t rows, int64_t vocab,
+                                      int32_t top, void* stream) {
+  const char* what = "token_logprobs_fwd";
+  const int rc = check_args(what, rows, vocab, row_stride, top, logits_bf16, logits);
+  if (rc) return rc;
+  if (rows == 0) return MHC_OK;
+  MHC_REQUIRE_PTR(logits);
+  MHC_REQUIRE_PTR(targets);
+  MHC_REQUIRE_PTR(logprob);
+  MHC_REQUIRE_PTR(entropy);
+  MHC_REQUIRE_PTR(stats);
+  if (top > 0) {
+    MHC_REQUIRE_PTR(top_logprob);
+    MHC_REQUIRE_PTR(top_id);
+  }
+  const FwdArgs p = {logits, row_stride, rows, vocab, targets, ignore_index, logprob, entropy, top_logprob, stats, top_id,
+                     (int)top, 0, targets_64 != 0};
+  return logits_bf16 ? pick_fwd<__nv_bfloat16>(p, (cudaStream_t)stream) : pick_fwd<float>(p, (cudaStream_t)stream);
+}
+
+extern "C" int mhc_token_logprobs_bwd(const void* logits, int32_t logits_bf16, int64_t row_stride, const void* targets,
+                                      int32_t targets_64, int64_t ignore_index, const float* stats, const float* entropy,
+                                      const int64_t* top_id, const float* grad_logprob, const float* grad_entropy,
+                                      const float* grad_top, void* grad_logits, int64_t rows, int64_t vocab, int32_t top,
+                                      void* stream) {
+  const char* what = "token_logprobs_bwd";
+  const int rc = check_args(what, rows, vocab, row_stride, top, logits_bf16, logits);
+  if (rc) return rc;
+  if (rows == 0) return MHC_OK;
+  MHC_REQUIRE_PTR(logits);
+  MHC_REQUIRE_PTR(targets);
+  MHC_REQUIRE_PTR(stats);
+  MHC_REQUIRE_PTR(entropy);
+  MHC_REQUIRE_PTR(grad_logits);
+  if (top > 0) {
+    MHC_REQUIRE_PTR(top_id);
+    MHC_REQUIRE_PTR(grad_top);
+  }
+  const int per = kPer / (logits_bf16 ? 8 : 4);
+  const int64_t count = (vocab + (logits_bf16 ? 8 : 4) - 1) / (logits_bf16 ? 8 : 4) + 1;  // with a start that is not aligned
+  int64_t threads = ((count + per - 1) / per + 31) / 32 * 32;
+  threads = threads > kBwdThreads ? kBwdThreads : threads;
+  const int64_t chunks = (count + threads * per - 1) / (threads * per);
+  MHC_REQUIRE(rows * chunks < (1ll << 31), MHC_ERR_UNSUPPORTED, "%s: %lld x %lld logits are too many", what, (long long)rows,
+              (long long)vocab);
+  const BwdArgs p = {logits, row_stride, rows, vocab, targets, ignore_index, stats, entropy, grad_logprob, grad_entropy,
+                     grad_top, top_id, grad_logits, (int)top, chunks, targets_64 != 0};
+  cudaStream_t st = (cudaStream_t)stream;
+  ProfScope prof(what, st);
+  if (logits_bf16) logprobs_bwd_kernel<__nv_bfloat16><<<(unsigned)(rows * chunks), (unsigned)threads, 0, st>>>(p);
+  else logprobs_bwd_kernel<float><<<(unsigned)(rows * chunks), (unsigned)threads, 0, st>>>(p);
+  return check_launch(what);
+}
