@@ -8,211 +8,254 @@
 #include "coded8.cuh"
 #include "dropout.cuh"
 #include "rows.cuh"
+#include "vec8.cuh"
 
 namespace mhc {
 namespace {
 
-template <typename TR, typename TB>
 struct FwdArgs {
-  const TR* res;
-  const TB* branch;
+  const void *res, *branch;
   const float* w;
-  TR* hidden;
-  float* rms;  // nullable
-  TB* out;     // plain output
+  void* hidden;
+  float* rms;     // nullable
+  void* out;      // plain output
   int8_t* codes;  // its checkpoint, or the codes (nullable in the plain form)
   uint8_t* exps;
   float* scales;
   int64_t rows, cols, pitch, groups;
   float eps;
-  bool int8, grouped;
+  bool int8, grouped, res16, branch16;
   DropSource drop;
 };
 
-// Sum of `a` and largest `m` over the row's threads, the same in each.
-template <bool WARP>
-__device__ __forceinline__ void row_sum_max(float& a, uint32_t& m, float* red, uint32_t* redm) {
+// Sum of `a` and largest `m` (NaN if any is) over the row's threads, the same in each.
+template <bool WARP, bool MAX>
+__device__ __forceinline__ void row_sum_max(float& a, float& m, float* red, float* redm) {
+  auto warp_max_nan = [](float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_abs_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
   a = warp_sum(a);
-  m = __reduce_max_sync(0xffffffffu, m);
+  if (MAX) m = warp_max_nan(m);
   if (WARP) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   if (lane == 0) {
     red[warp] = a;
-    redm[warp] = m;
+    if (MAX) redm[warp] = m;
   }
   __syncthreads();
   a = warp_sum(lane < nw ? red[lane] : 0.f);
-  m = __reduce_max_sync(0xffffffffu, lane < nw ? redm[lane] : 0u);
+  if (MAX) m = warp_max_nan(lane < nw ? redm[lane] : 0.f);
+}
+__device__ __forceinline__ float group_max(float m) {  // over 16 lanes, NaN if any is
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
 }
 
-__device__ __forceinline__ float rounded_as(float v, const float*) { return v; }
-__device__ __forceinline__ float rounded_as(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16_rn(v)); }
+constexpr int fwd_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : UPT == 2 ? 512 : 1024; }
 
-// h of a unit: residual + branch (dropped), rounded to the residual's type
-template <bool EVEN, typename TR, typename TB>
-__device__ __forceinline__ void add_unit(const FwdArgs<TR, TB>& p, const DropKey& key, int64_t row, int64_t c, float (&v)[8],
-                                         float (&b)[8]) {
-  if (p.drop.drop) {
-    const uint64_t i = (uint64_t)row * (uint64_t)p.cols + (uint64_t)c;
-    if (EVEN) drop_apply(drop_group(key, i / kDropGroup), p.drop.drop, p.drop.scale, b);
-    else drop_apply_at(key, i, p.drop.drop, p.drop.scale, b);
+// Rows that wide accesses fit.  A row stays in registers between the sum and the
+// output, UPT units a thread.  CODED: what is kept is h w, and its maxima are taken
+// with the sum (r > 0 is common to the row: max |y| = max |h w| / r), so that after
+// the barrier a value costs one product and its conversion.
+template <typename TR, typename TB, int UPT, bool WARP, bool CODED>
+__global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_kernel(const FwdArgs p) {
+  __shared__ float red[32], redm[32];
+  const int lane = threadIdx.x & 31, cols = (int)p.cols;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (WARP && row >= p.rows) return;
+  const int c0 = 8 * (WARP ? lane : (int)threadIdx.x), step = 8 * (WARP ? 32 : (int)blockDim.x);
+  const int64_t at = row * p.cols + c0;
+  const TR* rr = static_cast<const TR*>(p.res) + at;
+  const TB* br = static_cast<const TB*>(p.branch) + at;
+  TR* hr = static_cast<TR*>(p.hidden) + at;
+  Raw8<TR> a[UPT];
+  Raw8<TB> b[UPT];
+#pragma unroll
+  for (int k = 0; k < UPT; ++k) {
+    a[k].zero();
+    b[k].zero();
+    if (c0 + k * step < cols) {
+      a[k].load(rr + k * step);
+      b[k].load(br + k * step);
+    }
   }
+  const DropKey key = drop_key(p.drop);
+  V8 v[UPT];
+  float2 s2 = make_float2(0.f, 0.f);
+  float am = 0.f, gm[UPT];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = rounded_as(v[j] + b[j], p.hidden);
-}
-
-// Output of a unit: h in v, weights in wv
-template <bool EVEN, bool CODED, typename TR, typename TB>
-__device__ __forceinline__ void put_unit(const FwdArgs<TR, TB>& p, int64_t row, int64_t c, float (&v)[8], const float (&wv)[8],
-                                         float ir, float row_scale, float* mine) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = v[j] * ir * wv[j];
+  for (int k = 0; k < UPT; ++k) {
+    V8 x = b[k].values();
+    if (!CODED && p.drop.drop) {
+      float f[8];
+      v8_spread(x, f);
+      drop_apply(drop_group(key, (uint64_t)(at + k * step) / kDropGroup), p.drop.drop, p.drop.scale, f);
+      x = v8_gather(f);
+    }
+    v[k] = v8_add(a[k].values(), x);
+    const bool on = c0 + k * step < cols;
+    if (on) v8_save_rounded(hr + k * step, v[k]);
+    s2 = v8_dot(v[k], v[k], s2);
+    if (CODED) {
+      if (on) v[k] = v8_mul(v[k], v8_weights(p.w + c0 + k * step));
+      gm[k] = v8_max_abs(v[k]);
+      if (p.grouped) gm[k] = group_max(gm[k]);  // 16 lanes hold a group
+      else am = max_abs_nan(am, gm[k]);
+    }
+  }
+  float ss = s2.x + s2.y;
+  row_sum_max<WARP, CODED>(ss, am, red, redm);
+  const float r = sqrtf(ss / (float)cols + p.eps), ir = 1.0f / r;
+  const bool first = WARP ? lane == 0 : threadIdx.x == 0;
+  if (first && p.rms) p.rms[row] = r;
   if (CODED) {
-    float scale = row_scale;
-    if (p.grouped) {  // 16 lanes hold a group
-      uint32_t m = abs_bits(v[0]);
+    const float scale = coded_scale(am * ir, p.int8);
+    if (first && !p.grouped) p.scales[row] = scale;
+    uint8_t* to = reinterpret_cast<uint8_t*>(p.codes) + at;
 #pragma unroll
-      for (int j = 1; j < 8; ++j) m = max(m, abs_bits(v[j]));
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      scale = coded_scale(__uint_as_float(m), p.int8);
-      if (c < p.cols && (lane & 15) == 0) p.scales[row * p.groups + c / kCodedGroup] = scale;
+    for (int k = 0; k < UPT; ++k) {
+      const int c = c0 + k * step;
+      float s = scale;
+      if (p.grouped) {
+        s = coded_scale(gm[k] * ir, p.int8);
+        if ((lane & 15) == 0 && c < cols) p.scales[row * p.groups + c / kCodedGroup] = s;
+      }
+      float f[8];
+      v8_spread(v8_scale(v[k], ir * coded_inverse(s)), f);
+      if (c < cols) *reinterpret_cast<uint2*>(to + k * step) = coded_pack(f, p.int8);
     }
-    const float inv = 1.0f / scale;
+    return;
+  }
+  TB* out = static_cast<TB*>(p.out) + at;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= inv;
-    uint8_t* to = reinterpret_cast<uint8_t*>(p.codes) + row * p.cols;
-    if (EVEN) {
-      if (c < p.cols) *reinterpret_cast<uint2*>(to + c) = coded_pack(v, p.int8);
-    } else {
-      coded_save_any(to, c - 8 * lane, p.cols, mine, v, p.int8);
-    }
-  } else {
-    if (EVEN) {
-      if (c < p.cols) ck_save(p.out + row * p.cols + c, v);
-    } else {
-      ck_save_any(p.out + row * p.cols, c - 8 * lane, p.cols, mine, v);
+  for (int k = 0; k < UPT; ++k) {
+    const int c = c0 + k * step;
+    V8 y = v8_zero();
+    if (c < cols) {
+      y = v8_mul(v8_scale(v[k], ir), v8_weights(p.w + c));
+      v8_save_rounded(out + k * step, y);
     }
     if (p.codes) {  // of the output as it is returned
+      float f[8];
+      v8_spread(y, f);
+      ck_encode(f, p.codes + row * p.pitch, p.exps + row * (p.pitch / kCkBlock), c, c < p.pitch);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Any row: through shared memory, and types by a branch.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float rounded_as(float v, bool b16) { return b16 ? __bfloat162float(__float2bfloat16_rn(v)) : v; }
+
+// h of a unit: stored, and its share of the sum and of the maximum
+template <bool CODED>
+__device__ __forceinline__ void add_unit_any(const FwdArgs& p, const DropKey& key, int64_t row, int64_t c, float* mine,
+                                             float (&v)[8], float& ss, float& am) {
+  float b[8];
+  load_any(p.res, p.res16, row, c, p.cols, mine, v);
+  load_any(p.branch, p.branch16, row, c, p.cols, mine, b);
+  if (p.drop.drop) drop_apply_at(key, (uint64_t)row * (uint64_t)p.cols + (uint64_t)c, p.drop.drop, p.drop.scale, b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < p.cols ? rounded_as(v[j], p.out) : 0.f;  // 0 / r is NaN in a row of NaNs
+  for (int j = 0; j < 8; ++j) {
+    v[j] = rounded_as(v[j] + b[j], p.res16);
+    ss = fmaf(v[j], v[j], ss);
+  }
+  if (CODED && !p.grouped) {
+    float wv[8];
+    load_w(p.w, c, p.cols, wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) am = max_abs_nan(am, v[j] * wv[j]);
+  }
+  save_any(p.hidden, p.res16, row, c, p.cols, mine, v);
+}
+template <bool CODED>
+__device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int64_t c, float (&v)[8], float ir, float row_scale,
+                                             float* mine) {
+  const int lane = threadIdx.x & 31;
+  float wv[8];
+  load_w(p.w, c, p.cols, wv);
+  if (CODED) {
+    float scale = row_scale, m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] *= wv[j];
+      m = max_abs_nan(m, v[j]);
+    }
+    if (p.grouped) {
+      scale = coded_scale(group_max(m) * ir, p.int8);
+      if (c < p.cols && (lane & 15) == 0) p.scales[row * p.groups + c / kCodedGroup] = scale;
+    }
+    const float mult = ir * coded_inverse(scale);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= mult;
+    coded_save_any(reinterpret_cast<uint8_t*>(p.codes) + row * p.cols, c - 8 * lane, p.cols, mine, v, p.int8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * ir * wv[j];
+    save_any(p.out, p.branch16, row, c, p.cols, mine, v);
+    if (p.codes) {  // of the output as it is returned
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < p.cols ? rounded_as(v[j], p.branch16) : 0.f;  // 0 / r is NaN in a row of NaNs
       ck_encode(v, p.codes + row * p.pitch, p.exps + row * (p.pitch / kCkBlock), c, c < p.pitch);
     }
   }
 }
 
-constexpr int fwd_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : UPT == 2 ? 512 : 1024; }
-
-// A row stays in registers between the sum and the output, UPT units a thread.
-template <typename TR, typename TB, int UPT, bool WARP, bool EVEN, bool CODED>
-__global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_kernel(const FwdArgs<TR, TB> p) {
-  __shared__ float red[32];
-  __shared__ uint32_t redm[32];
-  extern __shared__ __align__(16) float sm[];  // uneven rows: 8 a thread
-  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
+template <int UPT, bool WARP, bool CODED>
+__global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_any_kernel(const FwdArgs p) {
+  __shared__ float red[32], redm[32];
+  __shared__ __align__(16) float sm[fwd_threads(UPT, WARP) * 8];
+  float* mine = sm + (threadIdx.x >> 5) * 256;
   const int lane = threadIdx.x & 31;
   const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
   if (WARP && row >= p.rows) return;
-  const TR* rr = p.res + row * p.cols;
-  const TB* br = p.branch + row * p.cols;
   const DropKey key = drop_key(p.drop);
-  float v[UPT][8], b[UPT][8];
+  float v[UPT][8];
+  float ss = 0.f, am = 0.f;
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) {
-    const int64_t c = unit_col<WARP>(k);
-    if (EVEN) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] = b[k][j] = 0.f;
-      if (c < p.cols) {
-        ck_load(rr + c, v[k]);
-        ck_load(br + c, b[k]);
-      }
-    } else {
-      ck_load_any(rr, c - 8 * lane, p.cols, mine, v[k]);
-      ck_load_any(br, c - 8 * lane, p.cols, mine, b[k]);
-    }
-  }
-  float ss = 0.f;
-  uint32_t am = 0u;
-#pragma unroll
-  for (int k = 0; k < UPT; ++k) {
-    const int64_t c = unit_col<WARP>(k);
-    add_unit<EVEN>(p, key, row, c, v[k], b[k]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[k][j], v[k][j], ss);
-    if (CODED && !p.grouped) {
-      float wv[8];
-      load_w(p.w, c, p.cols, wv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) am = max(am, abs_bits(v[k][j] * wv[j]));
-    }
-    if (EVEN) {
-      if (c < p.cols) ck_save(p.hidden + row * p.cols + c, v[k]);
-    } else {
-      ck_save_any(p.hidden + row * p.cols, c - 8 * lane, p.cols, mine, v[k]);
-    }
-  }
-  if (CODED) row_sum_max<WARP>(ss, am, red, redm);
-  else ss = row_total<WARP>(ss, red);
+  for (int k = 0; k < UPT; ++k) add_unit_any<CODED>(p, key, row, unit_col<WARP>(k), mine, v[k], ss, am);
+  row_sum_max<WARP, CODED>(ss, am, red, redm);
   const float r = sqrtf(ss / (float)p.cols + p.eps), ir = 1.0f / r;
-  const float scale = CODED ? coded_scale(__uint_as_float(am) * ir, p.int8) : 0.f;
+  const float scale = CODED ? coded_scale(am * ir, p.int8) : 0.f;
   if (WARP ? lane == 0 : threadIdx.x == 0) {
     if (p.rms) p.rms[row] = r;
     if (CODED && !p.grouped) p.scales[row] = scale;
   }
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) {
-    const int64_t c = unit_col<WARP>(k);
-    float wv[8];
-    load_w(p.w, c, p.cols, wv);
-    put_unit<EVEN, CODED>(p, row, c, v[k], wv, ir, scale, mine);
-  }
+  for (int k = 0; k < UPT; ++k) put_unit_any<CODED>(p, row, unit_col<WARP>(k), v[k], ir, scale, mine);
 }
 
 // Rows too long for registers: h is read again, from L2, by the thread that wrote it.
 constexpr int kLongThreads = 1024;
-template <typename TR, typename TB, bool CODED>
-__global__ void __launch_bounds__(kLongThreads) add_norm_fwd_long_kernel(const FwdArgs<TR, TB> p) {
-  __shared__ float red[32];
-  __shared__ uint32_t redm[32];
+template <bool CODED>
+__global__ void __launch_bounds__(kLongThreads) add_norm_fwd_long_kernel(const FwdArgs p) {
+  __shared__ float red[32], redm[32];
   __shared__ __align__(16) float sm[kLongThreads * 8];
   float* mine = sm + (threadIdx.x >> 5) * 256;
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x;
   const DropKey key = drop_key(p.drop);
-  float ss = 0.f;
-  uint32_t am = 0u;
+  float ss = 0.f, am = 0.f;
   for (int64_t c0 = (threadIdx.x >> 5) * 256; c0 < p.cols; c0 += 8 * kLongThreads) {
-    const int64_t c = c0 + 8 * lane;
-    float v[8], b[8];
-    ck_load_any(p.res + row * p.cols, c0, p.cols, mine, v);
-    ck_load_any(p.branch + row * p.cols, c0, p.cols, mine, b);
-    add_unit<false>(p, key, row, c, v, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-    if (CODED && !p.grouped) {
-      float wv[8];
-      load_w(p.w, c, p.cols, wv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) am = max(am, abs_bits(v[j] * wv[j]));
-    }
-    ck_save_any(p.hidden + row * p.cols, c0, p.cols, mine, v);
+    float v[8];
+    add_unit_any<CODED>(p, key, row, c0 + 8 * lane, mine, v, ss, am);
   }
-  row_sum_max<false>(ss, am, red, redm);
+  row_sum_max<false, CODED>(ss, am, red, redm);
   const float r = sqrtf(ss / (float)p.cols + p.eps), ir = 1.0f / r;
-  const float scale = CODED ? coded_scale(__uint_as_float(am) * ir, p.int8) : 0.f;
+  const float scale = CODED ? coded_scale(am * ir, p.int8) : 0.f;
   if (threadIdx.x == 0) {
     if (p.rms) p.rms[row] = r;
     if (CODED && !p.grouped) p.scales[row] = scale;
   }
   const int64_t end = CODED ? p.cols : p.pitch;
   for (int64_t c0 = (threadIdx.x >> 5) * 256; c0 < end; c0 += 8 * kLongThreads) {
-    const int64_t c = c0 + 8 * lane;
-    float v[8], wv[8];
-    ck_load_any(static_cast<const TR*>(p.hidden) + row * p.cols, c0, p.cols, mine, v);
-    load_w(p.w, c, p.cols, wv);
-    put_unit<false, CODED>(p, row, c, v, wv, ir, scale, mine);
+    float v[8];
+    load_any(p.hidden, p.res16, row, c0 + 8 * lane, p.cols, mine, v);
+    put_unit_any<CODED>(p, row, c0 + 8 * lane, v, ir, scale, mine);
   }
 }
 
@@ -229,20 +272,19 @@ FwdPlan fwd_plan(int64_t cols) {
 }
 
 template <bool CODED, typename TR, typename TB>
-int launch_fwd(const FwdArgs<TR, TB>& p, cudaStream_t st) {
+int launch_fwd(const FwdArgs& p, cudaStream_t st) {
   bool even = even_rows<TR>(p.res, p.cols, p.cols) && even_rows<TR>(p.hidden, p.cols, p.cols) &&
-              even_rows<TB>(p.branch, p.cols, p.cols);
+              even_rows<TB>(p.branch, p.cols, p.cols) && even_rows<float>(p.w, p.cols, p.cols);
   even = even && (CODED ? (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 : even_rows<TB>(p.out, p.cols, p.cols));
   const FwdPlan pl = fwd_plan(p.cols);
   const unsigned blocks = (unsigned)(pl.warp ? (p.rows + kWarpRows - 1) / kWarpRows : p.rows);
-  const size_t staging = even ? 0 : (size_t)pl.threads * 32;
   ProfScope prof(CODED ? "add_rmsnorm_coded" : "add_rmsnorm_fwd", st);
-#define MHC_GO(UPT, WARP)                                                                                       \
-  do {                                                                                                          \
-    if (even) add_norm_fwd_kernel<TR, TB, UPT, WARP, true, CODED><<<blocks, pl.threads, staging, st>>>(p);      \
-    else add_norm_fwd_kernel<TR, TB, UPT, WARP, false, CODED><<<blocks, pl.threads, staging, st>>>(p);          \
+#define MHC_GO(UPT, WARP)                                                                              \
+  do {                                                                                                 \
+    if (even) add_norm_fwd_kernel<TR, TB, UPT, WARP, CODED><<<blocks, pl.threads, 0, st>>>(p);         \
+    else add_norm_fwd_any_kernel<UPT, WARP, CODED><<<blocks, pl.threads, 0, st>>>(p);                  \
   } while (0)
-  if (pl.UPT == 0) add_norm_fwd_long_kernel<TR, TB, CODED><<<blocks, pl.threads, 0, st>>>(p);
+  if (pl.UPT == 0) add_norm_fwd_long_kernel<CODED><<<blocks, pl.threads, 0, st>>>(p);
   else if (pl.warp && pl.UPT == 1) MHC_GO(1, true);
   else if (pl.warp && pl.UPT == 2) MHC_GO(2, true);
   else if (pl.warp) MHC_GO(4, true);
@@ -325,9 +367,9 @@ extern "C" int mhc_add_rmsnorm_fwd(const void* residual, int32_t residual_bf16, 
   return with_types(residual_bf16, branch_bf16, [&](auto* r, auto* b) -> int {
     using TR = std::remove_pointer_t<decltype(r)>;
     using TB = std::remove_pointer_t<decltype(b)>;
-    FwdArgs<TR, TB> p = {(const TR*)residual, (const TB*)branch, weight, (TR*)hidden, rms, (TB*)out, codes, exponents, nullptr,
-                         rows, cols, ck_pitch(cols), 0, eps, false, false, drop_source(state, seed, position, drop)};
-    return launch_fwd<false>(p, (cudaStream_t)stream);
+    const FwdArgs p = {residual, branch, weight, hidden, rms, out, codes, exponents, nullptr, rows, cols, ck_pitch(cols), 0,
+                       eps, false, false, residual_bf16 != 0, branch_bf16 != 0, drop_source(state, seed, position, drop)};
+    return launch_fwd<false, TR, TB>(p, (cudaStream_t)stream);
   });
 }
 
@@ -347,10 +389,10 @@ extern "C" int mhc_add_rmsnorm_coded(const void* residual, int32_t residual_bf16
   return with_types(residual_bf16, branch_bf16, [&](auto* r, auto* b) -> int {
     using TR = std::remove_pointer_t<decltype(r)>;
     using TB = std::remove_pointer_t<decltype(b)>;
-    FwdArgs<TR, TB> p = {(const TR*)residual, (const TB*)branch, weight, (TR*)hidden, nullptr, nullptr, (int8_t*)codes,
-                         nullptr, scales, rows, cols, cols, coded_groups(cols, grouped != 0), eps, codes_int8 != 0,
-                         grouped != 0, drop_source(nullptr, 0, 0, 0)};
-    return launch_fwd<true>(p, (cudaStream_t)stream);
+    const FwdArgs p = {residual, branch, weight, hidden, nullptr, nullptr, (int8_t*)codes, nullptr, scales, rows, cols, cols,
+                       coded_groups(cols, grouped != 0), eps, codes_int8 != 0, grouped != 0, residual_bf16 != 0,
+                       branch_bf16 != 0, drop_source(nullptr, 0, 0, 0)};
+    return launch_fwd<true, TR, TB>(p, (cudaStream_t)stream);
   });
 }
 

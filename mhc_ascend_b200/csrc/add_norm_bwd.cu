@@ -6,75 +6,312 @@
 // output's.  A block (or warp) walks every (its count)-th row and keeps its
 // columns' share of gw in registers; the shares leave as one row a block and are
 // added in block order: no atomics, the same bits every time.
-#include "checkpoint8.cuh"
 #include "dropout.cuh"
 #include "rows.cuh"
 #include "tma.cuh"
+#include "vec8.cuh"
 
 namespace mhc {
 namespace {
 
-template <typename TR, typename TB>
 struct BwdArgs {
-  const TR* gh;  // nullable: zero
-  const TB* g;
-  const TR* h;
-  const float* w;
-  const float* rms;
-  TR* gr;
-  TB* gb;  // nullable: not wanted
+  const void* gh;  // nullable: zero
+  const void *g, *h;
+  const float *w, *rms;
+  void *gr, *gb;  // gb nullable: not wanted
   float* part;
   int64_t rows, cols;
+  bool res16, branch16;
   DropSource drop;
 };
 
-// gi of a unit -> both gradients
-template <bool EVEN, typename TR, typename TB>
-__device__ __forceinline__ void put_grads(const BwdArgs<TR, TB>& p, const DropKey& key, int64_t row, int64_t c, float (&o)[8],
-                                          float* mine) {
-  const int lane = threadIdx.x & 31;
-  const bool on = c < p.cols;
-  if (EVEN) {
-    if (on) ck_save(p.gr + row * p.cols + c, o);
-  } else {
-    ck_save_any(p.gr + row * p.cols, c - 8 * lane, p.cols, mine, o);
-  }
+// gi of a unit that starts at element i -> both gradients
+template <typename TR, typename TB>
+__device__ __forceinline__ void put_grads(const BwdArgs& p, const DropKey& key, int64_t i, const V8& gi) {
+  v8_save(static_cast<TR*>(p.gr) + i, gi);
   if (p.gb) {
+    V8 o = gi;
     if (p.drop.drop) {
-      const uint64_t i = (uint64_t)row * (uint64_t)p.cols + (uint64_t)c;
-      if (EVEN) drop_apply(drop_group(key, i / kDropGroup), p.drop.drop, p.drop.scale, o);
-      else drop_apply_at(key, i, p.drop.drop, p.drop.scale, o);
+      float f[8];
+      v8_spread(gi, f);
+      drop_apply(drop_group(key, (uint64_t)i / kDropGroup), p.drop.drop, p.drop.scale, f);
+      o = v8_gather(f);
     }
-    if (EVEN) {
-      if (on) ck_save(p.gb + row * p.cols + c, o);
-    } else {
-      ck_save_any(p.gb + row * p.cols, c - 8 * lane, p.cols, mine, o);
-    }
+    v8_save(static_cast<TB*>(p.gb) + i, o);
+  }
+}
+__device__ __forceinline__ void put_grads_any(const BwdArgs& p, const DropKey& key, int64_t row, int64_t c, float (&o)[8],
+                                              float* mine) {
+  save_any(p.gr, p.res16, row, c, p.cols, mine, o);
+  if (p.gb) {
+    if (p.drop.drop) drop_apply_at(key, (uint64_t)row * (uint64_t)p.cols + (uint64_t)c, p.drop.drop, p.drop.scale, o);
+    save_any(p.gb, p.branch16, row, c, p.cols, mine, o);
   }
 }
 
-template <bool EVEN, typename T>
-__device__ __forceinline__ void get_unit(const T* row, int64_t c, int64_t cols, float* mine, float (&v)[8]) {
-  if (EVEN) {
+// The warps' shares of the weight's gradient, added in warp order
+template <int UPT>
+__device__ __forceinline__ void put_warp_parts(const BwdArgs& p, const float (&acc)[UPT][8], float* sm) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if (c < cols) ck_load(row + c, v);
-  } else {
-    ck_load_any(row, c - 8 * (threadIdx.x & 31), cols, mine, v);
+  for (int k = 0; k < UPT; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sm[warp * 256 + j * 32 + lane] = acc[k][j];
+    __syncthreads();
+    float s = 0.f;
+    for (int q = 0; q < kWarpRows; ++q) s += sm[q * 256 + threadIdx.x];
+    const int64_t c = (k * 32 + lane) * 8 + warp;  // word j * 32 + lane holds column 8 lane + j
+    if (c < p.cols) p.part[(int64_t)blockIdx.x * p.cols + c] = s;
   }
 }
 
 // ---------------------------------------------------------------------------
-// Rows in registers: rows of a warp, and blocks' rows that wide accesses do not fit.
+// Rows of at most 1024 columns, one a warp.
 // ---------------------------------------------------------------------------
-constexpr int bwd_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : 512; }
+template <typename TR, typename TB, int UPT>
+__global__ void __launch_bounds__(32 * kWarpRows) add_norm_bwd_warp_kernel(const BwdArgs p) {
+  let_next_start();
+  __shared__ float sm[kWarpRows * 256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = (int)p.cols;
+  const DropKey key = drop_key(p.drop);
+  V8 acc[UPT];
+#pragma unroll
+  for (int k = 0; k < UPT; ++k) acc[k] = v8_zero();
+  for (int64_t row = (int64_t)blockIdx.x * kWarpRows + warp; row < p.rows; row += (int64_t)gridDim.x * kWarpRows) {
+    const int64_t at = row * cols + 8 * lane;
+    Raw8<TB> g[UPT];
+    Raw8<TR> h[UPT], o[UPT];
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      g[k].zero();
+      h[k].zero();
+      o[k].zero();
+      if (8 * (k * 32 + lane) < cols) {
+        g[k].load(static_cast<const TB*>(p.g) + at + k * 256);
+        h[k].load(static_cast<const TR*>(p.h) + at + k * 256);
+        if (p.gh) o[k].load(static_cast<const TR*>(p.gh) + at + k * 256);
+      }
+    }
+    const float r = p.rms[row], ir = 1.0f / r;
+    V8 gw[UPT];
+    float2 d2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      const V8 gv = g[k].values(), hv = h[k].values();
+      acc[k] = v8_fma(v8_scale(gv, ir), hv, acc[k]);
+      gw[k] = 8 * (k * 32 + lane) < cols ? v8_mul(gv, v8_weights(p.w + 8 * (k * 32 + lane))) : v8_zero();
+      d2 = v8_dot(gw[k], hv, d2);
+    }
+    const float coef = -warp_sum(d2.x + d2.y) / ((float)cols * r * r);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k)
+      if (8 * (k * 32 + lane) < cols)
+        put_grads<TR, TB>(p, key, at + k * 256, v8_fma(v8_fma(h[k].values(), coef, gw[k]), ir, o[k].values()));
+  }
+  float parts[UPT][8];
+#pragma unroll
+  for (int k = 0; k < UPT; ++k) v8_spread(acc[k], parts[k]);
+  put_warp_parts<UPT>(p, parts, sm);
+}
 
-template <typename TR, typename TB, int UPT, bool WARP, bool EVEN>
-__global__ void __launch_bounds__(bwd_threads(UPT, WARP), WARP ? 1 : 2) add_norm_bwd_kernel(const BwdArgs<TR, TB> p) {
+// ---------------------------------------------------------------------------
+// Rows of 1025 to 8192 columns that 16-byte copies fit: each thread copies its own
+// units of the rows ahead into shared memory (cp.async), `stages` rows deep, and
+// is the only one to read them, so the row's one barrier is that of its sum.
+// ---------------------------------------------------------------------------
+constexpr int kStagesMost = 4;
+constexpr int kStageBytes = 224 * 1024;  // of an SM's blocks together
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the latest n - 1 groups have landed, 1 <= n <= 4
+__device__ __forceinline__ void copies_wait(int n) {
+  if (n == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else if (n == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (n == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// A unit in shared memory: its 16-byte pieces `apart` bytes from each other, those of
+// all threads side by side.
+template <typename T>
+__device__ __forceinline__ void unit_copy(uint32_t to, uint32_t apart, const T* from) {
+  copy16(to, from);
+  if (sizeof(T) == 4) copy16(to + apart, from + 4);
+}
+__device__ __forceinline__ V8 unit_read(const unsigned char* at, uint32_t apart, const float*) {
+  const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + apart);
+  V8 v;
+  v.a[0] = make_float2(a.x, a.y);
+  v.a[1] = make_float2(a.z, a.w);
+  v.a[2] = make_float2(b.x, b.y);
+  v.a[3] = make_float2(b.z, b.w);
+  return v;
+}
+__device__ __forceinline__ V8 unit_read(const unsigned char* at, uint32_t, const __nv_bfloat16*) {
+  return v8_of(*reinterpret_cast<const uint4*>(at));
+}
+
+template <typename TR, typename TB, int UPT>
+__global__ void __launch_bounds__(512, 2) add_norm_bwd_ring_kernel(const BwdArgs p, int stages) {
+  let_next_start();
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float red[2][16];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, cols = (int)p.cols;
+  // a stage: pieces of gh, of h, of g, each 16 bytes for every unit
+  const uint32_t apart = 16u * UPT * blockDim.x;
+  constexpr uint32_t at_h = sizeof(TR) / 2, at_g = sizeof(TR);  // in pieces
+  const uint32_t stage = apart * (uint32_t)(sizeof(TR) + sizeof(TB) / 2);
+  const DropKey key = drop_key(p.drop);
+  // one unit a thread: its weights and what the sum was made of stay in registers;
+  // two: they are read again (64 registers a thread)
+  constexpr bool HOLD = UPT == 1;
+  V8 acc[UPT], wv = v8_zero();
+  bool on[UPT];
+#pragma unroll
+  for (int k = 0; k < UPT; ++k) {
+    const int c = 8 * (k * (int)blockDim.x + tid);
+    on[k] = c < cols;
+    if (HOLD && on[k]) wv = v8_weights(p.w + c);
+    acc[k] = v8_zero();
+  }
+  const int step = 8 * (int)blockDim.x;  // columns between a thread's units
+  const int64_t hop = (int64_t)gridDim.x * cols;
+  int64_t ahead = (int64_t)blockIdx.x * cols + 8 * tid;  // element of the next copies
+  const int64_t end = p.rows * cols;
+  const uint32_t mine = smem_u32(ring) + 16u * tid;
+  auto fetch = [&](uint32_t s) {
+    if (ahead < end) {
+#pragma unroll
+      for (int k = 0; k < UPT; ++k)
+        if (on[k]) {
+          const uint32_t to = mine + s + 16u * k * blockDim.x;
+          if (p.gh) unit_copy(to, apart, static_cast<const TR*>(p.gh) + ahead + k * step);
+          unit_copy(to + at_h * apart, apart, static_cast<const TR*>(p.h) + ahead + k * step);
+          unit_copy(to + at_g * apart, apart, static_cast<const TB*>(p.g) + ahead + k * step);
+        }
+    }
+    ahead += hop;
+    copies_end();  // a group each time, so that the count of groups is the count of rows
+  };
+  for (int s = 0; s < stages; ++s) fetch(s * stage);
+  uint32_t s = 0;
+  int buf = 0;
+  int64_t at = (int64_t)blockIdx.x * cols + 8 * tid;
+  float nr = p.rms[blockIdx.x];
+  const float share = 1.0f / (float)cols;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1, at += hop) {
+    const float ir = 1.0f / nr;
+    if (row + gridDim.x < p.rows) nr = p.rms[row + gridDim.x];
+    copies_wait(stages);
+    V8 gw, h;
+    float2 d2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k)
+      if (on[k]) {
+        const unsigned char* from = ring + s + 16u * (k * blockDim.x + tid);
+        const V8 g = unit_read(from + at_g * apart, apart, (const TB*)nullptr);
+        h = unit_read(from + at_h * apart, apart, (const TR*)nullptr);
+        acc[k] = v8_fma(v8_scale(g, ir), h, acc[k]);
+        gw = v8_mul(g, HOLD ? wv : v8_weights(p.w + 8 * tid + k * step));
+        d2 = v8_dot(gw, h, d2);
+      }
+    const float d = warp_sum(d2.x + d2.y);
+    if (lane == 0) red[buf][warp] = d;
+    __syncthreads();
+    float t = lane < nw ? red[buf][lane & 15] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);  // 16 warps at most
+    const float coef = -__shfl_sync(0xffffffffu, t, 0) * share * (ir * ir);
+#pragma unroll
+    for (int k = 0; k < UPT; ++k)
+      if (on[k]) {
+        const unsigned char* from = ring + s + 16u * (k * blockDim.x + tid);
+        if (!HOLD) {
+          h = unit_read(from + at_h * apart, apart, (const TR*)nullptr);
+          gw = v8_mul(unit_read(from + at_g * apart, apart, (const TB*)nullptr), v8_weights(p.w + 8 * tid + k * step));
+        }
+        const V8 o = p.gh ? unit_read(from, apart, (const TR*)nullptr) : v8_zero();
+        put_grads<TR, TB>(p, key, at + k * step, v8_fma(v8_fma(h, coef, gw), ir, o));
+      }
+    fetch(s);  // into what this thread has just read
+    s = s + stage == stages * stage ? 0 : s + stage;
+  }
+#pragma unroll
+  for (int k = 0; k < UPT; ++k)
+    if (on[k]) v8_save(p.part + (int64_t)blockIdx.x * cols + 8 * (k * (int)blockDim.x + tid), acc[k]);
+  copies_wait(1);
+}
+
+// ---------------------------------------------------------------------------
+// Longer rows: g and h are read twice (the second time from L2), and the block's
+// share of gw is kept in shared memory (KEEP) or, past kKeepCols columns, in its row
+// of partial sums.  Each unit is always the same thread's.
+// ---------------------------------------------------------------------------
+constexpr int kLongThreads = 512;
+constexpr int64_t kKeepCols = 49152;  // 192 KB
+
+template <typename TR, typename TB>
+__global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const BwdArgs p) {
+  let_next_start();
+  extern __shared__ __align__(16) unsigned char keep[];  // halves of a unit's eight sums apart
+  __shared__ float red[2][32];
+  const int cols = (int)p.cols, U = cols / 8;
+  float4* lo = reinterpret_cast<float4*>(keep);
+  float4* hi = lo + U;
+  for (int u = threadIdx.x; u < U; u += kLongThreads) lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const DropKey key = drop_key(p.drop);
+  int buf = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1) {
+    const float r = p.rms[row], ir = 1.0f / r;
+    const TB* g = static_cast<const TB*>(p.g) + row * cols;
+    const TR* h = static_cast<const TR*>(p.h) + row * cols;
+    float2 d2 = make_float2(0.f, 0.f);
+#pragma unroll 2
+    for (int u = threadIdx.x; u < U; u += kLongThreads) {
+      Raw8<TB> gq;
+      Raw8<TR> hq;
+      gq.load(g + 8 * u);
+      hq.load(h + 8 * u);
+      const V8 gv = gq.values(), hv = hq.values();
+      V8 a = unit_read(reinterpret_cast<const unsigned char*>(lo + u), 16u * U, (const float*)nullptr);
+      a = v8_fma(v8_scale(gv, ir), hv, a);
+      lo[u] = make_float4(a.a[0].x, a.a[0].y, a.a[1].x, a.a[1].y);
+      hi[u] = make_float4(a.a[2].x, a.a[2].y, a.a[3].x, a.a[3].y);
+      d2 = v8_dot(v8_mul(gv, v8_weights(p.w + 8 * u)), hv, d2);
+    }
+    const float coef = -row_total<false>(d2.x + d2.y, red[buf]) / ((float)cols * r * r);
+#pragma unroll 2
+    for (int u = threadIdx.x; u < U; u += kLongThreads) {
+      Raw8<TB> gq;
+      Raw8<TR> hq, o;
+      gq.load(g + 8 * u);
+      hq.load(h + 8 * u);
+      o.zero();
+      if (p.gh) o.load(static_cast<const TR*>(p.gh) + row * cols + 8 * u);
+      const V8 gw = v8_mul(gq.values(), v8_weights(p.w + 8 * u));
+      put_grads<TR, TB>(p, key, row * cols + 8 * u, v8_fma(v8_fma(hq.values(), coef, gw), ir, o.values()));
+    }
+  }
+  for (int u = threadIdx.x; u < U; u += kLongThreads)
+    v8_save(p.part + (int64_t)blockIdx.x * cols + 8 * u,
+            unit_read(reinterpret_cast<const unsigned char*>(lo + u), 16u * U, (const float*)nullptr));
+}
+
+// ---------------------------------------------------------------------------
+// Any row: through shared memory, types by a branch.  In registers up to 8192 columns:
+// ---------------------------------------------------------------------------
+constexpr int any_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : 512; }
+
+template <int UPT, bool WARP>
+__global__ void __launch_bounds__(any_threads(UPT, WARP)) add_norm_bwd_any_kernel(const BwdArgs p) {
   let_next_start();
   __shared__ float red[2][32];
-  __shared__ __align__(16) float sm[bwd_threads(UPT, WARP) * 8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ __align__(16) float sm[any_threads(UPT, WARP) * 8];
+  const int warp = threadIdx.x >> 5;
   float* mine = sm + warp * 256;
   const DropKey key = drop_key(p.drop);
   float acc[UPT][8];
@@ -87,24 +324,15 @@ __global__ void __launch_bounds__(bwd_threads(UPT, WARP), WARP ? 1 : 2) add_norm
   int buf = 0;
   for (int64_t row = first; row < p.rows; row += hop, buf ^= 1) {
     const float r = p.rms[row], ir = 1.0f / r;
-    float gw[UPT][8], h[UPT][8], o[UPT][8];
+    float gw[UPT][8], h[UPT][8];
     float d = 0.f;
 #pragma unroll
     for (int k = 0; k < UPT; ++k) {
       const int64_t c = unit_col<WARP>(k);
-      get_unit<EVEN>(p.g + row * p.cols, c, p.cols, mine, gw[k]);
-      get_unit<EVEN>(p.h + row * p.cols, c, p.cols, mine, h[k]);
-      if (p.gh) {
-        get_unit<EVEN>(p.gh + row * p.cols, c, p.cols, mine, o[k]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[k][j] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < UPT; ++k) {
+      load_any(p.g, p.branch16, row, c, p.cols, mine, gw[k]);
+      load_any(p.h, p.res16, row, c, p.cols, mine, h[k]);
       float wv[8];
-      load_w(p.w, unit_col<WARP>(k), p.cols, wv);
+      load_w(p.w, c, p.cols, wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         acc[k][j] = fmaf(gw[k][j] * ir, h[k][j], acc[k][j]);
@@ -116,23 +344,16 @@ __global__ void __launch_bounds__(bwd_threads(UPT, WARP), WARP ? 1 : 2) add_norm
     const float coef = row_total<WARP>(d, red[buf]) / ((float)p.cols * r * r);
 #pragma unroll
     for (int k = 0; k < UPT; ++k) {
+      const int64_t c = unit_col<WARP>(k);
+      float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (p.gh) load_any(p.gh, p.res16, row, c, p.cols, mine, o);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[k][j] = fmaf(gw[k][j] - h[k][j] * coef, ir, o[k][j]);
-      put_grads<EVEN>(p, key, row, unit_col<WARP>(k), o[k], mine);
+      for (int j = 0; j < 8; ++j) o[j] = fmaf(gw[k][j] - h[k][j] * coef, ir, o[j]);
+      put_grads_any(p, key, row, c, o, mine);
     }
   }
-  if (WARP) {  // the warps' shares, added in warp order
-#pragma unroll
-    for (int k = 0; k < UPT; ++k) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sm[warp * 256 + j * 32 + lane] = acc[k][j];
-      __syncthreads();
-      float s = 0.f;
-      for (int q = 0; q < kWarpRows; ++q) s += sm[q * 256 + threadIdx.x];
-      const int64_t c = (k * 32 + lane) * 8 + warp;  // word j * 32 + lane holds column 8 lane + j
-      if (c < p.cols) p.part[(int64_t)blockIdx.x * p.cols + c] = s;
-    }
+  if (WARP) {
+    put_warp_parts<UPT>(p, acc, sm);
   } else {
 #pragma unroll
     for (int k = 0; k < UPT; ++k)
@@ -144,156 +365,16 @@ __global__ void __launch_bounds__(bwd_threads(UPT, WARP), WARP ? 1 : 2) add_norm
   }
 }
 
-// ---------------------------------------------------------------------------
-// Rows of 1025 to 8192 columns that 16-byte copies fit: each thread copies its own
-// units of the rows ahead into shared memory (cp.async), `stages` rows deep, and
-// is the only one to read them, so the row's one barrier is that of its sum.
-// ---------------------------------------------------------------------------
-constexpr int kStagesMost = 4;
-constexpr int kStageBytes = 224 * 1024;  // of an SM's blocks together
-
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// all but the latest N groups have landed
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// A unit in shared memory: 16-byte pieces of all threads side by side.
-template <typename T>
-__device__ __forceinline__ void unit_copy(unsigned char* at, int unit, int units, const T* from) {
-#pragma unroll
-  for (int q = 0; q < (int)sizeof(T) / 2; ++q)
-    copy16(at + ((size_t)q * units + unit) * 16, reinterpret_cast<const unsigned char*>(from) + 16 * q);
-}
-__device__ __forceinline__ void unit_read(const unsigned char* at, int unit, int units, float (&v)[8], const float*) {
-  const float4 a = *reinterpret_cast<const float4*>(at + (size_t)unit * 16);
-  const float4 b = *reinterpret_cast<const float4*>(at + (size_t)(units + unit) * 16);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void unit_read(const unsigned char* at, int unit, int, float (&v)[8], const __nv_bfloat16*) {
-  const uint4 a = *reinterpret_cast<const uint4*>(at + (size_t)unit * 16);
-  const uint32_t r[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = __uint_as_float(r[j] << 16);
-    v[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
-  }
-}
-
-template <typename TR, typename TB, int UPT, int STAGES>
-__global__ void __launch_bounds__(512, 2) add_norm_bwd_ring_kernel(const BwdArgs<TR, TB> p) {
+template <bool KEEP>
+__global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_any_kernel(const BwdArgs p) {
   let_next_start();
-  extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float red[2][16];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  const int units = UPT * (int)blockDim.x;
-  constexpr int per = 8 * (2 * (int)sizeof(TR) + (int)sizeof(TB));  // bytes of a unit: gh, h, g
-  const size_t at_h = (size_t)units * 8 * sizeof(TR), at_g = 2 * at_h;
-  const DropKey key = drop_key(p.drop);
-  float acc[UPT][8], wv[UPT][8];
-  int c[UPT];
-  bool on[UPT];
-#pragma unroll
-  for (int k = 0; k < UPT; ++k) {
-    c[k] = 8 * (k * (int)blockDim.x + tid);
-    on[k] = c[k] < p.cols;
-    load_w(p.w, c[k], p.cols, wv[k]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[k][j] = 0.f;
-  }
-  auto fetch = [&](int64_t row, int s) {
-    unsigned char* at = ring + (size_t)s * units * per;
-    if (row < p.rows) {
-#pragma unroll
-      for (int k = 0; k < UPT; ++k)
-        if (on[k]) {
-          const int u = k * (int)blockDim.x + tid;
-          if (p.gh) unit_copy(at, u, units, p.gh + row * p.cols + c[k]);
-          unit_copy(at + at_h, u, units, p.h + row * p.cols + c[k]);
-          unit_copy(at + at_g, u, units, p.g + row * p.cols + c[k]);
-        }
-    }
-    copies_end();  // a group each time, so that the count of groups is the count of rows
-  };
-#pragma unroll
-  for (int s = 0; s < STAGES; ++s) fetch((int64_t)blockIdx.x + (int64_t)s * gridDim.x, s);
-  int s = 0, buf = 0;
-  float nr = p.rms[blockIdx.x];
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1) {
-    const unsigned char* at = ring + (size_t)s * units * per;
-    const float r = nr, ir = 1.0f / r;
-    if (row + gridDim.x < p.rows) nr = p.rms[row + gridDim.x];
-    copies_wait<STAGES - 1>();
-    float gw[UPT][8], h[UPT][8];
-    float d = 0.f;
-#pragma unroll
-    for (int k = 0; k < UPT; ++k)
-      if (on[k]) {
-        const int u = k * (int)blockDim.x + tid;
-        unit_read(at + at_g, u, units, gw[k], p.g);
-        unit_read(at + at_h, u, units, h[k], p.h);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          acc[k][j] = fmaf(gw[k][j] * ir, h[k][j], acc[k][j]);
-          gw[k][j] *= wv[k][j];
-          d = fmaf(gw[k][j], h[k][j], d);
-        }
-      }
-    d = warp_sum(d);
-    if (lane == 0) red[buf][warp] = d;
-    __syncthreads();
-    float t = lane < nw ? red[buf][lane & 15] : 0.f;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);  // 16 warps at most
-    const float coef = __shfl_sync(0xffffffffu, t, 0) / ((float)p.cols * r * r);
-#pragma unroll
-    for (int k = 0; k < UPT; ++k)
-      if (on[k]) {
-        float o[8];
-        if (p.gh) {
-          unit_read(at, k * (int)blockDim.x + tid, units, o, p.gh);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = fmaf(gw[k][j] - h[k][j] * coef, ir, o[j]);
-        put_grads<true>(p, key, row, c[k], o, nullptr);
-      }
-    fetch(row + (int64_t)STAGES * gridDim.x, s);  // into what this thread has just read
-    s = s + 1 == STAGES ? 0 : s + 1;
-  }
-#pragma unroll
-  for (int k = 0; k < UPT; ++k)
-    if (on[k]) {
-      float* q = p.part + (int64_t)blockIdx.x * p.cols + c[k];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = acc[k][j];
-    }
-  copies_wait<0>();
-}
-
-// ---------------------------------------------------------------------------
-// Longer rows: g and h are read twice (the second time from L2), and the block's
-// share of gw is kept in shared memory (KEEP) or, past kKeepCols columns, in its row
-// of partial sums.  Each unit is always the same thread's.
-// ---------------------------------------------------------------------------
-constexpr int kLongThreads = 512;
-constexpr int64_t kKeepCols = 49152;  // 192 KB
-
-template <typename TR, typename TB, bool EVEN, bool KEEP>
-__global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const BwdArgs<TR, TB> p) {
-  let_next_start();
-  extern __shared__ __align__(16) float keep[];  // [8][units]: value j of unit u at j * units + u
+  extern __shared__ __align__(16) unsigned char keep[];  // [8][units] floats: value j of unit u at j * units + u
   __shared__ float red[2][32];
-  __shared__ __align__(16) float sm[EVEN ? 1 : kLongThreads * 8];
-  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
+  __shared__ __align__(16) float sm[kLongThreads * 8];
+  float* mine = sm + (threadIdx.x >> 5) * 256;
   const int lane = threadIdx.x & 31;
   const int64_t units = (p.cols + 7) / 8;
-  float* a = KEEP ? keep : p.part + (int64_t)blockIdx.x * p.cols;
+  float* a = KEEP ? reinterpret_cast<float*>(keep) : p.part + (int64_t)blockIdx.x * p.cols;
   auto slot = [&](int64_t c, int j) -> int64_t { return KEEP ? j * units + c / 8 : c + j; };
   for (int64_t c = 8 * threadIdx.x; c < p.cols; c += 8 * kLongThreads)
 #pragma unroll
@@ -303,14 +384,12 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
   int buf = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1) {
     const float r = p.rms[row], ir = 1.0f / r;
-    const TB* gr = p.g + row * p.cols;
-    const TR* hr = p.h + row * p.cols;
     float d = 0.f;
     for (int64_t c0 = 8 * (threadIdx.x & ~31); c0 < p.cols; c0 += 8 * kLongThreads) {
       const int64_t c = c0 + 8 * lane;
       float g[8], h[8], wv[8];
-      get_unit<EVEN>(gr, c, p.cols, mine, g);
-      get_unit<EVEN>(hr, c, p.cols, mine, h);
+      load_any(p.g, p.branch16, row, c, p.cols, mine, g);
+      load_any(p.h, p.res16, row, c, p.cols, mine, h);
       load_w(p.w, c, p.cols, wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -321,16 +400,14 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
     const float coef = row_total<false>(d, red[buf]) / ((float)p.cols * r * r);
     for (int64_t c0 = 8 * (threadIdx.x & ~31); c0 < p.cols; c0 += 8 * kLongThreads) {
       const int64_t c = c0 + 8 * lane;
-      float g[8], h[8], wv[8], o[8];
-      get_unit<EVEN>(gr, c, p.cols, mine, g);
-      get_unit<EVEN>(hr, c, p.cols, mine, h);
+      float g[8], h[8], wv[8], o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      load_any(p.g, p.branch16, row, c, p.cols, mine, g);
+      load_any(p.h, p.res16, row, c, p.cols, mine, h);
       load_w(p.w, c, p.cols, wv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = 0.f;
-      if (p.gh) get_unit<EVEN>(p.gh + row * p.cols, c, p.cols, mine, o);
+      if (p.gh) load_any(p.gh, p.res16, row, c, p.cols, mine, o);
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = fmaf(g[j] * wv[j] - h[j] * coef, ir, o[j]);
-      put_grads<EVEN>(p, key, row, c, o, mine);
+      put_grads_any(p, key, row, c, o, mine);
     }
   }
   if (KEEP)
@@ -343,24 +420,24 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
 // ---------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------
-enum class Bwd { kWarp, kBlock, kRing, kLong };
+enum class Bwd { kWarp, kRing, kLong, kAny, kAnyWarp, kAnyLong };
 struct BwdPlan {
   Bwd kind;
   int UPT, threads, stages, per_sm;
   size_t smem;
 };
-// `unit`: bytes of 8 columns of gh, h and g
+// even: wide accesses fit; `unit`: bytes of 8 columns of gh, h and g
 BwdPlan bwd_plan(int64_t cols, bool even, size_t unit) {
   const int64_t U = (cols + 7) / 8;
   if (ck_pitch(cols) <= kWarpCols)
-    return {Bwd::kWarp, ck_pitch(cols) <= 256 ? 1 : ck_pitch(cols) <= 512 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
+    return {even ? Bwd::kWarp : Bwd::kAnyWarp, ck_pitch(cols) <= 256 ? 1 : ck_pitch(cols) <= 512 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
   if (U > 1024) {
     const size_t keep = cols <= kKeepCols ? (size_t)U * 8 * sizeof(float) : 0;
-    return {Bwd::kLong, 0, kLongThreads, 0, keep > 100 * 1024 ? 1 : 2, keep};
+    return {even && keep ? Bwd::kLong : Bwd::kAnyLong, 0, kLongThreads, 0, keep > 100 * 1024 ? 1 : 2, keep};
   }
   if (!even) {
     const int upt = U <= 256 ? 1 : 2;
-    return {Bwd::kBlock, upt, (int)(((U + upt - 1) / upt + 31) / 32 * 32), 0, 2, 0};
+    return {Bwd::kAny, upt, (int)(((U + upt - 1) / upt + 31) / 32 * 32), 0, 2, 0};
   }
   const int upt = U <= 512 ? 1 : 2, threads = (int)(((U + upt - 1) / upt + 31) / 32 * 32);
   const size_t stage = (size_t)upt * threads * unit;
@@ -375,57 +452,75 @@ BwdPlan bwd_plan(int64_t cols, bool even, size_t unit) {
 // Blocks: as many as run at once (gw leaves as one row a block), no more than
 // there are rows for.
 int bwd_blocks(const BwdPlan& pl, int64_t rows) {
-  const int64_t need = pl.kind == Bwd::kWarp ? (rows + kWarpRows - 1) / kWarpRows : rows;
+  const bool warp = pl.kind == Bwd::kWarp || pl.kind == Bwd::kAnyWarp;
+  const int64_t need = warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
   const int64_t most = pl.per_sm * (int64_t)num_sms();
   return (int)(need < most ? (need > 0 ? need : 1) : most);
 }
 
-template <typename K, typename P>
-int go(K kern, int blocks, const BwdPlan& pl, size_t most, const P& p, cudaStream_t st) {
-  // The limit on dynamic shared memory belongs to the kernel, not to the launch:
-  // it is always set to the most that any width asks for, so that host threads
-  // with other widths cannot lower it in between.
-  if (most && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
-    return fail(MHC_ERR_CUDA, "add_rmsnorm_bwd: cannot reserve %zu bytes of shared memory", most);
-  kern<<<blocks, pl.threads, pl.smem, st>>>(p);
-  return MHC_OK;
-}
-
-template <int UPT, typename TR, typename TB>
-int go_ring(int blocks, const BwdPlan& pl, const BwdArgs<TR, TB>& p, cudaStream_t st) {
-  constexpr size_t most = kStageBytes;
-  if (pl.stages == 2) return go(add_norm_bwd_ring_kernel<TR, TB, UPT, 2>, blocks, pl, most, p, st);
-  if (pl.stages == 3) return go(add_norm_bwd_ring_kernel<TR, TB, UPT, 3>, blocks, pl, most, p, st);
-  return go(add_norm_bwd_ring_kernel<TR, TB, UPT, 4>, blocks, pl, most, p, st);
+// The limit on dynamic shared memory belongs to the kernel, not to the launch: it is
+// always set to the most that any width asks for, so that host threads with other
+// widths cannot lower it in between.
+template <typename K>
+int allow(K kern, size_t most) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) == cudaSuccess
+             ? MHC_OK
+             : fail(MHC_ERR_CUDA, "add_rmsnorm_bwd: cannot reserve %zu bytes of shared memory", most);
 }
 
 template <typename TR, typename TB>
-int launch_bwd(BwdArgs<TR, TB> p, float* grad_weight, size_t workspace_bytes, cudaStream_t st) {
+int launch_bwd(const BwdArgs& p, float* grad_weight, size_t workspace_bytes, cudaStream_t st) {
   const bool even = even_rows<TR>(p.gh, p.cols, p.cols) && even_rows<TR>(p.h, p.cols, p.cols) &&
                     even_rows<TB>(p.g, p.cols, p.cols) && even_rows<TR>(p.gr, p.cols, p.cols) &&
-                    even_rows<TB>(p.gb, p.cols, p.cols);
+                    even_rows<TB>(p.gb, p.cols, p.cols) && even_rows<float>(p.w, p.cols, p.cols) &&
+                    even_rows<float>(p.part, p.cols, p.cols);
   const BwdPlan pl = bwd_plan(p.cols, even, 8 * (2 * sizeof(TR) + sizeof(TB)));
   const int blocks = bwd_blocks(pl, p.rows);
   MHC_REQUIRE(p.part != nullptr && workspace_bytes >= (size_t)blocks * (size_t)p.cols * sizeof(float), MHC_ERR_WORKSPACE,
               "add_rmsnorm_bwd: workspace too small");
+  constexpr size_t keep = kKeepCols * sizeof(float);
   int rc = MHC_OK;
   {
     ProfScope prof("add_rmsnorm_bwd", st);
-#define MHC_GO(UPT, WARP)                                                                             \
-  (even ? go(add_norm_bwd_kernel<TR, TB, UPT, WARP, true>, blocks, pl, 0, p, st)                      \
-        : go(add_norm_bwd_kernel<TR, TB, UPT, WARP, false>, blocks, pl, 0, p, st))
-    constexpr size_t keep = kKeepCols * sizeof(float);
-    if (pl.kind == Bwd::kRing) rc = pl.UPT == 1 ? go_ring<1>(blocks, pl, p, st) : go_ring<2>(blocks, pl, p, st);
-    else if (pl.kind == Bwd::kWarp) rc = pl.UPT == 1 ? MHC_GO(1, true) : pl.UPT == 2 ? MHC_GO(2, true) : MHC_GO(4, true);
-    else if (pl.kind == Bwd::kBlock)
-      rc = pl.UPT == 1 ? go(add_norm_bwd_kernel<TR, TB, 1, false, false>, blocks, pl, 0, p, st)
-                       : go(add_norm_bwd_kernel<TR, TB, 2, false, false>, blocks, pl, 0, p, st);
-    else if (pl.smem) rc = even ? go(add_norm_bwd_long_kernel<TR, TB, true, true>, blocks, pl, keep, p, st)
-                                : go(add_norm_bwd_long_kernel<TR, TB, false, true>, blocks, pl, keep, p, st);
-    else rc = even ? go(add_norm_bwd_long_kernel<TR, TB, true, false>, blocks, pl, 0, p, st)
-                   : go(add_norm_bwd_long_kernel<TR, TB, false, false>, blocks, pl, 0, p, st);
+#define MHC_GO(KERN, ...) KERN<<<blocks, pl.threads, pl.smem, st>>>(__VA_ARGS__)
+    switch (pl.kind) {
+      case Bwd::kWarp:
+        if (pl.UPT == 1) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 1>), p);
+        else if (pl.UPT == 2) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 2>), p);
+        else MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 4>), p);
+        break;
+      case Bwd::kRing: {
+        auto kern = pl.UPT == 1 ? add_norm_bwd_ring_kernel<TR, TB, 1> : add_norm_bwd_ring_kernel<TR, TB, 2>;
+        rc = allow(kern, kStageBytes);
+        if (rc) return rc;
+        MHC_GO(kern, p, pl.stages);
+        break;
+      }
+      case Bwd::kLong:
+        rc = allow(add_norm_bwd_long_kernel<TR, TB>, keep);
+        if (rc) return rc;
+        MHC_GO((add_norm_bwd_long_kernel<TR, TB>), p);
+        break;
+      case Bwd::kAnyWarp:
+        if (pl.UPT == 1) MHC_GO((add_norm_bwd_any_kernel<1, true>), p);
+        else if (pl.UPT == 2) MHC_GO((add_norm_bwd_any_kernel<2, true>), p);
+        else MHC_GO((add_norm_bwd_any_kernel<4, true>), p);
+        break;
+      case Bwd::kAny:
+        if (pl.UPT == 1) MHC_GO((add_norm_bwd_any_kernel<1, false>), p);
+        else MHC_GO((add_norm_bwd_any_kernel<2, false>), p);
+        break;
+      case Bwd::kAnyLong:
+        if (pl.smem) {
+          rc = allow(add_norm_bwd_long_any_kernel<true>, keep);
+          if (rc) return rc;
+          MHC_GO(add_norm_bwd_long_any_kernel<true>, p);
+        } else {
+          MHC_GO(add_norm_bwd_long_any_kernel<false>, p);
+        }
+    }
 #undef MHC_GO
-    if (rc == MHC_OK) rc = check_launch("add_rmsnorm_bwd");
+    rc = check_launch("add_rmsnorm_bwd");
     if (rc) return rc;
   }
   ProfScope prof("add_rmsnorm_gw", st);
@@ -478,9 +573,9 @@ extern "C" int mhc_add_rmsnorm_bwd(const void* grad_hidden, const void* grad_out
   auto run = [&](auto* r, auto* b) -> int {
     using TR = std::remove_pointer_t<decltype(r)>;
     using TB = std::remove_pointer_t<decltype(b)>;
-    const BwdArgs<TR, TB> p = {(const TR*)grad_hidden, (const TB*)grad_out, (const TR*)hidden, weight, rms, (TR*)grad_residual,
-                               (TB*)grad_branch, (float*)workspace, rows, cols, drop_source(state, seed, position, drop)};
-    return launch_bwd(p, grad_weight, workspace_bytes, st);
+    const BwdArgs p = {grad_hidden, grad_out, hidden, weight, rms, grad_residual, grad_branch, (float*)workspace, rows, cols,
+                       residual_bf16 != 0, branch_bf16 != 0, drop_source(state, seed, position, drop)};
+    return launch_bwd<TR, TB>(p, grad_weight, workspace_bytes, st);
   };
   if (residual_bf16)
     return branch_bf16 ? run((__nv_bfloat16*)nullptr, (__nv_bfloat16*)nullptr) : run((__nv_bfloat16*)nullptr, (float*)nullptr);

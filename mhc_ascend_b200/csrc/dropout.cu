@@ -6,7 +6,32 @@
 namespace mhc {
 namespace {
 
-constexpr int kThreads = 256, kUnits = 2;  // units of 8 values a thread
+constexpr int kThreads = 256, kUnits = 4;  // units of 8 values a thread
+
+__device__ __forceinline__ void load_raw(const float* p, float (&v)[8]) { ck_load(p, v); }
+__device__ __forceinline__ void load_raw(const __nv_bfloat16* p, uint4& v) { v = *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void put_unit(float* p, float (&v)[8], const uint4& n, uint32_t drop, float scale) {
+  drop_apply(n, drop, scale, v);
+  ck_save(p, v);
+}
+// Two bf16 values a word: scaled as pairs, dropped as halves of the result
+__device__ __forceinline__ void put_unit(__nv_bfloat16* p, uint4& v, const uint4& n, uint32_t drop, float scale) {
+  const uint32_t x[4] = {v.x, v.y, v.z, v.w}, w[4] = {n.x, n.y, n.z, n.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 s = __fmul2_rn(make_float2(__uint_as_float(x[j] << 16), __uint_as_float(x[j] & 0xffff0000u)),
+                                make_float2(scale, scale));
+    const __nv_bfloat162 b = __floats2bfloat162_rn(s.x, s.y);
+    uint32_t r = *reinterpret_cast<const uint32_t*>(&b);
+    if (!keeps_low(w[j], drop)) r &= 0xffff0000u;
+    if (!keeps_high(w[j], drop)) r &= 0x0000ffffu;
+    o[j] = r;
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+template <typename T> struct Raw { using type = float[8]; };
+template <> struct Raw<__nv_bfloat16> { using type = uint4; };
 
 // EVEN: 16- or 32-byte accesses; the tensor's last, incomplete unit goes value by
 // value.  Otherwise through shared memory (a start that is not aligned).
@@ -14,38 +39,42 @@ template <typename T, bool EVEN>
 __global__ void __launch_bounds__(kThreads)
     dropout_kernel(const T* __restrict__ x, T* __restrict__ out, int64_t count, DropSource src) {
   __shared__ __align__(16) float sm[EVEN ? 1 : kThreads * 8];
-  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
-  const int lane = threadIdx.x & 31;
   const int64_t first = (int64_t)blockIdx.x * (kThreads * kUnits) + threadIdx.x;
   const DropKey key = drop_key(src);
-  float v[kUnits][8];
+  if (EVEN && ((int64_t)blockIdx.x + 1) * (kThreads * kUnits * 8) <= count) {
+    typename Raw<T>::type v[kUnits];
+    x += 8 * first;
+    out += 8 * first;
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    const int64_t c = 8 * (first + k * kThreads);
-    if (EVEN) {
-      if (c + 8 <= count) ck_load(x + c, v[k]);
-    } else {
-      ck_load_any(x, c - 8 * lane, count, mine, v[k]);
-    }
+    for (int k = 0; k < kUnits; ++k) load_raw(x + k * kThreads * 8, v[k]);
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k)
+      put_unit(out + k * kThreads * 8, v[k], drop_group(key, first + k * kThreads), src.drop, src.scale);
+    return;
   }
-#pragma unroll
+  float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
   for (int k = 0; k < kUnits; ++k) {
     const int64_t u = first + k * kThreads, c = 8 * u;
-    if (EVEN) {
-      if (c + 8 <= count) {
-        drop_apply(drop_group(key, u), src.drop, src.scale, v[k]);
-        ck_save(out + c, v[k]);
-      } else if (c < count) {
+    float v[8];
+    if (EVEN && c + 8 <= count) {
+      ck_load(x + c, v);
+    } else if (EVEN) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[k][j] = c + j < count ? ck_f32(x[c + j]) : 0.f;
-        drop_apply(drop_group(key, u), src.drop, src.scale, v[k]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < count) ck_store(out + c + j, v[k][j]);
-      }
+      for (int j = 0; j < 8; ++j) v[j] = c + j < count ? ck_f32(x[c + j]) : 0.f;
     } else {
-      drop_apply(drop_group(key, u), src.drop, src.scale, v[k]);
-      ck_save_any(out, c - 8 * lane, count, mine, v[k]);
+      ck_load_any(x, c - 8 * lane, count, mine, v);
+    }
+    drop_apply(drop_group(key, u), src.drop, src.scale, v);
+    if (EVEN && c + 8 <= count) {
+      ck_save(out + c, v);
+    } else if (EVEN) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < count) ck_store(out + c + j, v[j]);
+    } else {
+      ck_save_any(out, c - 8 * lane, count, mine, v);
     }
   }
 }
@@ -57,7 +86,8 @@ int launch_dropout(const T* x, T* out, int64_t count, const DropSource& src, cud
   const int64_t blocks = ((count + 7) / 8 + kThreads * kUnits - 1) / (kThreads * kUnits);
   MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "dropout: %lld values are too many", (long long)count);
   ProfScope p("dropout", st);
-  if (even) dropout_kernel<T, true><<<(unsigned)blocks, kThreads, 0, st>>>(x, out, count, src);
+  if (src.drop >= kDropAll) cudaMemsetAsync(out, 0, (size_t)count * sizeof(T), st);
+  else if (even) dropout_kernel<T, true><<<(unsigned)blocks, kThreads, 0, st>>>(x, out, count, src);
   else dropout_kernel<T, false><<<(unsigned)blocks, kThreads, 0, st>>>(x, out, count, src);
   return check_launch("dropout");
 }

@@ -68,14 +68,25 @@ __device__ __forceinline__ uint4 drop_group(const DropKey& key, uint64_t group) 
   return make_uint4(x0, x1, x2, x3);
 }
 
+// Whether each of a word's two numbers keeps its value: the numbers are compared in
+// the upper half of a word, where what lies below does not matter.
+__device__ __forceinline__ bool keeps_low(uint32_t w, uint32_t drop) { return w << 16 >= drop << 16; }
+__device__ __forceinline__ bool keeps_high(uint32_t w, uint32_t drop) { return w >= drop << 16; }
+
 // Apply a group's numbers to eight values: 0 or v * scale (not fused with what
 // follows, so that a sum with a dropped value is the same wherever it is formed).
 __device__ __forceinline__ void drop_apply(const uint4& n, uint32_t drop, float scale, float (&v)[8]) {
   const uint32_t w[4] = {n.x, n.y, n.z, n.w};
+  if (drop >= kDropAll) {  // the shifted comparison has no room for it
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    v[2 * j] = (w[j] & 0xffffu) < drop ? 0.f : __fmul_rn(v[2 * j], scale);
-    v[2 * j + 1] = (w[j] >> 16) < drop ? 0.f : __fmul_rn(v[2 * j + 1], scale);
+    const float2 s = __fmul2_rn(make_float2(v[2 * j], v[2 * j + 1]), make_float2(scale, scale));
+    v[2 * j] = keeps_low(w[j], drop) ? s.x : 0.f;
+    v[2 * j + 1] = keeps_high(w[j], drop) ? s.y : 0.f;
   }
 }
 

@@ -4,9 +4,13 @@
 // With m = max x, s = sum exp(x - m) over a row of logits:
 //   log p_j = x_j - m - ln s,   H = ln s + sum exp(x - m) (m - x) / s
 // (both terms of H are >= 0: nothing cancels).  One pass over the row: a thread
-// keeps a running maximum, sum and sum of e t, t = (x - m) log2 e, and rescales
-// them when its maximum moves.  Minus infinity has probability 0 and adds nothing;
-// a row without anything else has s = 0.
+// keeps a running maximum, sum of e = exp(x - m) and sum of e (x - m), and rescales
+// them when its maximum moves.  x - m is formed before it is scaled to base 2, so
+// the largest value has e = 1 to the bit: s >= 1, no log probability is above 0 and
+// no entropy below.  -inf is read as -2^127, so that no product needs a check: it
+// has e = 0 and a finite x - m.  Rows whose maximum is past 1e38 (of masks alone, or
+// next to overflow) are scanned again value by value with those checks.  A row of
+// nothing but -inf has s = 0.
 //
 // The k most likely, ties to the lowest index, in the same pass: every thread also
 // notes the maximum of each of its 32-value segments.  The k-th largest of the
@@ -23,7 +27,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kPer = 32;          // values of a thread's segment
 constexpr int kMostTop = 32;
@@ -44,7 +48,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-constexpr float kTiny = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * inf out of e t
+constexpr float kTiny = -200.f;     // exp(-200) is 0 in fp32; keeps 0 * inf out of e (x - m) in the careful form
+constexpr float kFloor = -0x1p127f;  // what -inf is read as
+constexpr float kPlain = 1e38f;      // rows with a maximum up to this take the short form: x - m stays finite
+// x - m of a value with 0 probability can be anything from here on; keeps s (x - m) finite
+constexpr float kFar = -1e30f;
 
 // ---------------------------------------------------------------------------
 // A row as vectors of 16 bytes from the aligned address at or below its start;
@@ -99,25 +107,39 @@ __device__ __forceinline__ float2 two(const uint4& u, int i) {
   if (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
   return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
+// Values below -2^127 become that, NaNs stay
 template <typename T>
-__device__ __forceinline__ float vec_max(const uint4 (&u)[kPer / Row<T>::VE]) {
+__device__ __forceinline__ void floor_vec(uint4& u) {
+  auto up = [](uint32_t& w) {
+    if (sizeof(T) == 4) w = __float_as_uint(max_nan(__uint_as_float(w), kFloor));
+    else asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0xff00ff00u));
+  };
+  up(u.x);
+  up(u.y);
+  up(u.z);
+  up(u.w);
+}
+// Largest value of N vectors, NaNs aside
+template <typename T, int N>
+__device__ __forceinline__ float vec_max(const uint4 (&u)[N]) {
   if (sizeof(T) == 4) {
-    float m = minus_inf();
+    float m = kFloor;
 #pragma unroll
-    for (int q = 0; q < kPer / Row<T>::VE; ++q)
+    for (int q = 0; q < N; ++q)
       m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[q].x), __uint_as_float(u[q].y)),
                          fmaxf(__uint_as_float(u[q].z), __uint_as_float(u[q].w))));
     return m;
   }
-  uint32_t m = 0xff80ff80u;
-  auto up = [&](uint32_t w) { asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w)); };
+  uint32_t m = 0xff00ff00u, n = 0xff00ff00u;
+  auto up = [](uint32_t& m, uint32_t w) { asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w)); };
 #pragma unroll
-  for (int q = 0; q < kPer / Row<T>::VE; ++q) {
-    up(u[q].x);
-    up(u[q].y);
-    up(u[q].z);
-    up(u[q].w);
+  for (int q = 0; q < N; ++q) {
+    up(m, u[q].x);
+    up(n, u[q].y);
+    up(m, u[q].z);
+    up(n, u[q].w);
   }
+  up(m, n);
   return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
 }
 
@@ -163,16 +185,22 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t v) {
   return v;
 }
 
+// Sums of a part of a row around its maximum m.
 struct Part {
   float m, s, h;
 };
-// Bring a part to the maximum M >= its own
+__device__ __forceinline__ bool careful(float m) { return !(fabsf(m) <= kPlain); }
+// Sums around m as sums around M >= m
 __device__ __forceinline__ void rebase(Part& p, float M) {
-  const float t = fmaxf((p.m - M) * kLog2e, -1e30f), c = ex2(t);
-  p.h = c * fmaf(p.s, t, p.h);
+  const float d = fmaxf(p.m == M ? 0.f : p.m - M, kFar), c = ex2(d * kLog2e);  // equal infinities too
+  p.h = c * fmaf(p.s, d, p.h);
   p.s *= c;
   p.m = M;
 }
+__device__ __forceinline__ float logprob_of(float x, const Part& p) {
+  return p.s == 0.f ? minus_inf() : (x - p.m) - logf(p.s);
+}
+__device__ __forceinline__ float entropy_of(const Part& p) { return p.s == 0.f ? 0.f : logf(p.s) - p.h / p.s; }
 
 struct TopShared {
   uint64_t best[kMostTop], joined[kMostTop];  // of the block, of the row's blocks together
@@ -184,11 +212,17 @@ struct TopShared {
   int segments, candidates;
 };
 
-// The k largest keys of the vectors [v0, v1) of a row into sh.best, in order (0:
-// none left).  segmax: maxima of the threads' segments; tm: of all of a thread's.
+// A block's share [v0, v1) of a row's vectors.  It is walked as [i0, ve): whole
+// vectors first, a first one that is not whole (v0 < i0) in the place behind the last.
+struct Share {
+  int64_t v0, v1, i0, ve;
+  __device__ __forceinline__ int64_t at(int64_t v) const { return v == v1 ? v0 : v; }
+};
+
+// The k largest keys of a share into sh.best, in order (0: none left).  segmax:
+// maxima of the threads' segments; tm: of all of a thread's.
 template <typename T, int THREADS>
-__device__ void select_top(const Row<T>& r, int64_t v0, int64_t v1, int k, int tiles, const float* segmax, float tm,
-                           TopShared& sh) {
+__device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, const float* segmax, float tm, TopShared& sh) {
   constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float v = warp_sort(tm);
@@ -202,7 +236,7 @@ __device__ void select_top(const Row<T>& r, int64_t v0, int64_t v1, int k, int t
   if (tid == k - 1) sh.bound = v;  // k <= 32: a lane of warp 0
   __syncthreads();
   const float bound = sh.bound;
-  bool fast = bound > minus_inf();
+  bool fast = bound > kFloor;
   if (fast) {
     for (int it = 0; it < tiles; ++it)
       if (segmax[it * THREADS + tid] >= bound) {
@@ -215,8 +249,9 @@ __device__ void select_top(const Row<T>& r, int64_t v0, int64_t v1, int k, int t
     if (fast) {
       for (int i = tid; i < n * VPT; i += THREADS) {
         const int g = sh.seg[i / VPT];
-        const int64_t vec = v0 + (int64_t)(g / THREADS) * (THREADS * VPT) + (i % VPT) * THREADS + g % THREADS;
-        const uint4 u = load_vec(r, vec, v1);
+        const int64_t walk = z.i0 + (int64_t)(g / THREADS) * (THREADS * VPT) + (i % VPT) * THREADS + g % THREADS;
+        const int64_t vec = z.at(walk);
+        const uint4 u = load_vec(r, vec, walk < z.ve ? z.v1 : 0);
 #pragma unroll
         for (int j = 0; j < VE / 2; ++j) {
           const float2 x = two<T>(u, j);
@@ -246,8 +281,8 @@ __device__ void select_top(const Row<T>& r, int64_t v0, int64_t v1, int k, int t
   if (!fast) {  // one after the other; a thread looks again only when its best is taken
     auto below = [&](uint64_t prev) {
       uint64_t best = 0;
-      for (int64_t vec = v0 + tid; vec < v1; vec += THREADS) {
-        const uint4 u = load_vec(r, vec, v1);
+      for (int64_t vec = z.v0 + tid; vec < z.v1; vec += THREADS) {
+        const uint4 u = load_vec(r, vec, z.v1);
 #pragma unroll
         for (int j = 0; j < VE / 2; ++j) {
           const float2 x = two<T>(u, j);
@@ -289,98 +324,159 @@ __device__ __forceinline__ int64_t target_of(const void* t, bool ids64, int64_t 
 __device__ __forceinline__ float value_of(const float* p) { return *p; }
 __device__ __forceinline__ float value_of(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
+// Sums of N vectors around the thread's running maximum.
+struct Sums {
+  float m;
+  float2 s, h;
+};
+template <typename T, int N>
+__device__ __forceinline__ float add_vecs(Sums& a, uint4 (&u)[N]) {
+#pragma unroll
+  for (int q = 0; q < N; ++q) floor_vec<T>(u[q]);
+  const float mx = vec_max<T>(u);
+  if (mx > a.m) {
+    const float d = fmaxf(a.m - mx, kFar), c = ex2(d * kLog2e);
+    a.h.x = c * fmaf(a.s.x, d, a.h.x);
+    a.h.y = c * fmaf(a.s.y, d, a.h.y);
+    a.s.x *= c;
+    a.s.y *= c;
+    a.m = mx;
+  }
+  const float2 minus = make_float2(-a.m, -a.m), scale = make_float2(kLog2e, kLog2e);
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+#pragma unroll
+    for (int j = 0; j < Row<T>::VE / 2; ++j) {
+      const float2 d = __fadd2_rn(two<T>(u[q], j), minus), t = __fmul2_rn(d, scale);
+      const float2 e = make_float2(ex2(t.x), ex2(t.y));
+      a.s = __fadd2_rn(a.s, e);
+      a.h = __ffma2_rn(e, d, a.h);
+    }
+  return mx;
+}
+// The same for one vector in the careful form.
+template <typename T>
+__device__ __forceinline__ void add_careful(Sums& a, const uint4& u) {
+  for (int j = 0; j < Row<T>::VE; ++j) {
+    const float2 two_ = two<T>(u, j / 2);
+    const float x = j & 1 ? two_.y : two_.x;
+    if (x > a.m) {
+      const float d = fmaxf(a.m - x, kFar), c = ex2(d * kLog2e);
+      a.h.x = c * fmaf(a.s.x, d, a.h.x);
+      a.s.x *= c;
+      a.m = x;
+    }
+    const float d = max_nan(x - a.m, kTiny), e = ex2(d * kLog2e);
+    a.s.x += e;
+    a.h.x = fmaf(e, d, a.h.x);
+  }
+}
+
+// The block's threads' sums together, the same in each thread.
+template <int W>
+__device__ __forceinline__ Part block_part(const Sums& a, float (&red)[3][W]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Part p = {a.m, a.s.x + a.s.y, a.h.x + a.h.y};
+  auto join = [](Part& p) {
+    float M = p.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    rebase(p, M);
+    p.s = warp_sum(p.s);
+    p.h = warp_sum(p.h);
+  };
+  join(p);
+  if (lane == 0) {
+    red[0][warp] = p.m;
+    red[1][warp] = p.s;
+    red[2][warp] = p.h;
+  }
+  __syncthreads();
+  p = lane < W ? Part{red[0][lane], red[1][lane], red[2][lane]} : Part{kLowest, 0.f, 0.f};
+  join(p);
+  return p;
+}
+
+// Blocks an SM for the register budget: 16-bit values leave 40 a thread, 32-bit ones
+// (a segment is 32 registers) 64.
+template <typename T>
+constexpr int fwd_blocks(int threads) { return (sizeof(T) == 4 ? 1024 : 1536) / threads; }
+
 // One row a cluster of CL blocks, each over its share of the row's vectors; block
 // 0 joins the shares through distributed shared memory.
 template <typename T, int THREADS, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, 1536 / THREADS) logprobs_fwd_kernel(const FwdArgs p) {
-  constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32;
+__global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_kernel(const FwdArgs p) {
+  constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32, TILE = THREADS * VPT;
   extern __shared__ __align__(16) unsigned char dyn[];
   float* segmax = reinterpret_cast<float*>(dyn);
   TopShared& sh = *reinterpret_cast<TopShared*>(dyn + (size_t)p.tiles * THREADS * sizeof(float));
-  __shared__ float red[3][W];
-  __shared__ Part part;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ float red[2][3][W];
+  __shared__ Part shared_part;
+  const int tid = threadIdx.x;
   const int CL = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
   const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
   const int64_t row = CLUSTER ? blockIdx.x / CL : blockIdx.x;
   const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
   const int64_t each = (r.count + CL - 1) / CL;
-  const int64_t v0 = rank * each < r.count ? rank * each : r.count;
-  const int64_t v1 = v0 + each < r.count ? v0 + each : r.count;
+  Share z;
+  z.v0 = rank * each < r.count ? rank * each : r.count;
+  z.v1 = z.v0 + each < r.count ? z.v0 + each : r.count;
+  z.i0 = z.v0 > r.full0 ? z.v0 : r.full0;
+  z.i0 = z.i0 < z.v1 ? z.i0 : z.v1;
+  z.ve = z.v1 + (z.v0 < z.i0);
 
-  float m = kLowest, tm = minus_inf();
-  float2 s2 = make_float2(0.f, 0.f), h2 = make_float2(0.f, 0.f);
+  Sums a = {kFloor, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float tm = kFloor;
   int it = 0;
-  for (int64_t a = v0; a < v1; a += THREADS * VPT, ++it) {
+  const int64_t whole = z.v1 < r.full1 ? z.v1 : r.full1;
+  int64_t v = z.i0 + tid;
+  for (int64_t left = whole - z.i0; left >= TILE; left -= TILE, v += TILE, ++it) {
     uint4 u[VPT];
+    const uint4* from = reinterpret_cast<const uint4*>(r.base) + v;
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) u[q] = load_vec(r, a + q * THREADS + tid, v1);
-    const float mx = vec_max<T>(u);
+    for (int q = 0; q < VPT; ++q) u[q] = from[q * THREADS];
+    const float mx = add_vecs<T>(a, u);
     if (TOP) {
       segmax[it * THREADS + tid] = mx;
       tm = fmaxf(tm, mx);
     }
-    if (mx > m) {
-      const float t = fmaxf((m - mx) * kLog2e, -1e30f), c = ex2(t);
-      h2.x = c * fmaf(s2.x, t, h2.x);
-      h2.y = c * fmaf(s2.y, t, h2.y);
-      s2.x *= c;
-      s2.y *= c;
-      m = mx;
+  }
+  for (; v - tid < z.ve; v += TILE, ++it) {  // what is left, and the row's ends
+    uint4 u[VPT];
+#pragma unroll
+    for (int q = 0; q < VPT; ++q) {
+      const int64_t w = v + q * THREADS;
+      u[q] = load_vec(r, z.at(w), w < z.ve ? z.v1 : 0);
     }
-    const float2 minus = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
-#pragma unroll
-    for (int q = 0; q < VPT; ++q)
-#pragma unroll
-      for (int j = 0; j < VE / 2; ++j) {
-        float2 t = __fmul2_rn(__fadd2_rn(two<T>(u[q], j), minus), scale);
-        t.x = max_nan(t.x, kTiny);
-        t.y = max_nan(t.y, kTiny);
-        const float2 e = make_float2(ex2(t.x), ex2(t.y));
-        s2 = __fadd2_rn(s2, e);
-        h2 = __ffma2_rn(e, t, h2);
-      }
+    const float mx = add_vecs<T>(a, u);
+    if (TOP) {
+      segmax[it * THREADS + tid] = mx;
+      tm = fmaxf(tm, mx);
+    }
   }
-  // the threads' parts
-  Part mine = {m, s2.x + s2.y, h2.x + h2.y};
-  float M = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  rebase(mine, M);
-  mine.s = warp_sum(mine.s);
-  mine.h = warp_sum(mine.h);
-  if (lane == 0) {
-    red[0][warp] = M;
-    red[1][warp] = mine.s;
-    red[2][warp] = mine.h;
+  Part part = block_part<W>(a, red[0]);
+  if (careful(part.m)) {  // the same for the whole block
+    a = {kLowest, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    for (int64_t w = z.v0 + tid; w < z.v1; w += THREADS) add_careful<T>(a, load_vec(r, w, z.v1));
+    part = block_part<W>(a, red[1]);
   }
-  __syncthreads();
-  if (warp == 0) {
-    Part w = {kLowest, 0.f, 0.f};
-    if (lane < W) w = {red[0][lane], red[1][lane], red[2][lane]};
-    M = w.m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    rebase(w, M);
-    w.s = warp_sum(w.s);
-    w.h = warp_sum(w.h);
-    if (lane == 0) part = w;
-  }
-  if (TOP) select_top<T, THREADS>(r, v0, v1, p.top, it, segmax, tm, sh);
+  if (TOP) select_top<T, THREADS>(r, z, p.top, it, segmax, tm, sh);
   if (CLUSTER) {
+    if (tid == 0) shared_part = part;
     cg::this_cluster().sync();
     if (rank == 0) {
-      if (tid == 0) {
-        Part all = part;
-        for (int b = 1; b < CL; ++b) {
-          Part o = *cg::this_cluster().map_shared_rank(&part, b);
-          const float top = fmaxf(all.m, o.m);
-          rebase(all, top);
-          rebase(o, top);
-          all.s += o.s;
-          all.h += o.h;
+      for (int b = 1; b < CL; ++b) {
+        Part o = *cg::this_cluster().map_shared_rank(&shared_part, b);
+        if (o.s == 0.f) continue;
+        if (part.s == 0.f) {
+          part = o;
+          continue;
         }
-        part = all;
+        const float M = fmaxf(part.m, o.m);
+        rebase(part, M);
+        rebase(o, M);
+        part.s += o.s;
+        part.h += o.h;
       }
       if (TOP) {
         uint64_t* all = sh.cand;
@@ -397,29 +493,21 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) logprobs_fwd_kernel(c
     }
     cg::this_cluster().sync();  // the others' shared memory has been read
     if (rank != 0) return;
-  } else {
-    __syncthreads();
   }
-  const Part all = part;
-  const bool none = all.s == 0.f;
-  const float ln_s = logf(all.s);
-  if (TOP) {
-    const uint64_t* best = CLUSTER ? sh.joined : sh.best;
-    if (tid < p.top) {
-      const uint64_t key = best[tid];
-      p.top_logprob[row * p.top + tid] = none ? minus_inf() : (key_value(key) - all.m) - ln_s;
-      p.top_id[row * p.top + tid] = (int64_t)key_index(key);
-    }
+  if (TOP && tid < p.top) {
+    const uint64_t key = CLUSTER ? sh.joined[tid] : sh.best[tid];
+    p.top_logprob[row * p.top + tid] = logprob_of(key_value(key), part);
+    p.top_id[row * p.top + tid] = (int64_t)key_index(key);
   }
   if (tid == 0) {
     const int64_t t = target_of(p.targets, p.ids64, row);
     float lp = __uint_as_float(0x7fc00000u);
     if (t == p.ignore) lp = 0.f;
-    else if (t >= 0 && t < p.V) lp = none ? minus_inf() : (value_of(r.base + r.shift + t) - all.m) - ln_s;
+    else if (t >= 0 && t < p.V) lp = logprob_of(value_of(r.base + r.shift + t), part);
     p.logprob[row] = lp;
-    p.entropy[row] = none ? 0.f : ln_s - all.h * kLn2 / all.s;
-    p.stats[2 * row] = all.m;
-    p.stats[2 * row + 1] = all.s;
+    p.entropy[row] = entropy_of(part);
+    p.stats[2 * row] = part.m;
+    p.stats[2 * row + 1] = part.s;
   }
 }
 
@@ -427,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) logprobs_fwd_kernel(c
 // Gradient, from the row's m, s and H:
 //   gx_j = -p_j (G + gH (ln p_j + H)) + the given tokens' own gradients,
 //   G = g_logprob + sum g_top
-// and with t = (x - m) log2 e, e = 2^t: gx = e (A + B t).  The few places that have
+// and with e = exp(x - m): gx = e (A + B (x - m)).  The few places that have
 // a gradient of their own are written again after the block's others.
 // ---------------------------------------------------------------------------
 struct BwdArgs {
@@ -440,32 +528,68 @@ struct BwdArgs {
   void* gx;
   int top;
   int64_t chunks;
+  int tiles;
   bool ids64;
 };
-constexpr int kBwdThreads = 256;
+constexpr int kBwdThreads = 256, kBwdTiles = 4;
 
-__device__ __forceinline__ float grad_of(float x, float m, float A, float B) {
-  const float t = max_nan((x - m) * kLog2e, kTiny);
-  return ex2(t) * fmaf(B, t, A);
+// Coefficients of a row's gradient in either form
+struct Coef {
+  float m, A, B;
+};
+__device__ __forceinline__ float grad_of(float x, const Coef& k) {
+  const float d = x - k.m;
+  return ex2(d * kLog2e) * fmaf(k.B, max_nan(d, kTiny), k.A);
 }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename T>
+// Gradients of a vector in the short form.  H: with the entropy's (B != 0).
+template <typename T, bool H>
+__device__ __forceinline__ uint4 grad_vec(uint4 u, const Coef& k) {
+  constexpr int VE = Row<T>::VE;
+  if (H) floor_vec<T>(u);
+  const float2 A = make_float2(k.A, k.A), B = make_float2(k.B, k.B), minus = make_float2(-k.m, -k.m),
+               scale = make_float2(kLog2e, kLog2e);
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < VE / 2; ++j) {
+    const float2 d = __fadd2_rn(two<T>(u, j), minus), t = __fmul2_rn(d, scale);
+    const float2 g = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), H ? __ffma2_rn(B, d, A) : A);
+    if (sizeof(T) == 4) {
+      w[(2 * j) & 3] = __float_as_uint(g.x);
+      w[(2 * j + 1) & 3] = __float_as_uint(g.y);
+    } else {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(g.x, g.y);
+      w[j & 3] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A block takes `tiles` tiles of a row's vectors.
+template <typename T, bool H>
 __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs p) {
-  constexpr int VE = Row<T>::VE, VPT = kPer / VE;
+  constexpr int VE = Row<T>::VE, VPT = 4;
   __shared__ int64_t at[kMostTop + 1];
   __shared__ float own[kMostTop + 1];
+  __shared__ Coef shared_coef;
+  __shared__ bool mine;  // whether a place with a gradient of its own is in the block's range
   const int tid = threadIdx.x, B_ = blockDim.x;
   const int64_t row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
   const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
   T* out = static_cast<T*>(p.gx) + row * p.V;
-  const int64_t a = chunk * ((int64_t)B_ * VPT);
+  const int64_t first = chunk * ((int64_t)B_ * VPT * p.tiles);
+  int64_t end = first + (int64_t)B_ * VPT * p.tiles;
+  end = end < r.count ? end : r.count;
+  const bool same = ((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) == (uintptr_t)r.shift;
+  auto whole = [&](int64_t a) { return same && a >= r.full0 && a + B_ * VPT <= (end < r.full1 ? end : r.full1); };
   uint4 u[VPT];
+  const bool ahead = whole(first);
+  if (ahead) {
 #pragma unroll
-  for (int q = 0; q < VPT; ++q) u[q] = load_vec(r, a + q * B_ + tid, r.count);
-  const float m = p.stats[2 * row], s = p.stats[2 * row + 1];
-  const bool none = s == 0.f;
+    for (int q = 0; q < VPT; ++q) u[q] = reinterpret_cast<const uint4*>(r.base)[first + q * B_ + tid];
+  }
   for (int i = tid; i <= p.top; i += B_) {
     if (i == 0) {
       const int64_t t = target_of(p.targets, p.ids64, row);
@@ -478,67 +602,82 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
       own[i] = p.g_top[row * p.top + i - 1];
     }
   }
+  if (p.top) __syncthreads();
+  if (tid == 0) {
+    float G = own[0];
+    bool any = false;
+    const int64_t lo = r.index(first), hi = r.index(end);
+    for (int i = 0; i <= p.top; ++i) {
+      if (i) G += own[i];
+      any = any || (at[i] >= 0 && at[i] >= lo && at[i] < hi);
+    }
+    Coef k = {p.stats[2 * row], 0.f, 0.f};
+    const float s = p.stats[2 * row + 1];
+    if (s != 0.f) {
+      const float gh = H ? p.g_entropy[row] : 0.f, inv = 1.0f / s;
+      k.A = -inv * (H ? fmaf(gh, p.entropy[row] - logf(s), G) : G);
+      k.B = -inv * gh;
+    }
+    shared_coef = k;
+    mine = any && s != 0.f;
+  }
   __syncthreads();
-  float G = own[0];
-  for (int i = 1; i <= p.top; ++i) G += own[i];
-  float A = 0.f, B = 0.f;
-  if (!none) {
-    const float gh = p.g_entropy ? p.g_entropy[row] : 0.f, inv = 1.0f / s;
-    A = -inv * fmaf(gh, p.entropy[row] - logf(s), G);
-    B = -inv * gh * kLn2;
-  }
-  const bool same = ((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) == (uintptr_t)r.shift;
-  const float2 A2 = make_float2(A, A), B2 = make_float2(B, B), minus = make_float2(-m, -m),
-               scale = make_float2(kLog2e, kLog2e);
+  const Coef k = shared_coef;
+  if (careful(k.m)) {  // and rows without anything
+    for (int64_t v = first + tid; v < end; v += B_) {
+      const uint4 w = load_vec(r, v, end);
 #pragma unroll
-  for (int q = 0; q < VPT; ++q) {
-    const int64_t v = a + q * B_ + tid;
-    if (v >= r.count) continue;
-    float o[VE];
-#pragma unroll
-    for (int j = 0; j < VE / 2; ++j) {
-      float2 t = __fmul2_rn(__fadd2_rn(two<T>(u[q], j), minus), scale);
-      t.x = max_nan(t.x, kTiny);
-      t.y = max_nan(t.y, kTiny);
-      const float2 g = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), __ffma2_rn(B2, t, A2));
-      o[2 * j] = g.x;
-      o[2 * j + 1] = g.y;
-    }
-    const int64_t e = r.index(v);
-    if (same && v >= r.full0 && v < r.full1) {
-      uint4 w;
-      if (sizeof(T) == 4) {
-        w = make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
-      } else {
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(o[(2 * j) % VE], o[(2 * j + 1) % VE]);
-          h[j] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        w = make_uint4(h[0], h[1], h[2], h[3]);
+      for (int j = 0; j < VE; ++j) {
+        const float2 x = two<T>(w, j / 2);
+        const int64_t e = r.index(v) + j;
+        if (e >= 0 && e < p.V) put(out + e, grad_of(j & 1 ? x.y : x.x, k));
       }
-      *reinterpret_cast<uint4*>(out + e) = w;
-    } else {
+    }
+  } else {
+    for (int64_t a = first; a < end; a += B_ * VPT) {
+      if (whole(a)) {
+        const uint4* from = reinterpret_cast<const uint4*>(r.base) + a + tid;
+        uint4* to = reinterpret_cast<uint4*>(out - r.shift) + a + tid;
+        if (!(ahead && a == first)) {
 #pragma unroll
-      for (int j = 0; j < VE; ++j)
-        if (e + j >= 0 && e + j < p.V) put(out + e + j, o[j]);
+          for (int q = 0; q < VPT; ++q) u[q] = from[q * B_];
+        }
+#pragma unroll
+        for (int q = 0; q < VPT; ++q) to[q * B_] = grad_vec<T, H>(u[q], k);
+      } else {
+#pragma unroll
+        for (int q = 0; q < VPT; ++q) {
+          const int64_t v = a + q * B_ + tid;
+          if (v >= end) continue;
+          const uint4 g = grad_vec<T, H>(load_vec(r, v, end), k);
+          if (same && v >= r.full0 && v < r.full1) {
+            reinterpret_cast<uint4*>(out - r.shift)[v] = g;
+          } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+              const int64_t e = r.index(v) + j;
+              const float2 x = two<T>(g, j / 2);
+              if (e >= 0 && e < p.V) put(out + e, j & 1 ? x.y : x.x);
+            }
+          }
+        }
+      }
     }
   }
-  if (none) return;
+  if (!mine) return;
   __syncthreads();  // before these places are written again
-  const int64_t lo = r.index(a), hi = r.index(a + (int64_t)B_ * VPT);
+  const int64_t lo = r.index(first), hi = r.index(end);
   for (int i = tid; i <= p.top; i += B_) {
     const int64_t e = at[i];
     if (e < 0 || e >= p.V || e < lo || e >= hi) continue;
     float g = 0.f;
-    bool first = true;
+    bool earliest = true;
     for (int j = 0; j <= p.top; ++j)
       if (at[j] == e) {
-        first = first && j >= i;
+        earliest = earliest && j >= i;
         g += own[j];
       }
-    if (first) put(out + e, g + grad_of(value_of(r.base + r.shift + e), m, A, B));
+    if (earliest) put(out + e, g + grad_of(value_of(r.base + r.shift + e), k));
   }
 }
 
@@ -637,18 +776,29 @@ extern "C" int mhc_token_logprobs_bwd(const void* logits, int32_t logits_bf16, i
     MHC_REQUIRE_PTR(top_id);
     MHC_REQUIRE_PTR(grad_top);
   }
-  const int per = kPer / (logits_bf16 ? 8 : 4);
+  constexpr int per = 4;  // vectors of a thread and tile
   const int64_t count = (vocab + (logits_bf16 ? 8 : 4) - 1) / (logits_bf16 ? 8 : 4) + 1;  // with a start that is not aligned
   int64_t threads = ((count + per - 1) / per + 31) / 32 * 32;
   threads = threads > kBwdThreads ? kBwdThreads : threads;
-  const int64_t chunks = (count + threads * per - 1) / (threads * per);
+  // several tiles a block where that leaves enough blocks: its coefficients cost as much as a tile
+  int tiles = kBwdTiles;
+  while (tiles > 1 && rows * ((count + threads * per * tiles - 1) / (threads * per * tiles)) < 16 * (int64_t)num_sms()) --tiles;
+  const int64_t chunks = (count + threads * per * tiles - 1) / (threads * per * tiles);
   MHC_REQUIRE(rows * chunks < (1ll << 31), MHC_ERR_UNSUPPORTED, "%s: %lld x %lld logits are too many", what, (long long)rows,
               (long long)vocab);
   const BwdArgs p = {logits, row_stride, rows, vocab, targets, ignore_index, stats, entropy, grad_logprob, grad_entropy,
-                     grad_top, top_id, grad_logits, (int)top, chunks, targets_64 != 0};
+                     grad_top, top_id, grad_logits, (int)top, chunks, tiles, targets_64 != 0};
   cudaStream_t st = (cudaStream_t)stream;
   ProfScope prof(what, st);
-  if (logits_bf16) logprobs_bwd_kernel<__nv_bfloat16><<<(unsigned)(rows * chunks), (unsigned)threads, 0, st>>>(p);
-  else logprobs_bwd_kernel<float><<<(unsigned)(rows * chunks), (unsigned)threads, 0, st>>>(p);
+  const unsigned blocks = (unsigned)(rows * chunks);
+#define MHC_GO(T, H) logprobs_bwd_kernel<T, H><<<blocks, (unsigned)threads, 0, st>>>(p)
+  if (logits_bf16) {
+    if (grad_entropy) MHC_GO(__nv_bfloat16, true);
+    else MHC_GO(__nv_bfloat16, false);
+  } else {
+    if (grad_entropy) MHC_GO(float, true);
+    else MHC_GO(float, false);
+  }
+#undef MHC_GO
   return check_launch(what);
 }

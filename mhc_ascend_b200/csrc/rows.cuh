@@ -3,7 +3,7 @@
 // block, and need no barrier; longer ones to a block.
 #pragma once
 
-#include "common.cuh"
+#include "checkpoint8.cuh"
 
 namespace mhc {
 namespace {
@@ -58,6 +58,18 @@ __global__ void __launch_bounds__(256)
     for (int k = 0; k < 8; ++k) a += s[k][lane];
     gw[c] = a;
   }
+}
+
+// Units of rows that wide accesses do not fit, types by a branch
+__device__ __forceinline__ void load_any(const void* p, bool b16, int64_t row, int64_t c, int64_t cols, float* mine, float (&v)[8]) {
+  const int64_t c0 = c - 8 * (threadIdx.x & 31);
+  if (b16) ck_load_any(static_cast<const __nv_bfloat16*>(p) + row * cols, c0, cols, mine, v);
+  else ck_load_any(static_cast<const float*>(p) + row * cols, c0, cols, mine, v);
+}
+__device__ __forceinline__ void save_any(void* p, bool b16, int64_t row, int64_t c, int64_t cols, float* mine, const float (&v)[8]) {
+  const int64_t c0 = c - 8 * (threadIdx.x & 31);
+  if (b16) ck_save_any(static_cast<__nv_bfloat16*>(p) + row * cols, c0, cols, mine, v);
+  else ck_save_any(static_cast<float*>(p) + row * cols, c0, cols, mine, v);
 }
 
 template <typename T>

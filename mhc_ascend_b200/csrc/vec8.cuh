@@ -1,0 +1,140 @@
+// Eight consecutive values of a row as four pairs, for two-wide fp32 arithmetic.
+#pragma once
+
+#include "checkpoint8.cuh"
+
+namespace mhc {
+
+struct V8 {
+  float2 a[4];
+};
+__device__ __forceinline__ V8 v8_zero() {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = make_float2(0.f, 0.f);
+  return v;
+}
+__device__ __forceinline__ V8 v8_of(const uint4& u) {  // eight bf16 values
+  const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = make_float2(__uint_as_float(r[j] << 16), __uint_as_float(r[j] & 0xffff0000u));
+  return v;
+}
+__device__ __forceinline__ uint4 v8_bf16(const V8& v) {
+  uint32_t r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.a[j].x, v.a[j].y);
+    r[j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ void v8_spread(const V8& v, float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[2 * j] = v.a[j].x;
+    f[2 * j + 1] = v.a[j].y;
+  }
+}
+__device__ __forceinline__ V8 v8_gather(const float (&f)[8]) {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = make_float2(f[2 * j], f[2 * j + 1]);
+  return v;
+}
+
+// A unit as it lies in memory
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+  float f[8];
+  __device__ __forceinline__ void load(const float* p) { ck_load(p, f); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  }
+  __device__ __forceinline__ V8 values() const { return v8_gather(f); }
+};
+template <> struct Raw8<__nv_bfloat16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ V8 values() const { return v8_of(u); }
+};
+__device__ __forceinline__ void v8_save(float* p, const V8& v) {
+  float f[8];
+  v8_spread(v, f);
+  ck_save(p, f);
+}
+__device__ __forceinline__ void v8_save(__nv_bfloat16* p, const V8& v) { *reinterpret_cast<uint4*>(p) = v8_bf16(v); }
+// Store v and leave what was stored
+__device__ __forceinline__ void v8_save_rounded(float* p, V8& v) { v8_save(p, v); }
+__device__ __forceinline__ void v8_save_rounded(__nv_bfloat16* p, V8& v) {
+  const uint4 u = v8_bf16(v);
+  *reinterpret_cast<uint4*>(p) = u;
+  v = v8_of(u);
+}
+// Eight weights, 32-byte aligned
+__device__ __forceinline__ V8 v8_weights(const float* w) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(w)), b = __ldg(reinterpret_cast<const float4*>(w + 4));
+  V8 v;
+  v.a[0] = make_float2(a.x, a.y);
+  v.a[1] = make_float2(a.z, a.w);
+  v.a[2] = make_float2(b.x, b.y);
+  v.a[3] = make_float2(b.z, b.w);
+  return v;
+}
+
+__device__ __forceinline__ V8 v8_add(const V8& x, const V8& y) {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = __fadd2_rn(x.a[j], y.a[j]);
+  return v;
+}
+__device__ __forceinline__ V8 v8_mul(const V8& x, const V8& y) {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = __fmul2_rn(x.a[j], y.a[j]);
+  return v;
+}
+__device__ __forceinline__ V8 v8_scale(const V8& x, float s) {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = __fmul2_rn(x.a[j], make_float2(s, s));
+  return v;
+}
+__device__ __forceinline__ V8 v8_fma(const V8& x, const V8& y, const V8& z) {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = __ffma2_rn(x.a[j], y.a[j], z.a[j]);
+  return v;
+}
+__device__ __forceinline__ V8 v8_fma(const V8& x, float y, const V8& z) {
+  V8 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v.a[j] = __ffma2_rn(x.a[j], make_float2(y, y), z.a[j]);
+  return v;
+}
+// s + x . y, pair by pair
+__device__ __forceinline__ float2 v8_dot(const V8& x, const V8& y, float2 s) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s = __ffma2_rn(x.a[j], y.a[j], s);
+  return s;
+}
+// the larger of a and |b|; NaN if either is
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float y;
+  asm("{.reg .f32 t; abs.f32 t, %2; max.NaN.f32 %0, %1, t;}" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float v8_max_abs(const V8& x) {  // NaN if any value is
+  float m = 0.f, n = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    m = max_abs_nan(m, x.a[j].x);
+    n = max_abs_nan(n, x.a[j].y);
+  }
+  return max_abs_nan(m, n);
+}
+
+}  // namespace mhc

@@ -210,6 +210,34 @@ def test_rows_without_a_distribution(cuda, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,V", [(1, 40000), (2, 70), (300, 9001)])
+@pytest.mark.parametrize("most", [3e38, 1.5e38, 2e37, 5e36, -5e36, -2e37, -1.5e38, -3e38])
+def test_logits_next_to_overflow(cuda, T, V, dtype, most):
+    """Rows whose maximum is huge, with masked and far smaller logits beside it."""
+    x = torch.full((T, V), most)
+    x[:, V // 2:] = -INF
+    x[:, 0], x[:, 1], x[:, V - 1] = torch.finfo(dtype).min, 0.0 if most > 0 else most * 1.1, most
+    x = x.to(dtype)
+    t = torch.full((T,), V - 1)
+    count = int((x[0] == x[0].max()).sum())  # all others are infinitely far
+    got = mhc.token_logprobs(x.to(cuda).requires_grad_(True), t.to(cuda), 4)
+    assert got.logprob[0].item() == pytest.approx(-math.log(count), rel=4 * U, abs=2 * U)
+    assert got.entropy[0].item() == pytest.approx(math.log(count), rel=4 * U, abs=2 * U)
+    assert torch.equal(got.logprob, got.logprob[:1].expand(T))
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(got.top_id.cpu(), order)
+    r = mhc.token_logprobs_fwd(x.to(cuda), t.to(cuda))
+    one = torch.ones(T, device=cuda)
+    gx = mhc.token_logprobs_bwd(x.to(cuda), t.to(cuda), r, one, one).double().cpu()
+    p = (x == x[0].max()).double() / count  # log p and the entropy cancel: the gradient is the logprob's alone
+    want = -p
+    want[:, V - 1] += 1
+    # rounded once to its type: half a step of the value (1 - p of the given token is not exact in 24 bits); p by a few units
+    assert bool(((gx - want).abs() <= (UB if dtype == BF16 else U) * want.abs() + 64 * U * p).all())
+
+
+@pytest.mark.gpu
 def test_targets_outside(cuda):
     x, _ = make(5, 100, F32)
     t = torch.tensor([-100, 100, -1, 1 << 40, 99])
