@@ -14,10 +14,10 @@
 //
 // The k most likely, ties to the lowest index, in the same pass: every thread also
 // notes the maximum of each of its 32-value segments.  The k-th largest of the
-// threads' maxima bounds the k-th largest value from below, so only segments whose
-// maximum reaches it are read again (k of them unless values tie), and what reaches
-// it there is ranked by counting.  Where many values tie, or fewer than k threads
-// have any finite value, the k are taken one after the other instead.
+// maxima of 2 k or more groups of lanes bounds the k-th largest value from below, so
+// only segments whose maximum reaches it are read again (about k of them), and what
+// reaches it there is ranked by counting.  Where many values tie, or too few are
+// finite, the k are taken one after the other instead.
 #include <cooperative_groups.h>
 
 #include "checkpoint8.cuh"
@@ -31,9 +31,8 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kPer = 32;          // values of a thread's segment
 constexpr int kMostTop = 32;
-constexpr int kSegments = 128;    // segments and candidates that the fast selection takes
-constexpr int kCandidates = 512;
-constexpr int kMostTiles = 16;    // segments of a thread
+constexpr int kSegments = 128, kCandidates = 512;  // that the fast selection reads again, and ranks
+constexpr int kMostShare = 1 << 18;  // values of a block with alternatives: 32 KB of segments' maxima
 constexpr int kMostCluster = 8;
 
 __device__ __forceinline__ float minus_inf() { return __uint_as_float(0xff800000u); }
@@ -62,9 +61,8 @@ template <typename T>
 struct Row {
   static constexpr int VE = 16 / (int)sizeof(T);  // values of a vector
   const T* base;  // aligned; value e of the row is base[shift + e]
-  int shift;
-  int64_t full0, full1, count, V;  // whole vectors, all vectors
-  __device__ __forceinline__ Row(const T* row, int64_t vocab) {
+  int shift, full0, full1, count, V;  // whole vectors, all vectors; a row has at most 2^21 values
+  __device__ __forceinline__ Row(const T* row, int vocab) {
     shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     base = row - shift;
     V = vocab;
@@ -72,17 +70,17 @@ struct Row {
     full0 = shift ? 1 : 0;
     full1 = (shift + vocab) / VE;
   }
-  __device__ __forceinline__ int64_t index(int64_t v) const { return v * VE - shift; }  // of the vector's first value
+  __device__ __forceinline__ int index(int v) const { return v * VE - shift; }  // of the vector's first value
 };
 
 template <typename T>
-__device__ __forceinline__ uint4 load_vec(const Row<T>& r, int64_t v, int64_t end) {
+__device__ __forceinline__ uint4 load_vec(const Row<T>& r, int v, int end) {
   if (v >= r.full0 && v < r.full1 && v < end) return *reinterpret_cast<const uint4*>(r.base + v * Row<T>::VE);
   uint32_t w[4];
   if (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t e = r.index(v) + j;
+      const int e = r.index(v) + j;
       w[j] = v < end && e >= 0 && e < r.V ? reinterpret_cast<const uint32_t*>(r.base)[v * 4 + j] : 0xff800000u;
     }
   } else {
@@ -91,7 +89,7 @@ __device__ __forceinline__ uint4 load_vec(const Row<T>& r, int64_t v, int64_t en
       w[j] = 0u;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int64_t e = r.index(v) + 2 * j + i;
+        const int e = r.index(v) + 2 * j + i;
         const uint32_t h =
             v < end && e >= 0 && e < r.V ? reinterpret_cast<const uint16_t*>(r.base)[v * 8 + 2 * j + i] : 0xff80u;
         w[j] |= h << (16 * i);
@@ -147,10 +145,10 @@ __device__ __forceinline__ float vec_max(const uint4 (&u)[N]) {
 // Order of the alternatives: a 64-bit key, larger first; no two are equal.
 // NaNs come last.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint64_t key_of(float x, int64_t index) {
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
   const uint32_t b = __float_as_uint(x + 0.f);  // one zero
   const uint32_t o = x != x ? 0u : b ^ ((int32_t)b < 0 ? 0xffffffffu : 0x80000000u);
-  return (uint64_t)o << 32 | (uint32_t)~(uint32_t)index;
+  return (uint64_t)o << 32 | (uint32_t)~index;
 }
 __device__ __forceinline__ float key_value(uint64_t key) {
   const uint32_t o = (uint32_t)(key >> 32);
@@ -158,24 +156,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ float bitonic_step(float v, int j, bool larger_low) {
-  const float o = __shfl_xor_sync(0xffffffffu, v, j);
-  const bool low = ((threadIdx.x & 31) & j) == 0;
-  return low == larger_low ? fmaxf(v, o) : fminf(v, o);
-}
-// Largest in lane 0
-__device__ __forceinline__ float warp_sort(float v) {
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) v = bitonic_step(v, j, ((threadIdx.x & 31) & k) == 0);
-  return v;
-}
-__device__ __forceinline__ float warp_merge(float v) {  // of a bitonic sequence
-#pragma unroll
-  for (int j = 16; j > 0; j >>= 1) v = bitonic_step(v, j, true);
-  return v;
-}
 __device__ __forceinline__ uint64_t warp_max(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -205,8 +185,8 @@ __device__ __forceinline__ float entropy_of(const Part& p) { return p.s == 0.f ?
 struct TopShared {
   uint64_t best[kMostTop], joined[kMostTop];  // of the block, of the row's blocks together
   uint64_t cand[kCandidates];
-  float lists[16][32];
   uint64_t warps[16];
+  float maxima[4 * kMostTop];
   int seg[kSegments];
   float bound;
   int segments, candidates;
@@ -215,8 +195,8 @@ struct TopShared {
 // A block's share [v0, v1) of a row's vectors.  It is walked as [i0, ve): whole
 // vectors first, a first one that is not whole (v0 < i0) in the place behind the last.
 struct Share {
-  int64_t v0, v1, i0, ve;
-  __device__ __forceinline__ int64_t at(int64_t v) const { return v == v1 ? v0 : v; }
+  int v0, v1, i0, ve;
+  __device__ __forceinline__ int at(int v) const { return v == v1 ? v0 : v; }
 };
 
 // The k largest keys of a share into sh.best, in order (0: none left).  segmax:
@@ -225,68 +205,91 @@ template <typename T, int THREADS>
 __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, const float* segmax, float tm, TopShared& sh) {
   constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float v = warp_sort(tm);
   if (tid == 0) sh.segments = sh.candidates = 0;
+  // values of a vector that reach the bound, as candidates
+  auto push = [&](const uint4& u, int e0, float bound, bool all) {
+    uint32_t hits = 0;
 #pragma unroll
-  for (int half = W / 2; half > 0; half >>= 1) {
-    if (warp >= half && warp < 2 * half) sh.lists[warp][lane] = v;
-    __syncthreads();
-    if (warp < half) v = warp_merge(fmaxf(v, sh.lists[warp + half][31 - lane]));
-  }
-  if (tid == k - 1) sh.bound = v;  // k <= 32: a lane of warp 0
-  __syncthreads();
-  const float bound = sh.bound;
-  bool fast = bound > kFloor;
-  if (fast) {
-    for (int it = 0; it < tiles; ++it)
-      if (segmax[it * THREADS + tid] >= bound) {
-        const int i = atomicAdd(&sh.segments, 1);
-        if (i < kSegments) sh.seg[i] = it * THREADS + tid;
-      }
-    __syncthreads();
-    const int n = sh.segments;
-    fast = n <= kSegments;
-    if (fast) {
-      for (int i = tid; i < n * VPT; i += THREADS) {
-        const int g = sh.seg[i / VPT];
-        const int64_t walk = z.i0 + (int64_t)(g / THREADS) * (THREADS * VPT) + (i % VPT) * THREADS + g % THREADS;
-        const int64_t vec = z.at(walk);
-        const uint4 u = load_vec(r, vec, walk < z.ve ? z.v1 : 0);
-#pragma unroll
-        for (int j = 0; j < VE / 2; ++j) {
-          const float2 x = two<T>(u, j);
-          if (x.x >= bound) {
-            const int c = atomicAdd(&sh.candidates, 1);
-            if (c < kCandidates) sh.cand[c] = key_of(x.x, r.index(vec) + 2 * j);
-          }
-          if (x.y >= bound) {
-            const int c = atomicAdd(&sh.candidates, 1);
-            if (c < kCandidates) sh.cand[c] = key_of(x.y, r.index(vec) + 2 * j + 1);
-          }
-        }
-      }
-      __syncthreads();
-      const int c = sh.candidates;
-      fast = c <= kCandidates;
-      if (fast) {
-        for (int i = tid; i < c; i += THREADS) {
-          const uint64_t mine = sh.cand[i];
-          int rank = 0;
-          for (int j = 0; j < c; ++j) rank += sh.cand[j] > mine;
-          if (rank < k) sh.best[rank] = mine;
-        }
-      }
+    for (int j = 0; j < VE; ++j) {
+      const float2 x = two<T>(u, j / 2);
+      const bool in = e0 + j >= 0 && e0 + j < r.V;
+      if (in && (all || (j & 1 ? x.y : x.x) >= bound)) hits |= 1u << j;
     }
+    if (!hits) return;
+    int c = atomicAdd(&sh.candidates, __popc(hits));
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      if (hits >> j & 1) {
+        const float2 x = two<T>(u, j / 2);
+        if (c < kCandidates) sh.cand[c] = key_of(j & 1 ? x.y : x.x, e0 + j);
+        ++c;
+      }
+  };
+  bool fast;
+  const int lanes = z.ve - z.i0 < THREADS ? z.ve - z.i0 : THREADS;  // that have values
+  if (lanes < k) {  // 31 vectors at most: all of them
+    __syncthreads();
+    for (int vec = z.v0 + tid; vec < z.v1; vec += THREADS) push(load_vec(r, vec, z.v1), r.index(vec), 0.f, true);
+    fast = true;
+  } else {
+    int each = 32;  // lanes of a group
+    while (each > 1 && lanes < 2 * k * each) each >>= 1;
+    const int groups = (lanes + each - 1) / each;  // that have values: k to 4 k, or a warp each
+    float v = tm;
+    for (int o = 1; o < each; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (lane % each == 0 && tid / each < groups) sh.maxima[tid / each] = v;
+    __syncthreads();
+    if (tid < groups) {  // the place of each in their order
+      const float mine = sh.maxima[tid];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < groups; ++j) {
+        const float m = sh.maxima[j];
+        place += m > mine || (m == mine && j < tid);
+      }
+      if (place == k - 1) sh.bound = mine;
+    }
+    __syncthreads();
+    const float bound = sh.bound;
+    fast = bound > kFloor;  // too few values end below
+    if (fast) {
+      for (int it = 0; it < tiles; ++it)
+        if (segmax[it * THREADS + tid] >= bound) {
+          const int i = atomicAdd(&sh.segments, 1);
+          if (i < kSegments) sh.seg[i] = it * THREADS + tid;
+        }
+      __syncthreads();
+      const int n = sh.segments;
+      fast = n <= kSegments;
+      if (fast)
+        for (int i = tid; i < n * VPT; i += THREADS) {
+          const int g = sh.seg[i / VPT], walk = z.i0 + (g / THREADS) * (THREADS * VPT) + (i % VPT) * THREADS + g % THREADS;
+          if (walk < z.ve) push(load_vec(r, z.at(walk), z.v1), r.index(z.at(walk)), bound, false);
+        }
+    }
+  }
+  __syncthreads();
+  const int c = sh.candidates;
+  fast = fast && c <= kCandidates;
+  if (fast) {
+    for (int i = tid; i < c; i += THREADS) {
+      const uint64_t mine = sh.cand[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < c; ++j) rank += sh.cand[j] > mine;
+      if (rank < k) sh.best[rank] = mine;
+    }
+    if (tid >= c && tid < k) sh.best[tid] = 0;  // fewer than k
   }
   if (!fast) {  // one after the other; a thread looks again only when its best is taken
     auto below = [&](uint64_t prev) {
       uint64_t best = 0;
-      for (int64_t vec = z.v0 + tid; vec < z.v1; vec += THREADS) {
+      for (int vec = z.v0 + tid; vec < z.v1; vec += THREADS) {
         const uint4 u = load_vec(r, vec, z.v1);
 #pragma unroll
         for (int j = 0; j < VE / 2; ++j) {
           const float2 x = two<T>(u, j);
-          const int64_t e = r.index(vec) + 2 * j;
+          const int e = r.index(vec) + 2 * j;
           const uint64_t a = key_of(x.x, e), b = key_of(x.y, e + 1);
           if (e >= 0 && e < r.V && a < prev && a > best) best = a;
           if (e + 1 >= 0 && e + 1 < r.V && b < prev && b > best) best = b;
@@ -400,7 +403,7 @@ __device__ __forceinline__ Part block_part(const Sums& a, float (&red)[3][W]) {
 // Blocks an SM for the register budget: 16-bit values leave 40 a thread, 32-bit ones
 // (a segment is 32 registers) 64.
 template <typename T>
-constexpr int fwd_blocks(int threads) { return (sizeof(T) == 4 ? 1024 : 1536) / threads; }
+constexpr int fwd_blocks(int threads) { return threads == 32 ? 32 : (sizeof(T) == 4 ? 1024 : 1536) / threads; }
 
 // One row a cluster of CL blocks, each over its share of the row's vectors; block
 // 0 joins the shares through distributed shared memory.
@@ -416,8 +419,8 @@ __global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_
   const int CL = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
   const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
   const int64_t row = CLUSTER ? blockIdx.x / CL : blockIdx.x;
-  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
-  const int64_t each = (r.count + CL - 1) / CL;
+  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, (int)p.V);
+  const int each = (r.count + CL - 1) / CL;
   Share z;
   z.v0 = rank * each < r.count ? rank * each : r.count;
   z.v1 = z.v0 + each < r.count ? z.v0 + each : r.count;
@@ -428,9 +431,16 @@ __global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_
   Sums a = {kFloor, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   float tm = kFloor;
   int it = 0;
-  const int64_t whole = z.v1 < r.full1 ? z.v1 : r.full1;
-  int64_t v = z.i0 + tid;
-  for (int64_t left = whole - z.i0; left >= TILE; left -= TILE, v += TILE, ++it) {
+  // what the given token needs is on its way while the row is read
+  int64_t given = -1;
+  float at_given = __uint_as_float(0x7fc00000u);
+  if (rank == 0 && tid == 0) {
+    given = target_of(p.targets, p.ids64, row);
+    if (given >= 0 && given < p.V) at_given = value_of(r.base + r.shift + given);
+  }
+  const int whole = z.v1 < r.full1 ? z.v1 : r.full1;
+  int v = z.i0 + tid;
+  for (int left = whole - z.i0; left >= TILE; left -= TILE, v += TILE, ++it) {
     uint4 u[VPT];
     const uint4* from = reinterpret_cast<const uint4*>(r.base) + v;
 #pragma unroll
@@ -445,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_
     uint4 u[VPT];
 #pragma unroll
     for (int q = 0; q < VPT; ++q) {
-      const int64_t w = v + q * THREADS;
+      const int w = v + q * THREADS;
       u[q] = load_vec(r, z.at(w), w < z.ve ? z.v1 : 0);
     }
     const float mx = add_vecs<T>(a, u);
@@ -457,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_
   Part part = block_part<W>(a, red[0]);
   if (careful(part.m)) {  // the same for the whole block
     a = {kLowest, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    for (int64_t w = z.v0 + tid; w < z.v1; w += THREADS) add_careful<T>(a, load_vec(r, w, z.v1));
+    for (int w = z.v0 + tid; w < z.v1; w += THREADS) add_careful<T>(a, load_vec(r, w, z.v1));
     part = block_part<W>(a, red[1]);
   }
   if (TOP) select_top<T, THREADS>(r, z, p.top, it, segmax, tm, sh);
@@ -500,11 +510,8 @@ __global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_
     p.top_id[row * p.top + tid] = (int64_t)key_index(key);
   }
   if (tid == 0) {
-    const int64_t t = target_of(p.targets, p.ids64, row);
-    float lp = __uint_as_float(0x7fc00000u);
-    if (t == p.ignore) lp = 0.f;
-    else if (t >= 0 && t < p.V) lp = logprob_of(value_of(r.base + r.shift + t), part);
-    p.logprob[row] = lp;
+    const bool in = given >= 0 && given < p.V;
+    p.logprob[row] = given == p.ignore ? 0.f : in ? logprob_of(at_given, part) : at_given;
     p.entropy[row] = entropy_of(part);
     p.stats[2 * row] = part.m;
     p.stats[2 * row + 1] = part.s;
@@ -576,14 +583,15 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
   __shared__ Coef shared_coef;
   __shared__ bool mine;  // whether a place with a gradient of its own is in the block's range
   const int tid = threadIdx.x, B_ = blockDim.x;
-  const int64_t row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
-  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
+  const int64_t row = blockIdx.x / (uint32_t)p.chunks;
+  const int chunk = (int)(blockIdx.x - (uint32_t)row * (uint32_t)p.chunks);
+  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, (int)p.V);
   T* out = static_cast<T*>(p.gx) + row * p.V;
-  const int64_t first = chunk * ((int64_t)B_ * VPT * p.tiles);
-  int64_t end = first + (int64_t)B_ * VPT * p.tiles;
+  const int first = chunk * (B_ * VPT * p.tiles);
+  int end = first + B_ * VPT * p.tiles;
   end = end < r.count ? end : r.count;
   const bool same = ((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) == (uintptr_t)r.shift;
-  auto whole = [&](int64_t a) { return same && a >= r.full0 && a + B_ * VPT <= (end < r.full1 ? end : r.full1); };
+  auto whole = [&](int a) { return same && a >= r.full0 && a + B_ * VPT <= (end < r.full1 ? end : r.full1); };
   uint4 u[VPT];
   const bool ahead = whole(first);
   if (ahead) {
@@ -606,7 +614,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
   if (tid == 0) {
     float G = own[0];
     bool any = false;
-    const int64_t lo = r.index(first), hi = r.index(end);
+    const int lo = r.index(first), hi = r.index(end);
     for (int i = 0; i <= p.top; ++i) {
       if (i) G += own[i];
       any = any || (at[i] >= 0 && at[i] >= lo && at[i] < hi);
@@ -624,17 +632,17 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
   __syncthreads();
   const Coef k = shared_coef;
   if (careful(k.m)) {  // and rows without anything
-    for (int64_t v = first + tid; v < end; v += B_) {
+    for (int v = first + tid; v < end; v += B_) {
       const uint4 w = load_vec(r, v, end);
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
         const float2 x = two<T>(w, j / 2);
-        const int64_t e = r.index(v) + j;
+        const int e = r.index(v) + j;
         if (e >= 0 && e < p.V) put(out + e, grad_of(j & 1 ? x.y : x.x, k));
       }
     }
   } else {
-    for (int64_t a = first; a < end; a += B_ * VPT) {
+    for (int a = first; a < end; a += B_ * VPT) {
       if (whole(a)) {
         const uint4* from = reinterpret_cast<const uint4*>(r.base) + a + tid;
         uint4* to = reinterpret_cast<uint4*>(out - r.shift) + a + tid;
@@ -647,7 +655,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
       } else {
 #pragma unroll
         for (int q = 0; q < VPT; ++q) {
-          const int64_t v = a + q * B_ + tid;
+          const int v = a + q * B_ + tid;
           if (v >= end) continue;
           const uint4 g = grad_vec<T, H>(load_vec(r, v, end), k);
           if (same && v >= r.full0 && v < r.full1) {
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
           } else {
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-              const int64_t e = r.index(v) + j;
+              const int e = r.index(v) + j;
               const float2 x = two<T>(g, j / 2);
               if (e >= 0 && e < p.V) put(out + e, j & 1 ? x.y : x.x);
             }
@@ -666,7 +674,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
   }
   if (!mine) return;
   __syncthreads();  // before these places are written again
-  const int64_t lo = r.index(first), hi = r.index(end);
+  const int lo = r.index(first), hi = r.index(end);
   for (int i = tid; i <= p.top; i += B_) {
     const int64_t e = at[i];
     if (e < 0 || e >= p.V || e < lo || e >= hi) continue;
@@ -706,15 +714,21 @@ int launch_fwd(FwdArgs p, int CL, cudaStream_t st) {
 
 template <typename T>
 int pick_fwd(const FwdArgs& p, cudaStream_t st) {
-  // few rows: several blocks a row, so that the GPU is filled
+  // Few rows: several blocks a row while the GPU has room and a share stays long
+  // (joining shares costs 0.5 us, with alternatives 1 to 4: [1, 131072] fp32 8.3 us on
+  // one block, 5.9 on four, [1, 32768] 3.7 on one, 4.4 on four).
   int CL = 1;
-  while (CL < kMostCluster && p.rows * CL * 2 <= 2 * num_sms() && p.V >= (int64_t)CL * 2 * 2048) CL *= 2;
-  // a thread has at most kMostTiles segments
-  while (p.top > 0 && CL < kMostCluster && p.V + 16 > (int64_t)CL * 512 * kPer * kMostTiles) CL *= 2;
+  while (CL < kMostCluster && p.rows * CL * 2 <= num_sms() && p.V > (int64_t)CL * 49152) CL *= 2;
+  while (p.top > 0 && p.V > (int64_t)CL * kMostShare) CL *= 2;  // 8 at most: a row has up to 2^21 values
   MHC_REQUIRE(p.rows * CL < (1ll << 31), MHC_ERR_UNSUPPORTED, "token_logprobs: %lld rows are too many", (long long)p.rows);
-  const bool small = (p.V + CL - 1) / CL <= 8192;
-  if (p.top > 0) return small ? launch_fwd<T, 128, true>(p, CL, st) : launch_fwd<T, 512, true>(p, CL, st);
-  return small ? launch_fwd<T, 128, false>(p, CL, st) : launch_fwd<T, 512, false>(p, CL, st);
+  // Small blocks hide each other's ends where there are many rows ([32768, 4096] bf16: 53
+  // and 65 us with 32 and 128 threads, [19691, 13632]: 114, 137 and 184 us with 128, 256
+  // and 512); few rows want more threads each.
+  const int64_t share = (p.V + CL - 1) / CL, blocks = p.rows * CL;
+  const int th = share <= 8192 ? (blocks >= 4 * num_sms() ? 32 : 128) : blocks < 2 * num_sms() ? 512 : share <= 32768 ? 128 : 256;
+#define MHC_GO(TH) (p.top > 0 ? launch_fwd<T, TH, true>(p, CL, st) : launch_fwd<T, TH, false>(p, CL, st))
+  return th == 32 ? MHC_GO(32) : th == 128 ? MHC_GO(128) : th == 256 ? MHC_GO(256) : MHC_GO(512);
+#undef MHC_GO
 }
 
 int check_args(const char* what, int64_t rows, int64_t vocab, int64_t stride, int32_t top, int32_t bf16, const void* logits) {

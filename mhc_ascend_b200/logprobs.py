@@ -50,19 +50,21 @@ def token_logprobs_fwd(logits: torch.Tensor, targets: torch.Tensor, top: int = 0
     what = "token_logprobs"
     _check(what, logits, targets, top)
     x, stride = _rows2d(logits)
-    t = targets if targets.is_contiguous() else targets.contiguous()
+    t = _dense(targets)
     rows, vocab = x.shape
-    lead, dev, f32 = targets.shape, x.device, torch.float32
-    logprob = torch.empty(lead, dtype=f32, device=dev)
-    entropy = torch.empty(lead, dtype=f32, device=dev)
-    stats = torch.empty(rows, 2, dtype=f32, device=dev)
+    lead, dev = t.shape, x.device
+    logprob = torch.empty_like(t, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
     top_logprob = top_id = None
+    values = ids = 0
     if top:
-        top_logprob = torch.empty(*lead, top, dtype=f32, device=dev)
+        top_logprob = torch.empty(*lead, top, dtype=torch.float32, device=dev)
         top_id = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+        values, ids = top_logprob.data_ptr(), top_id.data_ptr()
     _launch("mhc_token_logprobs_fwd", dev, x.data_ptr(), x.dtype == torch.bfloat16, stride, t.data_ptr(),
-            t.dtype == torch.int64, int(ignore_index), logprob.data_ptr(), entropy.data_ptr(), _ptr(top_logprob),
-            _ptr(top_id), stats.data_ptr(), rows, vocab, top)
+            t.dtype == torch.int64, ignore_index, logprob.data_ptr(), entropy.data_ptr(), values, ids, stats.data_ptr(),
+            rows, vocab, top)
     return TokenLogprobs(logprob, entropy, top_logprob, top_id, stats)
 
 
