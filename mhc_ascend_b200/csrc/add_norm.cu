@@ -56,12 +56,18 @@ __device__ __forceinline__ float group_max(float m) {  // over 16 lanes, NaN if 
 
 constexpr int fwd_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : UPT == 2 ? 512 : 1024; }
 
+// Rows over threads of the kernels below; SMALL: four units a thread of at most 256,
+// four blocks an SM.
+enum class Lay { kWarp, kBlock, kSmall };
+
 // Rows that wide accesses fit.  A row stays in registers between the sum and the
 // output, UPT units a thread.  CODED: what is kept is h w, and its maxima are taken
 // with the sum (r > 0 is common to the row: max |y| = max |h w| / r), so that after
 // the barrier a value costs one product and its conversion.
-template <typename TR, typename TB, int UPT, bool WARP, bool CODED>
-__global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_kernel(const FwdArgs p) {
+template <typename TR, typename TB, int UPT, Lay LAY, bool CODED>
+__global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LAY == Lay::kWarp), LAY == Lay::kSmall ? 4 : 1)
+    add_norm_fwd_kernel(const FwdArgs p) {
+  constexpr bool WARP = LAY == Lay::kWarp;
   __shared__ float red[32], redm[32];
   const int lane = threadIdx.x & 31, cols = (int)p.cols;
   const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -260,15 +266,21 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_fwd_long_kernel(const F
 }
 
 struct FwdPlan {
+  Lay lay;
   int UPT, threads;  // UPT = 0: the long kernel
-  bool warp;
 };
-FwdPlan fwd_plan(int64_t cols) {
+// Rows of 1025 to 8192 columns: where there are many, four units a thread, since more and
+// smaller blocks overlap each other's barriers ([16384, 7168] bf16 to e4m3 with a scale for
+// each 128: 129 us, 6.4 TB/s, against 162 with two units and 448 threads, 175 with one and
+// 896); where there are few, as many threads as there are units ([1, 4096] 2.4 us against 3.3).
+FwdPlan fwd_plan(int64_t rows, int64_t cols, bool even) {
   const int64_t pitch = ck_pitch(cols), U = pitch / 8;
-  if (pitch <= kWarpCols) return {pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows, true};
+  if (pitch <= kWarpCols) return {Lay::kWarp, pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows};
+  auto threads = [&](int upt) { return (int)(((U + upt - 1) / upt + 31) / 32 * 32); };
+  if (even && U <= 1024 && rows >= 2 * num_sms()) return {Lay::kSmall, 4, threads(4)};
   for (int upt : {1, 2, 4})
-    if (U <= upt * fwd_threads(upt, false)) return {upt, (int)(((U + upt - 1) / upt + 31) / 32 * 32), false};
-  return {0, kLongThreads, false};
+    if (U <= upt * fwd_threads(upt, false)) return {Lay::kBlock, upt, threads(upt)};
+  return {Lay::kBlock, 0, kLongThreads};
 }
 
 template <bool CODED, typename TR, typename TB>
@@ -276,21 +288,22 @@ int launch_fwd(const FwdArgs& p, cudaStream_t st) {
   bool even = even_rows<TR>(p.res, p.cols, p.cols) && even_rows<TR>(p.hidden, p.cols, p.cols) &&
               even_rows<TB>(p.branch, p.cols, p.cols) && even_rows<float>(p.w, p.cols, p.cols);
   even = even && (CODED ? (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 : even_rows<TB>(p.out, p.cols, p.cols));
-  const FwdPlan pl = fwd_plan(p.cols);
-  const unsigned blocks = (unsigned)(pl.warp ? (p.rows + kWarpRows - 1) / kWarpRows : p.rows);
+  const FwdPlan pl = fwd_plan(p.rows, p.cols, even);
+  const unsigned blocks = (unsigned)(pl.lay == Lay::kWarp ? (p.rows + kWarpRows - 1) / kWarpRows : p.rows);
   ProfScope prof(CODED ? "add_rmsnorm_coded" : "add_rmsnorm_fwd", st);
-#define MHC_GO(UPT, WARP)                                                                              \
-  do {                                                                                                 \
-    if (even) add_norm_fwd_kernel<TR, TB, UPT, WARP, CODED><<<blocks, pl.threads, 0, st>>>(p);         \
-    else add_norm_fwd_any_kernel<UPT, WARP, CODED><<<blocks, pl.threads, 0, st>>>(p);                  \
+#define MHC_GO(UPT, LAY)                                                                                     \
+  do {                                                                                                       \
+    if (even) add_norm_fwd_kernel<TR, TB, UPT, LAY, CODED><<<blocks, pl.threads, 0, st>>>(p);                \
+    else add_norm_fwd_any_kernel<UPT, LAY == Lay::kWarp, CODED><<<blocks, pl.threads, 0, st>>>(p);           \
   } while (0)
   if (pl.UPT == 0) add_norm_fwd_long_kernel<CODED><<<blocks, pl.threads, 0, st>>>(p);
-  else if (pl.warp && pl.UPT == 1) MHC_GO(1, true);
-  else if (pl.warp && pl.UPT == 2) MHC_GO(2, true);
-  else if (pl.warp) MHC_GO(4, true);
-  else if (pl.UPT == 1) MHC_GO(1, false);
-  else if (pl.UPT == 2) MHC_GO(2, false);
-  else MHC_GO(4, false);
+  else if (pl.lay == Lay::kSmall) add_norm_fwd_kernel<TR, TB, 4, Lay::kSmall, CODED><<<blocks, pl.threads, 0, st>>>(p);
+  else if (pl.lay == Lay::kWarp && pl.UPT == 1) MHC_GO(1, Lay::kWarp);
+  else if (pl.lay == Lay::kWarp && pl.UPT == 2) MHC_GO(2, Lay::kWarp);
+  else if (pl.lay == Lay::kWarp) MHC_GO(4, Lay::kWarp);
+  else if (pl.UPT == 1) MHC_GO(1, Lay::kBlock);
+  else if (pl.UPT == 2) MHC_GO(2, Lay::kBlock);
+  else MHC_GO(4, Lay::kBlock);
 #undef MHC_GO
   return check_launch("add_rmsnorm");
 }
@@ -311,34 +324,48 @@ int with_types(int32_t a_bf16, int32_t b_bf16, F f) {
   return b_bf16 ? f((float*)nullptr, (__nv_bfloat16*)nullptr) : f((float*)nullptr, (float*)nullptr);
 }
 
-// Codes back to values: one unit of 8 a thread and turn.
+// Codes back to values: units of 8, four a thread and 256 apart.
+constexpr int kUnpackUnits = 4;
 template <typename T, bool EVEN>
 __global__ void __launch_bounds__(256)
     coded_unpack_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out,
                         int64_t rows, int64_t cols, int64_t U, int64_t groups, bool int8, bool grouped) {
   __shared__ __align__(16) float sm[EVEN ? 1 : 256 * 8];
   float* mine = sm + (EVEN ? 0 : (threadIdx.x >> 5) * 256);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t first = (int64_t)blockIdx.x * (256 * kUnpackUnits) + threadIdx.x;
   int64_t row, u;
-  if ((uint64_t)i >> 32 || (uint64_t)U >> 32) {
-    row = i / U;
-    u = i - row * U;
+  if ((uint64_t)first >> 32 || (uint64_t)U >> 32) {
+    row = first / U;
+    u = first - row * U;
   } else {  // a 64-bit division takes longer than the rest
-    row = (uint32_t)i / (uint32_t)U;
-    u = (uint32_t)i - (uint32_t)row * (uint32_t)U;
+    row = (uint32_t)first / (uint32_t)U;
+    u = (uint32_t)first - (uint32_t)row * (uint32_t)U;
   }
-  const int64_t c = 8 * u;
-  const bool on = row < rows && c < cols;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (on) {
-    const uint8_t* from = codes + row * cols;
-    const float scale = scales[row * groups + (grouped ? c / kCodedGroup : 0)];
-    coded_unpack(EVEN ? *reinterpret_cast<const uint2*>(from + c) : coded_load_any(from, c, cols), scale, int8, v);
+  int64_t at[kUnpackUnits], col[kUnpackUnits];
+  uint2 w[kUnpackUnits];
+  float scale[kUnpackUnits];
+#pragma unroll
+  for (int k = 0; k < kUnpackUnits; ++k) {
+    at[k] = row;
+    col[k] = 8 * u;
+    w[k] = make_uint2(0u, 0u);
+    scale[k] = 0.f;
+    if (row < rows && 8 * u < cols) {
+      const uint8_t* from = codes + row * cols;
+      scale[k] = scales[row * groups + (grouped ? 8 * u / kCodedGroup : 0)];
+      w[k] = EVEN ? *reinterpret_cast<const uint2*>(from + 8 * u) : coded_load_any(from, 8 * u, cols);
+    }
+    for (u += 256; u >= U; u -= U) ++row;
   }
-  if (EVEN) {
-    if (on) ck_save(out + row * cols + c, v);
-  } else {  // U % 32 == 0: the warp is in one row
-    ck_save_any(out + row * cols, c - 8 * (threadIdx.x & 31), row < rows ? cols : 0, mine, v);
+#pragma unroll
+  for (int k = 0; k < kUnpackUnits; ++k) {
+    float v[8];
+    coded_unpack(w[k], scale[k], int8, v);
+    if (EVEN) {
+      if (at[k] < rows && col[k] < cols) ck_save(out + at[k] * cols + col[k], v);
+    } else {  // U % 32 == 0: the warp is in one row
+      ck_save_any(out + at[k] * cols, col[k] - 8 * (threadIdx.x & 31), at[k] < rows ? cols : 0, mine, v);
+    }
   }
 }
 
@@ -409,7 +436,7 @@ extern "C" int mhc_coded8_unpack(const void* codes, int32_t codes_int8, const fl
   return with_types(out_bf16, 0, [&](auto* o, auto*) -> int {
     using T = std::remove_pointer_t<decltype(o)>;
     const bool even = even_rows<T>(out, cols, cols) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
-    const int64_t u = (cols + 7) / 8, U = even ? u : (u + 31) / 32 * 32, blocks = (rows * U + 255) / 256;
+    const int64_t u = (cols + 7) / 8, U = even ? u : (u + 31) / 32 * 32, blocks = (rows * U + 256 * kUnpackUnits - 1) / (256 * kUnpackUnits);
     MHC_REQUIRE(blocks < (1ll << 31), MHC_ERR_UNSUPPORTED, "coded8_unpack: %lld x %lld values are too many", (long long)rows,
                 (long long)cols);
     const int64_t groups = coded_groups(cols, grouped != 0);
