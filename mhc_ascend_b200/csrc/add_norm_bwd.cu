@@ -116,15 +116,25 @@ __global__ void __launch_bounds__(32 * kWarpRows) add_norm_bwd_warp_kernel(const
 }
 
 // ---------------------------------------------------------------------------
-// Rows of 1025 to 8192 columns that 16-byte copies fit: each thread copies its own
-// units of the rows ahead into shared memory (cp.async), `stages` rows deep, and
-// is the only one to read them, so the row's one barrier is that of its sum.
+// Rows of 1025 to 8192 columns, of any width: units are the tensor's own groups of
+// eight values, so that every access is aligned wherever a row starts; a row's first
+// and last unit may belong to its neighbours in part.  A block's rows are a multiple
+// of 8 apart (or of fewer, as the width allows): they all start at the same place of a
+// unit, and a thread keeps its columns, with their weights and sums, over all of them.
+// The rows ahead are copied into shared memory (cp.async), `stages` deep, each warp
+// what it will read itself, so the row's one barrier is that of its sum.  Copies of
+// 512 consecutive bytes a warp and 16-byte pieces stored crosswise: a 32-byte unit a
+// lane met every sector twice on its way in ([8192, 4096], fp32 residual, bf16 branch,
+// 122 us).
 // ---------------------------------------------------------------------------
 constexpr int kStagesMost = 4;
 constexpr int kStageBytes = 224 * 1024;  // of an SM's blocks together
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_part(uint32_t to, const void* from, uint32_t bytes) {  // zeros behind
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all but the latest n - 1 groups have landed, 1 <= n <= 4
@@ -135,64 +145,83 @@ __device__ __forceinline__ void copies_wait(int n) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// A unit in shared memory: its 16-byte pieces `apart` bytes from each other, those of
-// all threads side by side.
+// A warp's 256 consecutive values: its lanes copy pieces of 16 bytes side by side.
+// need: values that the row wants (a piece that holds none is left out); left: those
+// that the tensor has from the warp's first on.
 template <typename T>
-__device__ __forceinline__ void unit_copy(uint32_t to, uint32_t apart, const T* from) {
-  copy16(to, from);
-  if (sizeof(T) == 4) copy16(to + apart, from + 4);
+__device__ __forceinline__ void span_copy(uint32_t to, const T* from, int need, int64_t left) {
+  constexpr int per = 16 / (int)sizeof(T);  // values of a piece
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int q = 0; q < (int)sizeof(T) / 2; ++q) {
+    const int piece = 32 * q + lane, e = piece * per;
+    const uint32_t at = to + 16u * (sizeof(T) == 4 ? piece ^ ((piece >> 3) & 1) : piece);
+    if (e < need && e < left) {
+      if (e + per <= left) copy16(at, from + e);
+      else copy_part(at, from + e, (uint32_t)(left - e) * sizeof(T));
+    }
+  }
 }
-__device__ __forceinline__ V8 unit_read(const unsigned char* at, uint32_t apart, const float*) {
-  const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + apart);
+// The lane's unit of them
+__device__ __forceinline__ V8 span_read(const unsigned char* at, const float*) {
+  const int lane = threadIdx.x & 31, b = (lane >> 2) & 1;
+  const float4 x = *reinterpret_cast<const float4*>(at + 16 * ((2 * lane) ^ b));
+  const float4 y = *reinterpret_cast<const float4*>(at + 16 * ((2 * lane + 1) ^ b));
   V8 v;
-  v.a[0] = make_float2(a.x, a.y);
-  v.a[1] = make_float2(a.z, a.w);
-  v.a[2] = make_float2(b.x, b.y);
-  v.a[3] = make_float2(b.z, b.w);
+  v.a[0] = make_float2(x.x, x.y);
+  v.a[1] = make_float2(x.z, x.w);
+  v.a[2] = make_float2(y.x, y.y);
+  v.a[3] = make_float2(y.z, y.w);
   return v;
 }
-__device__ __forceinline__ V8 unit_read(const unsigned char* at, uint32_t, const __nv_bfloat16*) {
-  return v8_of(*reinterpret_cast<const uint4*>(at));
+__device__ __forceinline__ V8 span_read(const unsigned char* at, const __nv_bfloat16*) {
+  return v8_of(*reinterpret_cast<const uint4*>(at + 16 * (threadIdx.x & 31)));
+}
+// Values of a unit outside columns [0, cols) as zeros
+__device__ __forceinline__ V8 v8_inside(const V8& v, int c, int cols) {
+  float f[8];
+  v8_spread(v, f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = c + j >= 0 && c + j < cols ? f[j] : 0.f;
+  return v8_gather(f);
+}
+template <typename T>
+__device__ __forceinline__ void put_inside(T* to, const float (&f)[8], int c, int cols) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c + j >= 0 && c + j < cols) ck_store(to + j, f[j]);
 }
 
-template <typename TR, typename TB, int UPT>
-__global__ void __launch_bounds__(512, 2) add_norm_bwd_ring_kernel(const BwdArgs p, int stages) {
+template <typename TR, typename TB>
+__global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArgs p, int stages) {
   let_next_start();
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float red[2][16];
+  __shared__ float red[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, cols = (int)p.cols;
-  // a stage: pieces of gh, of h, of g, each 16 bytes for every unit
-  const uint32_t apart = 16u * UPT * blockDim.x;
-  constexpr uint32_t at_h = sizeof(TR) / 2, at_g = sizeof(TR);  // in pieces
-  const uint32_t stage = apart * (uint32_t)(sizeof(TR) + sizeof(TB) / 2);
+  const int shift = (int)(((int64_t)blockIdx.x * cols) & 7);
+  const int c = 8 * tid - shift;  // the unit's first column
+  const bool on = c < cols, edge = on && (c < 0 || c + 8 > cols);
+  // a stage: gh, h, g of all warps
+  const uint32_t span_r = 256u * sizeof(TR), at_h = nw * span_r, at_g = 2 * at_h;
+  const uint32_t stage = at_g + nw * 256u * sizeof(TB);
   const DropKey key = drop_key(p.drop);
-  // one unit a thread: its weights and what the sum was made of stay in registers;
-  // two: they are read again (64 registers a thread)
-  constexpr bool HOLD = UPT == 1;
-  V8 acc[UPT], wv = v8_zero();
-  bool on[UPT];
+  V8 acc = v8_zero(), wv;
+  {
+    float f[8];
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) {
-    const int c = 8 * (k * (int)blockDim.x + tid);
-    on[k] = c < cols;
-    if (HOLD && on[k]) wv = v8_weights(p.w + c);
-    acc[k] = v8_zero();
+    for (int j = 0; j < 8; ++j) f[j] = c + j >= 0 && c + j < cols ? __ldg(p.w + c + j) : 0.f;
+    wv = v8_gather(f);
   }
-  const int step = 8 * (int)blockDim.x;  // columns between a thread's units
-  const int64_t hop = (int64_t)gridDim.x * cols;
-  int64_t ahead = (int64_t)blockIdx.x * cols + 8 * tid;  // element of the next copies
-  const int64_t end = p.rows * cols;
-  const uint32_t mine = smem_u32(ring) + 16u * tid;
+  const int64_t hop = (int64_t)gridDim.x * cols, total = p.rows * cols;
+  const int need = shift + cols - 256 * warp;
+  int64_t ahead = (int64_t)blockIdx.x * cols - shift + 256 * warp;  // element of the warp's next copies
   auto fetch = [&](uint32_t s) {
-    if (ahead < end) {
-#pragma unroll
-      for (int k = 0; k < UPT; ++k)
-        if (on[k]) {
-          const uint32_t to = mine + s + 16u * k * blockDim.x;
-          if (p.gh) unit_copy(to, apart, static_cast<const TR*>(p.gh) + ahead + k * step);
-          unit_copy(to + at_h * apart, apart, static_cast<const TR*>(p.h) + ahead + k * step);
-          unit_copy(to + at_g * apart, apart, static_cast<const TB*>(p.g) + ahead + k * step);
-        }
+    if (ahead < total) {
+      const uint32_t to = smem_u32(ring) + s;
+      const int64_t left = total - ahead;
+      if (p.gh) span_copy(to + warp * span_r, static_cast<const TR*>(p.gh) + ahead, need, left);
+      span_copy(to + at_h + warp * span_r, static_cast<const TR*>(p.h) + ahead, need, left);
+      span_copy(to + at_g + warp * 256u * (uint32_t)sizeof(TB), static_cast<const TB*>(p.g) + ahead, need, left);
     }
     ahead += hop;
     copies_end();  // a group each time, so that the count of groups is the count of rows
@@ -200,49 +229,56 @@ __global__ void __launch_bounds__(512, 2) add_norm_bwd_ring_kernel(const BwdArgs
   for (int s = 0; s < stages; ++s) fetch(s * stage);
   uint32_t s = 0;
   int buf = 0;
-  int64_t at = (int64_t)blockIdx.x * cols + 8 * tid;
+  int64_t at = (int64_t)blockIdx.x * cols + c;
   float nr = p.rms[blockIdx.x];
   const float share = 1.0f / (float)cols;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1, at += hop) {
     const float ir = 1.0f / nr;
     if (row + gridDim.x < p.rows) nr = p.rms[row + gridDim.x];
     copies_wait(stages);
-    V8 gw, h;
+    __syncwarp();  // the other lanes' too
+    const unsigned char* from = ring + s;
+    V8 g = v8_zero(), h = g;
     float2 d2 = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < UPT; ++k)
-      if (on[k]) {
-        const unsigned char* from = ring + s + 16u * (k * blockDim.x + tid);
-        const V8 g = unit_read(from + at_g * apart, apart, (const TB*)nullptr);
-        h = unit_read(from + at_h * apart, apart, (const TR*)nullptr);
-        acc[k] = v8_fma(v8_scale(g, ir), h, acc[k]);
-        gw = v8_mul(g, HOLD ? wv : v8_weights(p.w + 8 * tid + k * step));
-        d2 = v8_dot(gw, h, d2);
+    if (on) {
+      g = span_read(from + at_g + warp * 256u * sizeof(TB), (const TB*)nullptr);
+      h = span_read(from + at_h + warp * span_r, (const TR*)nullptr);
+      if (edge) {
+        g = v8_inside(g, c, cols);
+        h = v8_inside(h, c, cols);
       }
+      acc = v8_fma(v8_scale(g, ir), h, acc);
+      g = v8_mul(g, wv);
+      d2 = v8_dot(g, h, d2);
+    }
     const float d = warp_sum(d2.x + d2.y);
     if (lane == 0) red[buf][warp] = d;
     __syncthreads();
-    float t = lane < nw ? red[buf][lane & 15] : 0.f;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);  // 16 warps at most
-    const float coef = -__shfl_sync(0xffffffffu, t, 0) * share * (ir * ir);
-#pragma unroll
-    for (int k = 0; k < UPT; ++k)
-      if (on[k]) {
-        const unsigned char* from = ring + s + 16u * (k * blockDim.x + tid);
-        if (!HOLD) {
-          h = unit_read(from + at_h * apart, apart, (const TR*)nullptr);
-          gw = v8_mul(unit_read(from + at_g * apart, apart, (const TB*)nullptr), v8_weights(p.w + 8 * tid + k * step));
+    const float coef = -warp_sum(lane < nw ? red[buf][lane] : 0.f) * share * (ir * ir);
+    if (on) {
+      const V8 o = p.gh ? span_read(from + warp * span_r, (const TR*)nullptr) : v8_zero();
+      const V8 gi = v8_fma(v8_fma(h, coef, g), ir, o);
+      if (!edge) {
+        put_grads<TR, TB>(p, key, at, gi);
+      } else {
+        float f[8];
+        v8_spread(gi, f);
+        put_inside(static_cast<TR*>(p.gr) + at, f, c, cols);
+        if (p.gb) {
+          if (p.drop.drop) drop_apply(drop_group(key, (uint64_t)at / kDropGroup), p.drop.drop, p.drop.scale, f);
+          put_inside(static_cast<TB*>(p.gb) + at, f, c, cols);
         }
-        const V8 o = p.gh ? unit_read(from, apart, (const TR*)nullptr) : v8_zero();
-        put_grads<TR, TB>(p, key, at + k * step, v8_fma(v8_fma(h, coef, gw), ir, o));
       }
-    fetch(s);  // into what this thread has just read
+    }
+    __syncwarp();  // everyone has read what is now copied over
+    fetch(s);
     s = s + stage == stages * stage ? 0 : s + stage;
   }
-#pragma unroll
-  for (int k = 0; k < UPT; ++k)
-    if (on[k]) v8_save(p.part + (int64_t)blockIdx.x * cols + 8 * (k * (int)blockDim.x + tid), acc[k]);
+  if (on) {
+    float f[8];
+    v8_spread(acc, f);
+    put_inside(p.part + (int64_t)blockIdx.x * cols + c, f, c, cols);
+  }
   copies_wait(1);
 }
 
@@ -253,6 +289,15 @@ __global__ void __launch_bounds__(512, 2) add_norm_bwd_ring_kernel(const BwdArgs
 // ---------------------------------------------------------------------------
 constexpr int kLongThreads = 512;
 constexpr int64_t kKeepCols = 49152;  // 192 KB
+
+__device__ __forceinline__ V8 sums_of(const float4& x, const float4& y) {
+  V8 v;
+  v.a[0] = make_float2(x.x, x.y);
+  v.a[1] = make_float2(x.z, x.w);
+  v.a[2] = make_float2(y.x, y.y);
+  v.a[3] = make_float2(y.z, y.w);
+  return v;
+}
 
 template <typename TR, typename TB>
 __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const BwdArgs p) {
@@ -277,7 +322,7 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
       gq.load(g + 8 * u);
       hq.load(h + 8 * u);
       const V8 gv = gq.values(), hv = hq.values();
-      V8 a = unit_read(reinterpret_cast<const unsigned char*>(lo + u), 16u * U, (const float*)nullptr);
+      V8 a = sums_of(lo[u], hi[u]);
       a = v8_fma(v8_scale(gv, ir), hv, a);
       lo[u] = make_float4(a.a[0].x, a.a[0].y, a.a[1].x, a.a[1].y);
       hi[u] = make_float4(a.a[2].x, a.a[2].y, a.a[3].x, a.a[3].y);
@@ -298,7 +343,7 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
   }
   for (int u = threadIdx.x; u < U; u += kLongThreads)
     v8_save(p.part + (int64_t)blockIdx.x * cols + 8 * u,
-            unit_read(reinterpret_cast<const unsigned char*>(lo + u), 16u * U, (const float*)nullptr));
+            sums_of(lo[u], hi[u]));
 }
 
 // ---------------------------------------------------------------------------
@@ -426,35 +471,41 @@ struct BwdPlan {
   int UPT, threads, stages, per_sm;
   size_t smem;
 };
-// even: wide accesses fit; `unit`: bytes of 8 columns of gh, h and g
-BwdPlan bwd_plan(int64_t cols, bool even, size_t unit) {
+// even: wide accesses fit rows; aligned: they fit the tensors' starts; `unit`: bytes of
+// 8 columns of gh, h and g
+BwdPlan bwd_plan(int64_t cols, bool even, bool aligned, size_t unit) {
   const int64_t U = (cols + 7) / 8;
   if (ck_pitch(cols) <= kWarpCols)
     return {even ? Bwd::kWarp : Bwd::kAnyWarp, ck_pitch(cols) <= 256 ? 1 : ck_pitch(cols) <= 512 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
+  const int64_t spread = cols % 8 ? U + 1 : U;  // units of a row wherever it starts
+  if (aligned && spread <= 1024) {
+    const int threads = (int)((spread + 31) / 32 * 32);
+    const size_t stage = threads * unit;
+    int per_sm = 1024 / threads;
+    per_sm = per_sm > 6 ? 6 : per_sm;
+    while (per_sm > 1 && 2 * stage > (size_t)kStageBytes / per_sm) --per_sm;
+    size_t s = (size_t)kStageBytes / per_sm / stage;
+    s = s > kStagesMost ? kStagesMost : s;
+    return {Bwd::kRing, 1, threads, (int)s, per_sm, s * stage};
+  }
   if (U > 1024) {
     const size_t keep = cols <= kKeepCols ? (size_t)U * 8 * sizeof(float) : 0;
     return {even && keep ? Bwd::kLong : Bwd::kAnyLong, 0, kLongThreads, 0, keep > 100 * 1024 ? 1 : 2, keep};
   }
-  if (!even) {
-    const int upt = U <= 256 ? 1 : 2;
-    return {Bwd::kAny, upt, (int)(((U + upt - 1) / upt + 31) / 32 * 32), 0, 2, 0};
-  }
-  const int upt = U <= 512 ? 1 : 2, threads = (int)(((U + upt - 1) / upt + 31) / 32 * 32);
-  const size_t stage = (size_t)upt * threads * unit;
-  int per_sm = 1024 / threads;
-  per_sm = per_sm < 2 ? 2 : per_sm > 6 ? 6 : per_sm;
-  while (per_sm > 1 && 2 * stage > (size_t)kStageBytes / per_sm) --per_sm;
-  size_t s = (size_t)kStageBytes / per_sm / stage;
-  s = s > kStagesMost ? kStagesMost : s;
-  return {Bwd::kRing, upt, threads, (int)s, per_sm, s * stage};
+  const int upt = U <= 256 ? 1 : 2;
+  return {Bwd::kAny, upt, (int)(((U + upt - 1) / upt + 31) / 32 * 32), 0, 2, 0};
 }
 
 // Blocks: as many as run at once (gw leaves as one row a block), no more than
-// there are rows for.
-int bwd_blocks(const BwdPlan& pl, int64_t rows) {
+// there are rows for; a ring's rows start at one place of a unit.
+int bwd_blocks(const BwdPlan& pl, int64_t rows, int64_t cols) {
   const bool warp = pl.kind == Bwd::kWarp || pl.kind == Bwd::kAnyWarp;
   const int64_t need = warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
-  const int64_t most = pl.per_sm * (int64_t)num_sms();
+  int64_t most = pl.per_sm * (int64_t)num_sms();
+  if (pl.kind == Bwd::kRing) {
+    const int64_t apart = cols % 2 ? 8 : cols % 4 ? 4 : cols % 8 ? 2 : 1;
+    most = most < apart ? apart : most / apart * apart;
+  }
   return (int)(need < most ? (need > 0 ? need : 1) : most);
 }
 
@@ -470,12 +521,11 @@ int allow(K kern, size_t most) {
 
 template <typename TR, typename TB>
 int launch_bwd(const BwdArgs& p, float* grad_weight, size_t workspace_bytes, cudaStream_t st) {
-  const bool even = even_rows<TR>(p.gh, p.cols, p.cols) && even_rows<TR>(p.h, p.cols, p.cols) &&
-                    even_rows<TB>(p.g, p.cols, p.cols) && even_rows<TR>(p.gr, p.cols, p.cols) &&
-                    even_rows<TB>(p.gb, p.cols, p.cols) && even_rows<float>(p.w, p.cols, p.cols) &&
-                    even_rows<float>(p.part, p.cols, p.cols);
-  const BwdPlan pl = bwd_plan(p.cols, even, 8 * (2 * sizeof(TR) + sizeof(TB)));
-  const int blocks = bwd_blocks(pl, p.rows);
+  const bool aligned = even_rows<TR>(p.gh, 8, 8) && even_rows<TR>(p.h, 8, 8) && even_rows<TB>(p.g, 8, 8) &&
+                       even_rows<TR>(p.gr, 8, 8) && even_rows<TB>(p.gb, 8, 8);
+  const bool even = aligned && p.cols % 8 == 0 && even_rows<float>(p.w, 8, 8) && even_rows<float>(p.part, 8, 8);
+  const BwdPlan pl = bwd_plan(p.cols, even, aligned, 8 * (2 * sizeof(TR) + sizeof(TB)));
+  const int blocks = bwd_blocks(pl, p.rows, p.cols);
   MHC_REQUIRE(p.part != nullptr && workspace_bytes >= (size_t)blocks * (size_t)p.cols * sizeof(float), MHC_ERR_WORKSPACE,
               "add_rmsnorm_bwd: workspace too small");
   constexpr size_t keep = kKeepCols * sizeof(float);
@@ -489,13 +539,11 @@ int launch_bwd(const BwdArgs& p, float* grad_weight, size_t workspace_bytes, cud
         else if (pl.UPT == 2) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 2>), p);
         else MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 4>), p);
         break;
-      case Bwd::kRing: {
-        auto kern = pl.UPT == 1 ? add_norm_bwd_ring_kernel<TR, TB, 1> : add_norm_bwd_ring_kernel<TR, TB, 2>;
-        rc = allow(kern, kStageBytes);
+      case Bwd::kRing:
+        rc = allow(add_norm_bwd_ring_kernel<TR, TB>, kStageBytes);
         if (rc) return rc;
-        MHC_GO(kern, p, pl.stages);
+        MHC_GO((add_norm_bwd_ring_kernel<TR, TB>), p, pl.stages);
         break;
-      }
       case Bwd::kLong:
         rc = allow(add_norm_bwd_long_kernel<TR, TB>, keep);
         if (rc) return rc;
@@ -539,8 +587,8 @@ extern "C" size_t mhc_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t cols
   // the plan depends on types and alignment too: enough for each
   int most = 1;
   for (size_t unit : {48, 64, 80, 96})
-    for (bool even : {false, true}) {
-      const int b = bwd_blocks(bwd_plan(cols, even, unit), rows);
+    for (int way = 0; way < 3; ++way) {
+      const int b = bwd_blocks(bwd_plan(cols, way == 2 && cols % 8 == 0, way >= 1, unit), rows, cols);
       most = b > most ? b : most;
     }
   return (size_t)most * (size_t)cols * sizeof(float);

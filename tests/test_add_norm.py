@@ -256,7 +256,7 @@ def check_grads(got, gh, go, hidden, w, keep, scale, C, R):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tr,tb", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
-@pytest.mark.parametrize("R,C", SIZES + [(3000, 2048), (1300, 1025), (5000, 40)])
+@pytest.mark.parametrize("R,C", SIZES + [(3000, 2048), (1300, 1025), (1200, 2050), (700, 2052), (330, 6001), (5000, 40)])
 def test_backward(cuda, R, C, tr, tb):
     res, br, w, gh, go = inputs(R, C, tr, tb)
     hidden, _, rms, _ = mhc.add_rmsnorm_fwd(res.to(cuda), br.to(cuda), w.to(cuda))
