@@ -148,16 +148,16 @@ __device__ __forceinline__ void copies_wait(int n) {
 // A warp's 256 consecutive values: its lanes copy pieces of 16 bytes side by side.
 // need: values that the row wants (a piece that holds none is left out); left: those
 // that the tensor has from the warp's first on.
-template <typename T>
-__device__ __forceinline__ void span_copy(uint32_t to, const T* from, int need, int64_t left) {
+template <bool EVEN, typename T>
+__device__ __forceinline__ void span_copy(uint32_t to, const T* from, int need, int left) {
   constexpr int per = 16 / (int)sizeof(T);  // values of a piece
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int q = 0; q < (int)sizeof(T) / 2; ++q) {
     const int piece = 32 * q + lane, e = piece * per;
     const uint32_t at = to + 16u * (sizeof(T) == 4 ? piece ^ ((piece >> 3) & 1) : piece);
-    if (e < need && e < left) {
-      if (e + per <= left) copy16(at, from + e);
+    if (e < need && (EVEN || e < left)) {
+      if (EVEN || e + per <= left) copy16(at, from + e);
       else copy_part(at, from + e, (uint32_t)(left - e) * sizeof(T));
     }
   }
@@ -192,18 +192,20 @@ __device__ __forceinline__ void put_inside(T* to, const float (&f)[8], int c, in
     if (c + j >= 0 && c + j < cols) ck_store(to + j, f[j]);
 }
 
-template <typename TR, typename TB>
+// EVEN: whole units (cols % 8 == 0).  One unit a thread: two (half the threads, twice
+// the registers) took as long within 3%.
+template <typename TR, typename TB, bool EVEN>
 __global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArgs p, int stages) {
   let_next_start();
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, cols = (int)p.cols;
-  const int shift = (int)(((int64_t)blockIdx.x * cols) & 7);
+  const int shift = EVEN ? 0 : (int)(((int64_t)blockIdx.x * cols) & 7);
   const int c = 8 * tid - shift;  // the unit's first column
-  const bool on = c < cols, edge = on && (c < 0 || c + 8 > cols);
+  const bool on = c < cols, edge = !EVEN && on && (c < 0 || c + 8 > cols);
   // a stage: gh, h, g of all warps
-  const uint32_t span_r = 256u * sizeof(TR), at_h = nw * span_r, at_g = 2 * at_h;
-  const uint32_t stage = at_g + nw * 256u * sizeof(TB);
+  const uint32_t span_r = 256u * sizeof(TR), span_b = 256u * sizeof(TB), at_h = nw * span_r, at_g = 2 * at_h;
+  const uint32_t stage = at_g + nw * span_b, ring_end = stages * stage;
   const DropKey key = drop_key(p.drop);
   V8 acc = v8_zero(), wv;
   {
@@ -215,13 +217,13 @@ __global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArg
   const int64_t hop = (int64_t)gridDim.x * cols, total = p.rows * cols;
   const int need = shift + cols - 256 * warp;
   int64_t ahead = (int64_t)blockIdx.x * cols - shift + 256 * warp;  // element of the warp's next copies
+  const uint32_t to_r = smem_u32(ring) + warp * span_r, to_b = smem_u32(ring) + at_g + warp * span_b;
   auto fetch = [&](uint32_t s) {
     if (ahead < total) {
-      const uint32_t to = smem_u32(ring) + s;
-      const int64_t left = total - ahead;
-      if (p.gh) span_copy(to + warp * span_r, static_cast<const TR*>(p.gh) + ahead, need, left);
-      span_copy(to + at_h + warp * span_r, static_cast<const TR*>(p.h) + ahead, need, left);
-      span_copy(to + at_g + warp * 256u * (uint32_t)sizeof(TB), static_cast<const TB*>(p.g) + ahead, need, left);
+      const int left = EVEN ? 0 : (int)min(total - ahead, (int64_t)1 << 20);
+      if (p.gh) span_copy<EVEN>(to_r + s, static_cast<const TR*>(p.gh) + ahead, need, left);
+      span_copy<EVEN>(to_r + at_h + s, static_cast<const TR*>(p.h) + ahead, need, left);
+      span_copy<EVEN>(to_b + s, static_cast<const TB*>(p.g) + ahead, need, left);
     }
     ahead += hop;
     copies_end();  // a group each time, so that the count of groups is the count of rows
@@ -233,16 +235,16 @@ __global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArg
   float nr = p.rms[blockIdx.x];
   const float share = 1.0f / (float)cols;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1, at += hop) {
-    const float ir = 1.0f / nr;
+    const float ir = __fdividef(1.0f, nr);
     if (row + gridDim.x < p.rows) nr = p.rms[row + gridDim.x];
     copies_wait(stages);
     __syncwarp();  // the other lanes' too
-    const unsigned char* from = ring + s;
+    const unsigned char* from = ring + s + warp * span_r;
     V8 g = v8_zero(), h = g;
     float2 d2 = make_float2(0.f, 0.f);
     if (on) {
-      g = span_read(from + at_g + warp * 256u * sizeof(TB), (const TB*)nullptr);
-      h = span_read(from + at_h + warp * span_r, (const TR*)nullptr);
+      g = span_read(ring + s + at_g + warp * span_b, (const TB*)nullptr);
+      h = span_read(from + at_h, (const TR*)nullptr);
       if (edge) {
         g = v8_inside(g, c, cols);
         h = v8_inside(h, c, cols);
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArg
     __syncthreads();
     const float coef = -warp_sum(lane < nw ? red[buf][lane] : 0.f) * share * (ir * ir);
     if (on) {
-      const V8 o = p.gh ? span_read(from + warp * span_r, (const TR*)nullptr) : v8_zero();
+      const V8 o = p.gh ? span_read(from, (const TR*)nullptr) : v8_zero();
       const V8 gi = v8_fma(v8_fma(h, coef, g), ir, o);
       if (!edge) {
         put_grads<TR, TB>(p, key, at, gi);
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArg
     }
     __syncwarp();  // everyone has read what is now copied over
     fetch(s);
-    s = s + stage == stages * stage ? 0 : s + stage;
+    s = s + stage == ring_end ? 0 : s + stage;
   }
   if (on) {
     float f[8];
@@ -530,6 +532,7 @@ int launch_bwd(const BwdArgs& p, float* grad_weight, size_t workspace_bytes, cud
               "add_rmsnorm_bwd: workspace too small");
   constexpr size_t keep = kKeepCols * sizeof(float);
   int rc = MHC_OK;
+  void (*kern)(const BwdArgs, int) = nullptr;
   {
     ProfScope prof("add_rmsnorm_bwd", st);
 #define MHC_GO(KERN, ...) KERN<<<blocks, pl.threads, pl.smem, st>>>(__VA_ARGS__)
@@ -540,9 +543,10 @@ int launch_bwd(const BwdArgs& p, float* grad_weight, size_t workspace_bytes, cud
         else MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 4>), p);
         break;
       case Bwd::kRing:
-        rc = allow(add_norm_bwd_ring_kernel<TR, TB>, kStageBytes);
+        kern = p.cols % 8 ? add_norm_bwd_ring_kernel<TR, TB, false> : add_norm_bwd_ring_kernel<TR, TB, true>;
+        rc = allow(kern, kStageBytes);
         if (rc) return rc;
-        MHC_GO((add_norm_bwd_ring_kernel<TR, TB>), p, pl.stages);
+        MHC_GO(kern, p, pl.stages);
         break;
       case Bwd::kLong:
         rc = allow(add_norm_bwd_long_kernel<TR, TB>, keep);
