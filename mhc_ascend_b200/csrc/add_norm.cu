@@ -60,30 +60,39 @@ constexpr int fwd_threads(int UPT, bool WARP) { return WARP || UPT == 1 ? 256 : 
 // four blocks an SM.
 enum class Lay { kWarp, kBlock, kSmall };
 
-// Rows that wide accesses fit.  A row stays in registers between the sum and the
-// output, UPT units a thread.  CODED: what is kept is h w, and its maxima are taken
-// with the sum (r > 0 is common to the row: max |y| = max |h w| / r), so that after
-// the barrier a value costs one product and its conversion.
-template <typename TR, typename TB, int UPT, Lay LAY, bool CODED>
-__global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LAY == Lay::kWarp), LAY == Lay::kSmall ? 4 : 1)
+// A row stays in registers between the sum and the output, UPT units a thread.  EVEN:
+// whole units; otherwise units of the tensor's own alignment (vec8.cuh), and the kept
+// codes, whose blocks begin with the row, pass through shared memory.  CODED: what is
+// kept in registers is h w, and its maxima are taken with the sum (r > 0 is common to
+// the row: max |y| = max |h w| / r), so that after the barrier a value costs one product
+// and its conversion.
+__device__ __forceinline__ int row_word(int c) { return c ^ ((c >> 5) & 7); }  // no bank twice, eight columns a lane
+
+template <typename TR, typename TB, int UPT, Lay LAY, bool CODED, bool EVEN>
+__global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LAY == Lay::kWarp),
+                                  LAY == Lay::kSmall ? 4 : LAY == Lay::kBlock && UPT == 2 ? 2 : 1)
     add_norm_fwd_kernel(const FwdArgs p) {
   constexpr bool WARP = LAY == Lay::kWarp;
   __shared__ float red[32], redm[32];
+  extern __shared__ __align__(16) float row_sm[];  // uneven rows with kept codes: pitch words a row
   const int lane = threadIdx.x & 31, cols = (int)p.cols;
   const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
   if (WARP && row >= p.rows) return;
-  const int c0 = 8 * (WARP ? lane : (int)threadIdx.x), step = 8 * (WARP ? 32 : (int)blockDim.x);
-  const int64_t at = row * p.cols + c0;
+  const int shift = EVEN ? 0 : (int)((row * p.cols) & 7);
+  const int c0 = 8 * (WARP ? lane : (int)threadIdx.x) - shift, step = 8 * (WARP ? 32 : (int)blockDim.x);
+  const int64_t at = row * p.cols + c0, total = p.rows * p.cols;
   const TR* rr = static_cast<const TR*>(p.res) + at;
   const TB* br = static_cast<const TB*>(p.branch) + at;
   TR* hr = static_cast<TR*>(p.hidden) + at;
+  auto edge = [&](int c) { return !EVEN && v8_edge(c, cols); };
+  auto weights = [&](int c) { return EVEN ? v8_weights(p.w + c) : v8_weights_inside(p.w, c, cols); };
   Raw8<TR> a[UPT];
   Raw8<TB> b[UPT];
 #pragma unroll
   for (int k = 0; k < UPT; ++k) {
     a[k].zero();
     b[k].zero();
-    if (c0 + k * step < cols) {
+    if (c0 + k * step < cols && (EVEN || at + k * step + 8 <= total)) {
       a[k].load(rr + k * step);
       b[k].load(br + k * step);
     }
@@ -94,21 +103,29 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
   float am = 0.f, gm[UPT];
 #pragma unroll
   for (int k = 0; k < UPT; ++k) {
-    V8 x = b[k].values();
+    const int c = c0 + k * step;
+    const bool on = c < cols;
+    V8 x = b[k].values(), y = a[k].values();
+    if (!EVEN && on && at + k * step + 8 > total) {  // the tensor's last
+      y = v8_load_part(rr + k * step, total - at - k * step);
+      x = v8_load_part(br + k * step, total - at - k * step);
+    }
     if (!CODED && p.drop.drop) {
       float f[8];
       v8_spread(x, f);
       drop_apply(drop_group(key, (uint64_t)(at + k * step) / kDropGroup), p.drop.drop, p.drop.scale, f);
       x = v8_gather(f);
     }
-    v[k] = v8_add(a[k].values(), x);
-    const bool on = c0 + k * step < cols;
-    if (on) v8_save_rounded(hr + k * step, v[k]);
+    v[k] = v8_add(y, x);
+    if (on) {
+      if (edge(c)) v8_save_inside(hr + k * step, v[k], c, cols);
+      else v8_save_rounded(hr + k * step, v[k]);
+    }
     s2 = v8_dot(v[k], v[k], s2);
     if (CODED) {
-      if (on) v[k] = v8_mul(v[k], v8_weights(p.w + c0 + k * step));
+      if (on) v[k] = v8_mul(v[k], weights(c));
       gm[k] = v8_max_abs(v[k]);
-      if (p.grouped) gm[k] = group_max(gm[k]);  // 16 lanes hold a group
+      if (EVEN && p.grouped) gm[k] = group_max(gm[k]);  // 16 lanes hold a group
       else am = max_abs_nan(am, gm[k]);
     }
   }
@@ -125,28 +142,58 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
     for (int k = 0; k < UPT; ++k) {
       const int c = c0 + k * step;
       float s = scale;
-      if (p.grouped) {
+      if (EVEN && p.grouped) {
         s = coded_scale(gm[k] * ir, p.int8);
         if ((lane & 15) == 0 && c < cols) p.scales[row * p.groups + c / kCodedGroup] = s;
       }
       float f[8];
       v8_spread(v8_scale(v[k], ir * coded_inverse(s)), f);
-      if (c < cols) *reinterpret_cast<uint2*>(to + k * step) = coded_pack(f, p.int8);
+      if (c < cols) {
+        const uint2 w = coded_pack(f, p.int8);
+        if (!edge(c)) {
+          *reinterpret_cast<uint2*>(to + k * step) = w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j >= 0 && c + j < cols) to[k * step + j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+        }
+      }
     }
     return;
   }
   TB* out = static_cast<TB*>(p.out) + at;
+  float* mine = row_sm + (WARP ? (threadIdx.x >> 5) * (int)p.pitch : 0);
 #pragma unroll
   for (int k = 0; k < UPT; ++k) {
     const int c = c0 + k * step;
     V8 y = v8_zero();
     if (c < cols) {
-      y = v8_mul(v8_scale(v[k], ir), v8_weights(p.w + c));
-      v8_save_rounded(out + k * step, y);
+      y = v8_mul(v8_quotient(v[k], minus_root(r), ir), weights(c));
+      if (edge(c)) v8_save_inside(out + k * step, y, c, cols);
+      else v8_save_rounded(out + k * step, y);
     }
-    if (p.codes) {  // of the output as it is returned
+    if (!p.codes) continue;
+    float f[8];
+    v8_spread(y, f);
+    if (EVEN) {  // of the output as it is returned
+      ck_encode(f, p.codes + row * p.pitch, p.exps + row * (p.pitch / kCkBlock), c, c < p.pitch);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j >= 0 && c + j < cols) mine[row_word(c + j)] = f[j];
+    }
+  }
+  if (!EVEN && p.codes) {
+    const int i0 = WARP ? lane : (int)threadIdx.x;
+    for (int c = cols + i0; c < p.pitch; c += step / 8) mine[row_word(c)] = 0.f;
+    if (WARP) __syncwarp();
+    else __syncthreads();
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      const int c = 8 * i0 + k * step;
       float f[8];
-      v8_spread(y, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = c < p.pitch ? mine[row_word(c + j)] : 0.f;
       ck_encode(f, p.codes + row * p.pitch, p.exps + row * (p.pitch / kCkBlock), c, c < p.pitch);
     }
   }
@@ -179,8 +226,8 @@ __device__ __forceinline__ void add_unit_any(const FwdArgs& p, const DropKey& ke
   save_any(p.hidden, p.res16, row, c, p.cols, mine, v);
 }
 template <bool CODED>
-__device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int64_t c, float (&v)[8], float ir, float row_scale,
-                                             float* mine) {
+__device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int64_t c, float (&v)[8], float minus_r, float ir,
+                                             float row_scale, float* mine) {
   const int lane = threadIdx.x & 31;
   float wv[8];
   load_w(p.w, c, p.cols, wv);
@@ -201,7 +248,10 @@ __device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int6
     coded_save_any(reinterpret_cast<uint8_t*>(p.codes) + row * p.cols, c - 8 * lane, p.cols, mine, v, p.int8);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * ir * wv[j];
+    for (int j = 0; j < 8; ++j) {
+      const float q = v[j] * ir;
+      v[j] = fmaf(fmaf(q, minus_r, v[j]), ir, q) * wv[j];
+    }
     save_any(p.out, p.branch16, row, c, p.cols, mine, v);
     if (p.codes) {  // of the output as it is returned
 #pragma unroll
@@ -232,7 +282,7 @@ __global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_any_kerne
     if (CODED && !p.grouped) p.scales[row] = scale;
   }
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) put_unit_any<CODED>(p, row, unit_col<WARP>(k), v[k], ir, scale, mine);
+  for (int k = 0; k < UPT; ++k) put_unit_any<CODED>(p, row, unit_col<WARP>(k), v[k], minus_root(r), ir, scale, mine);
 }
 
 // Rows too long for registers: h is read again, from L2, by the thread that wrote it.
@@ -261,11 +311,13 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_fwd_long_kernel(const F
   for (int64_t c0 = (threadIdx.x >> 5) * 256; c0 < end; c0 += 8 * kLongThreads) {
     float v[8];
     load_any(p.hidden, p.res16, row, c0 + 8 * lane, p.cols, mine, v);
-    put_unit_any<CODED>(p, row, c0 + 8 * lane, v, ir, scale, mine);
+    put_unit_any<CODED>(p, row, c0 + 8 * lane, v, minus_root(r), ir, scale, mine);
   }
 }
 
+enum class Way { kEven, kUneven, kAny };
 struct FwdPlan {
+  Way way;
   Lay lay;
   int UPT, threads;  // UPT = 0: the long kernel
 };
@@ -273,31 +325,57 @@ struct FwdPlan {
 // smaller blocks overlap each other's barriers ([16384, 7168] bf16 to e4m3 with a scale for
 // each 128: 129 us, 6.4 TB/s, against 162 with two units and 448 threads, 175 with one and
 // 896); where there are few, as many threads as there are units ([1, 4096] 2.4 us against 3.3).
-FwdPlan fwd_plan(int64_t rows, int64_t cols, bool even) {
-  const int64_t pitch = ck_pitch(cols), U = pitch / 8;
-  if (pitch <= kWarpCols) return {Lay::kWarp, pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows};
-  auto threads = [&](int upt) { return (int)(((U + upt - 1) / upt + 31) / 32 * 32); };
-  if (even && U <= 1024 && rows >= 2 * num_sms()) return {Lay::kSmall, 4, threads(4)};
+// Uneven rows take two units a thread (four spill: [8192, 4097] fp32 residual, bf16 branch,
+// kept codes 93 us against 114), and short ones of the plain form the kernel for any row
+// ([65536, 250] with kept codes 54 us against 75: its units begin with the row, as the
+// codes do; without them too, so that they change no bit of the output).
+// aligned: wide accesses fit the tensors' starts; by_column: scales belong to columns.
+FwdPlan fwd_plan(int64_t rows, int64_t cols, bool aligned, bool aligned_w, bool by_column, bool coded) {
+  const int64_t pitch = ck_pitch(cols), U = pitch / 8, spread = (cols + 7) / 8 + 1;
+  const int64_t most = spread > U ? spread : U;  // units of a row wherever it starts
+  auto threads = [](int64_t units, int upt) { return (int)(((units + upt - 1) / upt + 31) / 32 * 32); };
+  if (aligned && cols % 8 && !by_column) {
+    if (most <= 128 && coded) return {Way::kUneven, Lay::kWarp, most <= 32 ? 1 : most <= 64 ? 2 : 4, 32 * kWarpRows};
+    if (most > 128 && most <= 1024) return {Way::kUneven, Lay::kBlock, 2, threads(most, 2)};
+    if (most > 1024 && most <= 4096) return {Way::kUneven, Lay::kBlock, 4, threads(most, 4)};
+  }
+  const Way way = aligned && aligned_w && cols % 8 == 0 ? Way::kEven : Way::kAny;
+  if (pitch <= kWarpCols) return {way, Lay::kWarp, pitch <= 256 ? 1 : pitch <= 512 ? 2 : 4, 32 * kWarpRows};
+  if (way == Way::kEven && U <= 1024 && rows >= 2 * num_sms()) return {way, Lay::kSmall, 4, threads(U, 4)};
   for (int upt : {1, 2, 4})
-    if (U <= upt * fwd_threads(upt, false)) return {Lay::kBlock, upt, threads(upt)};
-  return {Lay::kBlock, 0, kLongThreads};
+    if (U <= upt * fwd_threads(upt, false)) return {way, Lay::kBlock, upt, threads(U, upt)};
+  return {Way::kAny, Lay::kBlock, 0, kLongThreads};
 }
 
 template <bool CODED, typename TR, typename TB>
 int launch_fwd(const FwdArgs& p, cudaStream_t st) {
-  bool even = even_rows<TR>(p.res, p.cols, p.cols) && even_rows<TR>(p.hidden, p.cols, p.cols) &&
-              even_rows<TB>(p.branch, p.cols, p.cols) && even_rows<float>(p.w, p.cols, p.cols);
-  even = even && (CODED ? (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 : even_rows<TB>(p.out, p.cols, p.cols));
-  const FwdPlan pl = fwd_plan(p.rows, p.cols, even);
+  const bool aligned = even_rows<TR>(p.res, 8, 8) && even_rows<TR>(p.hidden, 8, 8) && even_rows<TB>(p.branch, 8, 8) &&
+                       (CODED ? (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 : even_rows<TB>(p.out, 8, 8));
+  const FwdPlan pl = fwd_plan(p.rows, p.cols, aligned, even_rows<float>(p.w, 8, 8), p.grouped, CODED);
   const unsigned blocks = (unsigned)(pl.lay == Lay::kWarp ? (p.rows + kWarpRows - 1) / kWarpRows : p.rows);
+  const size_t smem = pl.way == Way::kUneven && p.codes && !CODED
+                          ? (size_t)p.pitch * sizeof(float) * (pl.lay == Lay::kWarp ? kWarpRows : 1) : 0;
   ProfScope prof(CODED ? "add_rmsnorm_coded" : "add_rmsnorm_fwd", st);
-#define MHC_GO(UPT, LAY)                                                                                     \
-  do {                                                                                                       \
-    if (even) add_norm_fwd_kernel<TR, TB, UPT, LAY, CODED><<<blocks, pl.threads, 0, st>>>(p);                \
-    else add_norm_fwd_any_kernel<UPT, LAY == Lay::kWarp, CODED><<<blocks, pl.threads, 0, st>>>(p);           \
+#define MHC_FIT(UPT, LAY, EVEN) add_norm_fwd_kernel<TR, TB, UPT, LAY, CODED, EVEN><<<blocks, pl.threads, smem, st>>>(p)
+#define MHC_GO(UPT, LAY)                                                                                    \
+  do {                                                                                                      \
+    if (pl.way == Way::kEven) MHC_FIT(UPT, LAY, true);                                                      \
+    else add_norm_fwd_any_kernel<UPT, LAY == Lay::kWarp, CODED><<<blocks, pl.threads, 0, st>>>(p);          \
   } while (0)
-  if (pl.UPT == 0) add_norm_fwd_long_kernel<CODED><<<blocks, pl.threads, 0, st>>>(p);
-  else if (pl.lay == Lay::kSmall) add_norm_fwd_kernel<TR, TB, 4, Lay::kSmall, CODED><<<blocks, pl.threads, 0, st>>>(p);
+  if (pl.way == Way::kUneven) {
+    if (pl.lay == Lay::kWarp && pl.UPT == 1) MHC_FIT(1, Lay::kWarp, false);
+    else if (pl.lay == Lay::kWarp && pl.UPT == 2) MHC_FIT(2, Lay::kWarp, false);
+    else if (pl.lay == Lay::kWarp) MHC_FIT(4, Lay::kWarp, false);
+    else if (pl.UPT == 2) MHC_FIT(2, Lay::kBlock, false);
+    else {
+      // the limit belongs to the kernel: always what its widest row asks for
+      if (smem && cudaFuncSetAttribute(add_norm_fwd_kernel<TR, TB, 4, Lay::kBlock, CODED, false>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, 4096 * 8 * (int)sizeof(float)) != cudaSuccess)
+        return fail(MHC_ERR_CUDA, "add_rmsnorm: cannot reserve shared memory for a row");
+      MHC_FIT(4, Lay::kBlock, false);
+    }
+  } else if (pl.UPT == 0) add_norm_fwd_long_kernel<CODED><<<blocks, pl.threads, 0, st>>>(p);
+  else if (pl.lay == Lay::kSmall) MHC_FIT(4, Lay::kSmall, true);
   else if (pl.lay == Lay::kWarp && pl.UPT == 1) MHC_GO(1, Lay::kWarp);
   else if (pl.lay == Lay::kWarp && pl.UPT == 2) MHC_GO(2, Lay::kWarp);
   else if (pl.lay == Lay::kWarp) MHC_GO(4, Lay::kWarp);
@@ -305,6 +383,7 @@ int launch_fwd(const FwdArgs& p, cudaStream_t st) {
   else if (pl.UPT == 2) MHC_GO(2, Lay::kBlock);
   else MHC_GO(4, Lay::kBlock);
 #undef MHC_GO
+#undef MHC_FIT
   return check_launch("add_rmsnorm");
 }
 

@@ -66,20 +66,40 @@ __device__ __forceinline__ void put_warp_parts(const BwdArgs& p, const float (&a
   }
 }
 
+// gi of a unit at its row's edge
+template <typename TR, typename TB>
+__device__ __forceinline__ void put_grads_edge(const BwdArgs& p, const DropKey& key, int64_t i, V8 gi, int c, int cols) {
+  V8 o = gi;
+  v8_save_inside(static_cast<TR*>(p.gr) + i, o, c, cols);
+  if (p.gb) {
+    if (p.drop.drop) {
+      float f[8];
+      v8_spread(gi, f);
+      drop_apply(drop_group(key, (uint64_t)i / kDropGroup), p.drop.drop, p.drop.scale, f);
+      gi = v8_gather(f);
+    }
+    v8_save_inside(static_cast<TB*>(p.gb) + i, gi, c, cols);
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Rows of at most 1024 columns, one a warp.
+// Rows of at most 1024 columns, one a warp, whose rows are a multiple of 8 apart.  EVEN:
+// whole units; otherwise units of the tensor's own alignment (vec8.cuh): a warp's rows
+// all start at the same place of a unit, and its sums go by column through shared memory.
 // ---------------------------------------------------------------------------
-template <typename TR, typename TB, int UPT>
+template <typename TR, typename TB, int UPT, bool EVEN>
 __global__ void __launch_bounds__(32 * kWarpRows) add_norm_bwd_warp_kernel(const BwdArgs p) {
   let_next_start();
-  __shared__ float sm[kWarpRows * 256];
+  __shared__ float sm[EVEN ? kWarpRows * 256 : kWarpRows * 256 * UPT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = (int)p.cols;
+  const int64_t row0 = (int64_t)blockIdx.x * kWarpRows + warp, total = p.rows * cols;
+  const int shift = EVEN ? 0 : (int)((row0 * cols) & 7), c0 = 8 * lane - shift;
   const DropKey key = drop_key(p.drop);
   V8 acc[UPT];
 #pragma unroll
   for (int k = 0; k < UPT; ++k) acc[k] = v8_zero();
-  for (int64_t row = (int64_t)blockIdx.x * kWarpRows + warp; row < p.rows; row += (int64_t)gridDim.x * kWarpRows) {
-    const int64_t at = row * cols + 8 * lane;
+  for (int64_t row = row0; row < p.rows; row += (int64_t)gridDim.x * kWarpRows) {
+    const int64_t at = row * cols + c0;
     Raw8<TB> g[UPT];
     Raw8<TR> h[UPT], o[UPT];
 #pragma unroll
@@ -87,32 +107,68 @@ __global__ void __launch_bounds__(32 * kWarpRows) add_norm_bwd_warp_kernel(const
       g[k].zero();
       h[k].zero();
       o[k].zero();
-      if (8 * (k * 32 + lane) < cols) {
+      if (c0 + k * 256 < cols && (EVEN || at + k * 256 + 8 <= total)) {
         g[k].load(static_cast<const TB*>(p.g) + at + k * 256);
         h[k].load(static_cast<const TR*>(p.h) + at + k * 256);
         if (p.gh) o[k].load(static_cast<const TR*>(p.gh) + at + k * 256);
       }
     }
     const float r = p.rms[row], ir = 1.0f / r;
-    V8 gw[UPT];
+    V8 gw[UPT], hv[UPT], ov[UPT];
     float2 d2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < UPT; ++k) {
-      const V8 gv = g[k].values(), hv = h[k].values();
-      acc[k] = v8_fma(v8_scale(gv, ir), hv, acc[k]);
-      gw[k] = 8 * (k * 32 + lane) < cols ? v8_mul(gv, v8_weights(p.w + 8 * (k * 32 + lane))) : v8_zero();
-      d2 = v8_dot(gw[k], hv, d2);
+      const int c = c0 + k * 256;
+      V8 gv = g[k].values();
+      hv[k] = h[k].values();
+      ov[k] = o[k].values();
+      if (!EVEN && c < cols && v8_edge(c, cols)) {
+        if (at + k * 256 + 8 > total) {  // the tensor's last
+          const int64_t left = total - at - k * 256;
+          gv = v8_load_part(static_cast<const TB*>(p.g) + at + k * 256, left);
+          hv[k] = v8_load_part(static_cast<const TR*>(p.h) + at + k * 256, left);
+          if (p.gh) ov[k] = v8_load_part(static_cast<const TR*>(p.gh) + at + k * 256, left);
+        }
+        gv = v8_inside(gv, c, cols);
+        hv[k] = v8_inside(hv[k], c, cols);
+      }
+      acc[k] = v8_fma(v8_scale(gv, ir), hv[k], acc[k]);
+      gw[k] = c < cols ? v8_mul(gv, EVEN ? v8_weights(p.w + c) : v8_weights_inside(p.w, c, cols)) : v8_zero();
+      d2 = v8_dot(gw[k], hv[k], d2);
     }
     const float coef = -warp_sum(d2.x + d2.y) / ((float)cols * r * r);
 #pragma unroll
-    for (int k = 0; k < UPT; ++k)
-      if (8 * (k * 32 + lane) < cols)
-        put_grads<TR, TB>(p, key, at + k * 256, v8_fma(v8_fma(h[k].values(), coef, gw[k]), ir, o[k].values()));
+    for (int k = 0; k < UPT; ++k) {
+      const int c = c0 + k * 256;
+      if (c >= cols) continue;
+      const V8 gi = v8_fma(v8_fma(hv[k], coef, gw[k]), ir, ov[k]);
+      if (!EVEN && v8_edge(c, cols)) put_grads_edge<TR, TB>(p, key, at + k * 256, gi, c, cols);
+      else put_grads<TR, TB>(p, key, at + k * 256, gi);
+    }
   }
-  float parts[UPT][8];
+  if (EVEN) {
+    float parts[UPT][8];
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) v8_spread(acc[k], parts[k]);
-  put_warp_parts<UPT>(p, parts, sm);
+    for (int k = 0; k < UPT; ++k) v8_spread(acc[k], parts[k]);
+    put_warp_parts<UPT>(p, parts, sm);
+  } else {
+#pragma unroll
+    for (int k = 0; k < UPT; ++k) {
+      float f[8];
+      v8_spread(acc[k], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = c0 + k * 256 + j;
+        if (c >= 0 && c < cols) sm[warp * (256 * UPT) + c] = f[j];
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += 32 * kWarpRows) {
+      float s = 0.f;
+      for (int q = 0; q < kWarpRows; ++q) s += sm[q * (256 * UPT) + c];
+      p.part[(int64_t)blockIdx.x * cols + c] = s;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -177,43 +233,26 @@ __device__ __forceinline__ V8 span_read(const unsigned char* at, const float*) {
 __device__ __forceinline__ V8 span_read(const unsigned char* at, const __nv_bfloat16*) {
   return v8_of(*reinterpret_cast<const uint4*>(at + 16 * (threadIdx.x & 31)));
 }
-// Values of a unit outside columns [0, cols) as zeros
-__device__ __forceinline__ V8 v8_inside(const V8& v, int c, int cols) {
-  float f[8];
-  v8_spread(v, f);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = c + j >= 0 && c + j < cols ? f[j] : 0.f;
-  return v8_gather(f);
-}
-template <typename T>
-__device__ __forceinline__ void put_inside(T* to, const float (&f)[8], int c, int cols) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j >= 0 && c + j < cols) ck_store(to + j, f[j]);
-}
+// Blocks of up to 576 threads twice an SM (56 registers a thread), larger ones once.
+constexpr int ring_blocks(int most) { return most > 576 ? 1 : 2; }
 
 // EVEN: whole units (cols % 8 == 0).  One unit a thread: two (half the threads, twice
 // the registers) took as long within 3%.
-template <typename TR, typename TB, bool EVEN>
-__global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArgs p, int stages) {
+template <typename TR, typename TB, bool EVEN, int MOST>
+__global__ void __launch_bounds__(MOST, ring_blocks(MOST)) add_norm_bwd_ring_kernel(const BwdArgs p, int stages) {
   let_next_start();
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, cols = (int)p.cols;
   const int shift = EVEN ? 0 : (int)(((int64_t)blockIdx.x * cols) & 7);
   const int c = 8 * tid - shift;  // the unit's first column
-  const bool on = c < cols, edge = !EVEN && on && (c < 0 || c + 8 > cols);
+  const bool on = c < cols, edge = !EVEN && on && v8_edge(c, cols);
   // a stage: gh, h, g of all warps
   const uint32_t span_r = 256u * sizeof(TR), span_b = 256u * sizeof(TB), at_h = nw * span_r, at_g = 2 * at_h;
   const uint32_t stage = at_g + nw * span_b, ring_end = stages * stage;
   const DropKey key = drop_key(p.drop);
-  V8 acc = v8_zero(), wv;
-  {
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = c + j >= 0 && c + j < cols ? __ldg(p.w + c + j) : 0.f;
-    wv = v8_gather(f);
-  }
+  V8 acc = v8_zero();
+  const V8 wv = v8_weights_inside(p.w, c, cols);
   const int64_t hop = (int64_t)gridDim.x * cols, total = p.rows * cols;
   const int need = shift + cols - 256 * warp;
   int64_t ahead = (int64_t)blockIdx.x * cols - shift + 256 * warp;  // element of the warp's next copies
@@ -260,27 +299,14 @@ __global__ void __launch_bounds__(1024, 1) add_norm_bwd_ring_kernel(const BwdArg
     if (on) {
       const V8 o = p.gh ? span_read(from, (const TR*)nullptr) : v8_zero();
       const V8 gi = v8_fma(v8_fma(h, coef, g), ir, o);
-      if (!edge) {
-        put_grads<TR, TB>(p, key, at, gi);
-      } else {
-        float f[8];
-        v8_spread(gi, f);
-        put_inside(static_cast<TR*>(p.gr) + at, f, c, cols);
-        if (p.gb) {
-          if (p.drop.drop) drop_apply(drop_group(key, (uint64_t)at / kDropGroup), p.drop.drop, p.drop.scale, f);
-          put_inside(static_cast<TB*>(p.gb) + at, f, c, cols);
-        }
-      }
+      if (edge) put_grads_edge<TR, TB>(p, key, at, gi, c, cols);
+      else put_grads<TR, TB>(p, key, at, gi);
     }
     __syncwarp();  // everyone has read what is now copied over
     fetch(s);
     s = s + stage == ring_end ? 0 : s + stage;
   }
-  if (on) {
-    float f[8];
-    v8_spread(acc, f);
-    put_inside(p.part + (int64_t)blockIdx.x * cols + c, f, c, cols);
-  }
+  if (on) v8_save_inside(p.part + (int64_t)blockIdx.x * cols + c, acc, c, cols);
   copies_wait(1);
 }
 
@@ -301,51 +327,61 @@ __device__ __forceinline__ V8 sums_of(const float4& x, const float4& y) {
   return v;
 }
 
-template <typename TR, typename TB>
+template <typename TR, typename TB, bool EVEN>
 __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const BwdArgs p) {
   let_next_start();
   extern __shared__ __align__(16) unsigned char keep[];  // halves of a unit's eight sums apart
   __shared__ float red[2][32];
-  const int cols = (int)p.cols, U = cols / 8;
+  const int cols = (int)p.cols;
+  const int shift = EVEN ? 0 : (int)(((int64_t)blockIdx.x * cols) & 7), U = (shift + cols + 7) / 8;
+  const int64_t total = p.rows * cols;
   float4* lo = reinterpret_cast<float4*>(keep);
   float4* hi = lo + U;
   for (int u = threadIdx.x; u < U; u += kLongThreads) lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
   const DropKey key = drop_key(p.drop);
+  auto weights = [&](int c) { return EVEN ? v8_weights(p.w + c) : v8_weights_inside(p.w, c, cols); };
+  auto load = [&](const auto* from, int64_t i) -> V8 {  // the unit at element i
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(from)>>;
+    if (!EVEN && i + 8 > total) return v8_load_part(from + i, total - i);
+    Raw8<T> q;
+    q.load(from + i);
+    return q.values();
+  };
   int buf = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1) {
     const float r = p.rms[row], ir = 1.0f / r;
-    const TB* g = static_cast<const TB*>(p.g) + row * cols;
-    const TR* h = static_cast<const TR*>(p.h) + row * cols;
+    const int64_t at = row * cols - shift;
     float2 d2 = make_float2(0.f, 0.f);
 #pragma unroll 2
     for (int u = threadIdx.x; u < U; u += kLongThreads) {
-      Raw8<TB> gq;
-      Raw8<TR> hq;
-      gq.load(g + 8 * u);
-      hq.load(h + 8 * u);
-      const V8 gv = gq.values(), hv = hq.values();
-      V8 a = sums_of(lo[u], hi[u]);
-      a = v8_fma(v8_scale(gv, ir), hv, a);
+      const int c = 8 * u - shift;
+      V8 gv = load(static_cast<const TB*>(p.g), at + 8 * u), hv = load(static_cast<const TR*>(p.h), at + 8 * u);
+      if (!EVEN && v8_edge(c, cols)) {
+        gv = v8_inside(gv, c, cols);
+        hv = v8_inside(hv, c, cols);
+      }
+      const V8 a = v8_fma(v8_scale(gv, ir), hv, sums_of(lo[u], hi[u]));
       lo[u] = make_float4(a.a[0].x, a.a[0].y, a.a[1].x, a.a[1].y);
       hi[u] = make_float4(a.a[2].x, a.a[2].y, a.a[3].x, a.a[3].y);
-      d2 = v8_dot(v8_mul(gv, v8_weights(p.w + 8 * u)), hv, d2);
+      d2 = v8_dot(v8_mul(gv, weights(c)), hv, d2);
     }
     const float coef = -row_total<false>(d2.x + d2.y, red[buf]) / ((float)cols * r * r);
 #pragma unroll 2
     for (int u = threadIdx.x; u < U; u += kLongThreads) {
-      Raw8<TB> gq;
-      Raw8<TR> hq, o;
-      gq.load(g + 8 * u);
-      hq.load(h + 8 * u);
-      o.zero();
-      if (p.gh) o.load(static_cast<const TR*>(p.gh) + row * cols + 8 * u);
-      const V8 gw = v8_mul(gq.values(), v8_weights(p.w + 8 * u));
-      put_grads<TR, TB>(p, key, row * cols + 8 * u, v8_fma(v8_fma(hq.values(), coef, gw), ir, o.values()));
+      const int c = 8 * u - shift;
+      const V8 gw = v8_mul(load(static_cast<const TB*>(p.g), at + 8 * u), weights(c));
+      const V8 o = p.gh ? load(static_cast<const TR*>(p.gh), at + 8 * u) : v8_zero();
+      const V8 gi = v8_fma(v8_fma(load(static_cast<const TR*>(p.h), at + 8 * u), coef, gw), ir, o);
+      if (!EVEN && v8_edge(c, cols)) put_grads_edge<TR, TB>(p, key, at + 8 * u, gi, c, cols);
+      else put_grads<TR, TB>(p, key, at + 8 * u, gi);
     }
   }
-  for (int u = threadIdx.x; u < U; u += kLongThreads)
-    v8_save(p.part + (int64_t)blockIdx.x * cols + 8 * u,
-            sums_of(lo[u], hi[u]));
+  for (int u = threadIdx.x; u < U; u += kLongThreads) {
+    V8 a = sums_of(lo[u], hi[u]);
+    float* to = p.part + (int64_t)blockIdx.x * cols - shift + 8 * u;
+    if (EVEN) v8_save(to, a);
+    else v8_save_inside(to, a, 8 * u - shift, cols);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -473,38 +509,42 @@ struct BwdPlan {
   int UPT, threads, stages, per_sm;
   size_t smem;
 };
-// even: wide accesses fit rows; aligned: they fit the tensors' starts; `unit`: bytes of
-// 8 columns of gh, h and g
-BwdPlan bwd_plan(int64_t cols, bool even, bool aligned, size_t unit) {
-  const int64_t U = (cols + 7) / 8;
-  if (ck_pitch(cols) <= kWarpCols)
-    return {even ? Bwd::kWarp : Bwd::kAnyWarp, ck_pitch(cols) <= 256 ? 1 : ck_pitch(cols) <= 512 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
-  const int64_t spread = cols % 8 ? U + 1 : U;  // units of a row wherever it starts
+// aligned: wide accesses fit the tensors' starts, aligned_w: the weights' and the sums'
+// too; `unit`: bytes of 8 columns of gh, h and g
+BwdPlan bwd_plan(int64_t rows, int64_t cols, bool aligned, bool aligned_w, size_t unit) {
+  const int64_t U = (cols + 7) / 8, spread = cols % 8 ? U + 1 : U;  // units of a row wherever it starts
+  const bool fit = aligned && (cols % 8 != 0 || aligned_w);
+  if (fit && spread <= 128)
+    return {Bwd::kWarp, spread <= 32 ? 1 : spread <= 64 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
   if (aligned && spread <= 1024) {
     const int threads = (int)((spread + 31) / 32 * 32);
     const size_t stage = threads * unit;
-    int per_sm = 1024 / threads;
-    per_sm = per_sm > 6 ? 6 : per_sm;
+    int per_sm = 1152 / threads;
+    per_sm = per_sm > 6 ? 6 : per_sm < 1 ? 1 : per_sm;
     while (per_sm > 1 && 2 * stage > (size_t)kStageBytes / per_sm) --per_sm;
+    // few rows: half the blocks of wide rows, twice the depth ([1001, 4097] fp32 18 us against 22)
+    if (threads > 288 && rows < 4 * per_sm * (int64_t)num_sms()) per_sm = 1;
     size_t s = (size_t)kStageBytes / per_sm / stage;
     s = s > kStagesMost ? kStagesMost : s;
     return {Bwd::kRing, 1, threads, (int)s, per_sm, s * stage};
   }
   if (U > 1024) {
-    const size_t keep = cols <= kKeepCols ? (size_t)U * 8 * sizeof(float) : 0;
-    return {even && keep ? Bwd::kLong : Bwd::kAnyLong, 0, kLongThreads, 0, keep > 100 * 1024 ? 1 : 2, keep};
+    const size_t keep = cols <= kKeepCols ? (size_t)spread * 8 * sizeof(float) : 0;
+    return {fit && keep ? Bwd::kLong : Bwd::kAnyLong, 0, kLongThreads, 0, keep > 100 * 1024 ? 1 : 2, keep};
   }
+  if (ck_pitch(cols) <= kWarpCols)
+    return {Bwd::kAnyWarp, ck_pitch(cols) <= 256 ? 1 : ck_pitch(cols) <= 512 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
   const int upt = U <= 256 ? 1 : 2;
   return {Bwd::kAny, upt, (int)(((U + upt - 1) / upt + 31) / 32 * 32), 0, 2, 0};
 }
 
 // Blocks: as many as run at once (gw leaves as one row a block), no more than
-// there are rows for; a ring's rows start at one place of a unit.
+// there are rows for; a block's rows in units start at one place of them.
 int bwd_blocks(const BwdPlan& pl, int64_t rows, int64_t cols) {
   const bool warp = pl.kind == Bwd::kWarp || pl.kind == Bwd::kAnyWarp;
   const int64_t need = warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
   int64_t most = pl.per_sm * (int64_t)num_sms();
-  if (pl.kind == Bwd::kRing) {
+  if (pl.kind == Bwd::kRing || pl.kind == Bwd::kLong) {
     const int64_t apart = cols % 2 ? 8 : cols % 4 ? 4 : cols % 8 ? 2 : 1;
     most = most < apart ? apart : most / apart * apart;
   }
@@ -525,33 +565,43 @@ template <typename TR, typename TB>
 int launch_bwd(const BwdArgs& p, float* grad_weight, size_t workspace_bytes, cudaStream_t st) {
   const bool aligned = even_rows<TR>(p.gh, 8, 8) && even_rows<TR>(p.h, 8, 8) && even_rows<TB>(p.g, 8, 8) &&
                        even_rows<TR>(p.gr, 8, 8) && even_rows<TB>(p.gb, 8, 8);
-  const bool even = aligned && p.cols % 8 == 0 && even_rows<float>(p.w, 8, 8) && even_rows<float>(p.part, 8, 8);
-  const BwdPlan pl = bwd_plan(p.cols, even, aligned, 8 * (2 * sizeof(TR) + sizeof(TB)));
+  const bool whole = p.cols % 8 == 0;
+  const BwdPlan pl = bwd_plan(p.rows, p.cols, aligned, even_rows<float>(p.w, 8, 8) && even_rows<float>(p.part, 8, 8),
+                              8 * (2 * sizeof(TR) + sizeof(TB)));
   const int blocks = bwd_blocks(pl, p.rows, p.cols);
   MHC_REQUIRE(p.part != nullptr && workspace_bytes >= (size_t)blocks * (size_t)p.cols * sizeof(float), MHC_ERR_WORKSPACE,
               "add_rmsnorm_bwd: workspace too small");
-  constexpr size_t keep = kKeepCols * sizeof(float);
+  constexpr size_t keep = (kKeepCols + 8) * sizeof(float);
   int rc = MHC_OK;
-  void (*kern)(const BwdArgs, int) = nullptr;
+  void (*ring)(const BwdArgs, int) = nullptr;
+  void (*plain)(const BwdArgs) = nullptr;
   {
     ProfScope prof("add_rmsnorm_bwd", st);
 #define MHC_GO(KERN, ...) KERN<<<blocks, pl.threads, pl.smem, st>>>(__VA_ARGS__)
     switch (pl.kind) {
       case Bwd::kWarp:
-        if (pl.UPT == 1) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 1>), p);
-        else if (pl.UPT == 2) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 2>), p);
-        else MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 4>), p);
+        if (whole) {
+          if (pl.UPT == 1) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 1, true>), p);
+          else if (pl.UPT == 2) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 2, true>), p);
+          else MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 4, true>), p);
+        } else {
+          if (pl.UPT == 1) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 1, false>), p);
+          else if (pl.UPT == 2) MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 2, false>), p);
+          else MHC_GO((add_norm_bwd_warp_kernel<TR, TB, 4, false>), p);
+        }
         break;
       case Bwd::kRing:
-        kern = p.cols % 8 ? add_norm_bwd_ring_kernel<TR, TB, false> : add_norm_bwd_ring_kernel<TR, TB, true>;
-        rc = allow(kern, kStageBytes);
+        if (pl.threads <= 576) ring = whole ? add_norm_bwd_ring_kernel<TR, TB, true, 576> : add_norm_bwd_ring_kernel<TR, TB, false, 576>;
+        else ring = whole ? add_norm_bwd_ring_kernel<TR, TB, true, 1024> : add_norm_bwd_ring_kernel<TR, TB, false, 1024>;
+        rc = allow(ring, kStageBytes);
         if (rc) return rc;
-        MHC_GO(kern, p, pl.stages);
+        MHC_GO(ring, p, pl.stages);
         break;
       case Bwd::kLong:
-        rc = allow(add_norm_bwd_long_kernel<TR, TB>, keep);
+        plain = whole ? add_norm_bwd_long_kernel<TR, TB, true> : add_norm_bwd_long_kernel<TR, TB, false>;
+        rc = allow(plain, keep);
         if (rc) return rc;
-        MHC_GO((add_norm_bwd_long_kernel<TR, TB>), p);
+        MHC_GO(plain, p);
         break;
       case Bwd::kAnyWarp:
         if (pl.UPT == 1) MHC_GO((add_norm_bwd_any_kernel<1, true>), p);
@@ -592,7 +642,7 @@ extern "C" size_t mhc_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t cols
   int most = 1;
   for (size_t unit : {48, 64, 80, 96})
     for (int way = 0; way < 3; ++way) {
-      const int b = bwd_blocks(bwd_plan(cols, way == 2 && cols % 8 == 0, way >= 1, unit), rows, cols);
+      const int b = bwd_blocks(bwd_plan(rows, cols, way >= 1, way == 2, unit), rows, cols);
       most = b > most ? b : most;
     }
   return (size_t)most * (size_t)cols * sizeof(float);

@@ -74,6 +74,50 @@ __device__ __forceinline__ void v8_save_rounded(__nv_bfloat16* p, V8& v) {
   *reinterpret_cast<uint4*>(p) = u;
   v = v8_of(u);
 }
+
+// Rows of any width in the tensor's own groups of eight values (units): every access is
+// aligned wherever a row starts, and a row's first and last unit may belong to its
+// neighbours in part.  Unit of columns c .. c + 7 of a row of cols, c as low as -7:
+__device__ __forceinline__ bool v8_edge(int c, int cols) { return c < 0 || c + 8 > cols; }
+// its values outside the row as zeros
+__device__ __forceinline__ V8 v8_inside(const V8& v, int c, int cols) {
+  float f[8];
+  v8_spread(v, f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = c + j >= 0 && c + j < cols ? f[j] : 0.f;
+  return v8_gather(f);
+}
+// those inside to memory; what was stored stays in v, zeros outside
+template <typename T>
+__device__ __forceinline__ void v8_save_inside(T* p, V8& v, int c, int cols) {
+  float f[8];
+  v8_spread(v, f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool in = c + j >= 0 && c + j < cols;
+    if (in) {
+      ck_store(p + j, f[j]);
+      if (sizeof(T) == 2) f[j] = __bfloat162float(__float2bfloat16_rn(f[j]));
+    } else {
+      f[j] = 0.f;
+    }
+  }
+  v = v8_gather(f);
+}
+// a unit of which the tensor has `left` values
+template <typename T>
+__device__ __forceinline__ V8 v8_load_part(const T* p, int64_t left) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = j < left ? ck_f32(p[j]) : 0.f;
+  return v8_gather(f);
+}
+__device__ __forceinline__ V8 v8_weights_inside(const float* w, int c, int cols) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = c + j >= 0 && c + j < cols ? __ldg(w + c + j) : 0.f;
+  return v8_gather(f);
+}
 // Eight weights, 32-byte aligned
 __device__ __forceinline__ V8 v8_weights(const float* w) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(w)), b = __ldg(reinterpret_cast<const float4*>(w + 4));
@@ -115,6 +159,14 @@ __device__ __forceinline__ V8 v8_fma(const V8& x, float y, const V8& z) {
   for (int j = 0; j < 4; ++j) v.a[j] = __ffma2_rn(x.a[j], make_float2(y, y), z.a[j]);
   return v;
 }
+// x / r to the last bit but for rare ties: the product with ir = 1 / r and one Newton step
+// on the quotient (x - q r is exact in a fused product).  minus_r = -r, or 0 where r is
+// infinite: the step then adds x * 0.
+__device__ __forceinline__ V8 v8_quotient(const V8& x, float minus_r, float ir) {
+  const V8 q = v8_scale(x, ir);
+  return v8_fma(v8_fma(q, minus_r, x), ir, q);
+}
+__device__ __forceinline__ float minus_root(float r) { return r > 3.402823466e38f ? 0.f : -r; }
 // s + x . y, pair by pair
 __device__ __forceinline__ float2 v8_dot(const V8& x, const V8& y, float2 s) {
 #pragma unroll

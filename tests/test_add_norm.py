@@ -40,7 +40,7 @@ def norm64(h, w, eps=EPS):
 
 SIZES = [(1, 1), (3, 7), (5, 8), (2, 9), (17, 100), (9, 128), (4, 129), (33, 256), (8, 264), (7, 512), (5, 1000), (3, 1024),
          (4, 1025), (6, 1032), (5, 2048), (3, 2056), (2, 4096), (600, 1100), (700, 264), (3, 4097), (2, 7168), (2, 8192), (3, 8200),
-         (2, 8191), (300, 2048), (310, 4104), (300, 8192), (2, 32768), (2, 32776), (3, 50001), (2, 49160)]
+         (2, 8191), (300, 2048), (310, 4104), (300, 8192), (2, 32768), (2, 32776), (5, 251), (67, 500), (9, 1015), (7, 1017), (5, 1019), (3, 9001), (4, 20002), (3, 32759), (3, 32761), (3, 50001), (2, 49160)]
 
 
 # ---------------------------------------------------------------------------
@@ -187,7 +187,8 @@ def test_rows_of_zeros_infinities_and_nans(cuda):
                                        (600, 264, F32, F32), (4, 1000, BF16, BF16), (4, 1025, F32, BF16), (3, 2048, BF16, BF16),
                                        (5, 4096, BF16, BF16), (2, 4097, F32, F32), (2, 7168, BF16, BF16),
                                        (2, 8200, F32, F32), (300, 1032, BF16, BF16), (301, 4000, F32, BF16),
-                                       (300, 7168, BF16, BF16), (300, 8192, BF16, F32), (2, 32770, BF16, F32), (2, 33024, F32, BF16)])
+                                       (300, 7168, BF16, BF16), (300, 8192, BF16, F32), (2, 32770, BF16, F32), (70, 251, BF16, BF16), (9, 1015, F32, BF16), (305, 2001, BF16, F32),
+                                       (4, 7999, BF16, BF16), (3, 20001, F32, F32), (2, 33024, F32, BF16)])
 def test_quantized(cuda, R, C, tr, tb, group, codes):
     res, br, w, _, _ = inputs(R, C, tr, tb)
     br[:, C // 2] *= 40  # a loud channel
@@ -256,7 +257,8 @@ def check_grads(got, gh, go, hidden, w, keep, scale, C, R):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tr,tb", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
-@pytest.mark.parametrize("R,C", SIZES + [(3000, 2048), (1300, 1025), (1200, 2050), (700, 2052), (330, 6001), (5000, 40)])
+@pytest.mark.parametrize("R,C", SIZES + [(3000, 2048), (1300, 1025), (1200, 2050), (700, 2052), (330, 6001), (5000, 40), (5100, 41),
+                                     (5003, 250), (5001, 500), (4999, 1010), (4990, 1018), (320, 12001), (310, 8194)])
 def test_backward(cuda, R, C, tr, tb):
     res, br, w, gh, go = inputs(R, C, tr, tb)
     hidden, _, rms, _ = mhc.add_rmsnorm_fwd(res.to(cuda), br.to(cuda), w.to(cuda))
