@@ -3,12 +3,14 @@
 Token ids become n residual streams (``StreamEmbedding``); each block mixes the
 streams (``MHCLayer``, streams kept in 8 bits) and adds a feed-forward branch
 whose norm and linear layers keep their inputs in 8 bits; the streams' mean is
-normalised and projected to the vocabulary.  Trains on one random batch:
+normalised and projected to the vocabulary, and the loss is the tokens' negative
+log probability (``token_logprobs``).  Trains on one random batch:
 
-    python examples/train_streams.py [--full] [--steps 30]
+    python examples/train_streams.py [--full] [--steps 30] [--dropout 0.1]
 
-``--full`` keeps the activations in full precision for comparison; the script
-prints the loss and what the activations of a step take.
+``--full`` keeps the activations in full precision for comparison, ``--dropout``
+drops branch outputs out; the script prints the loss, what the activations of a
+step take, and the most likely next tokens of the first text.
 """
 import argparse
 import os
@@ -24,9 +26,10 @@ from mhc_ascend_b200.ops import stream_mean  # noqa: E402
 
 
 class Block(nn.Module):
-    def __init__(self, hidden, n, eight):
+    def __init__(self, hidden, n, eight, dropout=0.0, seed=0):
         super().__init__()
         self.eight = eight
+        self.dropout = mhc.StreamDropout(dropout, seed)
         self.mix = mhc.MHCLayer(hidden, n, checkpoint_8bit=eight)
         self.norm = nn.Parameter(torch.ones(hidden))
         self.up = nn.Parameter(torch.randn(4 * hidden, hidden) * hidden ** -0.5)
@@ -40,14 +43,14 @@ class Block(nn.Module):
             h = mhc.linear_checkpoint8(F.gelu(h), self.down)
         else:
             h = F.linear(F.gelu(F.linear(mhc.rmsnorm(h, self.norm), self.up)), self.down)
-        return x + h.unsqueeze(1)
+        return x + self.dropout(h).unsqueeze(1)
 
 
 class Model(nn.Module):
-    def __init__(self, vocab=1000, hidden=256, n=4, blocks=2, eight=True):
+    def __init__(self, vocab=1000, hidden=256, n=4, blocks=2, eight=True, dropout=0.0):
         super().__init__()
         self.embed = mhc.StreamEmbedding(vocab, hidden, n, scale=[1.0, 0.5, 0.25, 0.125][:n], padding_idx=0)
-        self.blocks = nn.ModuleList(Block(hidden, n, eight) for _ in range(blocks))
+        self.blocks = nn.ModuleList(Block(hidden, n, eight, dropout, seed=i) for i in range(blocks))
         self.norm = nn.Parameter(torch.ones(hidden))
         self.head = nn.Parameter(torch.randn(vocab, hidden) * hidden ** -0.5)
         self.eight = eight
@@ -62,11 +65,18 @@ class Model(nn.Module):
         return F.linear(mhc.rmsnorm(h, self.norm), self.head)
 
 
-def train(steps=30, batch=8, length=64, vocab=1000, eight=True, device="cuda"):
+def loss_of(logits, targets):
+    """Mean negative log probability of the targets; token 0 is padding."""
+    logprob = mhc.token_logprobs(logits, targets, ignore_index=0).logprob
+    return -logprob.sum() / (targets != 0).sum()
+
+
+def train(steps=30, batch=8, length=64, vocab=1000, eight=True, dropout=0.0, device="cuda", answer=False):
     """Losses of `steps` steps on one batch, and the bytes that a step's
-    activations take."""
+    activations take; with `answer` also the five most likely next tokens at each
+    place of the first text, and their log probabilities."""
     torch.manual_seed(0)
-    model = Model(vocab, eight=eight).to(device)
+    model = Model(vocab, eight=eight, dropout=dropout).to(device)
     ids = torch.randint(1, vocab, (batch, length + 1), device=device)
     ids[:, -8:] = 0  # padding at the end
     opt = torch.optim.Adam(model.parameters(), lr=3e-3)
@@ -74,20 +84,28 @@ def train(steps=30, batch=8, length=64, vocab=1000, eight=True, device="cuda"):
     for _ in range(steps):
         opt.zero_grad()
         before = torch.cuda.memory_allocated(device)
-        loss = F.cross_entropy(model(ids[:, :-1]), ids[:, 1:].reshape(-1), ignore_index=0)
+        loss = loss_of(model(ids[:, :-1]), ids[:, 1:].reshape(-1))
         kept = torch.cuda.memory_allocated(device) - before
         loss.backward()
         opt.step()
         losses.append(loss.item())
-    return losses, kept
+    if not answer:
+        return losses, kept
+    with torch.no_grad():
+        best = mhc.token_logprobs(model.eval()(ids[:1, :-1]), ids[0, 1:], top=5)
+    return losses, kept, best.top_id, best.top_logprob
 
 
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=30)
     ap.add_argument("--full", action="store_true")
+    ap.add_argument("--dropout", type=float, default=0.0)
     a = ap.parse_args()
-    losses, kept = train(a.steps, eight=not a.full)
+    losses, kept, ids, logprobs = train(a.steps, eight=not a.full, dropout=a.dropout, answer=True)
     for i in range(0, len(losses), 5):
         print(f"step {i:3d}  loss {losses[i]:.4f}")
     print(f"last loss {losses[-1]:.4f}; activations of a step: {kept / 2 ** 20:.1f} MiB")
+    for place in range(3):
+        likely = ", ".join(f"{i} ({p:.2f})" for i, p in zip(ids[place].tolist(), logprobs[place].exp().tolist()))
+        print(f"after token {place}: {likely}")

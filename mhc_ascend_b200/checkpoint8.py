@@ -347,7 +347,8 @@ def checkpoint8_recompute(function, *tensors: torch.Tensor, kept: int = 1):
     bfloat16); the backward restores them and recomputes.  The gradients are
     those of ``function`` at the restored tensors.  ``function`` is called again
     with the same arguments and gradients on, as in the first pass: it draws no
-    random numbers, and what it differentiates by has to be among ``tensors``."""
+    random numbers but those of ``dropout`` at a given (seed, position), and what it
+    differentiates by has to be among ``tensors``."""
     if not 1 <= kept <= len(tensors):
         raise RuntimeError(f"checkpoint8_recompute: kept must be in [1, {len(tensors)}] (got {kept})")
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):

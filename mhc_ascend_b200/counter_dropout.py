@@ -68,7 +68,7 @@ def dropout_fwd(x: torch.Tensor, p: float, rng: Rng) -> torch.Tensor:
     drop = _drop(what, p)
     source = _source(what, rng, x.device)
     xc = x if x.is_contiguous() else x.detach().contiguous()
-    out = torch.empty_like(xc, requires_grad=False)
+    out = torch.empty_like(xc)
     _launch("mhc_dropout", x.device, xc.data_ptr(), x.dtype == torch.bfloat16, out.data_ptr(), xc.numel(), drop, *source)
     return out
 

@@ -12,6 +12,7 @@ import torch
 import torch.nn as nn
 
 from .checkpoint8 import checkpoint8_recompute, rmsnorm_checkpoint8
+from .counter_dropout import StreamDropout
 from .ops import (
     MHCLayerStaticFunction,
     compute_rms,
@@ -159,19 +160,31 @@ class MHCResidualWrapper(nn.Module):
     pass (n = 4, dynamic H, fp32) keeps the residual and the branch output in 8
     bits for the backward; elsewhere the layer keeps the n packed streams in 8
     bits.  ``use_post_norm`` is accepted and, as in the reference
-    (layer.py:261), forced off.
+    (layer.py:261), forced off.  With ``branch_dropout`` > 0 the branch output is
+    dropped out in training (``StreamDropout``, seed ``dropout_seed``: its position
+    is saved with the module, and no mask is kept).
     """
 
     def __init__(self, hidden_dim: int, expansion_rate: int = 4, residual_mode: str = "decay",
-                 use_post_norm: bool = True, **mhc_kwargs):
+                 use_post_norm: bool = True, branch_dropout: float = 0.0, dropout_seed: int = 0, **mhc_kwargs):
         super().__init__()
         self.hidden_dim = hidden_dim
         self.expansion_rate = expansion_rate
         self.residual_mode = residual_mode
         self.use_post_norm = False
         self.mhc = MHCLayer(hidden_dim=hidden_dim, expansion_rate=expansion_rate, **mhc_kwargs)
+        self.branch_dropout = StreamDropout(branch_dropout, dropout_seed) if branch_dropout else None
+
+    def _dropped(self, branch_output):
+        dropout = getattr(self, "branch_dropout", None)  # not there in modules pickled before it was an argument
+        if dropout is None or not self.training:
+            return branch_output
+        if branch_output.dtype not in (torch.float32, torch.bfloat16):
+            branch_output = branch_output.float()
+        return dropout(branch_output)
 
     def forward(self, residual: torch.Tensor, branch_output: torch.Tensor) -> torch.Tensor:
+        branch_output = self._dropped(branch_output)
         original_shape = residual.shape
         if len(original_shape) == 3:
             B, T, C = original_shape
@@ -225,7 +238,7 @@ class MHCResidualWrapper(nn.Module):
         if wrapper_fused_supported(r2, b2, self.expansion_rate, C, m.use_dynamic_h) and \
                 self.residual_mode in ("decay", "zero") and not keep:
             hidden, normed = wrapper_fused_dynamic_prenorm(
-                r2, b2, self.residual_mode, norm_weight, norm_eps, m.rmsnorm_weight, m.phi_pre,
+                r2, self._dropped(b2), self.residual_mode, norm_weight, norm_eps, m.rmsnorm_weight, m.phi_pre,
                 m.phi_post, m.phi_res, m.alpha_pre, m.alpha_post, m.alpha_res, m.b_pre, m.b_post,
                 m.b_res, m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
             return hidden.reshape(shape), normed.reshape(shape)

@@ -15,10 +15,11 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from .checkpoint8 import _check_float, _dense, _rows2d, _weight
+from .checkpoint8 import _FLOATS, _check_float, _dense, _rows2d, _weight
 from .ops import _launch, _ptr, _require_cuda
 
 MOST_TOP = 32
+_INTS = (torch.int64, torch.int32)
 
 
 class TokenLogprobs(NamedTuple):
@@ -31,11 +32,18 @@ class TokenLogprobs(NamedTuple):
 
 
 def _check(what, logits, targets, top):
+    try:  # all at once, for the calls that are right: a small call's time is the host's
+        if (logits.is_cuda and logits.device == targets.device and logits.dtype in _FLOATS and targets.dtype in _INTS
+                and targets.shape == logits.shape[:-1] and logits.dim() and 0 <= top <= MOST_TOP
+                and max(top, 1) <= logits.size(-1)):
+            return
+    except AttributeError:
+        pass
     _require_cuda(what, logits, targets)
     _check_float(what, "logits", logits)
     if logits.dim() == 0 or logits.size(-1) == 0:
         raise RuntimeError(f"{what}: logits must be [..., vocab] with a vocabulary of at least 1")
-    if targets.dtype not in (torch.int64, torch.int32):
+    if targets.dtype not in _INTS:
         raise RuntimeError(f"{what}: targets must be int64 or int32 (got {targets.dtype})")
     if targets.shape != logits.shape[:-1]:
         raise RuntimeError(f"{what}: targets must have the logits' leading dimensions {tuple(logits.shape[:-1])} "
