@@ -117,10 +117,11 @@ class AddRMSNormFunction(torch.autograd.Function):
         hidden, out, rms, kept = add_rmsnorm_fwd(residual, branch, weight, eps, p, rng, keep)
         ctx.p, ctx.rng = p, None
         saved = [hidden, weight, rms]
-        if torch.is_tensor(rng):
-            saved.append(rng)
-        elif rng is not None:
-            ctx.rng = tuple(rng)
+        if _drop("add_rmsnorm", p):
+            if torch.is_tensor(rng):
+                saved.append(rng)
+            else:
+                ctx.rng = tuple(rng)
         ctx.save_for_backward(*saved)
         ctx.set_materialize_grads(False)
         ctx.out_dtype = out.dtype

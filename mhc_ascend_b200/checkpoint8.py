@@ -24,6 +24,7 @@ from typing import Optional, Sequence
 import torch
 from torch.autograd.function import once_differentiable
 
+from .counter_dropout import no_new_numbers
 from .ops import _f32, _launch, _lib, _require_cuda, _workspace
 
 BLOCK, PITCH = 32, 128
@@ -315,7 +316,7 @@ class Checkpoint8Function(torch.autograd.Function):
         # and the backward differentiates what the forward returned.  The graph is
         # made for that alone: it saves nothing and goes with this call.
         inside = [t.detach().requires_grad_(n) for t, n in zip(tensors, ctx.needs_input_grad[2:])]
-        with torch.enable_grad(), torch.autograd.graph.saved_tensors_hooks(_forget, _forgotten):
+        with torch.enable_grad(), torch.autograd.graph.saved_tensors_hooks(_forget, _forgotten), no_new_numbers():
             out = function(*inside)
         outs = out if isinstance(out, tuple) else (out,)
         if any(map(_holds_tensors, outs)):  # autograd would hand them out without a graph
@@ -332,7 +333,7 @@ class Checkpoint8Function(torch.autograd.Function):
         tensors += [t.detach() for t in saved[2 * k:]]
         for t, n in zip(tensors, need):
             t.requires_grad_(n)
-        with torch.enable_grad(), torch.autocast("cuda", **ctx.autocast):
+        with torch.enable_grad(), torch.autocast("cuda", **ctx.autocast), no_new_numbers():
             out = ctx.function(*tensors)
         outs = out if isinstance(out, tuple) else (out,)
         pairs = [(o, g) for o, g in zip(outs, grad_out) if g is not None and o.requires_grad]

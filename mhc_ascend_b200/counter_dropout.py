@@ -9,7 +9,9 @@ The reference has no counterpart (its layers draw no random numbers).
 
 from __future__ import annotations
 
+import contextlib
 import math
+import threading
 from typing import Tuple, Union
 
 import torch
@@ -19,6 +21,7 @@ from torch.autograd.function import once_differentiable
 from .ops import _launch, _require_cuda
 
 GROUP = 8  # positions are counted in groups of eight values
+_running_twice = threading.local()  # .depth: functions that will run, or run, a second time
 _FLOATS = (torch.float32, torch.bfloat16)
 _WORD = (1 << 64) - 1
 
@@ -28,6 +31,16 @@ Rng = Union[Tuple[int, int], torch.Tensor]
 def dropout_groups(shape) -> int:
     """Positions that a tensor of this shape takes up."""
     return -(-math.prod(shape) // GROUP)
+
+
+@contextlib.contextmanager
+def no_new_numbers():
+    """While a function runs whose second run has to draw the same numbers."""
+    _running_twice.depth = getattr(_running_twice, "depth", 0) + 1
+    try:
+        yield
+    finally:
+        _running_twice.depth -= 1
 
 
 def _drop(what, p):
@@ -112,7 +125,11 @@ class DropoutCounter(nn.Module):
 
     def take(self, groups: int) -> torch.Tensor:
         """(seed, position) for the next ``groups`` groups as an int64 tensor of its
-        own, and the position moved past them."""
+        own, and the position moved past them.  Inside ``checkpoint8_recompute``, which
+        would take others when it runs again, it raises: take them before."""
+        if getattr(_running_twice, "depth", 0):
+            raise RuntimeError("DropoutCounter.take: a function under checkpoint8_recompute may not take new numbers: "
+                               "take them before and drop by them")
         _require_cuda("DropoutCounter.take", self.state)
         if self.state.dtype != torch.int64 or not self.state.is_contiguous():
             raise RuntimeError("DropoutCounter.take: state must be a contiguous int64 tensor")

@@ -604,6 +604,28 @@ __global__ void __launch_bounds__(kLongThreads)
         if (c + j < cols) part[(int64_t)blockIdx.x * cols + c + j] = p[slot(c, j)];
 }
 
+// gw[c] = sum of part[0..blocks)[c]: 32 columns a block, 8 threads a column,
+// each a fixed share of the partial rows.
+__global__ void __launch_bounds__(256)
+    norm_gw_kernel(const float* __restrict__ part, float* __restrict__ gw, int blocks, int64_t cols) {
+  __shared__ float s[8][32];
+  wait_for_previous();
+  const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float t = 0.f;
+  if (c < cols)
+#pragma unroll 4
+    for (int b = q; b < blocks; b += 8) t += part[(int64_t)b * cols + c];
+  s[q][lane] = t;
+  __syncthreads();
+  if (q == 0 && c < cols) {
+    float a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a += s[k][lane];
+    gw[c] = a;
+  }
+}
+
 // How a row is laid over threads: UPT units a thread, `threads` a block; warp:
 // one row a warp; UPT = 0: the row does not fit the registers.
 struct RowPlan {

@@ -91,8 +91,10 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, result: Toke
     _check(what, logits, targets, top)
     x, stride = _rows2d(logits)
     rows, vocab = x.shape
-    if result.stats is None or result.stats.shape != (rows, 2) or result.entropy.numel() != rows:
+    if result.stats is None or result.stats.shape != (rows, 2) or result.entropy.numel() != rows or \
+            (top and (result.top_id.shape != (*targets.shape, top) or result.top_id.dtype != torch.int64)):
         raise RuntimeError(f"{what}: result must be token_logprobs_fwd's for these logits")
+    _require_cuda(what, x, result.stats, result.entropy, *([result.top_id] if top else []))
     grads = []
     for name, g in (("grad_logprob", grad_logprob), ("grad_entropy", grad_entropy), ("grad_top", grad_top)):
         if g is not None:

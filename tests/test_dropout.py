@@ -239,6 +239,23 @@ def test_recomputation_draws_the_same_mask(cuda):
 
 
 @pytest.mark.gpu
+def test_recomputation_takes_no_new_numbers(cuda):
+    """A counter inside would draw another mask when the function runs again."""
+    layer = mhc.StreamDropout(0.3).to(cuda)
+    x = torch.randn(4, 64, device=cuda, requires_grad=True)
+    with pytest.raises(RuntimeError, match="may not take new numbers"):
+        mhc.checkpoint8_recompute(layer, x)
+    assert layer.counter.state.tolist() == [0, 0]
+    with torch.no_grad():  # runs once
+        mhc.checkpoint8_recompute(layer, x)
+    rng = layer.counter.take(mhc.dropout_groups(x.shape))
+    out = mhc.checkpoint8_recompute(lambda t: mhc.dropout(t, layer.p, rng), x)
+    out.sum().backward()
+    assert torch.equal(x.grad != 0, out != 0)
+    assert torch.equal(layer(x.detach()) != 0, mhc.dropout(x.detach(), 0.3, (0, 64)) != 0)  # and is free again
+
+
+@pytest.mark.gpu
 def test_gpu_refusals(cuda):
     x = torch.randn(8, device=cuda)
     for rng in (5, (1, 2, 3), "ab", torch.zeros(2, device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)):

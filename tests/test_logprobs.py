@@ -442,5 +442,10 @@ def test_refusals(cuda):
         mhc.token_logprobs_bwd(x, t, r, torch.ones(2, device=cuda))
     with pytest.raises(RuntimeError, match="for these logits"):
         mhc.token_logprobs_bwd(x, t, mhc.token_logprobs_fwd(x[:2], t[:2]), None)
+    for bad in (r._replace(stats=r.stats.cpu()), r._replace(entropy=r.entropy.cpu()), r._replace(top_id=r.top_id.cpu())):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            mhc.token_logprobs_bwd(x, t, bad, None, None, torch.ones(3, 2, device=cuda))
+    with pytest.raises(RuntimeError, match="for these logits"):
+        mhc.token_logprobs_bwd(x, t, r._replace(top_id=r.top_id.int()), None, None, torch.ones(3, 2, device=cuda))
     with pytest.raises(RuntimeError, match="at most"):
         mhc.token_logprobs(torch.empty(1, (1 << 21) + 1, device=cuda), t[:1])

@@ -78,7 +78,7 @@ def test_captured_step(cuda):
 
     def run():
         got, _ = step(leaves, ids, counter.take(groups), 0.2, True)
-        return (got.logprob, *torch.autograd.grad(-got.logprob.sum(), leaves))
+        return (got.logprob.detach(), *torch.autograd.grad(-got.logprob.sum(), leaves))
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
