@@ -328,7 +328,7 @@ __device__ __forceinline__ V8 sums_of(const float4& x, const float4& y) {
 }
 
 template <typename TR, typename TB, bool EVEN>
-__global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const BwdArgs p) {
+__global__ void __launch_bounds__(1024) add_norm_bwd_long_kernel(const BwdArgs p) {
   let_next_start();
   extern __shared__ __align__(16) unsigned char keep[];  // halves of a unit's eight sums apart
   __shared__ float red[2][32];
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
   const int64_t total = p.rows * cols;
   float4* lo = reinterpret_cast<float4*>(keep);
   float4* hi = lo + U;
-  for (int u = threadIdx.x; u < U; u += kLongThreads) lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int u = threadIdx.x; u < U; u += blockDim.x) lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
   const DropKey key = drop_key(p.drop);
   auto weights = [&](int c) { return EVEN ? v8_weights(p.w + c) : v8_weights_inside(p.w, c, cols); };
   auto load = [&](const auto* from, int64_t i) -> V8 {  // the unit at element i
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
     const int64_t at = row * cols - shift;
     float2 d2 = make_float2(0.f, 0.f);
 #pragma unroll 2
-    for (int u = threadIdx.x; u < U; u += kLongThreads) {
+    for (int u = threadIdx.x; u < U; u += blockDim.x) {
       const int c = 8 * u - shift;
       V8 gv = load(static_cast<const TB*>(p.g), at + 8 * u), hv = load(static_cast<const TR*>(p.h), at + 8 * u);
       if (!EVEN && v8_edge(c, cols)) {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
     }
     const float coef = -row_total<false>(d2.x + d2.y, red[buf]) / ((float)cols * r * r);
 #pragma unroll 2
-    for (int u = threadIdx.x; u < U; u += kLongThreads) {
+    for (int u = threadIdx.x; u < U; u += blockDim.x) {
       const int c = 8 * u - shift;
       const V8 gw = v8_mul(load(static_cast<const TB*>(p.g), at + 8 * u), weights(c));
       const V8 o = p.gh ? load(static_cast<const TR*>(p.gh), at + 8 * u) : v8_zero();
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_bwd_long_kernel(const B
       else put_grads<TR, TB>(p, key, at + 8 * u, gi);
     }
   }
-  for (int u = threadIdx.x; u < U; u += kLongThreads) {
+  for (int u = threadIdx.x; u < U; u += blockDim.x) {
     V8 a = sums_of(lo[u], hi[u]);
     float* to = p.part + (int64_t)blockIdx.x * cols - shift + 8 * u;
     if (EVEN) v8_save(to, a);
@@ -552,7 +552,9 @@ BwdPlan bwd_plan(int64_t rows, int64_t cols, bool aligned, bool aligned_w, size_
   }
   if (U > 1024) {
     const size_t keep = cols <= kKeepCols ? (size_t)spread * 8 * sizeof(float) : 0;
-    return {fit && keep ? Bwd::kLong : Bwd::kAnyLong, 0, kLongThreads, 0, keep > 100 * 1024 ? 1 : 2, keep};
+    const int per_sm = keep > 100 * 1024 ? 1 : 2;
+    if (fit && keep) return {Bwd::kLong, 0, 1024 / per_sm, 0, per_sm, keep};
+    return {Bwd::kAnyLong, 0, kLongThreads, 0, per_sm, keep};
   }
   if (ck_pitch(cols) <= kWarpCols)
     return {Bwd::kAnyWarp, ck_pitch(cols) <= 256 ? 1 : ck_pitch(cols) <= 512 ? 2 : 4, 32 * kWarpRows, 0, 4, 0};
