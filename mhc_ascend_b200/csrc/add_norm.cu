@@ -162,7 +162,6 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
     return;
   }
   TB* out = static_cast<TB*>(p.out) + at;
-  float* mine = row_sm + (WARP ? (threadIdx.x >> 5) * (int)p.pitch : 0);
 #pragma unroll
   for (int k = 0; k < UPT; ++k) {
     const int c = c0 + k * step;
@@ -180,20 +179,19 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j >= 0 && c + j < cols) mine[row_word(c + j)] = f[j];
+        if (c + j >= 0 && c + j < cols) row_sm[row_word(c + j)] = f[j];
     }
   }
   if (!EVEN && p.codes) {
-    const int i0 = WARP ? lane : (int)threadIdx.x;
-    for (int c = cols + i0; c < p.pitch; c += step / 8) mine[row_word(c)] = 0.f;
-    if (WARP) __syncwarp();
-    else __syncthreads();
+    static_assert(EVEN || CODED || !WARP, "a row's codes pass through the block's shared memory");
+    for (int c = cols + (int)threadIdx.x; c < p.pitch; c += blockDim.x) row_sm[row_word(c)] = 0.f;
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < UPT; ++k) {
-      const int c = 8 * i0 + k * step;
+      const int c = 8 * (int)threadIdx.x + k * step;
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = c < p.pitch ? mine[row_word(c + j)] : 0.f;
+      for (int j = 0; j < 8; ++j) f[j] = c < p.pitch ? row_sm[row_word(c + j)] : 0.f;
       ck_encode(f, p.codes + row * p.pitch, p.exps + row * (p.pitch / kCkBlock), c, c < p.pitch);
     }
   }
@@ -353,8 +351,7 @@ int launch_fwd(const FwdArgs& p, cudaStream_t st) {
                        (CODED ? (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 : even_rows<TB>(p.out, 8, 8));
   const FwdPlan pl = fwd_plan(p.rows, p.cols, aligned, even_rows<float>(p.w, 8, 8), p.grouped, CODED);
   const unsigned blocks = (unsigned)(pl.lay == Lay::kWarp ? (p.rows + kWarpRows - 1) / kWarpRows : p.rows);
-  const size_t smem = pl.way == Way::kUneven && p.codes && !CODED
-                          ? (size_t)p.pitch * sizeof(float) * (pl.lay == Lay::kWarp ? kWarpRows : 1) : 0;
+  const size_t smem = pl.way == Way::kUneven && p.codes && !CODED ? (size_t)p.pitch * sizeof(float) : 0;
   ProfScope prof(CODED ? "add_rmsnorm_coded" : "add_rmsnorm_fwd", st);
 #define MHC_FIT(UPT, LAY, EVEN) add_norm_fwd_kernel<TR, TB, UPT, LAY, CODED, EVEN><<<blocks, pl.threads, smem, st>>>(p)
 #define MHC_GO(UPT, LAY)                                                                                    \
@@ -363,11 +360,15 @@ int launch_fwd(const FwdArgs& p, cudaStream_t st) {
     else add_norm_fwd_any_kernel<UPT, LAY == Lay::kWarp, CODED><<<blocks, pl.threads, 0, st>>>(p);          \
   } while (0)
   if (pl.way == Way::kUneven) {
-    if (pl.lay == Lay::kWarp && pl.UPT == 1) MHC_FIT(1, Lay::kWarp, false);
-    else if (pl.lay == Lay::kWarp && pl.UPT == 2) MHC_FIT(2, Lay::kWarp, false);
-    else if (pl.lay == Lay::kWarp) MHC_FIT(4, Lay::kWarp, false);
-    else if (pl.UPT == 2) MHC_FIT(2, Lay::kBlock, false);
-    else {
+    if (pl.lay == Lay::kWarp) {
+      if constexpr (CODED) {  // the plain form's short rows take the kernel for any row
+        if (pl.UPT == 1) MHC_FIT(1, Lay::kWarp, false);
+        else if (pl.UPT == 2) MHC_FIT(2, Lay::kWarp, false);
+        else MHC_FIT(4, Lay::kWarp, false);
+      }
+    } else if (pl.UPT == 2) {
+      MHC_FIT(2, Lay::kBlock, false);
+    } else {
       // the limit belongs to the kernel: always what its widest row asks for
       if (smem && cudaFuncSetAttribute(add_norm_fwd_kernel<TR, TB, 4, Lay::kBlock, CODED, false>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 4096 * 8 * (int)sizeof(float)) != cudaSuccess)

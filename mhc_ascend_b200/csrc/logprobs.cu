@@ -707,8 +707,9 @@ int launch_fwd(FwdArgs p, int CL, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = CL > 1 ? 1 : 0;
-  if (CL > 1) cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, THREADS, TOP, true>, p);
-  else cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, THREADS, TOP, false>, p);
+  if (CL == 1) cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, THREADS, TOP, false>, p);
+  else if constexpr (THREADS == 512 || (THREADS == 256 && TOP)) cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, THREADS, TOP, true>, p);
+  else return fail(MHC_ERR_UNSUPPORTED, "token_logprobs: no kernel for %d blocks of %d threads a row", CL, THREADS);
   return check_launch("token_logprobs_fwd");
 }
 

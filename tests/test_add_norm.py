@@ -293,6 +293,40 @@ def test_backward_layouts(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tr,tb", [(F32, BF16), (BF16, F32)])
+@pytest.mark.parametrize("R,C", [(20, 100), (17, 500), (9, 1000), (5, 1500), (4, 6000), (3, 8190), (3, 20000), (2, 33000)])
+def test_starts_off_alignment(cuda, R, C, tr, tb):
+    """Views that begin one element into their storage: the kernels for any row."""
+    def off(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda)
+        flat[1:] = t.flatten().to(cuda)
+        return flat[1:].view(t.shape)
+
+    res, br, w, gh, go = inputs(R, C, tr, tb)
+    p, rng = 0.3, (6, 2 ** 32 - 5)
+    keep = mhc.dropout_fwd(torch.ones(R, C, device=cuda), p, rng).cpu() != 0
+    scale = 1 / (1 - round(p * 65536) / 65536)
+    hidden, out, rms, kept = mhc.add_rmsnorm_fwd(off(res), off(br), off(w), EPS, p, rng, keep=True)
+    dropped = torch.where(keep, br.float() * torch.tensor(scale).float(), 0.0)
+    assert torch.equal(hidden.cpu(), (res.float() + dropped).to(tr))
+    check_out(out.cpu(), hidden.cpu(), w, C, tb)
+    packed = mhc.checkpoint8_pack(out)
+    assert torch.equal(kept.codes, packed.codes) and torch.equal(kept.exponents, packed.exponents)
+    got = mhc.add_rmsnorm_bwd(off(gh), off(go), off(hidden), off(w), rms, p, rng)
+    check_grads(got, gh, go, hidden.cpu(), w, keep, scale, C, R)
+    for codes in (E4M3, INT8):
+        for group in (None, 128):
+            h, q = mhc.add_rmsnorm_quantized(off(res), off(br), off(w), EPS, codes, group)
+            want = mhc.add_rmsnorm_quantized(res.to(cuda), br.to(cuda), w.to(cuda), EPS, codes, group)
+            assert torch.equal(h, want[0])
+            # the same sum in another order: scales a few units apart, codes where they round the other way
+            assert bool(((q.scales - want[1].scales).abs() <= 2 * (terms(C) + 12) * U * want[1].scales).all())
+            step = q.scales.repeat_interleave(128 if group else C, 1)[:, :C]
+            apart = (q.unpack(F32) - want[1].unpack(F32)).abs()
+            assert bool((apart <= torch.clamp(q.unpack(F32).abs() * 2.0 ** -3, min=0) * 1.01 + step * 1.01).all())
+
+
+@pytest.mark.gpu
 def test_autograd_against_differences(cuda):
     R, C, p, rng = 6, 40, 0.25, (8, 1)
     res, br, w, gh, go = inputs(R, C, F32, F32)
