@@ -182,6 +182,13 @@ __device__ __forceinline__ float logprob_of(float x, const Part& p) {
 }
 __device__ __forceinline__ float entropy_of(const Part& p) { return p.s == 0.f ? 0.f : logf(p.s) - p.h / p.s; }
 
+// The threads of a row: a block, or a warp of one
+template <int THREADS>
+__device__ __forceinline__ void row_sync() {
+  if (THREADS == 32) __syncwarp();
+  else __syncthreads();
+}
+
 struct TopShared {
   uint64_t best[kMostTop], joined[kMostTop];  // of the block, of the row's blocks together
   uint64_t cand[kCandidates];
@@ -195,16 +202,29 @@ struct TopShared {
 // A block's share [v0, v1) of a row's vectors.  It is walked as [i0, ve): whole
 // vectors first, a first one that is not whole (v0 < i0) in the place behind the last.
 struct Share {
-  int v0, v1, i0, ve;
+  int v0, v1, i0, ve, full;  // full: tiles of whole vectors
+  // place of vector q of a thread's segment in tile `it`: the threads side by side in full
+  // tiles, the warps one behind the other in the last
+  template <int THREADS, int VPT>
+  __device__ __forceinline__ int walk(int it, int q, int t) const {
+    return i0 + it * (THREADS * VPT) + (it < full ? q * THREADS + t : (t & ~31) * VPT + q * 32 + (t & 31));
+  }
   __device__ __forceinline__ int at(int v) const { return v == v1 ? v0 : v; }
 };
+
+// Threads that the last tile's `left` vectors reach, from thread 0 on
+template <int VPT>
+__device__ __forceinline__ int lanes_of(int left) {
+  const int whole = left / (32 * VPT), rest = left - whole * (32 * VPT);
+  return 32 * whole + (rest < 32 ? rest : 32);
+}
 
 // The k largest keys of a share into sh.best, in order (0: none left).  segmax:
 // maxima of the threads' segments; tm: of all of a thread's.
 template <typename T, int THREADS>
 __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, const float* segmax, float tm, TopShared& sh) {
   constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) sh.segments = sh.candidates = 0;
   // values of a vector that reach the bound, as candidates
   auto push = [&](const uint4& u, int e0, float bound, bool all) {
@@ -226,9 +246,10 @@ __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, co
       }
   };
   bool fast;
-  const int lanes = z.ve - z.i0 < THREADS ? z.ve - z.i0 : THREADS;  // that have values
+  // threads that have values: all of them in a full tile, a warp's place and more in the last
+  const int left = z.ve - z.i0, lanes = z.full > 0 ? THREADS : left >= THREADS * VPT ? THREADS : lanes_of<VPT>(left);
   if (lanes < k) {  // 31 vectors at most: all of them
-    __syncthreads();
+    row_sync<THREADS>();
     for (int vec = z.v0 + tid; vec < z.v1; vec += THREADS) push(load_vec(r, vec, z.v1), r.index(vec), 0.f, true);
     fast = true;
   } else {
@@ -238,7 +259,7 @@ __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, co
     float v = tm;
     for (int o = 1; o < each; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (lane % each == 0 && tid / each < groups) sh.maxima[tid / each] = v;
-    __syncthreads();
+    row_sync<THREADS>();
     if (tid < groups) {  // the place of each in their order
       const float mine = sh.maxima[tid];
       int place = 0;
@@ -249,7 +270,7 @@ __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, co
       }
       if (place == k - 1) sh.bound = mine;
     }
-    __syncthreads();
+    row_sync<THREADS>();
     const float bound = sh.bound;
     fast = bound > kFloor;  // too few values end below
     if (fast) {
@@ -258,17 +279,17 @@ __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, co
           const int i = atomicAdd(&sh.segments, 1);
           if (i < kSegments) sh.seg[i] = it * THREADS + tid;
         }
-      __syncthreads();
+      row_sync<THREADS>();
       const int n = sh.segments;
       fast = n <= kSegments;
       if (fast)
         for (int i = tid; i < n * VPT; i += THREADS) {
-          const int g = sh.seg[i / VPT], walk = z.i0 + (g / THREADS) * (THREADS * VPT) + (i % VPT) * THREADS + g % THREADS;
+          const int g = sh.seg[i / VPT], walk = z.walk<THREADS, VPT>(g / THREADS, i % VPT, g % THREADS);
           if (walk < z.ve) push(load_vec(r, z.at(walk), z.v1), r.index(z.at(walk)), bound, false);
         }
     }
   }
-  __syncthreads();
+  row_sync<THREADS>();
   const int c = sh.candidates;
   fast = fast && c <= kCandidates;
   if (fast) {
@@ -300,15 +321,15 @@ __device__ void select_top(const Row<T>& r, const Share& z, int k, int tiles, co
     uint64_t mine = below(~0ull);
     for (int i = 0; i < k; ++i) {
       const uint64_t w = warp_max(mine);
-      __syncthreads();  // everyone has read the last round's
+      row_sync<THREADS>();  // everyone has read the last round's
       if (lane == 0) sh.warps[warp] = w;
-      __syncthreads();
+      row_sync<THREADS>();
       const uint64_t top = warp_max(lane < W ? sh.warps[lane] : 0ull);
       if (tid == 0) sh.best[i] = top;
       if (top != 0 && mine == top) mine = below(top);
     }
   }
-  __syncthreads();
+  row_sync<THREADS>();
 }
 
 struct FwdArgs {
@@ -375,9 +396,10 @@ __device__ __forceinline__ void add_careful(Sums& a, const uint4& u) {
   }
 }
 
-// The block's threads' sums together, the same in each thread.
-template <int W>
-__device__ __forceinline__ Part block_part(const Sums& a, float (&red)[3][W]) {
+// The row's threads' sums together, the same in each thread.
+template <int THREADS>
+__device__ __forceinline__ Part block_part(const Sums& a, float (&red)[3][THREADS / 32]) {
+  constexpr int W = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Part p = {a.m, a.s.x + a.s.y, a.h.x + a.h.y};
   auto join = [](Part& p) {
@@ -389,6 +411,7 @@ __device__ __forceinline__ Part block_part(const Sums& a, float (&red)[3][W]) {
     p.h = warp_sum(p.h);
   };
   join(p);
+  if (W == 1) return p;
   if (lane == 0) {
     red[0][warp] = p.m;
     red[1][warp] = p.s;
@@ -401,24 +424,34 @@ __device__ __forceinline__ Part block_part(const Sums& a, float (&red)[3][W]) {
 }
 
 // Blocks an SM for the register budget: 16-bit values leave 40 a thread, 32-bit ones
-// (a segment is 32 registers) 64.
+// (a segment is 32 registers) and rows of one warp 64.
 template <typename T>
-constexpr int fwd_blocks(int threads) { return threads == 32 ? 32 : (sizeof(T) == 4 ? 1024 : 1536) / threads; }
+constexpr int fwd_blocks(int threads) { return threads == 32 || sizeof(T) == 4 ? 1024 : 1536; }
+constexpr int kRows = 4;  // of a block, where a row takes one warp
+constexpr int block_threads(int threads) { return threads == 32 ? 32 * kRows : threads; }
+
+// Shared memory behind a row's segment maxima
+inline __host__ __device__ size_t top_bytes(int tiles, int threads) {
+  return (size_t)tiles * threads * sizeof(float) + sizeof(TopShared);
+}
 
 // One row a cluster of CL blocks, each over its share of the row's vectors; block
-// 0 joins the shares through distributed shared memory.
+// 0 joins the shares through distributed shared memory.  THREADS == 32: a row a warp.
 template <typename T, int THREADS, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_kernel(const FwdArgs p) {
+__global__ void __launch_bounds__(block_threads(THREADS), fwd_blocks<T>(THREADS) / block_threads(THREADS))
+    logprobs_fwd_kernel(const FwdArgs p) {
   constexpr int VE = Row<T>::VE, VPT = kPer / VE, W = THREADS / 32, TILE = THREADS * VPT;
   extern __shared__ __align__(16) unsigned char dyn[];
-  float* segmax = reinterpret_cast<float*>(dyn);
-  TopShared& sh = *reinterpret_cast<TopShared*>(dyn + (size_t)p.tiles * THREADS * sizeof(float));
+  const int tid = threadIdx.x % THREADS, lane = tid & 31, place = threadIdx.x / THREADS;
+  unsigned char* mine = dyn + (TOP ? place * top_bytes(p.tiles, THREADS) : 0);
+  float* segmax = reinterpret_cast<float*>(mine);
+  TopShared& sh = *reinterpret_cast<TopShared*>(mine + (size_t)p.tiles * THREADS * sizeof(float));
   __shared__ float red[2][3][W];
   __shared__ Part shared_part;
-  const int tid = threadIdx.x;
   const int CL = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
   const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
-  const int64_t row = CLUSTER ? blockIdx.x / CL : blockIdx.x;
+  const int64_t row = CLUSTER ? blockIdx.x / CL : THREADS == 32 ? (int64_t)blockIdx.x * kRows + place : blockIdx.x;
+  if (THREADS == 32 && row >= p.rows) return;
   const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, (int)p.V);
   const int each = (r.count + CL - 1) / CL;
   Share z;
@@ -451,24 +484,28 @@ __global__ void __launch_bounds__(THREADS, fwd_blocks<T>(THREADS)) logprobs_fwd_
       tm = fmaxf(tm, mx);
     }
   }
-  for (; v - tid < z.ve; v += TILE, ++it) {  // what is left, and the row's ends
-    uint4 u[VPT];
+  z.full = it;
+  for (; z.i0 + it * TILE < z.ve; ++it) {  // what is left, and the row's ends, to as few warps as it takes
+    float mx = kFloor;
+    if (z.walk<THREADS, VPT>(it, 0, tid - lane) < z.ve) {
+      uint4 u[VPT];
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) {
-      const int w = v + q * THREADS;
-      u[q] = load_vec(r, z.at(w), w < z.ve ? z.v1 : 0);
+      for (int q = 0; q < VPT; ++q) {
+        const int w = z.walk<THREADS, VPT>(it, q, tid);
+        u[q] = load_vec(r, z.at(w), w < z.ve ? z.v1 : 0);
+      }
+      mx = add_vecs<T>(a, u);
     }
-    const float mx = add_vecs<T>(a, u);
     if (TOP) {
       segmax[it * THREADS + tid] = mx;
       tm = fmaxf(tm, mx);
     }
   }
-  Part part = block_part<W>(a, red[0]);
+  Part part = block_part<THREADS>(a, red[0]);
   if (careful(part.m)) {  // the same for the whole block
     a = {kLowest, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     for (int w = z.v0 + tid; w < z.v1; w += THREADS) add_careful<T>(a, load_vec(r, w, z.v1));
-    part = block_part<W>(a, red[1]);
+    part = block_part<THREADS>(a, red[1]);
   }
   if (TOP) select_top<T, THREADS>(r, z, p.top, it, segmax, tm, sh);
   if (CLUSTER) {
@@ -691,18 +728,18 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
 
 template <typename T, int THREADS, bool TOP>
 int launch_fwd(FwdArgs p, int CL, cudaStream_t st) {
-  constexpr int VE = Row<T>::VE;
+  constexpr int VE = Row<T>::VE, rows = block_threads(THREADS) / THREADS;
   const int64_t count = (p.V + VE - 1) / VE + 1, each = (count + CL - 1) / CL;
   p.tiles = (int)((each + THREADS * (kPer / VE) - 1) / (THREADS * (kPer / VE)));
-  const size_t smem = TOP ? (size_t)p.tiles * THREADS * sizeof(float) + sizeof(TopShared) : 0;
+  const size_t smem = TOP ? rows * top_bytes(p.tiles, THREADS) : 0;
   ProfScope prof("token_logprobs_fwd", st);
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)CL;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.rows * CL));
-  cfg.blockDim = dim3(THREADS);
+  cfg.gridDim = dim3((unsigned)((p.rows + rows - 1) / rows * CL));
+  cfg.blockDim = dim3(block_threads(THREADS));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = at;
