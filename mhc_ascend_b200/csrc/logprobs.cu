@@ -611,17 +611,25 @@ __device__ __forceinline__ uint4 grad_vec(uint4 u, const Coef& k) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A block takes `tiles` tiles of a row's vectors.
-template <typename T, bool H>
-__global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs p) {
-  constexpr int VE = Row<T>::VE, VPT = 4;
-  __shared__ int64_t at[kMostTop + 1];
-  __shared__ float own[kMostTop + 1];
-  __shared__ Coef shared_coef;
-  __shared__ bool mine;  // whether a place with a gradient of its own is in the block's range
-  const int tid = threadIdx.x, B_ = blockDim.x;
-  const int64_t row = blockIdx.x / (uint32_t)p.chunks;
-  const int chunk = (int)(blockIdx.x - (uint32_t)row * (uint32_t)p.chunks);
+// A block takes `tiles` tiles of a row's vectors; WARP: rows of 128 vectors at most, one a
+// warp and kRows a block.
+template <typename T, bool H, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kRows : kBwdThreads) logprobs_bwd_kernel(const BwdArgs p) {
+  constexpr int VE = Row<T>::VE, VPT = 4, R = WARP ? kRows : 1;
+  __shared__ int64_t at_[R][kMostTop + 1];
+  __shared__ float own_[R][kMostTop + 1];
+  __shared__ Coef coef_[R];
+  __shared__ bool mine_[R];  // whether a place with a gradient of its own is in the range
+  const int place = WARP ? threadIdx.x >> 5 : 0, tid = WARP ? threadIdx.x & 31 : threadIdx.x, B_ = WARP ? 32 : blockDim.x;
+  int64_t* at = at_[place];
+  float* own = own_[place];
+  auto sync = [] {
+    if (WARP) __syncwarp();
+    else __syncthreads();
+  };
+  const int64_t row = WARP ? (int64_t)blockIdx.x * kRows + place : blockIdx.x / (uint32_t)p.chunks;
+  if (WARP && row >= p.rows) return;
+  const int chunk = WARP ? 0 : (int)(blockIdx.x - (uint32_t)row * (uint32_t)p.chunks);
   const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, (int)p.V);
   T* out = static_cast<T*>(p.gx) + row * p.V;
   const int first = chunk * (B_ * VPT * p.tiles);
@@ -630,11 +638,17 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
   const bool same = ((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) == (uintptr_t)r.shift;
   auto whole = [&](int a) { return same && a >= r.full0 && a + B_ * VPT <= (end < r.full1 ? end : r.full1); };
   uint4 u[VPT];
-  const bool ahead = whole(first);
-  if (ahead) {
+  auto load = [&](int a) {  // a tile
+    if (whole(a)) {
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) u[q] = reinterpret_cast<const uint4*>(r.base)[first + q * B_ + tid];
-  }
+      for (int q = 0; q < VPT; ++q) u[q] = reinterpret_cast<const uint4*>(r.base)[a + q * B_ + tid];
+    } else {
+#pragma unroll
+      for (int q = 0; q < VPT; ++q)
+        if (a + q * B_ + tid < end) u[q] = load_vec(r, a + q * B_ + tid, end);
+    }
+  };
+  load(first);
   for (int i = tid; i <= p.top; i += B_) {
     if (i == 0) {
       const int64_t t = target_of(p.targets, p.ids64, row);
@@ -647,7 +661,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
       own[i] = p.g_top[row * p.top + i - 1];
     }
   }
-  if (p.top) __syncthreads();
+  if (p.top) sync();
   if (tid == 0) {
     float G = own[0];
     bool any = false;
@@ -663,11 +677,11 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
       k.A = -inv * (H ? fmaf(gh, p.entropy[row] - logf(s), G) : G);
       k.B = -inv * gh;
     }
-    shared_coef = k;
-    mine = any && s != 0.f;
+    coef_[place] = k;
+    mine_[place] = any && s != 0.f;
   }
-  __syncthreads();
-  const Coef k = shared_coef;
+  sync();
+  const Coef k = coef_[place];
   if (careful(k.m)) {  // and rows without anything
     for (int v = first + tid; v < end; v += B_) {
       const uint4 w = load_vec(r, v, end);
@@ -680,13 +694,9 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
     }
   } else {
     for (int a = first; a < end; a += B_ * VPT) {
+      if (a != first) load(a);
+      uint4* to = reinterpret_cast<uint4*>(out - r.shift) + a + tid;
       if (whole(a)) {
-        const uint4* from = reinterpret_cast<const uint4*>(r.base) + a + tid;
-        uint4* to = reinterpret_cast<uint4*>(out - r.shift) + a + tid;
-        if (!(ahead && a == first)) {
-#pragma unroll
-          for (int q = 0; q < VPT; ++q) u[q] = from[q * B_];
-        }
 #pragma unroll
         for (int q = 0; q < VPT; ++q) to[q * B_] = grad_vec<T, H>(u[q], k);
       } else {
@@ -694,9 +704,9 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
         for (int q = 0; q < VPT; ++q) {
           const int v = a + q * B_ + tid;
           if (v >= end) continue;
-          const uint4 g = grad_vec<T, H>(load_vec(r, v, end), k);
+          const uint4 g = grad_vec<T, H>(u[q], k);
           if (same && v >= r.full0 && v < r.full1) {
-            reinterpret_cast<uint4*>(out - r.shift)[v] = g;
+            to[q * B_] = g;
           } else {
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
@@ -709,8 +719,8 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const BwdArgs
       }
     }
   }
-  if (!mine) return;
-  __syncthreads();  // before these places are written again
+  if (!mine_[place]) return;
+  sync();  // before these places are written again
   const int lo = r.index(first), hi = r.index(end);
   for (int i = tid; i <= p.top; i += B_) {
     const int64_t e = at[i];
@@ -829,21 +839,29 @@ extern "C" int mhc_token_logprobs_bwd(const void* logits, int32_t logits_bf16, i
     MHC_REQUIRE_PTR(grad_top);
   }
   constexpr int per = 4;  // vectors of a thread and tile
-  const int64_t count = (vocab + (logits_bf16 ? 8 : 4) - 1) / (logits_bf16 ? 8 : 4) + 1;  // with a start that is not aligned
+  const int64_t VE = logits_bf16 ? 8 : 4;
+  // where rows start in a vector: all at one place, or anywhere
+  const int64_t shift = rows == 1 || row_stride % VE == 0 ? (int64_t)(reinterpret_cast<uintptr_t>(logits) & 15) / (logits_bf16 ? 2 : 4) : VE - 1;
+  const int64_t count = (shift + vocab + VE - 1) / VE;
+  const bool warp = count <= 32 * per;
   int64_t threads = ((count + per - 1) / per + 31) / 32 * 32;
-  threads = threads > kBwdThreads ? kBwdThreads : threads;
+  threads = warp ? 32 * kRows : threads > kBwdThreads ? kBwdThreads : threads;
   // several tiles a block where that leaves enough blocks: its coefficients cost as much as a tile
-  int tiles = kBwdTiles;
+  int tiles = warp ? 1 : kBwdTiles;
   while (tiles > 1 && rows * ((count + threads * per * tiles - 1) / (threads * per * tiles)) < 16 * (int64_t)num_sms()) --tiles;
-  const int64_t chunks = (count + threads * per * tiles - 1) / (threads * per * tiles);
+  const int64_t chunks = warp ? 1 : (count + threads * per * tiles - 1) / (threads * per * tiles);
   MHC_REQUIRE(rows * chunks < (1ll << 31), MHC_ERR_UNSUPPORTED, "%s: %lld x %lld logits are too many", what, (long long)rows,
               (long long)vocab);
   const BwdArgs p = {logits, row_stride, rows, vocab, targets, ignore_index, stats, entropy, grad_logprob, grad_entropy,
                      grad_top, top_id, grad_logits, (int)top, chunks, tiles, targets_64 != 0};
   cudaStream_t st = (cudaStream_t)stream;
   ProfScope prof(what, st);
-  const unsigned blocks = (unsigned)(rows * chunks);
-#define MHC_GO(T, H) logprobs_bwd_kernel<T, H><<<blocks, (unsigned)threads, 0, st>>>(p)
+  const unsigned blocks = (unsigned)(warp ? (rows + kRows - 1) / kRows : rows * chunks);
+#define MHC_GO(T, H)                                                                          \
+  do {                                                                                        \
+    if (warp) logprobs_bwd_kernel<T, H, true><<<blocks, (unsigned)threads, 0, st>>>(p);       \
+    else logprobs_bwd_kernel<T, H, false><<<blocks, (unsigned)threads, 0, st>>>(p);           \
+  } while (0)
   if (logits_bf16) {
     if (grad_entropy) MHC_GO(__nv_bfloat16, true);
     else MHC_GO(__nv_bfloat16, false);
