@@ -116,7 +116,8 @@ class DropoutCounter(nn.Module):
     """Seed and position of a stream of random numbers, on the device: taking
     numbers is one small kernel and no host step, so a captured graph takes new
     ones each time it is replayed.  The state is a buffer of the module: it moves
-    with it and is saved with it."""
+    with it and is saved with it.  Ranks that are to draw different masks take
+    different seeds."""
 
     def __init__(self, seed: int = 0, position: int = 0):
         super().__init__()

@@ -26,10 +26,11 @@ struct FwdArgs {
   float eps;
   bool int8, grouped, res16, branch16;
   DropSource drop;
+  double share;  // 1 / cols
 };
 
 // Sum of `a` and largest `m` (NaN if any is) over the row's threads, the same in each.
-template <bool WARP, bool MAX>
+template <bool WARP>
 __device__ __forceinline__ void row_sum_max(float& a, float& m, float* red, float* redm) {
   auto warp_max_nan = [](float v) {
 #pragma unroll
@@ -37,16 +38,36 @@ __device__ __forceinline__ void row_sum_max(float& a, float& m, float* red, floa
     return v;
   };
   a = warp_sum(a);
-  if (MAX) m = warp_max_nan(m);
+  m = warp_max_nan(m);
   if (WARP) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   if (lane == 0) {
     red[warp] = a;
-    if (MAX) redm[warp] = m;
+    redm[warp] = m;
   }
   __syncthreads();
   a = warp_sum(lane < nw ? red[lane] : 0.f);
-  if (MAX) m = warp_max_nan(lane < nw ? redm[lane] : 0.f);
+  m = warp_max_nan(lane < nw ? redm[lane] : 0.f);
+}
+// Sum joined in 64 bits
+template <bool WARP>
+__device__ __forceinline__ double row_sum_d(float a, double* red) {
+  const double s = warp_sum_d((double)a);
+  if (WARP) return s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  if (lane == 0) red[warp] = s;
+  __syncthreads();
+  return warp_sum_d(lane < nw ? red[lane] : 0.0);
+}
+// Root of a row's mean square from the threads' shares, and the largest `m` (CODED).  The
+// plain form keeps what fp32 leaves out, since a step of the kept codes hangs on the last
+// bit of the output; codes with scales do without.
+template <bool WARP, bool CODED>
+__device__ __forceinline__ Root row_root(const FwdArgs& p, float cols, float a, float& m, double* red) {
+  if (!CODED) return root_of(row_sum_d<WARP>(a, red) * p.share + (double)p.eps);
+  row_sum_max<WARP>(a, m, reinterpret_cast<float*>(red), reinterpret_cast<float*>(red) + 32);
+  const float r = sqrtf(a / cols + p.eps);
+  return {r, 0.f, 1.0f / r};
 }
 __device__ __forceinline__ float group_max(float m) {  // over 16 lanes, NaN if any is
 #pragma unroll
@@ -73,7 +94,7 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
                                   LAY == Lay::kSmall ? 4 : LAY == Lay::kBlock && UPT == 2 ? 2 : 1)
     add_norm_fwd_kernel(const FwdArgs p) {
   constexpr bool WARP = LAY == Lay::kWarp;
-  __shared__ float red[32], redm[32];
+  __shared__ double red[32];
   extern __shared__ __align__(16) float row_sm[];  // uneven rows with kept codes: pitch words a row
   const int lane = threadIdx.x & 31, cols = (int)p.cols;
   const int64_t row = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -129,11 +150,10 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
       else am = max_abs_nan(am, gm[k]);
     }
   }
-  float ss = s2.x + s2.y;
-  row_sum_max<WARP, CODED>(ss, am, red, redm);
-  const float r = sqrtf(ss / (float)cols + p.eps), ir = 1.0f / r;
+  const Root root = row_root<WARP, CODED>(p, (float)cols, s2.x + s2.y, am, red);
+  const float ir = root.ir;
   const bool first = WARP ? lane == 0 : threadIdx.x == 0;
-  if (first && p.rms) p.rms[row] = r;
+  if (first && p.rms) p.rms[row] = root.r;
   if (CODED) {
     const float scale = coded_scale(am * ir, p.int8);
     if (first && !p.grouped) p.scales[row] = scale;
@@ -167,7 +187,7 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
     const int c = c0 + k * step;
     V8 y = v8_zero();
     if (c < cols) {
-      y = v8_mul(v8_quotient(v[k], minus_root(r), ir), weights(c));
+      y = v8_mul(v8_quotient(v[k], root), weights(c));
       if (edge(c)) v8_save_inside(out + k * step, y, c, cols);
       else v8_save_rounded(out + k * step, y);
     }
@@ -224,7 +244,7 @@ __device__ __forceinline__ void add_unit_any(const FwdArgs& p, const DropKey& ke
   save_any(p.hidden, p.res16, row, c, p.cols, mine, v);
 }
 template <bool CODED>
-__device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int64_t c, float (&v)[8], float minus_r, float ir,
+__device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int64_t c, float (&v)[8], const Root& root,
                                              float row_scale, float* mine) {
   const int lane = threadIdx.x & 31;
   float wv[8];
@@ -237,19 +257,16 @@ __device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int6
       m = max_abs_nan(m, v[j]);
     }
     if (p.grouped) {
-      scale = coded_scale(group_max(m) * ir, p.int8);
+      scale = coded_scale(group_max(m) * root.ir, p.int8);
       if (c < p.cols && (lane & 15) == 0) p.scales[row * p.groups + c / kCodedGroup] = scale;
     }
-    const float mult = ir * coded_inverse(scale);
+    const float mult = root.ir * coded_inverse(scale);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= mult;
     coded_save_any(reinterpret_cast<uint8_t*>(p.codes) + row * p.cols, c - 8 * lane, p.cols, mine, v, p.int8);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float q = v[j] * ir;
-      v[j] = fmaf(fmaf(q, minus_r, v[j]), ir, q) * wv[j];
-    }
+    for (int j = 0; j < 8; ++j) v[j] = quotient(v[j], root) * wv[j];
     save_any(p.out, p.branch16, row, c, p.cols, mine, v);
     if (p.codes) {  // of the output as it is returned
 #pragma unroll
@@ -261,7 +278,7 @@ __device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int6
 
 template <int UPT, bool WARP, bool CODED>
 __global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_any_kernel(const FwdArgs p) {
-  __shared__ float red[32], redm[32];
+  __shared__ double red[32];
   __shared__ __align__(16) float sm[fwd_threads(UPT, WARP) * 8];
   float* mine = sm + (threadIdx.x >> 5) * 256;
   const int lane = threadIdx.x & 31;
@@ -272,22 +289,21 @@ __global__ void __launch_bounds__(fwd_threads(UPT, WARP)) add_norm_fwd_any_kerne
   float ss = 0.f, am = 0.f;
 #pragma unroll
   for (int k = 0; k < UPT; ++k) add_unit_any<CODED>(p, key, row, unit_col<WARP>(k), mine, v[k], ss, am);
-  row_sum_max<WARP, CODED>(ss, am, red, redm);
-  const float r = sqrtf(ss / (float)p.cols + p.eps), ir = 1.0f / r;
-  const float scale = CODED ? coded_scale(am * ir, p.int8) : 0.f;
+  const Root root = row_root<WARP, CODED>(p, (float)p.cols, ss, am, red);
+  const float scale = CODED ? coded_scale(am * root.ir, p.int8) : 0.f;
   if (WARP ? lane == 0 : threadIdx.x == 0) {
-    if (p.rms) p.rms[row] = r;
+    if (p.rms) p.rms[row] = root.r;
     if (CODED && !p.grouped) p.scales[row] = scale;
   }
 #pragma unroll
-  for (int k = 0; k < UPT; ++k) put_unit_any<CODED>(p, row, unit_col<WARP>(k), v[k], minus_root(r), ir, scale, mine);
+  for (int k = 0; k < UPT; ++k) put_unit_any<CODED>(p, row, unit_col<WARP>(k), v[k], root, scale, mine);
 }
 
 // Rows too long for registers: h is read again, from L2, by the thread that wrote it.
 constexpr int kLongThreads = 1024;
 template <bool CODED>
 __global__ void __launch_bounds__(kLongThreads) add_norm_fwd_long_kernel(const FwdArgs p) {
-  __shared__ float red[32], redm[32];
+  __shared__ double red[32];
   __shared__ __align__(16) float sm[kLongThreads * 8];
   float* mine = sm + (threadIdx.x >> 5) * 256;
   const int lane = threadIdx.x & 31;
@@ -298,18 +314,17 @@ __global__ void __launch_bounds__(kLongThreads) add_norm_fwd_long_kernel(const F
     float v[8];
     add_unit_any<CODED>(p, key, row, c0 + 8 * lane, mine, v, ss, am);
   }
-  row_sum_max<false, CODED>(ss, am, red, redm);
-  const float r = sqrtf(ss / (float)p.cols + p.eps), ir = 1.0f / r;
-  const float scale = CODED ? coded_scale(am * ir, p.int8) : 0.f;
+  const Root root = row_root<false, CODED>(p, (float)p.cols, ss, am, red);
+  const float scale = CODED ? coded_scale(am * root.ir, p.int8) : 0.f;
   if (threadIdx.x == 0) {
-    if (p.rms) p.rms[row] = r;
+    if (p.rms) p.rms[row] = root.r;
     if (CODED && !p.grouped) p.scales[row] = scale;
   }
   const int64_t end = CODED ? p.cols : p.pitch;
   for (int64_t c0 = (threadIdx.x >> 5) * 256; c0 < end; c0 += 8 * kLongThreads) {
     float v[8];
     load_any(p.hidden, p.res16, row, c0 + 8 * lane, p.cols, mine, v);
-    put_unit_any<CODED>(p, row, c0 + 8 * lane, v, minus_root(r), ir, scale, mine);
+    put_unit_any<CODED>(p, row, c0 + 8 * lane, v, root, scale, mine);
   }
 }
 
@@ -475,7 +490,8 @@ extern "C" int mhc_add_rmsnorm_fwd(const void* residual, int32_t residual_bf16, 
     using TR = std::remove_pointer_t<decltype(r)>;
     using TB = std::remove_pointer_t<decltype(b)>;
     const FwdArgs p = {residual, branch, weight, hidden, rms, out, codes, exponents, nullptr, rows, cols, ck_pitch(cols), 0,
-                       eps, false, false, residual_bf16 != 0, branch_bf16 != 0, drop_source(state, seed, position, drop)};
+                       eps, false, false, residual_bf16 != 0, branch_bf16 != 0, drop_source(state, seed, position, drop),
+                       1.0 / (double)cols};
     return launch_fwd<false, TR, TB>(p, (cudaStream_t)stream);
   });
 }
@@ -498,7 +514,7 @@ extern "C" int mhc_add_rmsnorm_coded(const void* residual, int32_t residual_bf16
     using TB = std::remove_pointer_t<decltype(b)>;
     const FwdArgs p = {residual, branch, weight, hidden, nullptr, nullptr, (int8_t*)codes, nullptr, scales, rows, cols, cols,
                        coded_groups(cols, grouped != 0), eps, codes_int8 != 0, grouped != 0, residual_bf16 != 0,
-                       branch_bf16 != 0, drop_source(nullptr, 0, 0, 0)};
+                       branch_bf16 != 0, drop_source(nullptr, 0, 0, 0), 1.0 / (double)cols};
     return launch_fwd<true, TR, TB>(p, (cudaStream_t)stream);
   });
 }

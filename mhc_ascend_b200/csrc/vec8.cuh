@@ -159,14 +159,26 @@ __device__ __forceinline__ V8 v8_fma(const V8& x, float y, const V8& z) {
   for (int j = 0; j < 4; ++j) v.a[j] = __ffma2_rn(x.a[j], make_float2(y, y), z.a[j]);
   return v;
 }
-// x / r to the last bit but for rare ties: the product with ir = 1 / r and one Newton step
-// on the quotient (x - q r is exact in a fused product).  minus_r = -r, or 0 where r is
-// infinite: the step then adds x * 0.
-__device__ __forceinline__ V8 v8_quotient(const V8& x, float minus_r, float ir) {
-  const V8 q = v8_scale(x, ir);
-  return v8_fma(v8_fma(q, minus_r, x), ir, q);
+// r = sqrt(x) as a sum r + lo with a reciprocal, for quotients that are right to their own
+// rounding (one Newton step on the square root and, below, one on the quotient; the
+// residuals are exact in fused products).  An infinite or NaN root has no lo.
+struct Root {
+  float r, lo, ir;
+};
+__device__ __forceinline__ Root root_of(double x) {
+  const float hi = (float)x, r = sqrtf(hi), ir = 1.0f / r;
+  const float lo = (fmaf(-r, r, hi) + (float)(x - (double)hi)) * (0.5f * ir);
+  return {r, r > 0.f && r <= 3.402823466e38f ? lo : 0.f, ir};
 }
-__device__ __forceinline__ float minus_root(float r) { return r > 3.402823466e38f ? 0.f : -r; }
+__device__ __forceinline__ float quotient(float v, const Root& d) {
+  const float m = d.r <= 3.402823466e38f ? d.r : 0.f, q = v * d.ir;  // over an infinite root: v * 0 + v * 0
+  return fmaf(fmaf(-q, d.lo, fmaf(-q, m, v)), d.ir, q);
+}
+__device__ __forceinline__ V8 v8_quotient(const V8& x, const Root& d) {
+  const float m = d.r <= 3.402823466e38f ? -d.r : 0.f;
+  const V8 q = v8_scale(x, d.ir);
+  return v8_fma(v8_fma(q, -d.lo, v8_fma(q, m, x)), d.ir, q);
+}
 // s + x . y, pair by pair
 __device__ __forceinline__ float2 v8_dot(const V8& x, const V8& y, float2 s) {
 #pragma unroll

@@ -423,6 +423,38 @@ def test_captured_step_on_another_stream(cuda):
 
 
 @pytest.mark.gpu
+def test_widths_from_several_host_threads(cuda):
+    """Calls of several widths at once, each thread on a stream of its own: a kernel's limit
+    on shared memory belongs to the process, and so may not follow one call's width."""
+    import threading
+    work, errors = [], []
+    for R, C, tr, tb in ((40, 1032, F32, BF16), (40, 8192, F32, F32), (6, 28672, BF16, BF16), (6, 20001, F32, BF16)):
+        res, br, w, gh, go = (t.to(cuda) for t in inputs(R, C, tr, tb))
+
+        def run(res=res, br=br, w=w, gh=gh, go=go):
+            hidden, out, rms, kept = mhc.add_rmsnorm_fwd(res, br, w, EPS, 0.2, (1, 2), keep=True)
+            return hidden, out, kept.codes, *mhc.add_rmsnorm_bwd(gh, go, hidden, w, rms, 0.2, (1, 2))
+
+        work.append((run, run(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def repeat(run, want, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(60):
+                got = run()
+            if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                errors.append("another result")
+
+    threads = [threading.Thread(target=repeat, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+
+
+@pytest.mark.gpu
 def test_refusals(cuda):
     x, w = torch.randn(4, 16, device=cuda), torch.ones(16, device=cuda)
     with pytest.raises(RuntimeError, match="one shape"):
