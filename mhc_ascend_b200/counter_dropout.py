@@ -117,7 +117,8 @@ class DropoutCounter(nn.Module):
     numbers is one small kernel and no host step, so a captured graph takes new
     ones each time it is replayed.  The state is a buffer of the module: it moves
     with it and is saved with it.  Ranks that are to draw different masks take
-    different seeds."""
+    different seeds; a function that a checkpoint runs again has to be given its
+    numbers, taken before it."""
 
     def __init__(self, seed: int = 0, position: int = 0):
         super().__init__()
