@@ -17,9 +17,10 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import _C
 from .checkpoint8 import _FLOATS, _check_float, _dense, _empty, _weight
 from .counter_dropout import Rng, _drop, _source
-from .ops import _launch, _lib, _require_cuda, _workspace
+from .ops import _launch, _require_cuda
 
 GROUP = 128
 _CODES = (torch.float8_e4m3fn, torch.int8)
@@ -29,9 +30,9 @@ def _check_inputs(what, residual, branch, weight):
     try:  # all at once, for the calls that are right: a small call's time is the host's
         if (residual.is_cuda and residual.device == branch.device == weight.device and residual.dtype in _FLOATS
                 and branch.dtype in _FLOATS and residual.shape == branch.shape and weight.dim() == 1
-                and residual.shape[-1:] == weight.shape and len(weight) > 0):
+                and residual.size(-1) == weight.size(0) > 0):
             return
-    except AttributeError:
+    except (AttributeError, IndexError):
         pass
     _require_cuda(what, residual, branch, weight)
     _check_float(what, "residual", residual)
@@ -52,6 +53,10 @@ def _dropout_args(what, p, rng, device):
     if rng is None:
         raise RuntimeError(f"{what}: dropout needs rng = (seed, position)")
     return (drop, *_source(what, rng, device))
+
+
+def _workspace_bytes(rows, cols):
+    return _C.load().mhc_add_rmsnorm_bwd_workspace_bytes(rows, cols)
 
 
 def add_rmsnorm_fwd(residual: torch.Tensor, branch: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
@@ -84,15 +89,16 @@ def add_rmsnorm_bwd(grad_hidden: Optional[torch.Tensor], grad_out: torch.Tensor,
     and with one type the first two are one tensor."""
     what = "add_rmsnorm_bwd"
     _check_inputs(what, hidden, grad_out, weight)
-    _require_cuda(what, hidden, rms)
+    dev = hidden.device
     cols = hidden.size(-1)
     rows = hidden.numel() // cols
-    if rms.numel() != rows:
-        raise RuntimeError(f"{what}: rms must be [{rows}]")
-    drop = _dropout_args(what, p, rng, hidden.device)
+    if rms.device != dev or rms.numel() != rows:
+        raise RuntimeError(f"{what}: rms must be [{rows}] on {dev}")
+    drop = _dropout_args(what, p, rng, dev)
     gh = None
     if grad_hidden is not None:
-        _require_cuda(what, hidden, grad_hidden)
+        if grad_hidden.device != dev:
+            raise RuntimeError(f"{what}: grad_hidden must be on {dev}")
         if grad_hidden.shape != hidden.shape or grad_hidden.dtype != hidden.dtype:
             raise RuntimeError(f"{what}: grad_hidden must have hidden's shape and type")
         gh = _dense(grad_hidden)
@@ -100,11 +106,11 @@ def add_rmsnorm_bwd(grad_hidden: Optional[torch.Tensor], grad_out: torch.Tensor,
     gr = torch.empty_like(h)
     one = drop[0] == 0 and g.dtype == h.dtype
     gb = gr if one else torch.empty_like(g)
-    gw = torch.empty(cols, dtype=torch.float32, device=h.device)
-    ws = _workspace(_lib.mhc_add_rmsnorm_bwd_workspace_bytes(rows, cols), h.device)
-    _launch("mhc_add_rmsnorm_bwd", h.device, None if gh is None else gh.data_ptr(), g.data_ptr(), h.data_ptr(),
+    gw = torch.empty(cols, dtype=torch.float32, device=dev)
+    ws = torch.empty(_workspace_bytes(rows, cols), dtype=torch.uint8, device=dev)
+    _launch("mhc_add_rmsnorm_bwd", dev, 0 if gh is None else gh.data_ptr(), g.data_ptr(), h.data_ptr(),
             h.dtype == torch.bfloat16, g.dtype == torch.bfloat16, w.data_ptr(), r.data_ptr(), gr.data_ptr(),
-            None if one else gb.data_ptr(), gw.data_ptr(), rows, cols, *drop, ws.data_ptr(), ws.numel())
+            0 if one else gb.data_ptr(), gw.data_ptr(), rows, cols, *drop, ws.data_ptr(), ws.numel())
     return gr, gb, gw
 
 

@@ -94,11 +94,13 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, result: Toke
     if result.stats is None or result.stats.shape != (rows, 2) or result.entropy.numel() != rows or \
             (top and (result.top_id.shape != (*targets.shape, top) or result.top_id.dtype != torch.int64)):
         raise RuntimeError(f"{what}: result must be token_logprobs_fwd's for these logits")
-    _require_cuda(what, x, result.stats, result.entropy, *([result.top_id] if top else []))
+    dev = x.device
+    for t in (result.stats, result.entropy, result.top_id if top else None, grad_logprob, grad_entropy, grad_top):
+        if t is not None and t.device != dev:
+            _require_cuda(what, x, t)
     grads = []
     for name, g in (("grad_logprob", grad_logprob), ("grad_entropy", grad_entropy), ("grad_top", grad_top)):
         if g is not None:
-            _require_cuda(what, x, g)
             if name != "grad_top" and g.shape != targets.shape:
                 raise RuntimeError(f"{what}: {name} must have targets' shape")
             g = _weight(g)
@@ -106,7 +108,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, result: Toke
     t = _dense(targets)
     ids = _dense(result.top_id) if top else None
     stats, entropy = _weight(result.stats), _weight(result.entropy)
-    gx = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
+    gx = torch.empty_like(logits, memory_format=torch.contiguous_format)
     _launch("mhc_token_logprobs_bwd", x.device, x.data_ptr(), x.dtype == torch.bfloat16, stride, t.data_ptr(),
             t.dtype == torch.int64, int(ignore_index), stats.data_ptr(), entropy.data_ptr(), _ptr(ids), _ptr(grads[0]),
             _ptr(grads[1]), _ptr(grads[2]), gx.data_ptr(), rows, vocab, top)
