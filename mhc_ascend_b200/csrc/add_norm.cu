@@ -67,7 +67,7 @@ __device__ __forceinline__ Root row_root(const FwdArgs& p, float cols, float a, 
   if (!CODED) return root_of(row_sum_d<WARP>(a, red) * p.share + (double)p.eps);
   row_sum_max<WARP>(a, m, reinterpret_cast<float*>(red), reinterpret_cast<float*>(red) + 32);
   const float r = sqrtf(a / cols + p.eps);
-  return {r, 0.f, 1.0f / r};
+  return {r, 1.0f / r, 0.f};
 }
 __device__ __forceinline__ float group_max(float m) {  // over 16 lanes, NaN if any is
 #pragma unroll
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(LAY == Lay::kSmall ? 256 : fwd_threads(UPT, LA
     const int c = c0 + k * step;
     V8 y = v8_zero();
     if (c < cols) {
-      y = v8_mul(v8_quotient(v[k], root), weights(c));
+      y = v8_normed(v[k], weights(c), root);
       if (edge(c)) v8_save_inside(out + k * step, y, c, cols);
       else v8_save_rounded(out + k * step, y);
     }
@@ -268,7 +268,7 @@ __device__ __forceinline__ void put_unit_any(const FwdArgs& p, int64_t row, int6
     coded_save_any(reinterpret_cast<uint8_t*>(p.codes) + row * p.cols, c - 8 * lane, p.cols, mine, v, p.int8);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = quotient(v[j], root) * wv[j];
+    for (int j = 0; j < 8; ++j) v[j] = normed(v[j], wv[j], root);
     save_any(p.out, p.branch16, row, c, p.cols, mine, v);
     if (p.codes) {  // of the output as it is returned
 #pragma unroll

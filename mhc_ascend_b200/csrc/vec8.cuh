@@ -159,25 +159,33 @@ __device__ __forceinline__ V8 v8_fma(const V8& x, float y, const V8& z) {
   for (int j = 0; j < 4; ++j) v.a[j] = __ffma2_rn(x.a[j], make_float2(y, y), z.a[j]);
   return v;
 }
-// r = sqrt(x) as a sum r + lo with a reciprocal, for quotients that are right to their own
-// rounding (one Newton step on the square root and, below, one on the quotient; the
-// residuals are exact in fused products).  An infinite or NaN root has no lo.
+// r = sqrt(x) and its reciprocal as a sum ir + lo of two fp32 values (a Newton step each on
+// the root and on the reciprocal; the residuals are exact in fused products).  v / r * w is
+// then v c + v c', c + c' = w (ir + lo): one rounding that counts, in the five operations
+// that v / r by a Newton step and its product with w take, which round twice.
 struct Root {
-  float r, lo, ir;
+  float r, ir, lo;
 };
 __device__ __forceinline__ Root root_of(double x) {
   const float hi = (float)x, r = sqrtf(hi), ir = 1.0f / r;
-  const float lo = (fmaf(-r, r, hi) + (float)(x - (double)hi)) * (0.5f * ir);
-  return {r, r > 0.f && r <= 3.402823466e38f ? lo : 0.f, ir};
+  const float rest = (fmaf(-r, r, hi) + (float)(x - (double)hi)) * (0.5f * ir);  // the root is r + rest
+  const float lo = fmaf(-rest, ir, fmaf(-r, ir, 1.0f)) * ir;
+  return {r, ir, r > 0.f && r <= 3.402823466e38f ? lo : 0.f};
 }
-__device__ __forceinline__ float quotient(float v, const Root& d) {
-  const float m = d.r <= 3.402823466e38f ? d.r : 0.f, q = v * d.ir;  // over an infinite root: v * 0 + v * 0
-  return fmaf(fmaf(-q, d.lo, fmaf(-q, m, v)), d.ir, q);
+__device__ __forceinline__ float normed(float v, float w, const Root& d) {
+  const float c = w * d.ir;
+  return fmaf(v, c, v * fmaf(w, d.lo, fmaf(w, d.ir, -c)));
 }
-__device__ __forceinline__ V8 v8_quotient(const V8& x, const Root& d) {
-  const float m = d.r <= 3.402823466e38f ? -d.r : 0.f;
-  const V8 q = v8_scale(x, d.ir);
-  return v8_fma(v8_fma(q, -d.lo, v8_fma(q, m, x)), d.ir, q);
+__device__ __forceinline__ V8 v8_normed(const V8& v, const V8& w, const Root& d) {
+  V8 y;
+  const float2 ir = make_float2(d.ir, d.ir), lo = make_float2(d.lo, d.lo);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 c = __fmul2_rn(w.a[j], ir);
+    const float2 rest = __ffma2_rn(w.a[j], lo, __ffma2_rn(w.a[j], ir, make_float2(-c.x, -c.y)));
+    y.a[j] = __ffma2_rn(v.a[j], c, __fmul2_rn(v.a[j], rest));
+  }
+  return y;
 }
 // s + x . y, pair by pair
 __device__ __forceinline__ float2 v8_dot(const V8& x, const V8& y, float2 s) {
