@@ -449,3 +449,28 @@ def test_refusals(cuda):
         mhc.token_logprobs_bwd(x, t, r._replace(top_id=r.top_id.int()), None, None, torch.ones(3, 2, device=cuda))
     with pytest.raises(RuntimeError, match="at most"):
         mhc.token_logprobs(torch.empty(1, (1 << 21) + 1, device=cuda), t[:1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mask", ["-inf", "lowest"])
+@pytest.mark.parametrize("T,V", [(5, 200), (3, 1003), (2, 40000), (300, 9000)])
+def test_entropy_gradients_over_masked_logits(cuda, T, V, dtype, mask):
+    """Confident rows (a sum of exponentials of about 1) under entropy gradients above it."""
+    x, t = make(T, V, dtype, seed=5)
+    x[:, 3] = 30.0
+    x[:, V // 4:V // 2] = -INF if mask == "-inf" else torch.finfo(dtype).min
+    t[:] = V - 1
+    gl = torch.randn(T, generator=torch.Generator().manual_seed(V))
+    r = mhc.token_logprobs_fwd(x.to(cuda), t.to(cuda))
+    for size in (2.0, 3.0, 1e3, 65536.0, 1e30):
+        for sign in (1, -1):
+            ge = torch.full((T,), sign * size)
+            for a in (None, gl):
+                gx = mhc.token_logprobs_bwd(x.to(cuda), t.to(cuda), r, None if a is None else a.to(cuda), ge.to(cuda))
+                assert not gx[:, V // 4:V // 2].any()  # NaN counts as one
+                check_grad(gx, x, t, a, ge, None, None)
+    for loss in (lambda e: 3 * e.sum(), lambda e: (e + 5).exp().sum()):
+        leaf = x.to(cuda).requires_grad_(True)
+        loss(mhc.token_logprobs(leaf, t.to(cuda)).entropy).backward()
+        assert torch.isfinite(leaf.grad).all()
