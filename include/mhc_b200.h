@@ -495,7 +495,8 @@ MHC_API int mhc_token_logprobs_fwd(const void* logits, int32_t logits_bf16, int6
 /* Gradient of the logits [rows, vocab], contiguous, in their type, from the
  * gradients of the three results (each may be NULL; grad_top and top_id [rows, top]
  * with top > 0).  A row of nothing but -inf gets zeros; a target outside
- * [0, vocab) other than ignore_index gives its row NaNs. */
+ * [0, vocab) other than ignore_index gives its row NaNs if grad_logprob is given
+ * (the other results do not depend on it). */
 MHC_API int mhc_token_logprobs_bwd(const void* logits, int32_t logits_bf16, int64_t row_stride,
                                    const void* targets, int32_t targets_64, int64_t ignore_index,
                                    const float* stats, const float* entropy, const int64_t* top_id,

@@ -663,7 +663,8 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : kBwdThreads) logprobs_bwd_
       const float g = p.g_logprob ? p.g_logprob[row] : 0.f;
       const bool in = t >= 0 && t < p.V;
       at[0] = in && t != p.ignore ? t : -1;
-      own[0] = t == p.ignore ? 0.f : in ? g : g * __uint_as_float(0x7fc00000u);
+      // a target outside has a log probability of NaN, and nothing else depends on it
+      own[0] = t == p.ignore || !p.g_logprob ? 0.f : in ? g : g * __uint_as_float(0x7fc00000u);
     } else {
       at[i] = p.top_id[row * p.top + i - 1];
       own[i] = p.g_top[row * p.top + i - 1];

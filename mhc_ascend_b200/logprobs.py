@@ -148,7 +148,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, ig
     id; with autograd for all but the ids.
 
     A target equal to ``ignore_index`` has log probability 0 and gives no gradient;
-    any other outside the vocabulary gives NaNs.  A logit of -inf is a token that
+    any other outside the vocabulary has NaN, and so has the gradient through it
+    (entropy and alternatives do not depend on it).  A logit of -inf is a token that
     cannot come; a row of nothing else has log probabilities -inf, entropy 0 and no
     gradient."""
     return TokenLogprobs(*TokenLogprobsFunction.apply(logits, targets, top, ignore_index))

@@ -474,3 +474,23 @@ def test_entropy_gradients_over_masked_logits(cuda, T, V, dtype, mask):
         leaf = x.to(cuda).requires_grad_(True)
         loss(mhc.token_logprobs(leaf, t.to(cuda)).entropy).backward()
         assert torch.isfinite(leaf.grad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [100, 9001])
+def test_targets_outside_touch_the_log_probability_alone(cuda, V):
+    """Entropies and alternatives do not depend on the target, nor do their gradients."""
+    x, _ = make(4, V, F32)
+    t = torch.tensor([-1, V, 1 << 40, 5]).to(cuda)
+    r = mhc.token_logprobs_fwd(x.to(cuda), t, 3)
+    gen = torch.Generator().manual_seed(1)
+    ge, gt = torch.randn(4, generator=gen), torch.randn(4, 3, generator=gen)
+    zero = torch.zeros(4, dtype=torch.int64)
+    for a, b in ((ge, None), (None, gt), (ge, gt)):
+        dev = [None if g is None else g.to(cuda) for g in (a, b)]
+        check_grad(mhc.token_logprobs_bwd(x.to(cuda), t, r, None, *dev), x, zero, None, a, b, r.top_id.cpu())
+    gx = mhc.token_logprobs_bwd(x.to(cuda), t, r, ge.to(cuda))
+    assert torch.isnan(gx[:3]).all() and torch.isfinite(gx[3]).all()
+    leaf = x.to(cuda).requires_grad_(True)
+    mhc.token_logprobs(leaf, t).entropy.sum().backward()
+    assert torch.isfinite(leaf.grad).all()
