@@ -452,7 +452,8 @@ MHC_API int mhc_add_rmsnorm_fwd(const void* residual, int32_t residual_bf16, con
  * codes_int8) with fp32 scales: one a row, or, if grouped, one for each 128 columns
  * [rows, ceil(cols / 128)].  With a = max |out| of a group, scale =
  * max(a / 448, 2^-100) (int8: a / 127) and code = out / scale rounded to nearest,
- * ties to even; a group with an infinity or a NaN has a NaN scale. */
+ * ties to even; a group with an infinity or a NaN, also of hidden * weight, which is
+ * formed in fp32, has a NaN scale. */
 MHC_API int mhc_add_rmsnorm_coded(const void* residual, int32_t residual_bf16, const void* branch,
                                   int32_t branch_bf16, const float* weight, void* hidden,
                                   void* codes, int32_t codes_int8, float* scales, int32_t grouped,

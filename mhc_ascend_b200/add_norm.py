@@ -198,7 +198,8 @@ def add_rmsnorm_quantized(residual: torch.Tensor, branch: torch.Tensor, weight: 
     residual + branch, the output is ``add_rmsnorm``'s before it is rounded.
     ``codes``: torch.float8_e4m3fn or torch.int8; ``group``: None for a scale a row,
     128 for one for each 128 columns.  scale = max(largest |out| / 448 (127 for
-    int8), 2**-100); a row or group with an infinity or a NaN stands for NaNs."""
+    int8), 2**-100); a row or group with an infinity or a NaN, also of hidden * weight
+    in fp32, stands for NaNs."""
     what = "add_rmsnorm_quantized"
     _check_inputs(what, residual, branch, weight)
     if codes not in _CODES:

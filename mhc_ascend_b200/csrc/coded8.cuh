@@ -28,6 +28,9 @@ __device__ __forceinline__ float coded_inverse(float scale) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(scale));
   return y;
 }
+// Whether 1 / r times the reciprocal of a scale (2^100 at most) may pass fp32: h w is then
+// multiplied by one after the other.  The same for a whole row.
+__device__ __forceinline__ bool coded_apart(float ir) { return ir > 0x1p27f; }
 
 // Two codes from two values that have been divided by the scale, a in the low byte.
 __device__ __forceinline__ uint32_t coded_pair(float a, float b, bool int8) {

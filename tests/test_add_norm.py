@@ -489,3 +489,38 @@ def test_refusals(cuda):
     hidden.detach().add_(1.0)  # the backward pass reads it
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", [E4M3, INT8])
+@pytest.mark.parametrize("group", [None, 128])
+@pytest.mark.parametrize("R,C", [(3, 7), (3, 250), (5, 256), (4, 1000), (3, 1001), (4, 2048), (300, 2048), (2, 4097), (2, 8192),
+                                 (300, 8192), (2, 16384), (2, 33000)])
+def test_quantized_rows_of_tiny_values(cuda, R, C, group, codes):
+    """Rows, and groups of a row, whose scale is the least one, under a reciprocal of the root
+    past 2^28: their product is past fp32, the codes are those of the formula all the same."""
+    w = torch.ones(C, device=cuda)
+    x = torch.zeros(R, C, device=cuda)
+    x[1, 0] = 1e-12
+    with torch.no_grad():
+        for start in (0, 1):  # 1: off alignment, the kernels for any row
+            flat = torch.empty(R * C + start, device=cuda)
+            v = flat[start:].view(R, C)
+            v.copy_(x)
+            for eps in (1e-20, 1e-30, 0.0):
+                _, q = mhc.add_rmsnorm_quantized(v, torch.zeros_like(v), w, eps, codes, group)
+                back = q.unpack(F32)
+                if eps:
+                    assert not back[0].any() and not back[2:].any()  # NaN counts as one
+                assert not back[1, 1:].any()
+                want = 1e-12 / ((1e-24 / C) + eps) ** 0.5
+                # half a step of e4m3 (2^-4) or int8 at its largest code
+                assert back[1, 0].item() == pytest.approx(want, rel=2.0 ** -4)
+            # weights below the least scale: 1e-10 / 1e-10 * 1e-30, with h w below fp32's normal values
+            v.fill_(1e-10)
+            _, q = mhc.add_rmsnorm_quantized(v, torch.zeros_like(v), w * 1e-30, 0.0, codes, group)
+            assert bool((q.scales == 2.0 ** -100).all())
+            y = 1e-30
+            # half a step (of int8 half the scale), and half of h w's last bit, 2^-149 in 1e-40
+            tol = y * (2.0 ** -4 + 1e-4) if codes == E4M3 else 2.0 ** -101 + y * 1e-4
+            assert bool(((q.unpack(F32).double() - y).abs() <= tol).all())
