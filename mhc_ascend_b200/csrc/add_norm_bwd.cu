@@ -273,11 +273,18 @@ __global__ void __launch_bounds__(MOST, ring_blocks(MOST)) add_norm_bwd_ring_ker
   uint32_t s = 0;
   int buf = 0;
   int64_t at = (int64_t)blockIdx.x * cols + c;
-  float nr = p.rms[blockIdx.x];
+  // 1 / rms, rounded to nearest since it is common to a row's terms of gw: 32 of the block's
+  // rows at once, one a lane (a division a row in every thread: [8192, 2048] bf16 33.9 us, so 33.0)
+  float irs = 0.f;
+  int turn = 0;
   const float share = 1.0f / (float)cols;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1, at += hop) {
-    const float ir = __fdividef(1.0f, nr);
-    if (row + gridDim.x < p.rows) nr = p.rms[row + gridDim.x];
+    if (turn == 0) {
+      const int64_t mine = row + (int64_t)lane * gridDim.x;
+      if (mine < p.rows) irs = 1.0f / p.rms[mine];
+    }
+    const float ir = __shfl_sync(0xffffffffu, irs, turn);
+    turn = (turn + 1) & 31;
     copies_wait(stages);
     __syncwarp();  // the other lanes' too
     const unsigned char* from = ring + s + warp * span_r;

@@ -524,3 +524,15 @@ def test_quantized_rows_of_tiny_values(cuda, R, C, group, codes):
             # half a step (of int8 half the scale), and half of h w's last bit, 2^-149 in 1e-40
             tol = y * (2.0 ** -4 + 1e-4) if codes == E4M3 else 2.0 ** -101 + y * 1e-4
             assert bool(((q.unpack(F32).double() - y).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(200, 256), (200, 250), (2000, 2056), (2000, 2057), (2000, 4096), (2000, 8193)])
+def test_weight_gradient_has_a_rounded_reciprocal(cuda, R, C):
+    """Row i gives a gradient to column i alone: its sum is 1 / rms of that row, rounded once."""
+    R = min(R, C)
+    rms = torch.exp(torch.empty(R).uniform_(-7, 7, generator=torch.Generator().manual_seed(C))).to(cuda)
+    g = torch.eye(R, C, device=cuda)
+    gw = mhc.add_rmsnorm_bwd(None, g, torch.ones(R, C, device=cuda), torch.ones(C, device=cuda), rms)[2]
+    want = 1 / rms.double()
+    assert bool(((gw[:R].double() - want).abs() <= U * want).all()) and not gw[R:].any()
