@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _C
 from .checkpoint8 import _FLOATS, _check_float, _dense, _empty, _weight
-from .counter_dropout import Rng, _drop, _source
+from .counter_dropout import Rng, _drop, _source, dropout_fwd
 from .ops import _launch, _require_cuda
 
 GROUP = 128
@@ -139,9 +139,13 @@ class AddRMSNormFunction(torch.autograd.Function):
         hidden, weight, rms, *rng = ctx.saved_tensors
         if grad_hidden is None and grad_out is None:
             return (None,) * 7
-        if grad_out is None:
-            grad_out = torch.zeros_like(hidden, dtype=ctx.out_dtype)
-        gr, gb, gw = add_rmsnorm_bwd(grad_hidden, grad_out, hidden, weight, rms, ctx.p, rng[0] if rng else ctx.rng)
+        rng = rng[0] if rng else ctx.rng
+        if grad_out is None:  # the norm, which may have no gradient (rows of zeros, infinities), has no part in it
+            gb = grad_hidden
+            if rng is not None:  # the product in fp32, rounded once
+                gb = dropout_fwd(gb if gb.dtype == ctx.out_dtype else gb.float(), ctx.p, rng)
+            return grad_hidden, gb.to(ctx.out_dtype), torch.zeros_like(weight), None, None, None, None
+        gr, gb, gw = add_rmsnorm_bwd(grad_hidden, grad_out, hidden, weight, rms, ctx.p, rng)
         return gr, gb, gw.to(weight.dtype), None, None, None, None
 
 

@@ -536,3 +536,20 @@ def test_weight_gradient_has_a_rounded_reciprocal(cuda, R, C):
     gw = mhc.add_rmsnorm_bwd(None, g, torch.ones(R, C, device=cuda), torch.ones(C, device=cuda), rms)[2]
     want = 1 / rms.double()
     assert bool(((gw[:R].double() - want).abs() <= U * want).all()) and not gw[R:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tr,tb", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
+def test_gradient_of_hidden_alone(cuda, tr, tb):
+    """What reaches hidden and not the norm goes through as it is, whatever the row holds."""
+    res, br, w, gh, _ = (t.to(cuda) for t in inputs(6, 2056, tr, tb))
+    res[0], br[0] = 0.0, 0.0  # without eps its norm has no gradient
+    res[1, 5], res[2, 7] = float("inf"), float("nan")
+    for p in (0.0, 0.3, 1.0):
+        leaves = [t.clone().requires_grad_(True) for t in (res, br, w)]
+        hidden, _ = mhc.add_rmsnorm(*leaves, 0.0, p, (3, 4))
+        hidden.backward(gh)
+        assert torch.equal(leaves[0].grad, gh)
+        mask = mhc.dropout_fwd(torch.ones_like(gh, dtype=F32), p, (3, 4))  # 0 or the scale: one product
+        assert leaves[1].grad.dtype == tb and torch.equal(leaves[1].grad, (gh.float() * mask).to(tb))
+        assert not leaves[2].grad.any()
