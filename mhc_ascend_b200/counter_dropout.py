@@ -10,9 +10,11 @@ The reference has no counterpart (its layers draw no random numbers).
 from __future__ import annotations
 
 import contextlib
+import copy
+import itertools
 import math
 import threading
-from typing import Tuple, Union
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -24,6 +26,8 @@ GROUP = 8  # positions are counted in groups of eight values
 _running_twice = threading.local()  # .depth: functions that will run, or run, a second time
 _FLOATS = (torch.float32, torch.bfloat16)
 _WORD = (1 << 64) - 1
+_LAYERS = 0x9E3779B97F4A7C15  # odd: between the seeds of layers that are given none, so that few meet small given ones
+_made = itertools.count()  # such layers, in the order in which they are made
 
 Rng = Union[Tuple[int, int], torch.Tensor]
 
@@ -112,6 +116,11 @@ def dropout(x: torch.Tensor, p: float, rng: Rng) -> torch.Tensor:
     return DropoutFunction.apply(x, p, rng)
 
 
+def _int64(v):
+    v = int(v) & _WORD
+    return v - (1 << 64) if v >> 63 else v
+
+
 class DropoutCounter(nn.Module):
     """Seed and position of a stream of random numbers, on the device: taking
     numbers is one small kernel and no host step, so a captured graph takes new
@@ -122,8 +131,7 @@ class DropoutCounter(nn.Module):
 
     def __init__(self, seed: int = 0, position: int = 0):
         super().__init__()
-        words = [v & _WORD for v in (int(seed), int(position))]
-        self.register_buffer("state", torch.tensor([v - (1 << 64) if v >> 63 else v for v in words], dtype=torch.int64))
+        self.register_buffer("state", torch.tensor([_int64(seed), _int64(position)], dtype=torch.int64))
 
     def take(self, groups: int) -> torch.Tensor:
         """(seed, position) for the next ``groups`` groups as an int64 tensor of its
@@ -141,13 +149,27 @@ class DropoutCounter(nn.Module):
 
 
 class StreamDropout(nn.Module):
-    """Dropout layer over its own ``DropoutCounter``; the identity in evaluation."""
+    """Dropout layer over its own ``DropoutCounter``; the identity in evaluation.
 
-    def __init__(self, p: float, seed: int = 0):
+    Layers of one seed drop the same places.  Without a ``seed`` each layer gets another:
+    the process numbers them as they are made (the first has seed 0), and a deep copy
+    of such a layer counts as one more.  The order in which a program builds its model
+    decides them, not ``torch.manual_seed``; a layer restored by ``load_state_dict`` or
+    unpickled goes on with the seed that was saved."""
+
+    def __init__(self, p: float, seed: Optional[int] = None):
         super().__init__()
         _drop("StreamDropout", p)
         self.p = float(p)
-        self.counter = DropoutCounter(seed)
+        self.numbered = seed is None
+        self.counter = DropoutCounter(next(_made) * _LAYERS if seed is None else seed)
+
+    def __deepcopy__(self, memo):
+        made = memo[id(self)] = self.__class__.__new__(self.__class__)
+        made.__dict__ = copy.deepcopy(self.__dict__, memo)
+        if self.__dict__.get("numbered"):  # not there in layers pickled before it was
+            made.counter.state[0] = _int64(next(_made) * _LAYERS)
+        return made
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self.training or self.p == 0.0:

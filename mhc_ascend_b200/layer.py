@@ -8,6 +8,8 @@ reference checkpoint casts it to fp32 automatically.
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.nn as nn
 
@@ -161,12 +163,14 @@ class MHCResidualWrapper(nn.Module):
     bits for the backward; elsewhere the layer keeps the n packed streams in 8
     bits.  ``use_post_norm`` is accepted and, as in the reference
     (layer.py:261), forced off.  With ``branch_dropout`` > 0 the branch output is
-    dropped out in training (``StreamDropout``, seed ``dropout_seed``: its position
-    is saved with the module, and no mask is kept).
+    dropped out in training (``StreamDropout`` with seed ``dropout_seed``; without one
+    each wrapper draws other masks.  Seed and position are saved with the module, and
+    no mask is kept).
     """
 
     def __init__(self, hidden_dim: int, expansion_rate: int = 4, residual_mode: str = "decay",
-                 use_post_norm: bool = True, branch_dropout: float = 0.0, dropout_seed: int = 0, **mhc_kwargs):
+                 use_post_norm: bool = True, branch_dropout: float = 0.0, dropout_seed: Optional[int] = None,
+                 **mhc_kwargs):
         super().__init__()
         self.hidden_dim = hidden_dim
         self.expansion_rate = expansion_rate

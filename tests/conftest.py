@@ -26,6 +26,15 @@ def _native_library():
     yield
 
 
+@pytest.fixture(autouse=True)
+def _layers_numbered_from_zero(monkeypatch):
+    """Dropout layers without a seed are numbered by the process: each test by itself."""
+    import itertools
+
+    from mhc_ascend_b200 import counter_dropout
+    monkeypatch.setattr(counter_dropout, "_made", itertools.count())
+
+
 @pytest.fixture
 def cuda():
     import torch
