@@ -126,8 +126,9 @@ class DropoutCounter(nn.Module):
     numbers is one small kernel and no host step, so a captured graph takes new
     ones each time it is replayed.  The state is a buffer of the module: it moves
     with it and is saved with it.  Ranks that are to draw different masks take
-    different seeds; a function that a checkpoint runs again has to be given its
-    numbers, taken before it."""
+    different seeds.  A function that a checkpoint runs again has to be given its
+    numbers, taken before it: the second run would take others, and ``take`` raises
+    there."""
 
     def __init__(self, seed: int = 0, position: int = 0):
         super().__init__()
@@ -135,11 +136,15 @@ class DropoutCounter(nn.Module):
 
     def take(self, groups: int) -> torch.Tensor:
         """(seed, position) for the next ``groups`` groups as an int64 tensor of its
-        own, and the position moved past them.  Inside ``checkpoint8_recompute``, which
-        would take others when it runs again, it raises: take them before."""
+        own, and the position moved past them.  Inside ``checkpoint8_recompute``, and in a
+        backward pass, where ``torch.utils.checkpoint`` runs a function again, it raises:
+        take them before."""
         if getattr(_running_twice, "depth", 0):
             raise RuntimeError("DropoutCounter.take: a function under checkpoint8_recompute may not take new numbers: "
                                "take them before and drop by them")
+        if torch._C._current_graph_task_id() != -1:  # this thread is inside a backward pass
+            raise RuntimeError("DropoutCounter.take: a function that runs again in the backward pass would draw another "
+                               "mask than the first time: take them before and drop by them")
         _require_cuda("DropoutCounter.take", self.state)
         if self.state.dtype != torch.int64 or not self.state.is_contiguous():
             raise RuntimeError("DropoutCounter.take: state must be a contiguous int64 tensor")
@@ -171,10 +176,18 @@ class StreamDropout(nn.Module):
             made.counter.state[0] = _int64(next(_made) * _LAYERS)
         return made
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def take(self, shape) -> Optional[torch.Tensor]:
+        """Numbers for one call on a tensor of this shape, for a function that a checkpoint
+        runs again; None where the layer is the identity."""
+        if not self.training or self.p == 0.0:
+            return None
+        return self.counter.take(dropout_groups(shape))
+
+    def forward(self, x: torch.Tensor, rng: Optional[Rng] = None) -> torch.Tensor:
+        """x dropped by ``rng`` (``take``'s, or (seed, position)), by new numbers without one."""
         if not self.training or self.p == 0.0:
             return x
-        return dropout(x, self.p, self.counter.take(dropout_groups(x.shape)))
+        return dropout(x, self.p, self.counter.take(dropout_groups(x.shape)) if rng is None else rng)
 
     def extra_repr(self) -> str:
         return f"p={self.p}"

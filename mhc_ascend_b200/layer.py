@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from .checkpoint8 import checkpoint8_recompute, rmsnorm_checkpoint8
-from .counter_dropout import StreamDropout
+from .counter_dropout import Rng, StreamDropout
 from .ops import (
     MHCLayerStaticFunction,
     compute_rms,
@@ -179,16 +179,18 @@ class MHCResidualWrapper(nn.Module):
         self.mhc = MHCLayer(hidden_dim=hidden_dim, expansion_rate=expansion_rate, **mhc_kwargs)
         self.branch_dropout = StreamDropout(branch_dropout, dropout_seed) if branch_dropout else None
 
-    def _dropped(self, branch_output):
+    def _dropped(self, branch_output, rng):
         dropout = getattr(self, "branch_dropout", None)  # not there in modules pickled before it was an argument
         if dropout is None or not self.training:
             return branch_output
         if branch_output.dtype not in (torch.float32, torch.bfloat16):
             branch_output = branch_output.float()
-        return dropout(branch_output)
+        return dropout(branch_output) if rng is None else dropout(branch_output, rng)
 
-    def forward(self, residual: torch.Tensor, branch_output: torch.Tensor) -> torch.Tensor:
-        branch_output = self._dropped(branch_output)
+    def forward(self, residual: torch.Tensor, branch_output: torch.Tensor, dropout_rng: Optional[Rng] = None) -> torch.Tensor:
+        """The new residual.  Where a checkpoint runs this again, ``dropout_rng`` is what
+        ``branch_dropout.take(branch_output.shape)`` gave before it."""
+        branch_output = self._dropped(branch_output, dropout_rng)
         original_shape = residual.shape
         if len(original_shape) == 3:
             B, T, C = original_shape
@@ -225,7 +227,7 @@ class MHCResidualWrapper(nn.Module):
                                      m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
 
     def forward_prenorm(self, residual: torch.Tensor, branch_output: torch.Tensor,
-                        norm_weight: torch.Tensor, norm_eps: float = 1e-5):
+                        norm_weight: torch.Tensor, norm_eps: float = 1e-5, dropout_rng: Optional[Rng] = None):
         """forward() followed by the next branch's input RMSNorm, as a pre-norm
         block uses them: returns (hidden, rmsnorm(hidden, norm_weight,
         norm_eps)).  For n = 4, dynamic H, fp32 the normalised copy is written
@@ -242,11 +244,11 @@ class MHCResidualWrapper(nn.Module):
         if wrapper_fused_supported(r2, b2, self.expansion_rate, C, m.use_dynamic_h) and \
                 self.residual_mode in ("decay", "zero") and not keep:
             hidden, normed = wrapper_fused_dynamic_prenorm(
-                r2, self._dropped(b2), self.residual_mode, norm_weight, norm_eps, m.rmsnorm_weight, m.phi_pre,
+                r2, self._dropped(b2, dropout_rng), self.residual_mode, norm_weight, norm_eps, m.rmsnorm_weight, m.phi_pre,
                 m.phi_post, m.phi_res, m.alpha_pre, m.alpha_post, m.alpha_res, m.b_pre, m.b_post,
                 m.b_res, m.num_sinkhorn_iters, m.sinkhorn_eps, m.rmsnorm_eps)
             return hidden.reshape(shape), normed.reshape(shape)
-        hidden = self.forward(residual, branch_output)
+        hidden = self.forward(residual, branch_output, **({} if dropout_rng is None else {"dropout_rng": dropout_rng}))
         norm = rmsnorm_checkpoint8 if keep else rmsnorm
         return hidden, norm(hidden.reshape(-1, C), norm_weight, norm_eps).reshape(shape)
 
