@@ -27,6 +27,7 @@ _running_twice = threading.local()  # .depth: functions that will run, or run, a
 _FLOATS = (torch.float32, torch.bfloat16)
 _WORD = (1 << 64) - 1
 _LAYERS = 0x9E3779B97F4A7C15  # odd: between the seeds of layers that are given none, so that few meet small given ones
+_RANKS = 0xD1342543DE82EF95  # odd: between the seeds of ranks
 _made = itertools.count()  # such layers, in the order in which they are made
 
 Rng = Union[Tuple[int, int], torch.Tensor]
@@ -124,15 +125,56 @@ def _int64(v):
 class DropoutCounter(nn.Module):
     """Seed and position of a stream of random numbers, on the device: taking
     numbers is one small kernel and no host step, so a captured graph takes new
-    ones each time it is replayed.  The state is a buffer of the module: it moves
-    with it and is saved with it.  Ranks that are to draw different masks take
-    different seeds.  A function that a checkpoint runs again has to be given its
-    numbers, taken before it: the second run would take others, and ``take`` raises
-    there."""
+    ones each time it is replayed.  The state moves with the module and is saved with
+    it, but is no buffer: data-parallel wrappers broadcast buffers, and every rank would
+    go on with rank 0's.  Ranks that are to draw different masks take different seeds,
+    or one seed and a ``rank`` each: ``rank`` shifts the seed and is not saved, so that
+    every rank can load one rank's file and keeps numbers of its own.  A function that a
+    checkpoint runs again has to be given its numbers, taken before it: the second run
+    would take others, and ``take`` raises there."""
 
-    def __init__(self, seed: int = 0, position: int = 0):
+    rank = 0  # of modules pickled before it was an argument
+
+    def __init__(self, seed: int = 0, position: int = 0, rank: int = 0):
         super().__init__()
-        self.register_buffer("state", torch.tensor([_int64(seed), _int64(position)], dtype=torch.int64))
+        self.rank = int(rank)
+        self.state = torch.tensor([_int64(int(seed) + self.rank * _RANKS), _int64(position)], dtype=torch.int64)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.state = fn(self.state)
+        return self
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        state = self.state
+        if self.rank:
+            state = state.clone()
+            state[0] -= _int64(self.rank * _RANKS)
+        destination[prefix + "state"] = state
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        name = prefix + "state"
+        state = state_dict.get(name)
+        super()._load_from_state_dict({k: v for k, v in state_dict.items() if k != name}, prefix, local_metadata, strict,
+                                      missing_keys, unexpected_keys, error_msgs)
+        if state is None:
+            if strict:
+                missing_keys.append(name)
+        elif state.shape != self.state.shape:
+            error_msgs.append(f"size mismatch for {name}: {tuple(state.shape)} in place of {tuple(self.state.shape)}")
+        else:
+            if local_metadata.get("assign_to_params_buffers", False):
+                self.state = state.to(torch.int64, copy=True)
+            else:
+                self.state.copy_(state)  # in place: captured graphs hold its address
+            if self.rank:
+                self.state[0] += _int64(self.rank * _RANKS)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "state" in self._buffers:  # of modules pickled when it was one
+            self.state = self._buffers.pop("state")
 
     def take(self, groups: int) -> torch.Tensor:
         """(seed, position) for the next ``groups`` groups as an int64 tensor of its
@@ -159,21 +201,21 @@ class StreamDropout(nn.Module):
     Layers of one seed drop the same places.  Without a ``seed`` each layer gets another:
     the process numbers them as they are made (the first has seed 0), and a deep copy
     of such a layer counts as one more.  The order in which a program builds its model
-    decides them, not ``torch.manual_seed``; a layer restored by ``load_state_dict`` or
+    decides them, not ``torch.manual_seed``, and ``rank`` is as for the counter; a layer restored by ``load_state_dict`` or
     unpickled goes on with the seed that was saved."""
 
-    def __init__(self, p: float, seed: Optional[int] = None):
+    def __init__(self, p: float, seed: Optional[int] = None, rank: int = 0):
         super().__init__()
         _drop("StreamDropout", p)
         self.p = float(p)
         self.numbered = seed is None
-        self.counter = DropoutCounter(next(_made) * _LAYERS if seed is None else seed)
+        self.counter = DropoutCounter(next(_made) * _LAYERS if seed is None else seed, rank=rank)
 
     def __deepcopy__(self, memo):
         made = memo[id(self)] = self.__class__.__new__(self.__class__)
         made.__dict__ = copy.deepcopy(self.__dict__, memo)
         if self.__dict__.get("numbered"):  # not there in layers pickled before it was
-            made.counter.state[0] = _int64(next(_made) * _LAYERS)
+            made.counter.state[0] = _int64(next(_made) * _LAYERS + made.counter.rank * _RANKS)
         return made
 
     def take(self, shape) -> Optional[torch.Tensor]:

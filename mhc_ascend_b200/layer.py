@@ -164,20 +164,20 @@ class MHCResidualWrapper(nn.Module):
     bits.  ``use_post_norm`` is accepted and, as in the reference
     (layer.py:261), forced off.  With ``branch_dropout`` > 0 the branch output is
     dropped out in training (``StreamDropout`` with seed ``dropout_seed``; without one
-    each wrapper draws other masks.  Seed and position are saved with the module, and
-    no mask is kept).
+    each wrapper draws other masks, and ranks of data parallelism do by ``dropout_rank``.
+    Seed and position are saved with the module, and no mask is kept).
     """
 
     def __init__(self, hidden_dim: int, expansion_rate: int = 4, residual_mode: str = "decay",
                  use_post_norm: bool = True, branch_dropout: float = 0.0, dropout_seed: Optional[int] = None,
-                 **mhc_kwargs):
+                 dropout_rank: int = 0, **mhc_kwargs):
         super().__init__()
         self.hidden_dim = hidden_dim
         self.expansion_rate = expansion_rate
         self.residual_mode = residual_mode
         self.use_post_norm = False
         self.mhc = MHCLayer(hidden_dim=hidden_dim, expansion_rate=expansion_rate, **mhc_kwargs)
-        self.branch_dropout = StreamDropout(branch_dropout, dropout_seed) if branch_dropout else None
+        self.branch_dropout = StreamDropout(branch_dropout, dropout_seed, dropout_rank) if branch_dropout else None
 
     def _dropped(self, branch_output, rng):
         dropout = getattr(self, "branch_dropout", None)  # not there in modules pickled before it was an argument
