@@ -553,3 +553,24 @@ def test_gradient_of_hidden_alone(cuda, tr, tb):
         mask = mhc.dropout_fwd(torch.ones_like(gh, dtype=F32), p, (3, 4))  # 0 or the scale: one product
         assert leaves[1].grad.dtype == tb and torch.equal(leaves[1].grad, (gh.float() * mask).to(tb))
         assert not leaves[2].grad.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tr", [F32, BF16])
+@pytest.mark.parametrize("R,C", [(5, 256), (7, 1000), (300, 2048), (4, 2048), (3, 4097), (310, 4104), (300, 8192), (2, 8192),
+                                 (3, 9001), (2, 16384)])
+def test_dropout_of_a_16_bit_branch(cuda, R, C, tr):
+    """Rows that start on alignment: the mask is that of dropout, the product and the sum are
+    fp32's, and hidden is rounded once."""
+    res, br, w, gh, go = inputs(R, C, tr, BF16)
+    p, rng = 0.3, (6, 2 ** 32 - 5)
+    keep = mhc.dropout_fwd(torch.ones(R, C, device=cuda), p, rng).cpu() != 0
+    scale = 1 / (1 - round(p * 65536) / 65536)
+    hidden, out, rms, kept = mhc.add_rmsnorm_fwd(res.to(cuda), br.to(cuda), w.to(cuda), EPS, p, rng, keep=True)
+    dropped = torch.where(keep, br.float() * torch.tensor(scale).float(), 0.0)
+    assert torch.equal(hidden.cpu(), (res.float() + dropped).to(tr))
+    check_out(out.cpu(), hidden.cpu(), w, C, BF16)
+    packed = mhc.checkpoint8_pack(out)
+    assert torch.equal(kept.codes, packed.codes) and torch.equal(kept.exponents, packed.exponents)
+    got = mhc.add_rmsnorm_bwd(gh.to(cuda), go.to(cuda), hidden, w.to(cuda), rms, p, rng)
+    check_grads(got, gh, go, hidden.cpu(), w, keep, scale, C, R)
