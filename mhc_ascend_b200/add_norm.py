@@ -6,7 +6,7 @@ The blocks of a model that keep a plain residual stream beside the mHC ones run
 branch.  ``add_rmsnorm`` does both in one pass, forward and backward, and can
 write the output's 8-bit checkpoint with it, which ``linear_checkpoint8`` then
 need not pack.  ``add_rmsnorm_quantized`` is the serving form: the output as
-8-bit codes with scales, as 8-bit matrix products take them.  The reference has
+8-bit codes with scales, without padding; ``Coded8.unpack`` restores it.  The reference has
 no counterpart (it normalises by itself, ops.py:87-136).
 """
 

@@ -436,7 +436,8 @@ int with_types(int32_t a_bf16, int32_t b_bf16, F f) {
 }
 
 // Codes back to values: units of 8, four a thread and 256 apart, so that one division finds
-// the row of all ([16384, 7168] e4m3 to bf16 55 us, 6.4 TB/s; one unit a thread 69 us).
+// the row of all ([16384, 7168] e4m3 to bf16 55 us, 6.4 TB/s; one unit a thread 69 us).  Rows
+// of fewer than 256 units are stepped over one by one on the way.
 constexpr int kUnpackUnits = 4;
 template <typename T, bool EVEN>
 __global__ void __launch_bounds__(256)

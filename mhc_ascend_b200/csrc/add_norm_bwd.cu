@@ -554,7 +554,10 @@ BwdPlan bwd_plan(int64_t rows, int64_t cols, bool aligned, bool aligned_w, size_
     int per_sm = 1152 / threads;
     per_sm = per_sm > 6 ? 6 : per_sm < 1 ? 1 : per_sm;
     while (per_sm > 1 && 2 * stage > (size_t)kStageBytes / per_sm) --per_sm;
-    // few rows: half the blocks of wide rows, twice the depth ([1001, 4097] fp32 18 us against 22)
+    // few rows: half the blocks of wide rows, twice the depth (with the weight's sums, cold:
+    // [300, 4096] fp32 16.4 us against 18.4, [1001, 4097] fp32 26.6 against 27.2, [1000, 2560]
+    // bf16 18.4 against 20.5, [1100, 4600] bf16 24.6 against 26.6, fp32 residual and bf16 branch
+    // [1000, 3001] 24.6 against 25.5; [300, 4096] bf16 and [1100, 4096] fp32 the same)
     if (threads > 288 && rows < 4 * per_sm * (int64_t)num_sms()) per_sm = 1;
     size_t s = (size_t)kStageBytes / per_sm / stage;
     s = s > kStagesMost ? kStagesMost : s;

@@ -1,8 +1,11 @@
 // 8-bit codes with a fp32 scale for a row or for a group of 128 columns: e4m3 or
-// int8 codes [rows, cols] without padding, as 8-bit matrix products take them.
+// int8 codes [rows, cols] without padding; the scales are dense, one beside the other in a row.
 //   a = max |y| of the group, scale = max(a / 448, 2^-100) (int8: a / 127),
 //   code = y / scale rounded to nearest, ties to even; it stands for code * scale.
-// A group that holds an infinity or a NaN has a NaN scale and stands for NaNs.
+// A group that holds an infinity or a NaN has a NaN scale and stands for NaNs.  The scale is a
+// product with the rounded 1 / 448 or 1 / 127, and y / scale is h w times 1 / r and the scale's
+// approximate reciprocal: a few units of 2^-24 off the quotients, so that a value next to the
+// middle of two codes may take the other one.
 #pragma once
 
 #include "checkpoint8.cuh"

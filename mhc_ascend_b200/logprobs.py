@@ -4,8 +4,10 @@ alternatives, and the gradient of the logits.
 The end of a step beside ``StreamEmbedding`` at its start: ``-logprob`` of the
 next tokens is the training loss, the entropy its regulariser, and the
 alternatives are what a model answers with.  One pass over the logits, in the
-type they have; nothing of their size is kept or written but the gradient.  The
-reference has no counterpart (its layers end at the streams).
+type they have; nothing of their size is kept or written but the gradient, as long as
+they are one matrix of rows: a contiguous tensor, or two dimensions with any distance of
+rows.  Others, ``logits[:, :-1]`` of three dimensions among them, are copied in each
+pass.  The reference has no counterpart (its layers end at the streams).
 """
 
 from __future__ import annotations
