@@ -201,8 +201,9 @@ class StreamDropout(nn.Module):
     Layers of one seed drop the same places.  Without a ``seed`` each layer gets another:
     the process numbers them as they are made (the first has seed 0), and a deep copy
     of such a layer counts as one more.  The order in which a program builds its model
-    decides them, not ``torch.manual_seed``, and ``rank`` is as for the counter; a layer restored by ``load_state_dict`` or
-    unpickled goes on with the seed that was saved."""
+    decides them, not ``torch.manual_seed``, so ranks that build the same model draw the
+    same masks unless each has a ``rank`` (as for the counter).  A layer restored by
+    ``load_state_dict`` or unpickled goes on with the seed that was saved."""
 
     def __init__(self, p: float, seed: Optional[int] = None, rank: int = 0):
         super().__init__()
@@ -229,7 +230,9 @@ class StreamDropout(nn.Module):
         """x dropped by ``rng`` (``take``'s, or (seed, position)), by new numbers without one."""
         if not self.training or self.p == 0.0:
             return x
-        return dropout(x, self.p, self.counter.take(dropout_groups(x.shape)) if rng is None else rng)
+        if rng is None:  # replicas of torch.nn.DataParallel share the counter of the first device
+            rng = self.counter.take(dropout_groups(x.shape)).to(x.device)
+        return dropout(x, self.p, rng)
 
     def extra_repr(self) -> str:
         return f"p={self.p}"
