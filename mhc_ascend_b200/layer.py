@@ -187,7 +187,8 @@ class MHCResidualWrapper(nn.Module):
             branch_output = branch_output.float()
         return dropout(branch_output) if rng is None else dropout(branch_output, rng)
 
-    def forward(self, residual: torch.Tensor, branch_output: torch.Tensor, dropout_rng: Optional[Rng] = None) -> torch.Tensor:
+    def forward(self, residual: torch.Tensor, branch_output: torch.Tensor,
+                dropout_rng: Optional[Rng] = None) -> torch.Tensor:
         """The new residual.  Where a checkpoint runs this again, ``dropout_rng`` is what
         ``branch_dropout.take(branch_output.shape)`` gave before it."""
         branch_output = self._dropped(branch_output, dropout_rng)
@@ -233,6 +234,7 @@ class MHCResidualWrapper(nn.Module):
         norm_eps)).  For n = 4, dynamic H, fp32 the normalised copy is written
         by the same output pass as the hidden state (no second read of it);
         otherwise the two run back to back on this library's CUDA operators.
+        ``dropout_rng`` as for forward().
         The reference has no such entry: its model code would call
         MHCResidualWrapper.forward (layer.py:287-316) and then rmsnorm
         (ops.py:87-136)."""
